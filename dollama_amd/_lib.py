@@ -125,6 +125,16 @@ HIP_SIGNATURES = {
     "dlm_ln_fold_fp16": (I, [P, I, I, I, P, P, P, P, I, P, P, P]),
     "dlm_sdxl_embed_inputs_fp16": (I, [P, P, I, P, I, I, P, I, P, I, P]),
     "dlm_linear_small_fp16": (I, [P, I, P, P, P, I, I, I, I, I, I, I, P]),
+    "dlm_quantize_rows_fp16": (I, [P, I, P, I, P, I, I, P]),
+    "dlm_quantize_rows_f32": (I, [P, I, P, I, P, I, I, P]),
+    "dlm_dequantize_rows_fp16": (I, [P, I, P, P, I, I, I, P]),
+    "dlm_dequantize_rows_f32": (I, [P, I, P, P, I, I, I, P]),
+    "dlm_rms_norm_q8_fp16": (I, [P, I, P, I, P, I, P, P, I, P, I, I, F, P]),
+    "dlm_rms_norm_q8_f32": (I, [P, I, P, I, P, I, P, P, I, P, I, I, F, P]),
+    "dlm_layer_norm_q8_fp16": (I, [P, I, P, I, P, I, P, P, P, I, P, I, I, F, P]),
+    "dlm_layer_norm_q8_f32": (I, [P, I, P, I, P, I, P, P, P, I, P, I, I, F, P]),
+    "dlm_linear_q8_fp16": (I, [P, I, P, P, I, P, P, P, I, P, I, I, I, I, F, I, P]),
+    "dlm_linear_q8_f32out": (I, [P, I, P, P, I, P, P, P, I, P, I, I, I, I, F, I, P]),
     "dlm_euler_cfg_step": (I, [P, P, P, I, F, F, F, F, P]),
     "dlm_euler_step": (I, [P, P, P, I, F, F, F, P]),
     "dlm_scale_latent_fp16": (I, [P, P, I, F, I, P]),

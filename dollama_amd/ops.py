@@ -34,7 +34,8 @@ __all__ = [
     "launch_bias_add_rowvec", "launch_bias_add_channel", "launch_conv_bias_biasch",
     "launch_conv_bias_residual", "launch_timestep_embedding", "linear", "pack_conv_weight",
     "conv2d_nhwc", "group_norm_nhwc", "attention_strided", "pack_geglu", "nchw_to_nhwc",
-    "nhwc_to_nchw", "linear_small", "sdxl_embed_inputs",
+    "nhwc_to_nchw", "linear_small", "sdxl_embed_inputs", "quantize_rows", "dequantize_rows",
+    "rms_norm_q8", "layer_norm_q8", "linear_q8",
     "ACT_NONE", "ACT_SILU", "ACT_GEGLU", "ACT_GELU",
 ]
 
@@ -712,3 +713,172 @@ def scale_latent(latent: torch.Tensor, model_in: torch.Tensor, scale: float, cop
     _need(latent, n, "latent", dtype=torch.float32)
     _need(model_in, copies * n, "model_in")
     call("dlm_scale_latent_fp16", _p(latent), _p(model_in), n, float(scale), int(copies), _stream())
+
+
+# ---------------------------------------------------------------------------
+# Linears in 8-bit integers
+# ---------------------------------------------------------------------------
+# Rows here may be strided (a slice of the columns of a wider tensor): each
+# tensor is [rows, K] with consecutive values within a row.
+def _rows(t: Optional[torch.Tensor], shape, name: str, dtypes, device, optional=False) -> int:
+    """Row stride of t, a [rows, K] tensor of one of `dtypes` on `device`."""
+    if t is None:
+        if optional:
+            return 0
+        raise ValueError(f"{name} is None")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name} must be {' or '.join(map(str, dtypes))}, got {t.dtype}")
+    if t.dim() != 2 or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    if not t.is_cuda or t.device != device:
+        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    K = t.shape[1]
+    ld = t.stride(0) if t.shape[0] > 1 else max(K, t.stride(0))
+    if K > 1 and t.stride(1) != 1 or ld < K:
+        raise ValueError(f"{name} must have consecutive values in a row and rows that do not overlap")
+    if K < 1:
+        raise ValueError(f"{name} has rows of no values")
+    if max(ld, t.shape[0]) > 0x7fffffff:
+        raise ValueError(f"{name} passes the 32-bit range of rows and row strides")
+    return ld
+
+
+def _vector(t: Optional[torch.Tensor], numel: int, name: str, dtype, device, optional=False) -> None:
+    if t is None and optional:
+        return
+    _need(t, numel, name, dtype=dtype)
+    if t.numel() != numel or t.device != device:
+        raise ValueError(f"{name} must hold {numel} elements on {device}")
+
+
+def _here(t: torch.Tensor, name: str) -> torch.device:
+    """Device of t, which has to be the current one (its current stream is used)."""
+    if not t.is_cuda or t.dim() != 2:
+        raise ValueError(f"{name} must be a 2-D GPU tensor")
+    if t.device.index != torch._C._cuda_getDevice():
+        raise ValueError(f"{name} is on {t.device}, which is not the current device")
+    return t.device
+
+
+def _q8_out(rows: int, K: int, out, scale, device):
+    """8-bit rows and scales: the caller's, or new ones whose rows `linear_q8` takes."""
+    if out is None:
+        out = torch.empty(rows, (K + 15) // 16 * 16, dtype=torch.int8, device=device)[:, :K]
+    if scale is None:
+        scale = torch.empty(rows, dtype=torch.float32, device=device)
+    ld = _rows(out, (rows, K), "out", (torch.int8,), device)
+    _vector(scale, rows, "scale", torch.float32, device)
+    return out, ld, scale
+
+
+_STREAM_TYPES = (torch.float16, torch.float32)
+
+
+def quantize_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None,
+                  scale: Optional[torch.Tensor] = None):
+    """(q, scale) of fp16 or fp32 x [rows, K]: int8 q = round(127 x / max|x|) and
+    fp32 scale = max|x| / 127 per row.  For activations the rows are tokens, for
+    a weight [N, K] its output channels.  A row with an infinity or NaN gets
+    scale NaN.  New q rows start every K-rounded-up-to-16 bytes, as
+    ``linear_q8`` needs them."""
+    dev = _here(x, "x")
+    rows, K = x.shape
+    ldx = _rows(x, (rows, K), "x", _STREAM_TYPES, dev)
+    out, ldq, scale = _q8_out(rows, K, out, scale, dev)
+    call("dlm_quantize_rows_fp16" if x.dtype == torch.float16 else "dlm_quantize_rows_f32", x.data_ptr(), ldx,
+         out.data_ptr(), ldq, scale.data_ptr(), rows, K, _stream())
+    return out, scale
+
+
+def dequantize_rows(q: torch.Tensor, scale: torch.Tensor, dtype=torch.float16,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """q [rows, K] * scale [rows] as fp16 or fp32."""
+    dev = _here(q, "q")
+    rows, K = q.shape
+    ldq = _rows(q, (rows, K), "q", (torch.int8,), dev)
+    _vector(scale, rows, "scale", torch.float32, dev)
+    if out is None:
+        if dtype not in _STREAM_TYPES:
+            raise ValueError(f"dtype must be float16 or float32, got {dtype}")
+        out = torch.empty(rows, K, dtype=dtype, device=dev)
+    ldy = _rows(out, (rows, K), "out", _STREAM_TYPES, dev)
+    call("dlm_dequantize_rows_fp16" if out.dtype == torch.float16 else "dlm_dequantize_rows_f32", q.data_ptr(), ldq,
+         scale.data_ptr(), out.data_ptr(), ldy, rows, K, _stream())
+    return out
+
+
+def _norm_q8(name, x, gamma, beta, residual, eps, sum_out, out, scale):
+    dev = _here(x, "x")
+    rows, K = x.shape
+    same = (x.dtype,)
+    ldx = _rows(x, (rows, K), "x", _STREAM_TYPES, dev)
+    ldr = _rows(residual, (rows, K), "residual", same, dev, optional=True)
+    if residual is None and sum_out is not None:
+        raise ValueError("sum_out needs a residual")
+    if residual is not None and sum_out is None:
+        sum_out = torch.empty(rows, K, dtype=x.dtype, device=dev)
+    ldh = _rows(sum_out, (rows, K), "sum_out", same, dev, optional=True)
+    _vector(gamma, K, "gamma", torch.float16, dev, optional=True)
+    _vector(beta, K, "beta", torch.float16, dev, optional=True)
+    out, ldq, scale = _q8_out(rows, K, out, scale, dev)
+    affine = (_p(gamma),) if name == "rms" else (_p(gamma), _p(beta))
+    call(f"dlm_{name}_norm_q8_{'fp16' if x.dtype == torch.float16 else 'f32'}", x.data_ptr(), ldx, _p(residual), ldr,
+         _p(sum_out), ldh, *affine, out.data_ptr(), ldq, scale.data_ptr(), rows, K, float(eps), _stream())
+    return (out, scale) if residual is None else (out, scale, sum_out)
+
+
+def rms_norm_q8(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+                eps: float = 1e-6, sum_out: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                scale: Optional[torch.Tensor] = None):
+    """RMS norm of h = x + residual as 8-bit rows: (q, scale) of
+    h / sqrt(mean(h^2) + eps) * gamma, as ``quantize_rows`` forms them, and h
+    too where there is a residual.  x, residual and h are fp16 or fp32; sum_out
+    receives h and may be x or residual itself."""
+    return _norm_q8("rms", x, gamma, None, residual, eps, sum_out, out, scale)
+
+
+def layer_norm_q8(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, beta: Optional[torch.Tensor] = None,
+                  residual: Optional[torch.Tensor] = None, eps: float = 1e-5,
+                  sum_out: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                  scale: Optional[torch.Tensor] = None):
+    """``rms_norm_q8`` with a LayerNorm: rows of (h - mean) / sqrt(var + eps) * gamma + beta."""
+    return _norm_q8("layer", x, gamma, beta, residual, eps, sum_out, out, scale)
+
+
+def linear_q8(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.Tensor, bias=None, residual=None,
+              act=ACT_NONE, out: Optional[torch.Tensor] = None, beta=1.0, dtype=torch.float16) -> torch.Tensor:
+    """y = act(sx * sw * (xq @ wq.T) + bias) + beta * residual in fp16 or fp32, for int8
+    xq [M, K] and wq [N, K] with fp32 scales sx [M] and sw [N], as ``quantize_rows`` and
+    the norms make them.  For ACT_GEGLU, wq / sw / bias hold a weight packed with
+    ``pack_geglu`` (quantised after it) and y has N/2 columns.  out may be residual."""
+    dev = _here(xq, "xq")
+    M, K = xq.shape
+    if wq is None or wq.dim() != 2:
+        raise ValueError("wq must be a 2-D GPU tensor")
+    N = wq.shape[0]
+    if act == ACT_GEGLU and N % 16:
+        raise ValueError("GEGLU needs wq.shape[0] % 16 == 0")
+    ncols = N // 2 if act == ACT_GEGLU else N
+    ldx = _rows(xq, (M, K), "xq", (torch.int8,), dev)
+    ldw = _rows(wq, (N, K), "wq", (torch.int8,), dev)
+    k16 = (K + 15) // 16 * 16
+    for t, name, ld in ((xq, "xq", ldx), (wq, "wq", ldw)):
+        # one row may come without the stride it would have among others
+        if ld < k16 and t.shape[0] > 1 or ld % 16 and t.shape[0] > 1 or t.data_ptr() % 16:
+            raise ValueError(f"{name} needs 16-byte aligned rows: make it with quantize_rows or a norm")
+        end = t.storage_offset() + (t.shape[0] - 1) * ld + k16
+        if t.shape[0] and end > t.untyped_storage().nbytes():
+            raise ValueError(f"{name}: the last row has no room up to the next multiple of 16 bytes")
+    _vector(sx, M, "sx", torch.float32, dev)
+    _vector(sw, N, "sw", torch.float32, dev)
+    _vector(bias, N, "bias", torch.float16, dev, optional=True)
+    if out is None:
+        if dtype not in _STREAM_TYPES:
+            raise ValueError(f"dtype must be float16 or float32, got {dtype}")
+        out = torch.empty(M, ncols, dtype=dtype, device=dev)
+    ldy = _rows(out, (M, ncols), "out", _STREAM_TYPES, dev)
+    ldr = _rows(residual, (M, ncols), "residual", (out.dtype,), dev, optional=True)
+    call("dlm_linear_q8_fp16" if out.dtype == torch.float16 else "dlm_linear_q8_f32out", xq.data_ptr(),
+         ldx if M > 1 else k16, sx.data_ptr(), wq.data_ptr(), ldw if N > 1 else k16, sw.data_ptr(), _p(bias),
+         _p(residual), ldr, out.data_ptr(), ldy, M, N, K, float(beta), int(act), _stream())
+    return out

@@ -476,6 +476,79 @@ int dlm_linear_small_fp16(const void* X, int ldx, const void* W, const void* bia
                           int ldy, int M, int N, int K, int silu_in, int act, int accumulate,
                           void* stream);
 
+/* ------------------------------------------------------------------ */
+/* Linears in 8-bit integers                                           */
+/* ------------------------------------------------------------------ */
+
+/* Rows in 8 bits.  A row v of K values is stored as int8 q and one fp32
+ * scale:
+ *   a = max |v|,  q[k] = round(127 v[k] / a) (halves to the even integer),
+ *   scale = a / 127,  so v[k] ~ q[k] * scale and |q| <= 127.
+ * A row of zeros has scale 0 and q 0.  A row that holds an infinity or NaN
+ * (or, in the norms, whose sum of squares overflows fp32) has scale NaN and
+ * q 0, so that everything computed from it is NaN.  A row's result depends on
+ * that row alone.  Where v is exact in fp32 (fp16 rows; their products with an
+ * fp16 gamma) q is the exact quotient's nearest integer.
+ * x [rows, K] with row stride ldx (elements, >= K; any alignment of an
+ * element); q has row stride ldq >= K bytes, of which K are written; a stride
+ * of K rounded up to 16 on a 16-byte aligned q makes it an operand of
+ * dlm_linear_q8_fp16.  Outputs may not overlap inputs.
+ * No counterpart in the reference, whose transformer is fp16 throughout
+ * (src/infer/unet.cu:677-802). */
+int dlm_quantize_rows_fp16(const void* x, int ldx, void* q, int ldq, float* scale, int rows, int K,
+                           void* stream);
+int dlm_quantize_rows_f32(const float* x, int ldx, void* q, int ldq, float* scale, int rows, int K,
+                          void* stream);
+/* y[m, k] = q[m, k] * scale[m], an fp32 product rounded to y's type. */
+int dlm_dequantize_rows_fp16(const void* q, int ldq, const float* scale, void* y, int ldy, int rows,
+                             int K, void* stream);
+int dlm_dequantize_rows_f32(const void* q, int ldq, const float* scale, float* y, int ldy, int rows,
+                            int K, void* stream);
+
+/* The residual's addition, a norm, and its output in 8 bits (as above):
+ *   h = x + R, rounded to their type (R may be NULL: h = x),
+ *   RMS norm:  v = h gamma / sqrt(mean(h^2) + eps)
+ *   LayerNorm: v = (h - mean) / sqrt(var + eps) gamma + beta
+ * with the statistics in fp32 over the stored h.  H (may be NULL; only with
+ * R) receives h and may be x or R itself (same pointer and row stride), but
+ * not overlap them otherwise.  gamma and beta are fp16 [K] and may be NULL
+ * (1 and 0).  x, R, H are fp16 or, in the _f32 forms, fp32. */
+int dlm_rms_norm_q8_fp16(const void* x, int ldx, const void* R, int ldr, void* H, int ldh,
+                         const void* gamma, void* q, int ldq, float* scale, int rows, int K, float eps,
+                         void* stream);
+int dlm_rms_norm_q8_f32(const float* x, int ldx, const float* R, int ldr, float* H, int ldh,
+                        const void* gamma, void* q, int ldq, float* scale, int rows, int K, float eps,
+                        void* stream);
+int dlm_layer_norm_q8_fp16(const void* x, int ldx, const void* R, int ldr, void* H, int ldh,
+                           const void* gamma, const void* beta, void* q, int ldq, float* scale,
+                           int rows, int K, float eps, void* stream);
+int dlm_layer_norm_q8_f32(const float* x, int ldx, const float* R, int ldr, float* H, int ldh,
+                          const void* gamma, const void* beta, void* q, int ldq, float* scale,
+                          int rows, int K, float eps, void* stream);
+
+/* Y[m, n] = act(sx[m] sw[n] sum_k X[m, k] W[n, k] + bias[n]) + beta * R[m, n]
+ * with int8 X [M, K] and W [N, K], one fp32 scale for each row of X (token)
+ * and of W (output channel), int32 sums, and fp32 arithmetic behind them,
+ * rounded once to Y's type (fp16, or fp32 in the _f32out form, whose R is fp32
+ * too).  bias is fp16 [N]; bias and R may be NULL; act = DLM_ACT_*.  For
+ * DLM_ACT_GEGLU the weight rows (with sw and bias) are interleaved as
+ * dlm_geglu_pack_fp16 does (quantise the packed weight), N % 16 == 0, and Y
+ * and R have N/2 columns.  The sums are exact, so a row's result depends on
+ * neither M nor the other rows.
+ * X and W start at 16-byte aligned addresses with row strides ldx, ldw that
+ * are multiples of 16 bytes and at least K rounded up to 16; K <= 131071 (the
+ * range of the sums).  Bytes of a row past K are read but have no effect.  Y
+ * and R take any element-aligned address and row stride (even ones that are
+ * multiples of 16 bytes are the fast ones).  Y may be R (same pointer and row
+ * stride) and not overlap an input otherwise.  Uses no workspace: calls on any
+ * streams, captured or not, are independent. */
+int dlm_linear_q8_fp16(const void* X, int ldx, const float* sx, const void* W, int ldw,
+                       const float* sw, const void* bias, const void* R, int ldr, void* Y, int ldy,
+                       int M, int N, int K, float beta, int act, void* stream);
+int dlm_linear_q8_f32out(const void* X, int ldx, const float* sx, const void* W, int ldw,
+                         const float* sw, const void* bias, const float* R, int ldr, float* Y, int ldy,
+                         int M, int N, int K, float beta, int act, void* stream);
+
 /* Euler step fused with classifier-free guidance (reference
  * src/infer/diffusion.cu:968-973 and src/infer/scheduler.hpp:112-143):
  * eps = u + g (c - u) from noise [2, n] (cond slice first, uncond second),

@@ -1,0 +1,477 @@
+"""The 8-bit rows, norms and linear against float64 on the CPU (GPU).
+
+Every case prints its name before it launches.  Integers are compared exactly
+where the quotient they round is exact in the kernel's inputs (fp16 rows of the
+plain and the RMS kind, fp32 rows of the plain kind); elsewhere an integer may
+differ from the oracle's only where the oracle's quotient lies within the fp32
+rounding error of a half.  u = 2^-24 is fp32's rounding, fp16's is 2^-11.
+"""
+import math
+
+import pytest
+import torch
+
+from dollama_amd import ops
+from oracle import quant_ref as Q
+from oracle import ref_ops as R
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+WIDTHS = [1, 2, 7, 8, 9, 15, 16, 17, 63, 64, 511, 512, 513, 640, 1003, 1024, 1031, 1280, 1536, 1537, 2048, 2500,
+          4096, 4101, 8192, 8200, 16384, 16385, 20000]
+
+
+def announce(msg):
+    print(f"[case] {msg}", flush=True)
+
+
+def cpu(shape, seed, dtype=torch.float16, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * std).to(dtype)
+
+
+def spread(rows, K, seed, dtype=torch.float16):
+    """Rows with channels of unequal spread, as activations have them."""
+    g = torch.Generator().manual_seed(seed)
+    ch = torch.exp(0.7 * torch.randn(K, generator=g))
+    return (torch.randn(rows, K, generator=g) * ch).to(dtype)
+
+
+def gpu_rows(rows, K, dtype):
+    """[rows, K] filled with a sentinel, inside a wider tensor that has to keep it."""
+    whole = torch.full((rows + 2, K + 24), 77, dtype=dtype, device="cuda")
+    return whole, whole[1:rows + 1, 8:8 + K]
+
+
+def untouched(whole, rows, K):
+    w = whole.clone()
+    w[1:rows + 1, 8:8 + K] = 77
+    return bool((w == 77).all())
+
+
+def sum_steps(K):
+    """Most fp32 additions a value of a row passes through: 32 in a thread's
+    registers (or every K / 1024th value of long rows), 6 in a wave, 16 waves."""
+    return max(32, K // 1024 + 1) + 6 + 16
+
+
+# --------------------------------------------------------------- quantise ---
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("K", WIDTHS)
+def test_quantize_rows_is_the_nearest_integer(gpu, K, dtype):
+    rows = 7
+    announce(f"quantize {rows}x{K} {dtype}")
+    x = spread(rows, K, K, dtype)
+    # exact halves: values that are odd multiples of max / 254
+    x[1] = (torch.arange(K) % 255 - 127).to(dtype)
+    x[2] = ((torch.arange(K) * 2 + 1) % 255).to(dtype)
+    x[2, 0] = 254
+    x[3] = 0
+    x[4] = torch.tensor([2.0 ** -24, -2.0 ** -23])[torch.arange(K) % 2].to(dtype)
+    _, q, s = Q.rows(x.double())
+    wq, out = gpu_rows(rows, K, torch.int8)
+    got, scale = ops.quantize_rows(x.cuda(), out=out)
+    assert got is out and untouched(wq, rows, K)
+    assert torch.equal(out.cpu().double(), q)
+    # max / 127 is one fp32 division
+    assert torch.equal(scale.cpu(), x.abs().amax(1).float() / 127.0)
+    assert float((scale.cpu().double() - s).abs().max()) <= U * float(s.max())
+
+
+def test_quantize_rows_of_tiny_and_huge_fp32(gpu):
+    announce("quantize fp32 rows near the ends of the range")
+    x = spread(8, 333, 5, torch.float32)
+    f = torch.tensor([1e-44, 1e-38, 1e-37, 2.0 ** -101, 2.0 ** -99, 1e30, 1e38, 1.0])
+    x = x / x.abs().amax(1, keepdim=True) * f[:, None]
+    t, q, _ = Q.rows(x.double())
+    got, scale = ops.quantize_rows(x.cuda())
+    assert torch.equal(got.cpu().double(), q)
+    assert torch.equal(scale.cpu(), x.abs().amax(1) / 127.0)
+
+
+@pytest.mark.parametrize("K", [5, 320, 1500, 3000, 9000, 17000])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_rows_with_infinity_or_nan_come_out_as_nan_alone(gpu, K, dtype):
+    announce(f"non-finite rows K={K} {dtype}")
+    x = spread(6, K, 3, dtype)
+    x[1, K - 1] = float("inf")
+    x[2, 0] = -float("inf")
+    x[4, K // 2] = float("nan")
+    clean = torch.tensor([0, 3, 5])
+    ok = [r for r in clean.tolist()]
+    g = cpu((K,), 4) * 0.3 + 1
+    for name, call in (("quantize", lambda v: ops.quantize_rows(v)),
+                       ("rms", lambda v: ops.rms_norm_q8(v, g.cuda())),
+                       ("layer", lambda v: ops.layer_norm_q8(v, g.cuda(), g.cuda()))):
+        q, s = call(x.cuda())
+        q0, s0 = call(x[clean].cuda())
+        assert torch.isnan(s[[1, 2, 4]]).all(), name
+        assert (q[[1, 2, 4]] == 0).all(), name
+        assert torch.equal(q[ok], q0) and torch.equal(s[ok], s0), f"{name}: a row depends on its neighbours"
+        y = ops.dequantize_rows(q, s)
+        assert torch.isnan(y[[1, 2, 4]]).all() and torch.isfinite(y[ok]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,K", [(1, 1), (3, 15), (5, 16), (4, 17), (33, 640), (7, 1003), (2, 20000)])
+def test_dequantize_rows(gpu, rows, K, dtype):
+    announce(f"dequantize {rows}x{K} {dtype}")
+    g = torch.Generator().manual_seed(K)
+    q = torch.randint(-128, 128, (rows, K), generator=g, dtype=torch.int8)
+    s = torch.rand(rows, generator=g) * 0.3
+    wide = torch.zeros(rows, K + 11, dtype=torch.int8, device="cuda")
+    wide[:, 3:3 + K] = q.cuda()
+    wy, out = gpu_rows(rows, K, dtype)
+    ops.dequantize_rows(wide[:, 3:3 + K], s.cuda(), out=out)
+    assert untouched(wy, rows, K)
+    assert torch.equal(out.cpu(), (q.float() * s[:, None]).to(dtype))
+    assert torch.equal(ops.dequantize_rows(q.cuda(), s.cuda(), dtype=dtype).cpu(), out.cpu())
+
+
+# ------------------------------------------------------------------ norms ---
+def check_rows(q, scale, v, err, what):
+    """q and scale of the oracle's rows v, whose values the kernel has within
+    err (absolute, per row)."""
+    t, ref, s = Q.rows(v)
+    top = v.abs().amax(1)
+    slack = 127.0 * 2.0 * err / top.clamp_min(1e-300)  # v and its maximum
+    off = (t - q.double()).abs()
+    assert bool((off <= 0.5 + slack[:, None]).all()), f"{what}: off by {float(off.max())}"
+    far = ((t - torch.floor(t) - 0.5).abs() > slack[:, None])
+    assert torch.equal(q.double()[far], ref[far]), f"{what}: an integer away from a half differs"
+    bound = err / 127.0 + 2 * U * s
+    assert bool(((scale.double() - s).abs() <= bound).all()), f"{what}: scale"
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("residual,gamma", [(False, False), (False, True), (True, True)])
+@pytest.mark.parametrize("K", WIDTHS)
+def test_rms_norm_q8(gpu, K, residual, gamma, dtype):
+    rows, eps = 5, 1e-5
+    announce(f"rms_norm_q8 {rows}x{K} residual={residual} gamma={gamma} {dtype}")
+    x = spread(rows, K, K + 1, dtype)
+    x[3] = 0
+    r = cpu((rows, K), 2, dtype) if residual else None
+    if residual:
+        r[3] = 0
+    g = cpu((K,), 3) * 0.3 + 1 if gamma else None
+    h = (x.float() + r.float()).to(dtype) if residual else x
+    wq, out = gpu_rows(rows, K, torch.int8)
+    wh, ho = gpu_rows(rows, K, dtype) if residual else (None, None)
+    res = ops.rms_norm_q8(x.cuda(), None if g is None else g.cuda(), None if r is None else r.cuda(), eps=eps,
+                          sum_out=ho, out=out)
+    assert untouched(wq, rows, K)
+    if residual:
+        assert untouched(wh, rows, K) and torch.equal(res[2].cpu(), h)
+    hd = h.double()
+    gd = None if g is None else g.double()
+    prod = hd if g is None else hd * gd
+    if dtype == torch.float32:
+        prod = (h if g is None else h * g.float()).double()  # one fp32 rounding
+    # the integers come from the products alone, exact to the last half
+    _, q, _ = Q.rows(prod)
+    assert torch.equal(out.cpu().double(), q)
+    v = Q.rms_norm(hd, gd, eps)
+    top = v.abs().amax(1)
+    # a square, its sum's roundings (halved by the root), mean, root, quotient, product of scale
+    rel = U * (0.5 * (sum_steps(K) + 2) + 5)
+    s = top / 127.0
+    assert bool(((res[1].cpu().double() - s).abs() <= rel * s).all())
+    assert float(res[1][3]) == 0.0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("residual,affine", [(False, False), (False, True), (True, True)])
+@pytest.mark.parametrize("K", WIDTHS)
+def test_layer_norm_q8(gpu, K, residual, affine, dtype):
+    rows, eps = 5, 1e-5
+    announce(f"layer_norm_q8 {rows}x{K} residual={residual} affine={affine} {dtype}")
+    x = spread(rows, K, K + 1, dtype)
+    x[1] += 40  # a mean far from 0
+    x[3] = 0
+    r = cpu((rows, K), 2, dtype) if residual else None
+    g = cpu((K,), 3) * 0.3 + 1 if affine else None
+    b = cpu((K,), 4) * 0.2 if affine else None
+    h = (x.float() + r.float()).to(dtype) if residual else x
+    wq, out = gpu_rows(rows, K, torch.int8)
+    wh, ho = gpu_rows(rows, K, dtype) if residual else (None, None)
+    up = lambda t: None if t is None else t.cuda()  # noqa: E731
+    res = ops.layer_norm_q8(x.cuda(), up(g), up(b), up(r), eps=eps, sum_out=ho, out=out)
+    assert untouched(wq, rows, K)
+    if residual:
+        assert untouched(wh, rows, K) and torch.equal(res[2].cpu(), h)
+    hd = h.double()
+    v = Q.layer_norm(hd, None if g is None else g.double(), None if b is None else b.double(), eps)
+    gmax = 1.0 if g is None else float(g.double().abs().max())
+    d = hd - hd.mean(1, keepdim=True)
+    rs = 1.0 / torch.sqrt((d * d).mean(1) + eps)
+    # the mean is off by the sum's roundings of mean |h| at most, and shifts
+    # every value by as much; the root's relative error as in the RMS norm;
+    # difference, product, affine and its rounding: 4 more
+    n = sum_steps(K)
+    shift = U * (n + 2) * hd.abs().mean(1)
+    dmax = d.abs().amax(1)
+    rel = U * (0.5 * (n + 4) + 6) + 0.5 * (shift * rs) ** 2
+    err = gmax * rs * (shift + dmax * rel + U * hd.abs().amax(1)) + U * v.abs().amax(1)
+    check_rows(out.cpu(), res[1].cpu(), v, err, f"layer_norm {K}")
+
+
+def test_norms_write_the_sum_in_place_and_read_strided_rows(gpu):
+    announce("norms: sum over x or over the residual, rows inside wider tensors")
+    for K in (40, 640, 2052, 5000, 17000):
+        for dtype in (torch.float16, torch.float32):
+            x, r, g = spread(9, K, 1, dtype).cuda(), cpu((9, K), 2, dtype).cuda(), (cpu((K,), 3) + 1).cuda()
+            for norm in (ops.rms_norm_q8, ops.layer_norm_q8):
+                q, s, h = norm(x, g, residual=r)
+                for target in ("x", "residual"):
+                    xi, ri = x.clone(), r.clone()
+                    t = xi if target == "x" else ri
+                    qi, si, hi = norm(xi, g, residual=ri, sum_out=t)
+                    assert hi is t and torch.equal(hi, h) and torch.equal(qi, q) and torch.equal(si, s)
+                wx, xs = gpu_rows(9, K, dtype)
+                wr, rs = gpu_rows(9, K, dtype)
+                xs.copy_(x)
+                rs.copy_(r)
+                qi, si, hi = norm(xs, g, residual=rs)
+                assert torch.equal(hi, h) and torch.equal(qi, q) and torch.equal(si, s)
+                # a row's result does not depend on the others
+                q1, s1, h1 = norm(x[4:5], g, residual=r[4:5])
+                assert torch.equal(q1, q[4:5]) and torch.equal(s1, s[4:5]) and torch.equal(h1, h[4:5])
+
+
+# ----------------------------------------------------------------- linear ---
+def int8_rows(rows, K, seed, low=-127):
+    """Random 8-bit rows at a 16-byte row stride whose padding holds garbage."""
+    g = torch.Generator().manual_seed(seed)
+    whole = torch.randint(low, 128, (rows, (K + 15) // 16 * 16), generator=g, dtype=torch.int8)
+    whole[:, K:] = 113
+    return whole.cuda()[:, :K], whole[:, :K]
+
+
+def check_linear(M, N, K, act="none", bias=True, residual=True, dtype=torch.float16, beta=1.0, seed=1, low=-127):
+    announce(f"linear_q8 {M}x{N}x{K} act={act} bias={bias} residual={residual} beta={beta} {dtype}")
+    xg, x = int8_rows(M, K, seed, low)
+    wg, w = int8_rows(N, K, seed + 1, low)
+    g = torch.Generator().manual_seed(seed + 2)
+    sx = (torch.rand(M, generator=g) + 0.5) * (1.5 / (64 * math.sqrt(K)))
+    sw = (torch.rand(N, generator=g) + 0.5) / 64
+    cols = N // 2 if act == "geglu" else N
+    b = cpu((N,), seed + 3) if bias else None
+    r = cpu((M, cols), seed + 4, dtype) if residual else None
+    ref, mag = Q.linear(x, sx, w, sw, b, r, act, beta)
+    up = lambda t: None if t is None else t.cuda()  # noqa: E731
+    wy, out = gpu_rows(M, cols, dtype)
+    code = {"none": ops.ACT_NONE, "silu": ops.ACT_SILU, "gelu": ops.ACT_GELU, "geglu": ops.ACT_GEGLU}[act]
+    y = ops.linear_q8(xg, sx.cuda(), wg, sw.cuda(), bias=up(b), residual=up(r), act=code, out=out, beta=beta)
+    assert y is out and untouched(wy, M, cols), "wrote outside its rows"
+    # conversion, two scales, bias, residual: u each of what they act on, times
+    # at most 1.13 (the activations' slopes); the activations add 4 u (silu) or
+    # the 1.5e-7 of the erf approximation on half the value
+    tol = 8 * U * mag + (0 if act == "none" else 4e-7 * mag)
+    if dtype == torch.float16:
+        tol = tol + 2.0 ** -11 * ref.abs() * 1.001 + 2.0 ** -25
+    off = (out.cpu().double() - ref).abs()
+    assert bool((off <= tol).all()), f"off by {float((off / tol).max()):.2f} of the bound"
+    plain = ops.linear_q8(xg, sx.cuda(), wg, sw.cuda(), bias=up(b), residual=up(r), act=code, dtype=dtype, beta=beta)
+    assert torch.equal(plain, out), "the output's layout shows in its values"
+    return xg, sx, wg, sw, b, r, out
+
+
+SHAPES = [(1, 1, 1), (1, 16, 64), (1, 1280, 640), (1, 63, 1003), (2, 17, 15), (3, 40, 16), (5, 333, 17), (7, 128, 4099),
+          (13, 320, 2560), (16, 96, 63), (17, 96, 65), (31, 130, 100), (32, 64, 1000), (33, 64, 128), (64, 80, 640),
+          (65, 77, 127), (100, 1283, 200), (128, 256, 256), (154, 640, 2048), (200, 1, 513), (257, 300, 1280),
+          (300, 161, 1000), (513, 640, 640), (1000, 320, 333), (2100, 200, 130)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_linear_q8(gpu, M, N, K, dtype):
+    check_linear(M, N, K, dtype=dtype)
+    check_linear(M, N, K, bias=False, residual=False, dtype=dtype, seed=9)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("act", ["silu", "gelu", "geglu"])
+@pytest.mark.parametrize("M,N,K", [(1, 16, 40), (1, 640, 320), (9, 320, 1003), (40, 96, 64), (154, 1280, 640),
+                                   (300, 336, 200), (1030, 640, 320)])
+def test_linear_q8_activations(gpu, M, N, K, act, dtype):
+    check_linear(M, N, K, act=act, dtype=dtype, residual=False)
+    check_linear(M, N, K, act=act, dtype=dtype, beta=-0.75, seed=5)
+
+
+@pytest.mark.parametrize("M", [1, 20, 300])
+def test_linear_q8_sums_reach_the_ends_of_their_range(gpu, M):
+    """K = 131071 products of -128 x -128 stay below 2^31; the sums are exact
+    also where fp32 sums would not be (one odd unit among 2^31)."""
+    announce(f"largest K, M={M}")
+    K, N = 131071, 24
+    x = torch.full((M, 131072), -128, dtype=torch.int8, device="cuda")[:, :K]
+    w = torch.full((N, 131072), -128, dtype=torch.int8, device="cuda")[:, :K]
+    one_m, one_n = torch.ones(M, device="cuda"), torch.ones(N, device="cuda")
+    y = ops.linear_q8(x, one_m, w, one_n, dtype=torch.float32)
+    assert (y == float(128 * 128 * K)).all()  # 2^14 (2^17 - 1): exact in fp32
+    check_linear(M, N, 4096, low=-128, dtype=torch.float32)
+
+
+def test_linear_q8_in_place_residual_and_nan_rows(gpu):
+    for M, N, K in ((3, 64, 100), (70, 200, 640), (300, 640, 640)):
+        xg, sx, wg, sw, b, r, out = check_linear(M, N, K)
+        y = r.cuda()
+        ops.linear_q8(xg, sx.cuda(), wg, sw.cuda(), bias=b.cuda(), residual=y, out=y)
+        assert torch.equal(y, out)
+        sx = sx.clone()
+        sx[M // 2] = float("nan")
+        y = ops.linear_q8(xg, sx.cuda(), wg, sw.cuda(), bias=b.cuda(), residual=r.cuda())
+        assert torch.isnan(y[M // 2]).all()
+        rest = [i for i in range(M) if i != M // 2]
+        assert torch.equal(y[rest], out[rest])
+
+
+def test_linear_q8_row_results_do_not_depend_on_the_batch(gpu):
+    announce("linear_q8: a row alone, in small batches and in a large one")
+    M, N, K = 700, 640, 1280
+    xg, sx, wg, sw, b, r, out = check_linear(M, N, K, act="gelu")
+    for lo, n in ((0, 1), (5, 3), (16, 16), (100, 40), (333, 154), (0, 512)):
+        y = ops.linear_q8(xg[lo:lo + n], sx[lo:lo + n].cuda(), wg, sw.cuda(), bias=b.cuda(),
+                          residual=r[lo:lo + n].cuda(), act=ops.ACT_GELU)
+        assert torch.equal(y, out[lo:lo + n]), f"rows {lo}..{lo + n}"
+
+
+# --------------------------------------------------------------- together ---
+class Block:
+    """Norm, gated projection, row quantisation, projection back and residual:
+    a feed-forward layer in 8 bits."""
+
+    def __init__(self, C, F, seed):
+        k = lambda *s, i=0: cpu(s, seed + i)  # noqa: E731
+        self.gamma, self.beta = (k(C, i=1) * 0.2 + 1).cuda(), (k(C, i=2) * 0.1).cuda()
+        self.w1, self.b1 = (k(2 * F, C, i=3).float() / math.sqrt(C)).half(), k(2 * F, i=4) * 0.1
+        self.w2, self.b2 = (k(C, F, i=5).float() / math.sqrt(F)).half(), k(C, i=6) * 0.1
+        wp, self.b1p = ops.pack_geglu(self.w1.cuda(), self.b1.cuda())
+        self.q1, self.s1 = ops.quantize_rows(wp)
+        self.q2, self.s2 = ops.quantize_rows(self.w2.cuda())
+        self.b2g = self.b2.cuda()
+
+    def __call__(self, x, attn, rms=False):
+        if rms:
+            q, s, h = ops.rms_norm_q8(x, self.gamma, residual=attn)
+        else:
+            q, s, h = ops.layer_norm_q8(x, self.gamma, self.beta, residual=attn)
+        f = ops.linear_q8(q, s, self.q1, self.s1, bias=self.b1p, act=ops.ACT_GEGLU)
+        q, s = ops.quantize_rows(f)
+        return ops.linear_q8(q, s, self.q2, self.s2, bias=self.b2g, residual=h, out=h)
+
+    def exact(self, x, attn, rms=False):
+        """The unquantised layer in float64."""
+        h = x.double() + attn.double()
+        g = self.gamma.cpu().double()
+        n = Q.rms_norm(h, g, 1e-6) if rms else Q.layer_norm(h, g, self.beta.cpu().double(), 1e-5)
+        z = n @ self.w1.double().t() + self.b1.double()
+        v, t = z.chunk(2, 1)
+        return h, (v * (t * torch.special.ndtr(t))) @ self.w2.double().t() + self.b2.double()
+
+
+@pytest.mark.parametrize("rms", [False, True])
+@pytest.mark.parametrize("M", [1, 2, 33, 154, 1024])
+def test_feed_forward_in_8_bits(gpu, M, rms):
+    """Against the unquantised layer.  A rounding to 8 bits is off by a / 254 at
+    most and a / 254 / sqrt(3) in the root mean square; with a about 4 times a
+    row's root mean square, that is 0.9% of it.  Four such sources (two
+    activations, two weights) add up to 2%; the gate's slope and the product of
+    two of them leave it below 4%."""
+    announce(f"feed-forward block M={M} rms={rms}")
+    C, F = 640, 2560
+    blk = Block(C, F, 100)
+    x, a = cpu((M, C), 1), cpu((M, C), 2)
+    h, ff = blk.exact(x, a, rms)
+    y = blk(x.cuda(), a.cuda(), rms)
+    got = y.cpu().double() - h
+    assert float((got - ff).norm() / ff.norm()) <= 0.04
+
+
+def test_feed_forward_on_other_streams_and_in_graphs(gpu):
+    """Eager on the default stream = eager on another = captured and replayed,
+    two graphs replayed at the same time on two streams included."""
+    announce("feed-forward block: streams and graphs")
+    blk = Block(320, 1280, 50)
+    xs = [cpu((M, 320), M).cuda() for M in (1, 48, 600)]
+    at = [cpu((M, 320), M + 1).cuda() for M in (1, 48, 600)]
+    ref = [blk(x, a) for x, a in zip(xs, at)]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = [blk(x, a) for x, a in zip(xs, at)]
+    side.synchronize()
+    for r, g in zip(ref, got):
+        assert torch.equal(r, g)
+    graphs = []
+    for x, a in zip(xs, at):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = blk(x, a)
+        graphs.append((g, y))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for i in range(4):
+        for (g, y), s in zip(graphs, streams):
+            y.zero_()
+        torch.cuda.synchronize()
+        for (g, y), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        junk = torch.randn(256, 256, device="cuda") @ torch.randn(256, 256, device="cuda")
+        torch.cuda.synchronize()
+        for (g, y), r in zip(graphs, ref):
+            assert torch.equal(y, r), f"replay {i}"
+        del junk
+    xs[1].copy_(cpu((48, 320), 999).cuda())  # new values in the captured inputs
+    torch.cuda.synchronize()
+    graphs[1][0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(graphs[1][1], blk(xs[1], at[1]))
+
+
+# --------------------------------------------------------------- refusals ---
+def test_refusals(gpu):
+    announce("refusals (no kernel is launched)")
+    x = cpu((4, 64), 1).cuda()
+    q, s = ops.quantize_rows(x)
+    w, sw = ops.quantize_rows(cpu((32, 64), 2).cuda())
+    g = torch.ones(64, dtype=torch.float16, device="cuda")
+    no = lambda f, *a, **k: pytest.raises((ValueError, RuntimeError), f, *a, **k)  # noqa: E731
+    no(ops.quantize_rows, x.cpu())
+    no(ops.quantize_rows, x[0])
+    no(ops.quantize_rows, x.t())
+    no(ops.quantize_rows, x.to(torch.bfloat16))
+    no(ops.quantize_rows, x[:1].expand(4, 64))
+    no(ops.quantize_rows, x[:, :0])
+    no(ops.quantize_rows, x, out=torch.empty(4, 63, dtype=torch.int8, device="cuda"))
+    no(ops.quantize_rows, x, scale=torch.empty(3, device="cuda"))
+    no(ops.quantize_rows, x, out=x.view(torch.int8)[:, :64])  # over its own input
+    no(ops.dequantize_rows, q, s, dtype=torch.bfloat16)
+    no(ops.dequantize_rows, q, s[:3])
+    no(ops.rms_norm_q8, x, g[:63])
+    no(ops.rms_norm_q8, x, g.float())
+    no(ops.rms_norm_q8, x, g, sum_out=x)
+    no(ops.rms_norm_q8, x, g, residual=x.float())
+    no(ops.rms_norm_q8, x, g, eps=-1.0)
+    no(ops.rms_norm_q8, x, g, eps=float("nan"))
+    wide = torch.zeros(5, 64, dtype=torch.float16, device="cuda")
+    no(ops.rms_norm_q8, wide[:4], g, residual=x, sum_out=wide[1:])  # rows shifted by one
+    no(ops.layer_norm_q8, x, g, g[:60])
+    no(ops.linear_q8, q, s, w[:, :63], sw)
+    no(ops.linear_q8, q, s[:3], w, sw)
+    no(ops.linear_q8, q, s, w, sw.half())
+    no(ops.linear_q8, q, s, w, sw, act=7)
+    no(ops.linear_q8, q, s, w[:24], sw[:24], act=ops.ACT_GEGLU)
+    no(ops.linear_q8, q, s, w, sw, dtype=torch.bfloat16)
+    no(ops.linear_q8, q, s, w, sw, bias=torch.zeros(31, dtype=torch.float16, device="cuda"))
+    no(ops.linear_q8, q, s, w, sw, residual=torch.zeros(4, 32, device="cuda"))  # fp32 with an fp16 output
+    no(ops.linear_q8, q, s, w, sw, out=q.view(torch.float16)[:, :32])  # over an input
+    ragged = torch.zeros(4 * 50, dtype=torch.int8, device="cuda").view(4, 50)
+    no(ops.linear_q8, ragged, s, torch.zeros(8, 64, dtype=torch.int8, device="cuda")[:, :50], sw[:8])
+    tight = torch.zeros(3 * 64 + 50, dtype=torch.int8, device="cuda").as_strided((4, 50), (64, 1))
+    no(ops.linear_q8, tight, s, torch.zeros(8, 64, dtype=torch.int8, device="cuda")[:, :50], sw[:8])
+    # no rows: empty results
+    assert ops.linear_q8(q[:0], s[:0], w, sw).shape == (0, 32)
+    assert ops.rms_norm_q8(x[:0], g)[0].shape == (0, 64)
