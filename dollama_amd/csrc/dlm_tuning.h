@@ -46,6 +46,9 @@ int dlm_gemm_force_split(int splits);
  * as on a full device). */
 int dlm_gemm_set_variant(int variant);
 
+/* The same for the 8-bit linears (dlm_linear_q8_*), 0 = automatic. */
+int dlm_q8_force_tile(int tile_id);
+
 /* Counter calibration: `blocks` workgroups of 4 waves, each wave `iters`
  * rounds of eight v_mfma_f32_32x32x16_f16 on register operands (no memory
  * traffic in the loop): blocks * 4 * iters * 8 * 32768 FLOP per launch,
