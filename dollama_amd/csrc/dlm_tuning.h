@@ -46,7 +46,10 @@ int dlm_gemm_force_split(int splits);
  * as on a full device). */
 int dlm_gemm_set_variant(int variant);
 
-/* The same for the 8-bit linears (dlm_linear_q8_*), 0 = automatic. */
+/* The same for the 8-bit linears (dlm_linear_q8_*), 0 = automatic: 1-2 the row
+ * kernel with 16 and 8 waves, 3-11 output tiles of 32x32, 64x32, 64x64, 64x128,
+ * 128x128 (four stages), 128x96, 128x128 (two), 192x128, 128x256 (ping-pong).
+ * Outputs narrower than 16 columns stay with the row kernel. */
 int dlm_q8_force_tile(int tile_id);
 
 /* Counter calibration: `blocks` workgroups of 4 waves, each wave `iters`

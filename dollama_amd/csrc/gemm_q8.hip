@@ -55,100 +55,81 @@ __device__ __forceinline__ float act_f(float v, int act) {
   return v;
 }
 
-// Output row `row`, columns col .. col + 3 of the sums in a.
-template <class T>
-__device__ __forceinline__ void epi4(const i32x4& a, int row, int col, const Q8Gemm& p) {
-  if (row >= p.M) return;
-  const float sx = p.sx[row];
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int c = col + t;
-    if (c >= p.N) continue;
-    float v = (float)a[t] * p.sw[c] * sx;
-    if (p.bias) v += (float)p.bias[c];
-    v = act_f(v, p.act);
-    if (p.res) v = __builtin_fmaf(p.beta, (float)((const T*)p.res)[(size_t)row * p.ldr + c], v);
-    ((T*)p.y)[(size_t)row * p.ldy + c] = (T)v;
-  }
-}
+// Every kernel forms an output by the same operations in the same order, so that
+// it does not depend on the kernel that the shape selects:
+//   v = fma(float(sum) * sw, sx, bias), act(v), fma(beta, R, .), round to T
 
-// GEGLU: packed columns 8q + [0, 4) are values, 8q + 4 + [0, 4) their gates,
-// so values and gates lie in lanes 16 apart; each of the two finishes two
-// outputs.  N is a multiple of 16.
-template <class T>
-__device__ __forceinline__ void epi4_geglu(const i32x4& a, int row, int col, const Q8Gemm& p) {
-  const auto s02 = __builtin_amdgcn_permlane16_swap((unsigned)a[0], (unsigned)a[2], false, false);
-  const auto s13 = __builtin_amdgcn_permlane16_swap((unsigned)a[1], (unsigned)a[3], false, false);
-  if (row >= p.M || col >= p.N) return;
-  const float sx = p.sx[row];
-  const int vc = col & ~4, t0 = (col & 4) ? 2 : 0;
-  const int sv[2] = {(int)s02[0], (int)s13[0]}, sg[2] = {(int)s02[1], (int)s13[1]};
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    float v = (float)sv[t] * p.sw[vc + t0 + t] * sx, g = (float)sg[t] * p.sw[vc + 4 + t0 + t] * sx;
-    if (p.bias) {
-      v += (float)p.bias[vc + t0 + t];
-      g += (float)p.bias[vc + 4 + t0 + t];
-    }
-    v *= gelu_erf_fast(g);
-    const size_t o = (vc >> 1) + t0 + t;
-    if (p.res) v = __builtin_fmaf(p.beta, (float)((const T*)p.res)[(size_t)row * p.ldr + o], v);
-    ((T*)p.y)[(size_t)row * p.ldy + o] = (T)v;
-  }
-}
-
-// 16 columns and 16 TM rows a workgroup, K dealt to its NW waves in groups
-// of 128 bytes, G groups of a wave in flight at a time; operands go from
-// memory to the MFMA's registers, and the waves' sums meet in LDS.
-template <class T, int TM, int NW, int G>
+// 16 columns and 16 rows a workgroup, for few rows: K is dealt to its NW waves
+// in groups of 128 bytes, G groups of a wave in flight at a time.  Operands go
+// from memory to the MFMA's registers, and the waves' sums meet in LDS.  What
+// the first wave needs to finish them is requested ahead of the operands.
+template <class T, int NW, int G>
 __global__ void __launch_bounds__(NW * 64) q8_rows_kernel(Q8Gemm p) {
   constexpr int U = 2 * G;
-  __shared__ i32x4 red[NW][TM][64];
+  __shared__ i32x4 red[NW][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * TM;
   const int l15 = lane & 15, kl = 16 * (lane >> 4);
+  const int row = blockIdx.y * 16 + l15, col = blockIdx.x * 16 + 4 * (lane >> 4);
+  const int xrow = min(row, p.M - 1);
+  const bool geglu = p.act == DLM_ACT_GEGLU;
+  // GEGLU: packed columns 8q + [0, 4) are values, 8q + 4 + [0, 4) their gates,
+  // in lanes 16 apart; each of the two finishes two outputs
+  const int cols = geglu ? p.N >> 1 : p.N, w = geglu ? 2 : 4;
+  const int ocol = geglu ? (col >> 3) * 4 + (col & 4 ? 2 : 0) : col;
+  float sw[4], bias[4];
+  T res[4] = {};
+  const float sx = p.sx[xrow];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int c = min(col + t, p.N - 1);
+    sw[t] = p.sw[c];
+    bias[t] = p.bias ? (float)p.bias[c] : 0.0f;
+    if (p.res) res[t] = ((const T*)p.res)[(size_t)xrow * p.ldr + min(ocol + t, cols - 1)];
+  }
   const int klast = (p.K - 1) & ~15;
-  const int8_t* wp = p.w + (size_t)min(n0 + l15, p.N - 1) * p.ldw;
-  const int8_t* xp[TM];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) xp[i] = p.x + (size_t)min(m0 + 16 * i + l15, p.M - 1) * p.ldx;
-  i32x4 acc[TM];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) acc[i] = i32x4{0, 0, 0, 0};
+  const int8_t* wp = p.w + (size_t)min((int)blockIdx.x * 16 + l15, p.N - 1) * p.ldw;
+  const int8_t* xp = p.x + (size_t)xrow * p.ldx;
+  i32x4 acc{0, 0, 0, 0};
   const int steps = (p.K + 63) >> 6;
   auto step = [&](int s0, int u) { return s0 + (u >> 1) * 2 * NW + (u & 1); };
   for (int s0 = 2 * wave; s0 < steps; s0 += U * NW) {
-    i32x4 fw[U], fx[U][TM];
+    i32x4 fw[U], fx[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int k = min(64 * step(s0, u) + kl, klast);
       fw[u] = *reinterpret_cast<const i32x4*>(wp + k);
-#pragma unroll
-      for (int i = 0; i < TM; ++i) fx[u][i] = *reinterpret_cast<const i32x4*>(xp[i] + k);
+      fx[u] = *reinterpret_cast<const i32x4*>(xp + k);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int s = step(s0, u);
-      if (64 * s + 64 > p.K) {  // uniform: past the end of K, or across it
-#pragma unroll
-        for (int i = 0; i < TM; ++i) fx[u][i] = keep_bytes(fx[u][i], p.K - 64 * s - kl);
-      }
-#pragma unroll
-      for (int i = 0; i < TM; ++i) acc[i] = mfma16x16x64(fw[u], fx[u][i], acc[i]);
+      if (64 * s + 64 > p.K)  // uniform: past the end of K, or across it
+        fx[u] = keep_bytes(fx[u], p.K - 64 * s - kl);
+      acc = mfma16x16x64(fw[u], fx[u], acc);
     }
   }
-#pragma unroll
-  for (int i = 0; i < TM; ++i) red[wave][i][lane] = acc[i];
+  red[wave][lane] = acc;
   __syncthreads();
-  if (wave >= TM) return;
-  i32x4 a = red[0][wave][lane];
+  if (wave > 0) return;
 #pragma unroll
-  for (int w = 1; w < NW; ++w) a += red[w][wave][lane];
-  const int row = m0 + 16 * wave + l15, col = n0 + 4 * (lane >> 4);
-  if (p.act == DLM_ACT_GEGLU)
-    epi4_geglu<T>(a, row, col, p);
-  else
-    epi4<T>(a, row, col, p);
+  for (int i = 1; i < NW; ++i) acc += red[i][lane];
+  float v[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) v[t] = __builtin_fmaf((float)acc[t] * sw[t], sx, bias[t]);
+  if (geglu) {
+    const auto s02 = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[0]), __float_as_uint(v[2]), false, false);
+    const auto s13 = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[1]), __float_as_uint(v[3]), false, false);
+    v[0] = __uint_as_float(s02[0]) * gelu_erf_fast(__uint_as_float(s02[1]));
+    v[1] = __uint_as_float(s13[0]) * gelu_erf_fast(__uint_as_float(s13[1]));
+  } else {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) v[t] = act_f(v[t], p.act);
+  }
+  if (row >= p.M) return;
+  T* y = (T*)p.y + (size_t)row * p.ldy + ocol;
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+    if (t < w && ocol + t < cols) y[t] = (T)__builtin_fmaf(p.beta, (float)res[t], v[t]);
 }
 
 // ---------------------------------------------------------------------------
@@ -203,103 +184,152 @@ __device__ __forceinline__ typename Vec4<T>::type load4(const T* p) {
   return v;
 }
 
-// A wave's TM x TN blocks: lane holds row row0 + 16 i and columns col0 + 16 j
-// + [0, 4) of block (i, j).  Loads go to addresses clamped into the tensors
-// and are issued together; the last column group of an N that is no multiple
-// of four goes value by value.  N >= 16.
-template <class T, int TM, int TN>
-__device__ __forceinline__ void epi_tile(const i32x4 (&acc)[TM][TN], int row0, int col0, const Q8Gemm& p) {
-  f32x4 cs[TN];
-  f16x4 cb[TN];
-  float sx[TM];
+// Epilogue of a wave's TM x TN blocks at (m0, n0).  The blocks hold four columns
+// of a row a lane; stored from there, an instruction covers 32 bytes of each of
+// 16 rows, and the stores take longer than everything else (8192x1920x640:
+// QQ -> QQ us).  So the scaled sums go through the wave's part of the (now
+// free) operand ring, CI blocks' rows at a time, and are finished and stored
+// row by row, 16 bytes a lane.
+// v * sw * sx + bias is formed on the way in; activation, residual and the one
+// rounding to T on the way out.
+template <class T, int TM, int TN, int BYTES>
+__device__ __forceinline__ void epi_tile(const i32x4 (&acc)[TM][TN], float DLM_LDS* st, int m0, int n0, int lane,
+                                         const Q8Gemm& p) {
+  constexpr int WN = TN * 16, LD = WN + 4;  // rows 4 (2 WN + 1) banks apart: writes touch each bank once
+  constexpr int FIT = BYTES / (16 * LD * 4);
+  static_assert(FIT >= 1, "a block's rows do not fit");
+  constexpr int CI = TM % 4 == 0 && FIT >= 4 ? 4 : TM % 2 == 0 && FIT >= 2 ? 2 : 1;
+  constexpr int V = 16 / sizeof(T), VR = WN / V, N_IT = (16 * CI * VR + 63) / 64;
+  typedef T VecT __attribute__((ext_vector_type(V)));
+  const int l15 = lane & 15, c4 = 4 * (lane >> 4);
+  f32x4 cs[TN], cb[TN];
 #pragma unroll
-  for (int j = 0; j < TN; ++j) cs[j] = load4(p.sw + min(col0 + 16 * j, p.N - 4));
-  if (p.bias) {
+  for (int j = 0; j < TN; ++j) {
+    const int c = min(n0 + 16 * j + c4, p.N - 4);
+    // a last group of fewer than four columns starts short of the end
+    const int d = n0 + 16 * j + c4 - c;
+    cs[j] = load4(p.sw + c);
+    f16x4 h = {};
+    if (p.bias) h = load4(p.bias + c);
 #pragma unroll
-    for (int j = 0; j < TN; ++j) cb[j] = load4(p.bias + min(col0 + 16 * j, p.N - 4));
-  }
-#pragma unroll
-  for (int i = 0; i < TM; ++i) sx[i] = p.sx[min(row0 + 16 * i, p.M - 1)];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int row = row0 + 16 * i, r = min(row, p.M - 1);
-    typename Vec4<T>::type rv[TN];
-    if (p.res) {
-      const T* res = (const T*)p.res + (size_t)r * p.ldr;
-#pragma unroll
-      for (int j = 0; j < TN; ++j) rv[j] = load4(res + min(col0 + 16 * j, p.N - 4));
-    }
-    T* y = (T*)p.y + (size_t)r * p.ldy;
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int col = col0 + 16 * j;
-      typename Vec4<T>::type o;
+    for (int t = 0; t < 4; ++t) cb[j][t] = (float)h[t];
+    if (d > 0) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        float v = (float)acc[i][j][t] * cs[j][t] * sx[i];
-        if (p.bias) v += (float)cb[j][t];
-        v = act_f(v, p.act);
-        if (p.res) v = __builtin_fmaf(p.beta, (float)rv[j][t], v);
-        o[t] = (T)v;
-      }
-      if (row < p.M) {
-        if (col + 4 <= p.N)
-          __builtin_memcpy(y + col, &o, sizeof(o));
-        else
-          epi4<T>(acc[i][j], row, col, p);
+        cs[j][t] = p.sw[min(c + d + t, p.N - 1)];
+        cb[j][t] = p.bias ? (float)p.bias[min(c + d + t, p.N - 1)] : 0.0f;
       }
     }
+  }
+  float sx[TM];
+#pragma unroll
+  for (int i = 0; i < TM; ++i) sx[i] = p.sx[min(m0 + 16 * i + l15, p.M - 1)];
+  // stores the finished row vector: its columns col .. col + V - 1
+  auto put = [&](int row, int col, int cols, const VecT& o) {
+    if (row >= p.M || col >= cols) return;
+    T* y = (T*)p.y + (size_t)row * p.ldy + col;
+    if (col + V <= cols) {
+      __builtin_memcpy(y, &o, sizeof(o));
+    } else {
+#pragma unroll
+      for (int t = 0; t < V - 1; ++t)
+        if (col + t < cols) y[t] = o[t];
+    }
+  };
+  auto get_res = [&](int row, int col, int cols) {
+    VecT r = {};
+    const T* q = (const T*)p.res + (size_t)min(row, p.M - 1) * p.ldr;
+    if (col + V <= cols) {
+      __builtin_memcpy(&r, q + col, sizeof(r));
+    } else {
+#pragma unroll
+      for (int t = 0; t < V - 1; ++t)
+        if (col + t < cols) r[t] = q[col + t];
+    }
+    return r;
+  };
+#pragma unroll
+  for (int c = 0; c < TM / CI; ++c) {
+    const int r0 = m0 + 16 * CI * c;
+    VecT rv[N_IT];
+    if (p.res && p.act == DLM_ACT_NONE) {  // requested ahead of the exchange
+#pragma unroll
+      for (int it = 0; it < N_IT; ++it) {
+        const int idx = it * 64 + lane;
+        rv[it] = get_res(r0 + idx / VR, n0 + idx % VR * V, p.N);
+      }
+    }
+#pragma unroll
+    for (int ii = 0; ii < CI; ++ii)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const i32x4& a = acc[c * CI + ii][j];
+        f32x4 v;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) v[t] = __builtin_fmaf((float)a[t] * cs[j][t], sx[c * CI + ii], cb[j][t]);
+        *reinterpret_cast<f32x4 DLM_LDS*>(st + (ii * 16 + l15) * LD + j * 16 + c4) = v;
+      }
+    // the LDS takes a wave's accesses in order
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
+    if (p.act == DLM_ACT_NONE) {
+#pragma unroll
+      for (int it = 0; it < N_IT; ++it) {
+        const int idx = it * 64 + lane, r = idx / VR, col = idx % VR * V;
+        if ((16 * CI * VR) % 64 && idx >= 16 * CI * VR) break;
+        VecT o;
+#pragma unroll
+        for (int u = 0; u < V / 4; ++u) {
+          const f32x4 v = *reinterpret_cast<const f32x4 DLM_LDS*>(st + r * LD + col + 4 * u);
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            o[4 * u + t] = (T)(p.res ? __builtin_fmaf(p.beta, (float)rv[it][4 * u + t], v[t]) : v[t]);
+        }
+        put(r0 + r, n0 + col, p.N, o);
+      }
+    } else if (p.act == DLM_ACT_GEGLU) {
+      // output vector: V values and V gates, in groups of four of each
+      constexpr int VG = WN / (2 * V);
+#pragma unroll 1
+      for (int idx = lane; idx < 16 * CI * VG; idx += 64) {
+        const int r = idx / VG, col = idx % VG * V;
+        VecT o, rg = {};
+        if (p.res) rg = get_res(r0 + r, (n0 >> 1) + col, p.N >> 1);
+#pragma unroll
+        for (int u = 0; u < V / 4; ++u) {
+          const float DLM_LDS* q = st + r * LD + 2 * col + 8 * u;
+          const f32x4 v = *reinterpret_cast<const f32x4 DLM_LDS*>(q);
+          const f32x4 g = *reinterpret_cast<const f32x4 DLM_LDS*>(q + 4);
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            o[4 * u + t] = (T)__builtin_fmaf(p.beta, (float)rg[4 * u + t], v[t] * gelu_erf_fast(g[t]));
+        }
+        put(r0 + r, (n0 >> 1) + col, p.N >> 1, o);
+      }
+    } else {
+#pragma unroll 1
+      for (int idx = lane; idx < 16 * CI * VR; idx += 64) {
+        const int r = idx / VR, col = idx % VR * V;
+        VecT o, rg = {};
+        if (p.res) rg = get_res(r0 + r, n0 + col, p.N);
+#pragma unroll
+        for (int u = 0; u < V / 4; ++u) {
+          const f32x4 v = *reinterpret_cast<const f32x4 DLM_LDS*>(st + r * LD + col + 4 * u);
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            o[4 * u + t] = (T)__builtin_fmaf(p.beta, (float)rg[4 * u + t], act_f(v[t], p.act));
+        }
+        put(r0 + r, n0 + col, p.N, o);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+    asm volatile("" ::: "memory");
   }
 }
 
-template <class T, int TM, int TN>
-__device__ __forceinline__ void epi_tile_geglu(const i32x4 (&acc)[TM][TN], int row0, int col0, const Q8Gemm& p) {
-  const int t0 = (col0 & 4) ? 2 : 0;
-  float sv[TN][2], sg[TN][2], bv[TN][2], bg[TN][2], sx[TM];
-#pragma unroll
-  for (int j = 0; j < TN; ++j) {
-    const int vc = min((col0 + 16 * j) & ~4, p.N - 8) + t0;
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      sv[j][t] = p.sw[vc + t];
-      sg[j][t] = p.sw[vc + 4 + t];
-      bv[j][t] = p.bias ? (float)p.bias[vc + t] : 0.0f;
-      bg[j][t] = p.bias ? (float)p.bias[vc + 4 + t] : 0.0f;
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < TM; ++i) sx[i] = p.sx[min(row0 + 16 * i, p.M - 1)];
-#pragma unroll
-  for (int i = 0; i < TM; ++i) {
-    const int row = row0 + 16 * i, r = min(row, p.M - 1);
-    float rv[TN][2];
-    if (p.res) {
-#pragma unroll
-      for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          rv[j][t] = (float)((const T*)p.res)[(size_t)r * p.ldr + (min((col0 + 16 * j) & ~4, p.N - 8) >> 1) + t0 + t];
-    }
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const i32x4& a = acc[i][j];
-      const auto s02 = __builtin_amdgcn_permlane16_swap((unsigned)a[0], (unsigned)a[2], false, false);
-      const auto s13 = __builtin_amdgcn_permlane16_swap((unsigned)a[1], (unsigned)a[3], false, false);
-      const int vc = (col0 + 16 * j) & ~4;
-      const int v2[2] = {(int)s02[0], (int)s13[0]}, g2[2] = {(int)s02[1], (int)s13[1]};
-      T o[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        float v = (float)v2[t] * sv[j][t] * sx[i] + bv[j][t];
-        const float g = (float)g2[t] * sg[j][t] * sx[i] + bg[j][t];
-        v *= gelu_erf_fast(g);
-        if (p.res) v = __builtin_fmaf(p.beta, rv[j][t], v);
-        o[t] = (T)v;
-      }
-      if (row < p.M && vc < p.N) __builtin_memcpy((T*)p.y + (size_t)row * p.ldy + (vc >> 1) + t0, o, sizeof(o));
-    }
-  }
-}
+// Waves a SIMD is to hold: those of as many workgroups as the LDS takes, two at
+// most counted.
+constexpr int waves_per_simd(int lds, int waves) { return (lds <= 80 * 1024 ? 2 : 1) * waves / 4; }
 
 // K advances in slices of 128 bytes, copied by DMA into a ring of NS stages
 // (LDS rows of 128 bytes, 16-byte chunks XOR-swizzled by (row >> 1) & 7: a
@@ -317,7 +347,8 @@ __device__ __forceinline__ void epi_tile_geglu(const i32x4 (&acc)[TM][TN], int r
 // The last 1 to 15 values of a K that is no multiple of 16 follow the loop:
 // one MFMA a block on fragments from memory, with what lies past K zeroed.
 template <class T, int BM, int BN, int WM, int WN, int NS, int SCH>
-__global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64) q8_tile_kernel(Q8Gemm p, int tiles_m, int tiles_n) {
+__global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64, waves_per_simd(NS* (BM + BN) * kSlice, (BM / WM) * (BN / WN)))
+q8_tile_kernel(Q8Gemm p, int tiles_m, int tiles_n) {
   constexpr int WAVES_N = BN / WN, NW = (BM / WM) * WAVES_N;
   constexpr int TM = WM / 16, TN = WN / 16;
   constexpr int KS = kSlice / 64;
@@ -485,12 +516,9 @@ __global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64) q8_tile_kernel(Q8G
     mma(fa, fb);
   }
 
-  // ------------------------------ epilogue ------------------------------
-  const int row0 = m0 + wm * WM + l15, col0 = n0 + wn * WN + 4 * (lane >> 4);
-  if (p.act == DLM_ACT_GEGLU)
-    epi_tile_geglu<T>(acc, row0, col0, p);
-  else
-    epi_tile<T>(acc, row0, col0, p);
+  __syncthreads();  // every wave is done with the ring
+  constexpr int PART = NS * STAGE / NW & ~15;
+  epi_tile<T, TM, TN, PART>(acc, (float DLM_LDS*)(smem + wave * PART), m0 + wm * WM, n0 + wn * WN, lane, p);
 }
 
 template <class T, int BM, int BN, int WM, int WN, int NS, int SCH>
@@ -505,68 +533,92 @@ void launch_tile(const Q8Gemm& p, hipStream_t s) {
          tn);
 }
 
-template <class T, int TM, int NW = 8, int G = 2>
+template <class T, int NW, int G>
 void launch_rows(const Q8Gemm& p, hipStream_t s) {
   static const std::string name = std::string("q8_rows_kernel<") + (sizeof(T) == 2 ? "_Float16" : "float") + ", " +
-                                  std::to_string(TM) + ", " + std::to_string(NW) + ", " + std::to_string(G) + ">";
+                                  std::to_string(NW) + ", " + std::to_string(G) + ">";
   note_kernel(name.c_str());
   note_dims(p.M, p.N, p.K, (p.res ? 1 : 0) | (p.act << 4));
-  launch((q8_rows_kernel<T, TM, NW, G>), dim3((p.N + 15) / 16, (p.M + 16 * TM - 1) / (16 * TM)), dim3(NW * 64), 0, s, p);
+  launch((q8_rows_kernel<T, NW, G>), dim3((p.N + 15) / 16, (p.M + 15) / 16), dim3(NW * 64), 0, s, p);
 }
 
+// Tile override of dlm_q8_force_tile (0 = the plan below).
 thread_local int g_q8_tile = 0;
+
+// A launch's time is modelled as
+//   base + (fix + slices * slice) * (1 + more * (ceil(grid / 256) - 1))   [us]
+// grid: output tiles, slices: 128-byte slices of K, more: what each further
+// workgroup on a CU adds, relative to the first (over 1 where it has to queue
+// for the LDS).  The constants are fits to the launches of 479 shapes (1-8192
+// rows, 16-12000 columns, K = 64-8192), graph-replayed; the modelled choice
+// takes 0.7% longer than the fastest of the eleven in the mean and 19% at
+// worst (1024 columns x 21 rows, 4.8 us against 4.05).
+struct Q8Tile {
+  int bm, bn;
+  float base, fix, slice, more;
+};
+constexpr int kRowTiles = 2;  // the first two are q8_rows_kernel's
+constexpr Q8Tile kQ8Tiles[] = {
+    {16, 16, 2.61f, 0.25f, 0.064f, 1.18f},    // 1: 16 waves, one group in flight
+    {16, 16, 2.90f, 0.13f, 0.074f, 1.27f},    // 2: 8 waves, two groups
+    {32, 32, 2.30f, 0.63f, 0.147f, 0.67f},    // 3
+    {64, 32, 2.56f, 0.67f, 0.164f, 0.97f},    // 4
+    {64, 64, 2.49f, 1.27f, 0.205f, 1.08f},    // 5
+    {64, 128, 1.73f, 2.24f, 0.298f, 1.30f},   // 6
+    {128, 128, 1.62f, 3.37f, 0.460f, 1.22f},  // 7: one workgroup a CU, four stages
+    {128, 96, 1.50f, 3.44f, 0.422f, 1.10f},   // 8
+    {128, 128, 1.50f, 2.90f, 0.745f, 0.70f},  // 9: two workgroups a CU, two stages
+    {192, 128, 1.50f, 4.23f, 0.904f, 0.70f},  // 10: the same
+    {128, 256, 1.93f, 5.41f, 0.691f, 1.29f},  // 11: ping-pong
+};
+constexpr int kQ8TileCount = sizeof(kQ8Tiles) / sizeof(kQ8Tiles[0]);
+
+// Rows too far apart for a tile's 32-bit offsets, and outputs narrower than
+// one MFMA block, which the tiles' epilogue does not take.
+bool only_rows(const Q8Gemm& p) { return p.N < 16 || std::max(p.ldx, p.ldw) > (1 << 22); }
+
+// The row kernels read W once for every 16 rows: up to 64 where there is a choice.
+int plan_q8(const Q8Gemm& p) {
+  const bool rows = only_rows(p);
+  const int slices = (p.K + 127) / 128;
+  int best = 1;
+  float best_us = 3e38f;
+  for (int i = 0; i < (rows ? kRowTiles : kQ8TileCount); ++i) {
+    if (i < kRowTiles && !rows && p.M > 64) continue;
+    const Q8Tile& t = kQ8Tiles[i];
+    const long long grid = (long long)((p.M + t.bm - 1) / t.bm) * ((p.N + t.bn - 1) / t.bn);
+    const float us =
+        t.base + (t.fix + (float)slices * t.slice) * (1.0f + t.more * (float)((grid + 255) / 256 - 1));
+    if (us < best_us) {
+      best_us = us;
+      best = i + 1;
+    }
+  }
+  return best;
+}
 
 template <class T>
 void q8_gemm(const Q8Gemm& p, hipStream_t s) {
-  switch (g_q8_tile) {
-    case 1: return launch_tile<T, 256, 160, 64, 80, 3, kPingPong>(p, s);
-    case 3: return launch_tile<T, 128, 160, 32, 80, 4, kPlain>(p, s);
-    case 4: return launch_tile<T, 128, 128, 64, 32, 4, kPlain>(p, s);
-    case 5: return launch_tile<T, 128, 64, 64, 32, 4, kPlain>(p, s);
-    case 6: return launch_tile<T, 128, 80, 16, 80, 4, kPlain>(p, s);
-    case 7: return launch_tile<T, 64, 64, 32, 32, 4, kPlain>(p, s);
-    case 8: return launch_tile<T, 64, 32, 16, 32, 4, kPlain>(p, s);
-    case 10: return launch_tile<T, 256, 128, 64, 64, 3, kPingPong>(p, s);
-    case 12: return launch_tile<T, 128, 128, 32, 64, 2, kPlain>(p, s);
-    case 13: return launch_rows<T, 1>(p, s);
-    case 14: return launch_rows<T, 2>(p, s);
-    case 15: return launch_rows<T, 4>(p, s);
-    case 16: return launch_tile<T, 64, 128, 32, 32, 4, kPlain>(p, s);
-    case 17: return launch_tile<T, 32, 64, 16, 16, 4, kPlain>(p, s);
-    case 18: return launch_tile<T, 64, 16, 16, 16, 4, kPlain>(p, s);
-    case 19: return launch_tile<T, 128, 256, 64, 64, 3, kPingPong>(p, s);
-    case 20: return launch_tile<T, 128, 160, 64, 80, 2, kPlain>(p, s);
-    case 21: return launch_tile<T, 128, 128, 64, 64, 2, kPlain>(p, s);
-    case 22: return launch_tile<T, 128, 80, 32, 80, 3, kPlain>(p, s);
-    case 23: return launch_tile<T, 64, 160, 32, 80, 2, kPlain>(p, s);
-    case 24: return launch_tile<T, 32, 32, 16, 16, 4, kPlain>(p, s);
-    case 25: return launch_tile<T, 64, 32, 32, 16, 6, kPlain>(p, s);
-    case 26: return launch_tile<T, 64, 64, 32, 32, 8, kPlain>(p, s);
-    case 27: return launch_tile<T, 64, 64, 32, 16, 8, kPlain>(p, s);
-    case 28: return launch_tile<T, 64, 32, 16, 32, 8, kPlain>(p, s);
-    case 30: return launch_rows<T, 1, 8, 4>(p, s);
-    case 31: return launch_rows<T, 1, 16, 2>(p, s);
-    case 32: return launch_rows<T, 1, 16, 1>(p, s);
-    case 33: return launch_rows<T, 2, 8, 4>(p, s);
-    case 34: return launch_rows<T, 2, 16, 2>(p, s);
-    case 35: return launch_rows<T, 4, 16, 2>(p, s);
-    case 36: return launch_rows<T, 4, 8, 1>(p, s);
-    case 37: return launch_rows<T, 1, 4, 4>(p, s);
-    case 38: return launch_rows<T, 4, 16, 1>(p, s);
-    default: break;
+  const bool as_planned = g_q8_tile <= 0 || (g_q8_tile > kRowTiles && only_rows(p));
+  switch (as_planned ? plan_q8(p) : g_q8_tile) {
+    case 1: return launch_rows<T, 16, 1>(p, s);
+    case 2: return launch_rows<T, 8, 2>(p, s);
+    case 3: return launch_tile<T, 32, 32, 16, 16, 4, kPlain>(p, s);
+    case 4: return launch_tile<T, 64, 32, 16, 32, 4, kPlain>(p, s);
+    case 5: return launch_tile<T, 64, 64, 32, 32, 4, kPlain>(p, s);
+    case 6: return launch_tile<T, 64, 128, 32, 32, 4, kPlain>(p, s);
+    case 7: return launch_tile<T, 128, 128, 64, 32, 4, kPlain>(p, s);
+    case 8: return launch_tile<T, 128, 96, 32, 48, 3, kPlain>(p, s);
+    case 9: return launch_tile<T, 128, 128, 64, 32, 2, kPlain>(p, s);
+    case 10: return launch_tile<T, 192, 128, 48, 64, 2, kPlain>(p, s);
+    default: return launch_tile<T, 128, 256, 64, 64, 3, kPingPong>(p, s);
   }
-  if (p.M <= 16)
-    launch_rows<T, 1>(p, s);
-  else if (p.M <= 32)
-    launch_rows<T, 2>(p, s);
-  else
-    launch_rows<T, 4>(p, s);
 }
 
 // Largest K: 128 * 128 * K stays below 2^31.
 constexpr int kMaxK = 131071;
-// Rows of one launch: the grid's y.
-constexpr int kMaxRows = 1 << 21;
+// Columns a row of workgroups takes: a launch counts threads in 32 bits.
+constexpr int kMaxN = 1 << 25;
 
 template <class T>
 int linear_q8(const char* fn, Q8Gemm p, hipStream_t s) {
@@ -574,6 +626,7 @@ int linear_q8(const char* fn, Q8Gemm p, hipStream_t s) {
   if (!p.x || !p.w || !p.sx || !p.sw || !p.y) return bad("NULL pointer");
   if (p.act < DLM_ACT_NONE || p.act > DLM_ACT_GELU) return bad("unknown activation");
   if (p.K > kMaxK) return bad("K over " + std::to_string(kMaxK) + " may overflow the 32-bit sums");
+  if (p.N > kMaxN) return bad("N over " + std::to_string(kMaxN));
   const int k16 = (p.K + 15) & ~15, cols = p.act == DLM_ACT_GEGLU ? p.N / 2 : p.N;
   if (p.act == DLM_ACT_GEGLU && p.N % 16) return bad("GEGLU needs N % 16 == 0");
   if (p.ldx % 16 || p.ldw % 16 || !dlm_aligned16(p.x) || !dlm_aligned16(p.w))
@@ -583,6 +636,7 @@ int linear_q8(const char* fn, Q8Gemm p, hipStream_t s) {
   if ((uintptr_t)p.y % sizeof(T) || (uintptr_t)p.res % sizeof(T) || (uintptr_t)p.bias % 2 || (uintptr_t)p.sx % 4 ||
       (uintptr_t)p.sw % 4)
     return bad("pointer not aligned to its element");
+  if (!p.res) p.beta = 0.0f;  // kernels that add beta times nothing stay clear of infinities
   const uintptr_t y0 = (uintptr_t)p.y, y1 = y0 + ((uintptr_t)(p.M - 1) * p.ldy + cols) * sizeof(T);
   struct {
     const char* name;
@@ -599,14 +653,17 @@ int linear_q8(const char* fn, Q8Gemm p, hipStream_t s) {
     if (i.p == p.res && p.res == p.y && p.ldr == p.ldy) continue;  // added in place
     return bad(std::string("Y overlaps ") + i.name);
   }
-  for (int left = p.M; left > 0; left -= kMaxRows) {
-    p.M = std::min(left, kMaxRows);
+  // rows of one launch: at most 2^28 outputs (2^26 threads of the smallest
+  // tile) and 2^19 rows (the grid's y)
+  const int part = std::max(1 << 8, std::min(1 << 19, (1 << 28) / p.N & ~255));
+  for (int left = p.M; left > 0; left -= part) {
+    p.M = std::min(left, part);
     q8_gemm<T>(p, s);
     DLM_LAUNCH_CHECK();
-    p.x += kMaxRows * p.ldx;
-    p.sx += kMaxRows;
-    p.y = (T*)p.y + kMaxRows * p.ldy;
-    if (p.res) p.res = (const T*)p.res + kMaxRows * p.ldr;
+    p.x += part * p.ldx;
+    p.sx += part;
+    p.y = (T*)p.y + part * p.ldy;
+    if (p.res) p.res = (const T*)p.res + part * p.ldr;
   }
   return DLM_OK;
 }

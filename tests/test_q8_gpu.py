@@ -300,6 +300,26 @@ def test_linear_q8_activations(gpu, M, N, K, act, dtype):
     check_linear(M, N, K, act=act, dtype=dtype, beta=-0.75, seed=5)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("tile", range(1, 12))
+def test_linear_q8_every_kernel(gpu, tile, dtype):
+    """Every kernel and tile the plan chooses among (dlm_q8_force_tile), on shapes
+    with ragged last tiles in both directions, K from less than a slice to more
+    than the ring, odd N, K tails of 1 to 15 values, and rows of padding."""
+    from dollama_amd import _lib
+    try:
+        _lib.call("dlm_q8_force_tile", tile)
+        for M, N, K in ((300, 340, 648), (70, 161, 1003), (200, 16, 5), (1, 35, 127), (129, 129, 128), (260, 272, 1297),
+                        (513, 78, 384), (16, 2, 640)):
+            check_linear(M, N, K, dtype=dtype)
+        check_linear(300, 340, 648, act="silu", dtype=dtype, residual=False, seed=21)
+        check_linear(257, 99, 200, act="gelu", dtype=dtype, beta=0.5, seed=23)
+        check_linear(300, 336, 648, act="geglu", dtype=dtype, residual=False, seed=25)
+        check_linear(131, 144, 333, act="geglu", dtype=dtype, beta=-2.0, seed=27)
+    finally:
+        _lib.call("dlm_q8_force_tile", 0)
+
+
 @pytest.mark.parametrize("M", [1, 20, 300])
 def test_linear_q8_sums_reach_the_ends_of_their_range(gpu, M):
     """K = 131071 products of -128 x -128 stay below 2^31; the sums are exact
