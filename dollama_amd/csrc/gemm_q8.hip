@@ -55,83 +55,6 @@ __device__ __forceinline__ float act_f(float v, int act) {
   return v;
 }
 
-// Every kernel forms an output by the same operations in the same order, so that
-// it does not depend on the kernel that the shape selects:
-//   v = fma(float(sum) * sw, sx, bias), act(v), fma(beta, R, .), round to T
-
-// 16 columns and 16 rows a workgroup, for few rows: K is dealt to its NW waves
-// in groups of 128 bytes, G groups of a wave in flight at a time.  Operands go
-// from memory to the MFMA's registers, and the waves' sums meet in LDS.  What
-// the first wave needs to finish them is requested ahead of the operands.
-template <class T, int NW, int G>
-__global__ void __launch_bounds__(NW * 64) q8_rows_kernel(Q8Gemm p) {
-  constexpr int U = 2 * G;
-  __shared__ i32x4 red[NW][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int l15 = lane & 15, kl = 16 * (lane >> 4);
-  const int row = blockIdx.y * 16 + l15, col = blockIdx.x * 16 + 4 * (lane >> 4);
-  const int xrow = min(row, p.M - 1);
-  const bool geglu = p.act == DLM_ACT_GEGLU;
-  // GEGLU: packed columns 8q + [0, 4) are values, 8q + 4 + [0, 4) their gates,
-  // in lanes 16 apart; each of the two finishes two outputs
-  const int cols = geglu ? p.N >> 1 : p.N, w = geglu ? 2 : 4;
-  const int ocol = geglu ? (col >> 3) * 4 + (col & 4 ? 2 : 0) : col;
-  float sw[4], bias[4];
-  T res[4] = {};
-  const float sx = p.sx[xrow];
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int c = min(col + t, p.N - 1);
-    sw[t] = p.sw[c];
-    bias[t] = p.bias ? (float)p.bias[c] : 0.0f;
-    if (p.res) res[t] = ((const T*)p.res)[(size_t)xrow * p.ldr + min(ocol + t, cols - 1)];
-  }
-  const int klast = (p.K - 1) & ~15;
-  const int8_t* wp = p.w + (size_t)min((int)blockIdx.x * 16 + l15, p.N - 1) * p.ldw;
-  const int8_t* xp = p.x + (size_t)xrow * p.ldx;
-  i32x4 acc{0, 0, 0, 0};
-  const int steps = (p.K + 63) >> 6;
-  auto step = [&](int s0, int u) { return s0 + (u >> 1) * 2 * NW + (u & 1); };
-  for (int s0 = 2 * wave; s0 < steps; s0 += U * NW) {
-    i32x4 fw[U], fx[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = min(64 * step(s0, u) + kl, klast);
-      fw[u] = *reinterpret_cast<const i32x4*>(wp + k);
-      fx[u] = *reinterpret_cast<const i32x4*>(xp + k);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int s = step(s0, u);
-      if (64 * s + 64 > p.K)  // uniform: past the end of K, or across it
-        fx[u] = keep_bytes(fx[u], p.K - 64 * s - kl);
-      acc = mfma16x16x64(fw[u], fx[u], acc);
-    }
-  }
-  red[wave][lane] = acc;
-  __syncthreads();
-  if (wave > 0) return;
-#pragma unroll
-  for (int i = 1; i < NW; ++i) acc += red[i][lane];
-  float v[4];
-#pragma unroll
-  for (int t = 0; t < 4; ++t) v[t] = __builtin_fmaf((float)acc[t] * sw[t], sx, bias[t]);
-  if (geglu) {
-    const auto s02 = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[0]), __float_as_uint(v[2]), false, false);
-    const auto s13 = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[1]), __float_as_uint(v[3]), false, false);
-    v[0] = __uint_as_float(s02[0]) * gelu_erf_fast(__uint_as_float(s02[1]));
-    v[1] = __uint_as_float(s13[0]) * gelu_erf_fast(__uint_as_float(s13[1]));
-  } else {
-#pragma unroll
-    for (int t = 0; t < 4; ++t) v[t] = act_f(v[t], p.act);
-  }
-  if (row >= p.M) return;
-  T* y = (T*)p.y + (size_t)row * p.ldy + ocol;
-#pragma unroll
-  for (int t = 0; t < 4; ++t)
-    if (t < w && ocol + t < cols) y[t] = (T)__builtin_fmaf(p.beta, (float)res[t], v[t]);
-}
-
 // ---------------------------------------------------------------------------
 // Output tiles of BM x BN, operands through LDS.
 // ---------------------------------------------------------------------------
@@ -192,40 +115,75 @@ __device__ __forceinline__ typename Vec4<T>::type load4(const T* p) {
 // row by row, 16 bytes a lane.
 // v * sw * sx + bias is formed on the way in; activation, residual and the one
 // rounding to T on the way out.
+// Small wave tiles request the scales, bias and residual ahead of the main loop
+// (request), the others once their accumulators are done with.
 template <class T, int TM, int TN, int BYTES>
-__device__ __forceinline__ void epi_tile(const i32x4 (&acc)[TM][TN], float DLM_LDS* st, int m0, int n0, int lane,
-                                         const Q8Gemm& p) {
-  constexpr int WN = TN * 16, LD = WN + 4;  // rows 4 (2 WN + 1) banks apart: writes touch each bank once
-  constexpr int FIT = BYTES / (16 * LD * 4);
+struct Epilogue {
+  static constexpr int WN = TN * 16, LD = WN + 4;  // rows 4 (2 WN + 1) banks apart: writes touch each bank once
+  static constexpr int FIT = BYTES / (16 * LD * 4);
   static_assert(FIT >= 1, "a block's rows do not fit");
-  constexpr int CI = TM % 4 == 0 && FIT >= 4 ? 4 : TM % 2 == 0 && FIT >= 2 ? 2 : 1;
-  constexpr int V = 16 / sizeof(T), VR = WN / V, N_IT = (16 * CI * VR + 63) / 64;
+  static constexpr int CI = TM % 4 == 0 && FIT >= 4 ? 4 : TM % 2 == 0 && FIT >= 2 ? 2 : 1;
+  static constexpr int V = 16 / sizeof(T), VR = WN / V, N_IT = (16 * CI * VR + 63) / 64;
+  static constexpr bool EARLY = TM * TN <= 8, EARLY_RES = TM * TN <= 4 && CI == TM;
   typedef T VecT __attribute__((ext_vector_type(V)));
-  const int l15 = lane & 15, c4 = 4 * (lane >> 4);
-  f32x4 cs[TN], cb[TN];
+  const Q8Gemm& p;
+  int m0, n0, lane;
+  f32x4 cs[TN];
+  f16x4 cb[TN];
+  float sx[TM];
+  VecT rv[N_IT];
+
+  __device__ Epilogue(const Q8Gemm& p_, int m0_, int n0_, int lane_) : p(p_), m0(m0_), n0(n0_), lane(lane_) {
+    if (EARLY) scales();
+    if (EARLY_RES) residual(0);
+  }
+  __device__ __forceinline__ void scales() {
 #pragma unroll
-  for (int j = 0; j < TN; ++j) {
-    const int c = min(n0 + 16 * j + c4, p.N - 4);
-    // a last group of fewer than four columns starts short of the end
-    const int d = n0 + 16 * j + c4 - c;
-    cs[j] = load4(p.sw + c);
-    f16x4 h = {};
-    if (p.bias) h = load4(p.bias + c);
+    for (int j = 0; j < TN; ++j) {
+      const int col = n0 + 16 * j + 4 * (lane >> 4);
+      const int c = p.N >= 4 ? min(col, p.N - 4) : 0;
+      cb[j] = f16x4{};
+      if (p.N >= 4) {
+        cs[j] = load4(p.sw + c);
+        if (p.bias) cb[j] = load4(p.bias + c);
+      }
+      if (col != c || p.N < 4) {  // fewer than four columns are left
 #pragma unroll
-    for (int t = 0; t < 4; ++t) cb[j][t] = (float)h[t];
-    if (d > 0) {
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        cs[j][t] = p.sw[min(c + d + t, p.N - 1)];
-        cb[j][t] = p.bias ? (float)p.bias[min(c + d + t, p.N - 1)] : 0.0f;
+        for (int t = 0; t < 4; ++t) {
+          cs[j][t] = p.sw[min(col + t, p.N - 1)];
+          if (p.bias) cb[j][t] = p.bias[min(col + t, p.N - 1)];
+        }
       }
     }
-  }
-  float sx[TM];
 #pragma unroll
-  for (int i = 0; i < TM; ++i) sx[i] = p.sx[min(m0 + 16 * i + l15, p.M - 1)];
-  // stores the finished row vector: its columns col .. col + V - 1
-  auto put = [&](int row, int col, int cols, const VecT& o) {
+    for (int i = 0; i < TM; ++i) sx[i] = p.sx[min(m0 + 16 * i + (lane & 15), p.M - 1)];
+  }
+  // Residual vector of columns col .. col + V - 1.  `whole`: the wave's columns
+  // all lie in N, so that no load stands in a branch of lanes (its result
+  // would be waited for there).
+  __device__ __forceinline__ VecT get_res(int row, int col, int cols, bool whole) const {
+    VecT r = {};
+    const T* q = (const T*)p.res + (size_t)min(row, p.M - 1) * p.ldr + col;
+    if (whole || col + V <= cols) {
+      __builtin_memcpy(&r, q, sizeof(r));
+    } else {
+#pragma unroll
+      for (int t = 0; t < V - 1; ++t)
+        if (col + t < cols) r[t] = q[t];
+    }
+    return r;
+  }
+  __device__ __forceinline__ void residual(int c) {
+    if (!p.res || p.act != DLM_ACT_NONE) return;
+    const bool whole = n0 + WN <= p.N;
+#pragma unroll
+    for (int it = 0; it < N_IT; ++it) {
+      const int idx = it * 64 + lane;
+      rv[it] = get_res(m0 + 16 * CI * c + idx / VR, n0 + idx % VR * V, p.N, whole);
+    }
+  }
+  // Stores a finished vector, columns col .. col + V - 1 of a row.
+  __device__ __forceinline__ void put(int row, int col, int cols, const VecT& o) const {
     if (row >= p.M || col >= cols) return;
     T* y = (T*)p.y + (size_t)row * p.ldy + col;
     if (col + V <= cols) {
@@ -235,97 +193,83 @@ __device__ __forceinline__ void epi_tile(const i32x4 (&acc)[TM][TN], float DLM_L
       for (int t = 0; t < V - 1; ++t)
         if (col + t < cols) y[t] = o[t];
     }
-  };
-  auto get_res = [&](int row, int col, int cols) {
-    VecT r = {};
-    const T* q = (const T*)p.res + (size_t)min(row, p.M - 1) * p.ldr;
-    if (col + V <= cols) {
-      __builtin_memcpy(&r, q + col, sizeof(r));
-    } else {
-#pragma unroll
-      for (int t = 0; t < V - 1; ++t)
-        if (col + t < cols) r[t] = q[col + t];
-    }
-    return r;
-  };
-#pragma unroll
-  for (int c = 0; c < TM / CI; ++c) {
-    const int r0 = m0 + 16 * CI * c;
-    VecT rv[N_IT];
-    if (p.res && p.act == DLM_ACT_NONE) {  // requested ahead of the exchange
-#pragma unroll
-      for (int it = 0; it < N_IT; ++it) {
-        const int idx = it * 64 + lane;
-        rv[it] = get_res(r0 + idx / VR, n0 + idx % VR * V, p.N);
-      }
-    }
-#pragma unroll
-    for (int ii = 0; ii < CI; ++ii)
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const i32x4& a = acc[c * CI + ii][j];
-        f32x4 v;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) v[t] = __builtin_fmaf((float)a[t] * cs[j][t], sx[c * CI + ii], cb[j][t]);
-        *reinterpret_cast<f32x4 DLM_LDS*>(st + (ii * 16 + l15) * LD + j * 16 + c4) = v;
-      }
-    // the LDS takes a wave's accesses in order
-    __builtin_amdgcn_wave_barrier();
-    asm volatile("" ::: "memory");
-    if (p.act == DLM_ACT_NONE) {
-#pragma unroll
-      for (int it = 0; it < N_IT; ++it) {
-        const int idx = it * 64 + lane, r = idx / VR, col = idx % VR * V;
-        if ((16 * CI * VR) % 64 && idx >= 16 * CI * VR) break;
-        VecT o;
-#pragma unroll
-        for (int u = 0; u < V / 4; ++u) {
-          const f32x4 v = *reinterpret_cast<const f32x4 DLM_LDS*>(st + r * LD + col + 4 * u);
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-            o[4 * u + t] = (T)(p.res ? __builtin_fmaf(p.beta, (float)rv[it][4 * u + t], v[t]) : v[t]);
-        }
-        put(r0 + r, n0 + col, p.N, o);
-      }
-    } else if (p.act == DLM_ACT_GEGLU) {
-      // output vector: V values and V gates, in groups of four of each
-      constexpr int VG = WN / (2 * V);
-#pragma unroll 1
-      for (int idx = lane; idx < 16 * CI * VG; idx += 64) {
-        const int r = idx / VG, col = idx % VG * V;
-        VecT o, rg = {};
-        if (p.res) rg = get_res(r0 + r, (n0 >> 1) + col, p.N >> 1);
-#pragma unroll
-        for (int u = 0; u < V / 4; ++u) {
-          const float DLM_LDS* q = st + r * LD + 2 * col + 8 * u;
-          const f32x4 v = *reinterpret_cast<const f32x4 DLM_LDS*>(q);
-          const f32x4 g = *reinterpret_cast<const f32x4 DLM_LDS*>(q + 4);
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-            o[4 * u + t] = (T)__builtin_fmaf(p.beta, (float)rg[4 * u + t], v[t] * gelu_erf_fast(g[t]));
-        }
-        put(r0 + r, (n0 >> 1) + col, p.N >> 1, o);
-      }
-    } else {
-#pragma unroll 1
-      for (int idx = lane; idx < 16 * CI * VR; idx += 64) {
-        const int r = idx / VR, col = idx % VR * V;
-        VecT o, rg = {};
-        if (p.res) rg = get_res(r0 + r, n0 + col, p.N);
-#pragma unroll
-        for (int u = 0; u < V / 4; ++u) {
-          const f32x4 v = *reinterpret_cast<const f32x4 DLM_LDS*>(st + r * LD + col + 4 * u);
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-            o[4 * u + t] = (T)__builtin_fmaf(p.beta, (float)rg[4 * u + t], act_f(v[t], p.act));
-        }
-        put(r0 + r, n0 + col, p.N, o);
-      }
-    }
-    __builtin_amdgcn_wave_barrier();
-    asm volatile("" ::: "memory");
   }
-}
+  __device__ __forceinline__ void finish(const i32x4 (&acc)[TM][TN], float DLM_LDS* st) {
+    const int l15 = lane & 15, c4 = 4 * (lane >> 4);
+    if (!EARLY) scales();
+#pragma unroll
+    for (int c = 0; c < TM / CI; ++c) {
+      const int r0 = m0 + 16 * CI * c;
+      if (!EARLY_RES) residual(c);
+#pragma unroll
+      for (int ii = 0; ii < CI; ++ii)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const i32x4& a = acc[c * CI + ii][j];
+          f32x4 v;
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            v[t] = __builtin_fmaf((float)a[t] * cs[j][t], sx[c * CI + ii], (float)cb[j][t]);
+          *reinterpret_cast<f32x4 DLM_LDS*>(st + (ii * 16 + l15) * LD + j * 16 + c4) = v;
+        }
+      // the LDS takes a wave's accesses in order
+      __builtin_amdgcn_wave_barrier();
+      asm volatile("" ::: "memory");
+      if (p.act == DLM_ACT_NONE) {
+#pragma unroll
+        for (int it = 0; it < N_IT; ++it) {
+          const int idx = it * 64 + lane, r = idx / VR, col = idx % VR * V;
+          if ((16 * CI * VR) % 64 && idx >= 16 * CI * VR) break;
+          VecT o;
+#pragma unroll
+          for (int u = 0; u < V / 4; ++u) {
+            const f32x4 v = *reinterpret_cast<const f32x4 DLM_LDS*>(st + r * LD + col + 4 * u);
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+              o[4 * u + t] = (T)(p.res ? __builtin_fmaf(p.beta, (float)rv[it][4 * u + t], v[t]) : v[t]);
+          }
+          put(r0 + r, n0 + col, p.N, o);
+        }
+      } else if (p.act == DLM_ACT_GEGLU) {
+        // V outputs from V values and V gates, which alternate in groups of four
+        constexpr int VG = (WN / 2 + V - 1) / V;
+#pragma unroll 1
+        for (int idx = lane; idx < 16 * CI * VG; idx += 64) {
+          const int r = idx / VG, col = idx % VG * V;
+          VecT o, rg = {};
+          if (p.res) rg = get_res(r0 + r, (n0 >> 1) + col, p.N >> 1, false);
+#pragma unroll
+          for (int u = 0; u < V / 4; ++u) {
+            const float DLM_LDS* q = st + r * LD + 2 * col + 8 * u;
+            const f32x4 v = *reinterpret_cast<const f32x4 DLM_LDS*>(q);
+            const f32x4 g = *reinterpret_cast<const f32x4 DLM_LDS*>(q + 4);
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+              o[4 * u + t] = (T)__builtin_fmaf(p.beta, (float)rg[4 * u + t], v[t] * gelu_erf_fast(g[t]));
+          }
+          put(r0 + r, (n0 >> 1) + col, p.N >> 1, o);
+        }
+      } else {
+#pragma unroll 1
+        for (int idx = lane; idx < 16 * CI * VR; idx += 64) {
+          const int r = idx / VR, col = idx % VR * V;
+          VecT o, rg = {};
+          if (p.res) rg = get_res(r0 + r, n0 + col, p.N, false);
+#pragma unroll
+          for (int u = 0; u < V / 4; ++u) {
+            const f32x4 v = *reinterpret_cast<const f32x4 DLM_LDS*>(st + r * LD + col + 4 * u);
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+              o[4 * u + t] = (T)__builtin_fmaf(p.beta, (float)rg[4 * u + t], act_f(v[t], p.act));
+          }
+          put(r0 + r, n0 + col, p.N, o);
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+      asm volatile("" ::: "memory");
+    }
+  }
+};
 
 // Waves a SIMD is to hold: those of as many workgroups as the LDS takes, two at
 // most counted.
@@ -344,24 +288,32 @@ constexpr int waves_per_simd(int lds, int waves) { return (lds <= 80 * 1024 ? 2 
 // reads of a stage (the late half's) before the phase that refills it; it
 // waits for its own part of the next slice a barrier before either half reads
 // that.
+// KG > 1 (few rows, where a grid of one workgroup a tile would leave most of
+// the chip waiting for one workgroup's slices): KG groups of waves take the
+// slices in turn, each with a ring of its own, and add their sums up in LDS.
 // The last 1 to 15 values of a K that is no multiple of 16 follow the loop:
 // one MFMA a block on fragments from memory, with what lies past K zeroed.
-template <class T, int BM, int BN, int WM, int WN, int NS, int SCH>
-__global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64, waves_per_simd(NS* (BM + BN) * kSlice, (BM / WM) * (BN / WN)))
+template <class T, int BM, int BN, int WM, int WN, int NS, int SCH, int KG>
+__global__ void __launch_bounds__((BM / WM) * (BN / WN) * KG * 64,
+                                  waves_per_simd(KG* NS* (BM + BN) * kSlice, (BM / WM) * (BN / WN) * KG))
 q8_tile_kernel(Q8Gemm p, int tiles_m, int tiles_n) {
-  constexpr int WAVES_N = BN / WN, NW = (BM / WM) * WAVES_N;
+  constexpr int WAVES_N = BN / WN, NW = (BM / WM) * WAVES_N;  // waves of a K group
   constexpr int TM = WM / 16, TN = WN / 16;
   constexpr int KS = kSlice / 64;
   constexpr int SA = BM * kSlice, STAGE = (BM + BN) * kSlice;
   constexpr int GA = BM / 8, GB = BN / 8;
   constexpr int IA = (GA + NW - 1) / NW, IB = (GB + NW - 1) / NW;
   static_assert(BM % 8 == 0 && BN % 8 == 0 && WM % 16 == 0 && WN % 16 == 0 && NW % 2 == 0 && NS >= 2, "tile");
-  static_assert(NS * STAGE <= 160 * 1024, "ring larger than the LDS");
-  __shared__ __attribute__((aligned(1024))) unsigned char smem_generic[NS * STAGE];
-  unsigned char DLM_LDS* smem = (unsigned char DLM_LDS*)smem_generic;
+  static_assert(KG == 1 || SCH == kPlain, "K groups use the plain loop");
+  static_assert(KG * NS * STAGE <= 160 * 1024, "ring larger than the LDS");
+  static_assert((KG - 1) * BM * BN * 4 <= KG * NS * STAGE, "the K groups' sums do not fit the ring");
+  __shared__ __attribute__((aligned(1024))) unsigned char smem_generic[KG * NS * STAGE];
 
   const int lane = threadIdx.x & 63, l15 = lane & 15;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kg = wave_all / NW, wave = wave_all % NW;
+  unsigned char DLM_LDS* all = (unsigned char DLM_LDS*)smem_generic;
+  unsigned char DLM_LDS* smem = all + kg * (NS * STAGE);
   const int wm = wave / WAVES_N, wn = wave % WAVES_N;
   int tmi, tni;
   tile_coords(blockIdx.x, tiles_m, tiles_n, tmi, tni);
@@ -369,7 +321,10 @@ q8_tile_kernel(Q8Gemm p, int tiles_m, int tiles_n) {
   const int K16 = p.K & ~15;
   Q8Rows<IA> al(p.x + (size_t)m0 * p.ldx, p.ldx, min(BM, p.M - m0), K16, NW, wave, lane);
   Q8Rows<IB> bl(p.w + (size_t)n0 * p.ldw, p.ldw, min(BN, p.N - n0), K16, NW, wave, lane);
-  const int ke = (K16 + kSlice - 1) / kSlice;
+  constexpr int PART = (KG * NS * STAGE - (KG - 1) * BM * BN * 4) / NW & ~15;
+  Epilogue<T, TM, TN, PART> ep(p, m0 + wm * WM, n0 + wn * WN, lane);
+  // slices of a group: kg, kg + KG, ...; one past the end of K reads zeros
+  const int ke = (K16 + KG * kSlice - 1) / (KG * kSlice);
 
   i32x4 acc[TM][TN];
 #pragma unroll
@@ -387,8 +342,8 @@ q8_tile_kernel(Q8Gemm p, int tiles_m, int tiles_n) {
   };
 #pragma unroll
   for (int s = 0; s < NS - 1; ++s) {
-    al.prepare(min(s, ke - 1));
-    bl.prepare(min(s, ke - 1));
+    al.prepare(min(s, ke - 1) * KG + kg);
+    bl.prepare(min(s, ke - 1) * KG + kg);
 #pragma unroll
     for (int i = 0; i < IA; ++i) dma_a(smem + s * STAGE, i);
 #pragma unroll
@@ -476,8 +431,8 @@ q8_tile_kernel(Q8Gemm p, int tiles_m, int tiles_n) {
       const unsigned char DLM_LDS* st = smem + slot * STAGE;
       unsigned char DLM_LDS* nst = smem + nslot * STAGE;
       const int nkt = min(kt + NS - 1, ke - 1);
-      al.prepare(nkt);
-      bl.prepare(nkt);
+      al.prepare(nkt * KG + kg);
+      bl.prepare(nkt * KG + kg);
       i32x4 fa[2][TM], fb[2][TN];
       rd(st, 0, fa[0], fb[0]);
 #pragma unroll
@@ -500,7 +455,7 @@ q8_tile_kernel(Q8Gemm p, int tiles_m, int tiles_n) {
 #undef DLM_WAIT_SLICES
   DLM_WAIT_VM(0);  // no DMA may still be writing this workgroup's LDS at exit
 
-  if (p.K & 15) {
+  if ((p.K & 15) && kg == 0) {
     const bool mine = lane < 16;  // the first 16 values of the k-step
     i32x4 fa[TM], fb[TN];
 #pragma unroll
@@ -517,29 +472,42 @@ q8_tile_kernel(Q8Gemm p, int tiles_m, int tiles_n) {
   }
 
   __syncthreads();  // every wave is done with the ring
-  constexpr int PART = NS * STAGE / NW & ~15;
-  epi_tile<T, TM, TN, PART>(acc, (float DLM_LDS*)(smem + wave * PART), m0 + wm * WM, n0 + wn * WN, lane, p);
+  if constexpr (KG > 1) {
+    i32x4 DLM_LDS* part = (i32x4 DLM_LDS*)all;
+    auto at = [&](int g, int i, int j) { return (((g - 1) * NW + wave) * TM * TN + i * TN + j) * 64 + lane; };
+    if (kg > 0) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) part[at(kg, i, j)] = acc[i][j];
+    }
+    __syncthreads();
+    if (kg > 0) return;
+#pragma unroll
+    for (int g = 1; g < KG; ++g)
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] += part[at(g, i, j)];
+    // the first group alone goes on: its waves' parts of the ring, once all
+    // of them have read the sums there
+    static_assert(KG * NS * STAGE - (KG - 1) * BM * BN * 4 >= NW * 16 * (WN + 4) * 4, "no room beside the sums");
+    smem = all + (KG - 1) * BM * BN * 4;
+  }
+  ep.finish(acc, (float DLM_LDS*)(smem + wave * PART));
 }
 
-template <class T, int BM, int BN, int WM, int WN, int NS, int SCH>
+template <class T, int BM, int BN, int WM, int WN, int NS, int SCH, int KG = 1>
 void launch_tile(const Q8Gemm& p, hipStream_t s) {
   static const std::string name = std::string("q8_tile_kernel<") + (sizeof(T) == 2 ? "_Float16" : "float") + ", " +
                                   std::to_string(BM) + ", " + std::to_string(BN) + ", " + std::to_string(WM) + ", " +
-                                  std::to_string(WN) + ", " + std::to_string(NS) + ", " + std::to_string(SCH) + ">";
+                                  std::to_string(WN) + ", " + std::to_string(NS) + ", " + std::to_string(SCH) + ", " +
+                                  std::to_string(KG) + ">";
   const int tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
   note_kernel(name.c_str());
   note_dims(p.M, p.N, p.K, (p.res ? 1 : 0) | (p.act << 4));
-  launch((q8_tile_kernel<T, BM, BN, WM, WN, NS, SCH>), dim3(tm * tn), dim3((BM / WM) * (BN / WN) * 64), 0, s, p, tm,
-         tn);
-}
-
-template <class T, int NW, int G>
-void launch_rows(const Q8Gemm& p, hipStream_t s) {
-  static const std::string name = std::string("q8_rows_kernel<") + (sizeof(T) == 2 ? "_Float16" : "float") + ", " +
-                                  std::to_string(NW) + ", " + std::to_string(G) + ">";
-  note_kernel(name.c_str());
-  note_dims(p.M, p.N, p.K, (p.res ? 1 : 0) | (p.act << 4));
-  launch((q8_rows_kernel<T, NW, G>), dim3((p.N + 15) / 16, (p.M + 15) / 16), dim3(NW * 64), 0, s, p);
+  launch((q8_tile_kernel<T, BM, BN, WM, WN, NS, SCH, KG>), dim3(tm * tn), dim3((BM / WM) * (BN / WN) * KG * 64), 0, s,
+         p, tm, tn);
 }
 
 // Tile override of dlm_q8_force_tile (0 = the plan below).
@@ -547,51 +515,43 @@ thread_local int g_q8_tile = 0;
 
 // A launch's time is modelled as
 //   base + (fix + slices * slice) * (1 + more * (ceil(grid / 256) - 1))   [us]
-// grid: output tiles, slices: 128-byte slices of K, more: what each further
-// workgroup on a CU adds, relative to the first (over 1 where it has to queue
-// for the LDS).  The constants are fits to the launches of 479 shapes (1-8192
-// rows, 16-12000 columns, K = 64-8192), graph-replayed; the modelled choice
-// takes 0.7% longer than the fastest of the eleven in the mean and 19% at
-// worst (1024 columns x 21 rows, 4.8 us against 4.05).
+// grid: output tiles, slices: of 128 bytes of K, more: what each further
+// workgroup on a CU adds, relative to the first (over 1 where it queues for
+// the LDS).  The constants are fits to the launches of 503 shapes (1-8192 rows,
+// 16-12000 columns, K = 64-8192), graph-replayed; the modelled choice takes
+// 0.3% longer than the fastest of the eleven in the mean and 12% at worst
+// (829x1184x224, 4.6 us against 4.2).  Split K for few rows (us, without and
+// with K groups): 1x4096x4096 6.8 -> 5.9, 13x1280x5120 9.2 -> 6.2, 1x2560x8192
+// 12.5 -> 6.9.
 struct Q8Tile {
   int bm, bn;
   float base, fix, slice, more;
 };
-constexpr int kRowTiles = 2;  // the first two are q8_rows_kernel's
 constexpr Q8Tile kQ8Tiles[] = {
-    {16, 16, 2.61f, 0.25f, 0.064f, 1.18f},    // 1: 16 waves, one group in flight
-    {16, 16, 2.90f, 0.13f, 0.074f, 1.27f},    // 2: 8 waves, two groups
-    {32, 32, 2.30f, 0.63f, 0.147f, 0.67f},    // 3
-    {64, 32, 2.56f, 0.67f, 0.164f, 0.97f},    // 4
-    {64, 64, 2.49f, 1.27f, 0.205f, 1.08f},    // 5
-    {64, 128, 1.73f, 2.24f, 0.298f, 1.30f},   // 6
-    {128, 128, 1.62f, 3.37f, 0.460f, 1.22f},  // 7: one workgroup a CU, four stages
-    {128, 96, 1.50f, 3.44f, 0.422f, 1.10f},   // 8
-    {128, 128, 1.50f, 2.90f, 0.745f, 0.70f},  // 9: two workgroups a CU, two stages
-    {192, 128, 1.50f, 4.23f, 0.904f, 0.70f},  // 10: the same
-    {128, 256, 1.93f, 5.41f, 0.691f, 1.29f},  // 11: ping-pong
+    {16, 32, 1.91f, 1.53f, 0.064f, 1.30f},    // 1: four K groups
+    {16, 32, 2.48f, 0.49f, 0.095f, 0.77f},    // 2: two K groups
+    {32, 32, 2.29f, 0.61f, 0.149f, 0.68f},    // 3
+    {32, 32, 2.24f, 1.13f, 0.101f, 0.88f},    // 4: two K groups
+    {64, 32, 2.45f, 0.66f, 0.169f, 0.93f},    // 5
+    {64, 64, 2.23f, 1.42f, 0.216f, 0.88f},    // 6
+    {64, 128, 1.80f, 2.16f, 0.289f, 1.21f},   // 7
+    {128, 128, 1.50f, 3.85f, 0.467f, 1.09f},  // 8: four stages, one workgroup a CU
+    {128, 128, 1.50f, 2.84f, 0.796f, 0.64f},  // 9: two stages, two workgroups
+    {192, 128, 1.50f, 4.01f, 0.939f, 0.66f},  // 10: the same
+    {128, 256, 1.50f, 5.62f, 0.690f, 1.21f},  // 11: ping-pong
 };
-constexpr int kQ8TileCount = sizeof(kQ8Tiles) / sizeof(kQ8Tiles[0]);
 
-// Rows too far apart for a tile's 32-bit offsets, and outputs narrower than
-// one MFMA block, which the tiles' epilogue does not take.
-bool only_rows(const Q8Gemm& p) { return p.N < 16 || std::max(p.ldx, p.ldw) > (1 << 22); }
-
-// The row kernels read W once for every 16 rows: up to 64 where there is a choice.
 int plan_q8(const Q8Gemm& p) {
-  const bool rows = only_rows(p);
-  const int slices = (p.K + 127) / 128;
+  const int slices = (p.K + kSlice - 1) / kSlice;
   int best = 1;
   float best_us = 3e38f;
-  for (int i = 0; i < (rows ? kRowTiles : kQ8TileCount); ++i) {
-    if (i < kRowTiles && !rows && p.M > 64) continue;
-    const Q8Tile& t = kQ8Tiles[i];
+  for (const Q8Tile& t : kQ8Tiles) {
     const long long grid = (long long)((p.M + t.bm - 1) / t.bm) * ((p.N + t.bn - 1) / t.bn);
     const float us =
         t.base + (t.fix + (float)slices * t.slice) * (1.0f + t.more * (float)((grid + 255) / 256 - 1));
     if (us < best_us) {
       best_us = us;
-      best = i + 1;
+      best = (int)(&t - kQ8Tiles) + 1;
     }
   }
   return best;
@@ -599,16 +559,15 @@ int plan_q8(const Q8Gemm& p) {
 
 template <class T>
 void q8_gemm(const Q8Gemm& p, hipStream_t s) {
-  const bool as_planned = g_q8_tile <= 0 || (g_q8_tile > kRowTiles && only_rows(p));
-  switch (as_planned ? plan_q8(p) : g_q8_tile) {
-    case 1: return launch_rows<T, 16, 1>(p, s);
-    case 2: return launch_rows<T, 8, 2>(p, s);
+  switch (g_q8_tile > 0 ? g_q8_tile : plan_q8(p)) {
+    case 1: return launch_tile<T, 16, 32, 16, 16, 4, kPlain, 4>(p, s);
+    case 2: return launch_tile<T, 16, 32, 16, 16, 3, kPlain, 2>(p, s);
     case 3: return launch_tile<T, 32, 32, 16, 16, 4, kPlain>(p, s);
-    case 4: return launch_tile<T, 64, 32, 16, 32, 4, kPlain>(p, s);
-    case 5: return launch_tile<T, 64, 64, 32, 32, 4, kPlain>(p, s);
-    case 6: return launch_tile<T, 64, 128, 32, 32, 4, kPlain>(p, s);
-    case 7: return launch_tile<T, 128, 128, 64, 32, 4, kPlain>(p, s);
-    case 8: return launch_tile<T, 128, 96, 32, 48, 3, kPlain>(p, s);
+    case 4: return launch_tile<T, 32, 32, 16, 16, 4, kPlain, 2>(p, s);
+    case 5: return launch_tile<T, 64, 32, 16, 32, 4, kPlain>(p, s);
+    case 6: return launch_tile<T, 64, 64, 32, 32, 4, kPlain>(p, s);
+    case 7: return launch_tile<T, 64, 128, 32, 32, 4, kPlain>(p, s);
+    case 8: return launch_tile<T, 128, 128, 64, 32, 4, kPlain>(p, s);
     case 9: return launch_tile<T, 128, 128, 64, 32, 2, kPlain>(p, s);
     case 10: return launch_tile<T, 192, 128, 48, 64, 2, kPlain>(p, s);
     default: return launch_tile<T, 128, 256, 64, 64, 3, kPingPong>(p, s);
@@ -617,6 +576,8 @@ void q8_gemm(const Q8Gemm& p, hipStream_t s) {
 
 // Largest K: 128 * 128 * K stays below 2^31.
 constexpr int kMaxK = 131071;
+// Largest row stride: 256 rows of a tile stay within 32-bit offsets.
+constexpr int kMaxLd = 1 << 22;
 // Columns a row of workgroups takes: a launch counts threads in 32 bits.
 constexpr int kMaxN = 1 << 25;
 
@@ -626,6 +587,7 @@ int linear_q8(const char* fn, Q8Gemm p, hipStream_t s) {
   if (!p.x || !p.w || !p.sx || !p.sw || !p.y) return bad("NULL pointer");
   if (p.act < DLM_ACT_NONE || p.act > DLM_ACT_GELU) return bad("unknown activation");
   if (p.K > kMaxK) return bad("K over " + std::to_string(kMaxK) + " may overflow the 32-bit sums");
+  if (p.ldx > kMaxLd || p.ldw > kMaxLd) return bad("row stride of X or W over " + std::to_string(kMaxLd));
   if (p.N > kMaxN) return bad("N over " + std::to_string(kMaxN));
   const int k16 = (p.K + 15) & ~15, cols = p.act == DLM_ACT_GEGLU ? p.N / 2 : p.N;
   if (p.act == DLM_ACT_GEGLU && p.N % 16) return bad("GEGLU needs N % 16 == 0");
@@ -653,9 +615,8 @@ int linear_q8(const char* fn, Q8Gemm p, hipStream_t s) {
     if (i.p == p.res && p.res == p.y && p.ldr == p.ldy) continue;  // added in place
     return bad(std::string("Y overlaps ") + i.name);
   }
-  // rows of one launch: at most 2^28 outputs (2^26 threads of the smallest
-  // tile) and 2^19 rows (the grid's y)
-  const int part = std::max(1 << 8, std::min(1 << 19, (1 << 28) / p.N & ~255));
+  // rows of one launch: at most 2^28 outputs (2^28 threads of the smallest tile)
+  const int part = std::max(1 << 8, std::min(1 << 24, (1 << 28) / p.N & ~255));
   for (int left = p.M; left > 0; left -= part) {
     p.M = std::min(left, part);
     q8_gemm<T>(p, s);

@@ -536,10 +536,10 @@ int dlm_layer_norm_q8_f32(const float* x, int ldx, const float* R, int ldr, floa
  * and R have N/2 columns.  The sums are exact, so a row's result depends on
  * neither M nor the other rows.
  * X and W start at 16-byte aligned addresses with row strides ldx, ldw that
- * are multiples of 16 bytes and at least K rounded up to 16; K <= 131071 (the
- * range of the sums), N <= 2^25.  Bytes of a row past K are read but have no effect.  Y
- * and R take any element-aligned address and row stride (even ones that are
- * multiples of 16 bytes are the fast ones).  Y may be R (same pointer and row
+ * are multiples of 16 bytes, at least K rounded up to 16 and at most 2^22; K <=
+ * 131071 (the range of the sums), N <= 2^25.  Bytes of a row past K, up to the
+ * next multiple of 16, are read but have no effect.  Y and R take any
+ * element-aligned address and row stride.  Y may be R (same pointer and row
  * stride) and not overlap an input otherwise.  Uses no workspace: calls on any
  * streams, captured or not, are independent. */
 int dlm_linear_q8_fp16(const void* X, int ldx, const float* sx, const void* W, int ldw,

@@ -72,6 +72,8 @@ def test_linear_entries_refuse(lib):
         assert call(act=-1) == INVALID and "activation" in err()
         assert call(act=2, N=24) == INVALID and "GEGLU" in err()
         assert call(K=131072, ldx=131072, ldw=131072) == INVALID and "K" in err()
+        assert call(ldx=(1 << 22) + 16) == INVALID and "4194304" in err()
+        assert call(N=(1 << 25) + 1, ldy=(1 << 25) + 1) == INVALID and "33554432" in err()
         assert call(X=A + 8) == INVALID and "16-byte" in err()
         assert call(ldw=72) == INVALID and "16-byte" in err()
         assert call(K=65) == INVALID and "rounded up" in err()
