@@ -11,19 +11,22 @@
 //               root cancels in q, so q is formed from h gamma / max|h gamma|
 //               and only the scale sees it: the largest magnitude and the sum
 //               of squares come out of one pass over the row.
-//   LayerNorm   v = (h - mean) / sqrt(var + eps) gamma + beta
+//   LayerNorm   v = (h - mean) / sqrt(var + eps) gamma + beta, the variance from
+//               the differences (rows whose mean is far from 0 keep theirs)
 //
-// Rounding.  127 v / a is formed as v * (127 / a) in fp32, which may fall on
-// the wrong side of a half by 2^-17 at most (2^-24 relative error of 127 / a
-// on values up to 127).  Quotients within 2^-16 of a half (one in 30,000) are
-// decided again by comparing 254 v with (2k + 1) a in fp64, where both
+// Rounding.  127 v / a is formed as v * (127 * rcp(a)) in fp32, which is off by
+// 2.3e-5 at most (relative errors of 2^-23 and 2^-24 on values up to 127).
+// Quotients within 2^-15 of a half (one in 16,000) are decided again by comparing 254 v with (2k + 1) a in fp64, where both
 // products are exact.  So q is the quotient's nearest integer whatever the
 // launch looks like; for fp16 rows (and fp16 gamma) of the first two kinds,
 // where v is exact in fp32, that is the mathematically exact result.
 //
 // What bounds them: memory, one pass.  A row stays in registers between its
-// statistics and its output (up to 64 values a thread); rows of up to 1536
-// values take one wave, so a workgroup needs no barrier.
+// statistics and its output, in 8 to 512 threads by its length.  Measured (graph
+// replays, inputs that no cache holds): quantise 8192x1280 fp16 8.2 us (3.8 TB/s,
+// of which the launch is 2 us), RMS norm with residual 13.5 us (5.4 TB/s; fp32
+// 26.7 us, 5.1), LayerNorm 10.8 us (2.9 TB/s, three reductions in a chain); a 1 GiB
+// copy reaches 5.15 TB/s.  One row: 2.3 us, 2.9 and 3.2.
 #include <algorithm>
 
 #include "common.hpp"
@@ -43,83 +46,70 @@ struct RowArgs {
   float* scale;
   long long ldx, ldr, ldh, ldq;
   int rows, K;
-  float eps;
+  float eps, inv_k;
 };
 
-template <class T>
-struct Vec8;  // eight elements as loaded
-template <>
-struct Vec8<f16> {
-  typedef f16x8 type;
-};
-template <>
-struct Vec8<float> {
-  typedef float type __attribute__((ext_vector_type(8)));
-};
 typedef float f32x8 __attribute__((ext_vector_type(8)));
+template <class T>
+using Vec8 = T __attribute__((ext_vector_type(8)));
 
 // Eight elements at any element-aligned address: one 16-byte access (two for
 // fp32), which the hardware takes at any alignment.
 template <class T>
-__device__ __forceinline__ f32x8 load8(const T* p) {
-  typename Vec8<T>::type v;
+__device__ __forceinline__ Vec8<T> load8(const T* p) {
+  Vec8<T> v;
   __builtin_memcpy(&v, p, sizeof(v));
-  f32x8 r;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = (float)v[i];
-  return r;
+  return v;
 }
 template <class T>
-__device__ __forceinline__ void store8(T* p, const f32x8& x) {
-  typename Vec8<T>::type v;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = (T)x[i];
+__device__ __forceinline__ void store8(T* p, const Vec8<T>& v) {
   __builtin_memcpy(p, &v, sizeof(v));
 }
+// Largest magnitude, NaN where one of the two is NaN (v_maximum3_f32 for two
+// values at a time).
+__device__ __forceinline__ float max_abs(float m, float v) { return __builtin_elementwise_maximum(m, fabsf(v)); }
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 // What a row's values are multiplied by on their way to q.
 struct RowScale {
   float r;     // 127 / (a m), 0 for rows without a finite positive maximum
   float a;     // a m
-  float m;     // fp32 rows: 2^100 where a is so small that 127 / a would overflow; else 1
+  float m;     // fp32 rows: a power of two that keeps 127 / a and its reciprocal normal numbers; else 1
   float unit;  // a / 127, NaN for a row that holds an infinity or NaN
 };
-// top: bits of max |v| (of the largest NaN, if there is one).  Values of fp16
-// rows are no smaller than 2^-48 where they are not 0 (LayerNorm's 2^-112).
+// a: max |v|, NaN if there is one.  Values of fp16 rows are no smaller than
+// 2^-48 where they are not 0 (LayerNorm's 2^-112).
 template <class T>
-__device__ __forceinline__ RowScale row_scale(unsigned top, bool bad) {
+__device__ __forceinline__ RowScale row_scale(float a, bool bad) {
   RowScale s;
-  const float a = __uint_as_float(top);
-  bad = bad || top >= 0x7f800000u;
-  s.m = sizeof(T) == 4 && a < 0x1p-100f ? 0x1p100f : 1.0f;
+  bad = bad || !(a < INFINITY);
+  s.m = sizeof(T) == 2 ? 1.0f : a < 0x1p-100f ? 0x1p100f : a > 0x1p100f ? 0x1p-100f : 1.0f;
   s.a = a * s.m;
-  s.r = bad || top == 0 ? 0.0f : 127.0f / s.a;
+  s.r = bad || a == 0.0f ? 0.0f : 127.0f * __builtin_amdgcn_rcpf(s.a);
   s.unit = bad ? __uint_as_float(0x7fc00000u) : a / 127.0f;
   return s;
 }
 
 // Eight values to eight bytes.  Adding 1.5 * 2^23 rounds to an integer (ties
-// to even) and leaves it in the low byte.  A row with an infinity or NaN
-// (r = 0) becomes zeros: its values go through a select, as 0 * inf is NaN.
+// to even) and leaves it in the low byte.
 constexpr float kRound = 12582912.0f;
 template <class T>
 __device__ __forceinline__ u32x2 quant8(const f32x8& v, const RowScale& s) {
-  float far = 0.0f;
+  float far = 0.0f, x[8];
   unsigned u[8];
-  float x[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    x[i] = s.r == 0.0f ? 0.0f : sizeof(T) == 4 ? v[i] * s.m : v[i];
+    x[i] = sizeof(T) == 4 ? v[i] * s.m : v[i];
     const float t = __builtin_fmaf(x[i], s.r, kRound);
     u[i] = __float_as_uint(t);
-    far = fmaxf(far, fabsf(__builtin_fmaf(x[i], s.r, -(t - kRound))));
+    far = max_abs(far, __builtin_fmaf(x[i], s.r, -(t - kRound)));
   }
-  if (far > 0.5f - 0x1p-16f) {
+  if (far > 0.5f - 0x1p-15f) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float n = __uint_as_float(u[i]) - kRound;
       const float d = __builtin_fmaf(x[i], s.r, -n);
-      if (fabsf(d) > 0.5f - 0x1p-16f) {
+      if (fabsf(d) > 0.5f - 0x1p-15f) {
         const float k = d > 0.0f ? n : n - 1.0f;  // between k and k + 1
         const double e = 254.0 * (double)x[i] - (double)(2.0f * k + 1.0f) * (double)s.a;
         const bool up = e > 0.0 || (e == 0.0 && ((int)k & 1));
@@ -132,205 +122,282 @@ __device__ __forceinline__ u32x2 quant8(const f32x8& v, const RowScale& s) {
   for (int j = 0; j < 2; ++j) {
     const unsigned lo = __builtin_amdgcn_perm(u[4 * j + 1], u[4 * j], 0x0c0c0400u);
     const unsigned hi = __builtin_amdgcn_perm(u[4 * j + 3], u[4 * j + 2], 0x04000c0cu);
-    o[j] = lo | hi;
+    o[j] = s.r == 0.0f ? 0u : lo | hi;  // zeros, or a row with an infinity or NaN
   }
   return o;
 }
 
-__device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-__device__ __forceinline__ unsigned wave_umax(unsigned v) {
-  return wave_reduce(v, [](unsigned a, unsigned b) { return a > b ? a : b; });
-}
-
-// Reductions over the threads of a row: a wave, or the waves of a workgroup
-// through LDS (`slot`: another part of it for each use).
-template <int WAVES, typename V, typename Op>
-__device__ __forceinline__ V row_reduce(V v, Op op, V* lds) {
-  v = wave_reduce(v, op);
-  if constexpr (WAVES > 1) {
-    const int w = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) lds[w] = v;
+// Reductions over the TPR threads of a row: 8, 16 or 32 lanes of a wave, a wave,
+// or the waves of a workgroup through LDS (`lds`: another part of it for each
+// use).  All lanes have to take part.
+template <int TPR, typename Op>
+__device__ __forceinline__ float row_reduce(float v, Op op, float* lds) {
+  if constexpr (TPR >= 64) {
+    v = wave_reduce(v, op);
+  } else {
+    auto dpp = [&](auto ctrl) {
+      v = op(v, __uint_as_float(dpp_u32<decltype(ctrl)::value>(__float_as_uint(v))));
+    };
+    dpp(std::integral_constant<int, kDppXor1>{});
+    dpp(std::integral_constant<int, kDppXor2>{});
+    dpp(std::integral_constant<int, kDppHalfMirror>{});
+    if constexpr (TPR > 8) dpp(std::integral_constant<int, kDppMirror>{});
+    if constexpr (TPR == 32) {
+      const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+      v = op(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    }
+  }
+  if constexpr (TPR > 64) {
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
     v = lds[0];
 #pragma unroll
-    for (int i = 1; i < WAVES; ++i) v = op(v, lds[i]);
+    for (int i = 1; i < TPR / 64; ++i) v = op(v, lds[i]);
   }
   return v;
 }
+constexpr auto kSum = [](float a, float b) { return a + b; };
+constexpr auto kMax = [](float a, float b) { return max_nan(a, b); };
 
-// A row in the registers of WAVES waves, VPT vectors of eight values a
-// thread (K >= 8).  Vector j of a thread starts at 8 (thread + threads j); the
-// row's last one starts at K - 8 and repeats values of the one before, which
-// sums leave out and whose results are the same bytes.  All loads are issued
-// before any is used, at addresses inside the row.
-template <class T, RowKind KIND, int WAVES, int VPT>
-__global__ void __launch_bounds__(WAVES == 1 ? 256 : WAVES * 64) row_q8_kernel(RowArgs p) {
-  constexpr int TPR = WAVES * 64;
-  __shared__ float red[3][WAVES];
+// A row in the registers of TPR threads, VPT vectors of eight values each
+// (K >= 8).  Vector j of a thread starts at 8 (thread + TPR j); the row's last
+// one starts at K - 8 and repeats values of the one before, which sums leave
+// out and whose results are the same bytes.  All loads are issued before any
+// is used, at addresses inside the row.
+template <class T, RowKind KIND, int TPR, int VPT>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) row_q8_kernel(RowArgs p) {
+  constexpr int ROWS = TPR < 256 ? 256 / TPR : 1;  // of a workgroup
+  __shared__ float red[3][TPR > 64 ? TPR / 64 : 1];
   const int t = threadIdx.x & (TPR - 1);
-  const int row = WAVES == 1 ? blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
-  if (WAVES == 1 && row >= p.rows) return;
+  const int row_at = ROWS == 1 ? (int)blockIdx.x : (int)blockIdx.x * ROWS + (int)threadIdx.x / TPR;
+  const int row = min(row_at, p.rows - 1);  // lanes past the last row repeat it, and store nothing
   const int K = p.K, S = (K + 7) >> 3;
+  const bool ragged = K & 7;
   const T* x = (const T*)p.x + (size_t)row * p.ldx;
   const T* res = (const T*)p.res + (size_t)row * p.ldr;
-  f32x8 v[VPT], g[VPT], b[VPT], r[VPT];
+  Vec8<T> h[VPT], r[VPT];
+  f16x8 g[VPT], b[VPT];
   int at[VPT];
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
     at[j] = min(min(t + TPR * j, S - 1) * 8, K - 8);
-    v[j] = load8(x + at[j]);
+    h[j] = load8(x + at[j]);
     if (KIND != kQuant && p.res) r[j] = load8(res + at[j]);
     if (KIND != kQuant && p.gamma) g[j] = load8(p.gamma + at[j]);
     if (KIND == kLayer && p.beta) b[j] = load8(p.beta + at[j]);
   }
-  // first new value of vector j (8: the thread has none)
-  auto skip = [&](int j) { return t + TPR * j < S ? (t + TPR * j) * 8 - at[j] : 8; };
   if (KIND != kQuant && p.res) {
+    // in T: the sum of two fp16 values rounded once, as through fp32
 #pragma unroll
-    for (int j = 0; j < VPT; ++j)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[j][i] = (float)(T)(v[j][i] + r[j][i]);
+    for (int j = 0; j < VPT; ++j) h[j] = h[j] + r[j];
   }
-  const f32x8* h = v;  // the stream as it is stored
-  f32x8 y[KIND == kQuant ? 1 : VPT];
-  float rstd = 1.0f;
-  bool bad = false;
-  if constexpr (KIND == kRms) {
-    float ss = 0.0f;
-#pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-      const int s0 = skip(j);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        ss += i >= s0 ? v[j][i] * v[j][i] : 0.0f;
-        y[j][i] = p.gamma ? v[j][i] * g[j][i] : v[j][i];
-      }
-    }
-    ss = row_reduce<WAVES>(ss, [](float a, float c) { return a + c; }, red[0]);
-    bad = !(ss < INFINITY);
-    rstd = 1.0f / sqrtf(ss / (float)K + p.eps);
-  } else if constexpr (KIND == kLayer) {
+  // sum of f(j, i) over the row's values, each once
+  auto row_sum = [&](auto f, float* lds) {
     float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-      const int s0 = skip(j);
+      float part = 0.0f;
+      if (ragged) {
+        const int skip = (t + TPR * j) * 8 - at[j];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += i >= s0 ? v[j][i] : 0.0f;
-    }
-    const float mean = row_reduce<WAVES>(sum, [](float a, float c) { return a + c; }, red[0]) / (float)K;
-    float sq = 0.0f;
+        for (int i = 0; i < 8; ++i) part += i >= skip ? f(j, i) : 0.0f;
+      } else {
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-      const int s0 = skip(j);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = v[j][i] - mean;
-        sq += i >= s0 ? d * d : 0.0f;
+        for (int i = 0; i < 8; ++i) part += f(j, i);
       }
+      sum += t + TPR * j < S ? part : 0.0f;
     }
-    sq = row_reduce<WAVES>(sq, [](float a, float c) { return a + c; }, red[1]);
-    bad = !(sq < INFINITY);
-    const float rs = 1.0f / sqrtf(sq / (float)K + p.eps);
+    return row_reduce<TPR>(sum, kSum, lds);
+  };
+  f32x8 y[VPT];
+  float rstd = 1.0f;
+  bool bad = false;
+  if constexpr (KIND == kQuant) {
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) y[j] = __builtin_convertvector(h[j], f32x8);
+  } else if constexpr (KIND == kRms) {
 #pragma unroll
     for (int j = 0; j < VPT; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float n = (v[j][i] - mean) * rs;
-        y[j][i] = __builtin_fmaf(n, p.gamma ? g[j][i] : 1.0f, p.beta ? b[j][i] : 0.0f);
-      }
+      for (int i = 0; i < 8; ++i) y[j][i] = p.gamma ? (float)h[j][i] * (float)g[j][i] : (float)h[j][i];
+    const float ss = row_sum([&](int j, int i) { return (float)h[j][i] * (float)h[j][i]; }, red[0]);
+    bad = !(ss < INFINITY);
+    rstd = rsqrtf(ss * p.inv_k + p.eps);
+  } else {
+    const float mean = row_sum([&](int j, int i) { return (float)h[j][i]; }, red[0]) / (float)K;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[j][i] = (float)h[j][i] - mean;
+    const float sq = row_sum([&](int j, int i) { return y[j][i] * y[j][i]; }, red[1]);
+    bad = !(sq < INFINITY);
+    const float rs = rsqrtf(sq * p.inv_k + p.eps);
+#pragma unroll
+    for (int j = 0; j < VPT; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        y[j][i] = __builtin_fmaf(y[j][i] * rs, p.gamma ? (float)g[j][i] : 1.0f, p.beta ? (float)b[j][i] : 0.0f);
   }
-  const f32x8* out = KIND == kQuant ? v : y;
-  unsigned top = 0;
+  float top = 0.0f;
 #pragma unroll
   for (int j = 0; j < VPT; ++j)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, abs_bits(out[j][i]));
-  top = row_reduce<WAVES>(top, [](unsigned a, unsigned c) { return a > c ? a : c; }, (unsigned*)red[2]);
-  const RowScale s = row_scale<T>(top, bad);
+    for (int i = 0; i < 8; ++i) top = max_abs(top, y[j][i]);
+  const RowScale s = row_scale<T>(row_reduce<TPR>(top, kMax, red[2]), bad);
+  if (ROWS > 1 && row_at >= p.rows) return;
   int8_t* q = p.q + (size_t)row * p.ldq;
   T* ho = (T*)p.h + (size_t)row * p.ldh;
 #pragma unroll
   for (int j = 0; j < VPT; ++j) {
     if (t + TPR * j >= S) continue;
     if (KIND != kQuant && p.h) store8(ho + at[j], h[j]);
-    const u32x2 o = quant8<T>(out[j], s);
+    const u32x2 o = quant8<T>(y[j], s);
     __builtin_memcpy(q + at[j], &o, 8);
   }
-  if (t == 0) p.scale[row] = KIND == kRms ? rstd * s.unit : s.unit;
+  if (t == 0) p.scale[row] = s.unit == 0.0f ? 0.0f : rstd * s.unit;
 }
 
-// Rows of fewer than 8 values, or of more than the registers of a workgroup
-// hold: one workgroup a row, which reads it again for every statistic (from
-// the L2).  With a residual the sums are read back from h where the caller
-// takes them, from x and the residual otherwise (h may be either of them:
-// then h holds what the sum was).
-template <class T, RowKind KIND, int WAVES>
-__global__ void __launch_bounds__(WAVES * 64) row_q8_long_kernel(RowArgs p) {
-  constexpr int NT = WAVES * 64;
-  __shared__ float red[3][WAVES];
-  const int row = blockIdx.x;
-  const int K = p.K;
+// Rows of more values than the registers of a workgroup hold: one workgroup a
+// row, which reads it again for every statistic (from the L2).  With a
+// residual the sums are read back from h where the caller takes them, from x
+// and the residual otherwise.  h may be either of them, so each value is read
+// and replaced by one thread: vectors of eight, and the row's last values one
+// by one.
+template <class T, RowKind KIND>
+__global__ void __launch_bounds__(1024) row_q8_long_kernel(RowArgs p) {
+  constexpr int NT = 1024;
+  __shared__ float red[3][NT / 64];
+  const int row = blockIdx.x, t = threadIdx.x;
+  const int K = p.K, S = K >> 3, tail = S * 8 + t;
   const T* x = (const T*)p.x + (size_t)row * p.ldx;
   const T* res = (const T*)p.res + (size_t)row * p.ldr;
   T* ho = (T*)p.h + (size_t)row * p.ldh;
-  const bool sum_first = KIND != kQuant && p.res;
-  auto first = [&](int k) {
-    float v = (float)x[k];
-    if (sum_first) {
-      v = (float)(T)(v + (float)res[k]);
-      if (p.h) ho[k] = (T)v;
+  const bool add = KIND != kQuant && p.res;
+  bool first = true;
+  // f(values, gamma, beta, n, k) for each of the row's vectors
+  auto each = [&](auto f) {
+    for (int s = t; s < S; s += NT) {
+      const int k = s * 8;
+      const bool back = add && p.h && !first;
+      Vec8<T> v = load8(back ? ho + k : x + k);
+      if (add && !back) {
+        v = v + load8(res + k);
+        if (p.h) store8(ho + k, v);
+      }
+      f16x8 g{}, b{};
+      if (KIND != kQuant && p.gamma) g = load8(p.gamma + k);
+      if (KIND == kLayer && p.beta) b = load8(p.beta + k);
+      f(__builtin_convertvector(v, f32x8), __builtin_convertvector(g, f32x8), __builtin_convertvector(b, f32x8), 8, k);
     }
-    return v;
-  };
-  auto again = [&](int k) -> float {
-    if (sum_first && p.h) return (float)ho[k];
-    return sum_first ? (float)(T)((float)x[k] + (float)res[k]) : (float)x[k];
+    if (tail < K) {
+      const bool back = add && p.h && !first;
+      T v = back ? ho[tail] : x[tail];
+      if (add && !back) {
+        v = v + res[tail];
+        if (p.h) ho[tail] = v;
+      }
+      f32x8 v8{}, g{}, b{};
+      v8[0] = (float)v;
+      if (KIND != kQuant && p.gamma) g[0] = (float)p.gamma[tail];
+      if (KIND == kLayer && p.beta) b[0] = (float)p.beta[tail];
+      f(v8, g, b, 1, tail);
+    }
+    first = false;
   };
   float rstd = 1.0f, mean = 0.0f, rs = 1.0f;
   bool bad = false;
-  auto value = [&](int k, float v) {
-    if constexpr (KIND == kRms) return p.gamma ? v * (float)p.gamma[k] : v;
-    if constexpr (KIND == kLayer)
-      return __builtin_fmaf((v - mean) * rs, p.gamma ? (float)p.gamma[k] : 1.0f, p.beta ? (float)p.beta[k] : 0.0f);
+  auto value = [&](float v, float g, float b) {
+    if constexpr (KIND == kRms) return p.gamma ? v * g : v;
+    if constexpr (KIND == kLayer) return __builtin_fmaf((v - mean) * rs, p.gamma ? g : 1.0f, p.beta ? b : 0.0f);
     return v;
   };
-  auto add = [](float a, float c) { return a + c; };
-  unsigned top = 0;
+  float top = 0.0f;
   if constexpr (KIND == kLayer) {
-    float sum = 0.0f;
-    for (int k = threadIdx.x; k < K; k += NT) sum += first(k);
-    mean = row_reduce<WAVES>(sum, add, red[0]) / (float)K;
-    float sq = 0.0f;
-    for (int k = threadIdx.x; k < K; k += NT) {
-      const float d = again(k) - mean;
-      sq += d * d;
-    }
-    sq = row_reduce<WAVES>(sq, add, red[1]);
+    float sum = 0.0f, sq = 0.0f;
+    each([&](const f32x8& v, const f32x8&, const f32x8&, int n, int) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += i < n ? v[i] : 0.0f;
+    });
+    mean = row_reduce<NT>(sum, kSum, red[0]) / (float)K;
+    each([&](const f32x8& v, const f32x8&, const f32x8&, int n, int) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sq += i < n ? (v[i] - mean) * (v[i] - mean) : 0.0f;
+    });
+    sq = row_reduce<NT>(sq, kSum, red[1]);
     bad = !(sq < INFINITY);
-    rs = 1.0f / sqrtf(sq / (float)K + p.eps);
-    for (int k = threadIdx.x; k < K; k += NT) top = max(top, abs_bits(value(k, again(k))));
+    rs = rsqrtf(sq * p.inv_k + p.eps);
+    each([&](const f32x8& v, const f32x8& g, const f32x8& b, int n, int) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = i < n ? max_abs(top, value(v[i], g[i], b[i])) : top;
+    });
   } else {
     float ss = 0.0f;
-    for (int k = threadIdx.x; k < K; k += NT) {
-      const float v = first(k);
-      ss += v * v;
-      top = max(top, abs_bits(value(k, v)));
-    }
+    each([&](const f32x8& v, const f32x8& g, const f32x8& b, int n, int) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        ss += v[i] * v[i];
+        top = max_abs(top, value(v[i], g[i], b[i]));  // past n: zeros
+      }
+    });
     if constexpr (KIND == kRms) {
-      ss = row_reduce<WAVES>(ss, add, red[0]);
+      ss = row_reduce<NT>(ss, kSum, red[0]);
       bad = !(ss < INFINITY);
-      rstd = 1.0f / sqrtf(ss / (float)K + p.eps);
+      rstd = rsqrtf(ss * p.inv_k + p.eps);
     }
   }
-  top = row_reduce<WAVES>(top, [](unsigned a, unsigned c) { return a > c ? a : c; }, (unsigned*)red[2]);
-  const RowScale s = row_scale<T>(top, bad);
+  const RowScale s = row_scale<T>(row_reduce<NT>(top, kMax, red[2]), bad);
   int8_t* q = p.q + (size_t)row * p.ldq;
-  for (int k = threadIdx.x; k < K; k += NT) {
-    const float v = value(k, again(k));
-    const u32x2 o = quant8<T>(f32x8{v, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f}, s);
-    q[k] = (int8_t)(o[0] & 0xff);
+  each([&](const f32x8& v, const f32x8& g, const f32x8& b, int n, int k) {
+    f32x8 y;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = value(v[i], g[i], b[i]);
+    const u32x2 o = quant8<T>(y, s);
+    if (n == 8)
+      __builtin_memcpy(q + k, &o, 8);
+    else
+      q[k] = (int8_t)(o[0] & 0xff);
+  });
+  if (t == 0) p.scale[row] = s.unit == 0.0f ? 0.0f : rstd * s.unit;
+}
+
+// Rows of fewer than eight values: a thread a row.
+template <class T, RowKind KIND>
+__global__ void __launch_bounds__(256) row_q8_short_kernel(RowArgs p) {
+  const int row = blockIdx.x * 256 + threadIdx.x;
+  if (row >= p.rows) return;
+  const T* x = (const T*)p.x + (size_t)row * p.ldx;
+  f32x8 y{};
+  float sum = 0.0f, sq = 0.0f, top = 0.0f, rstd = 1.0f;
+#pragma unroll
+  for (int k = 0; k < 7; ++k) {
+    if (k >= p.K) break;
+    T v = x[k];
+    if (KIND != kQuant && p.res) v = v + ((const T*)p.res)[(size_t)row * p.ldr + k];
+    if (KIND != kQuant && p.h) ((T*)p.h)[(size_t)row * p.ldh + k] = v;
+    y[k] = (float)v;
+    sum += y[k];
   }
-  if (threadIdx.x == 0) p.scale[row] = KIND == kRms ? rstd * s.unit : s.unit;
+  const float mean = KIND == kLayer ? sum / (float)p.K : 0.0f;
+#pragma unroll
+  for (int k = 0; k < 7; ++k) sq += k < p.K ? (y[k] - mean) * (y[k] - mean) : 0.0f;
+  const bool bad = KIND != kQuant && !(sq < INFINITY);
+  const float rs = rsqrtf(sq * p.inv_k + p.eps);
+  if (KIND == kRms) rstd = rs;
+#pragma unroll
+  for (int k = 0; k < 7; ++k) {
+    if (k >= p.K) break;
+    const float g = KIND != kQuant && p.gamma ? (float)p.gamma[k] : 1.0f;
+    if (KIND == kRms) y[k] = y[k] * g;
+    if (KIND == kLayer) y[k] = __builtin_fmaf((y[k] - mean) * rs, g, p.beta ? (float)p.beta[k] : 0.0f);
+    top = max_abs(top, y[k]);
+  }
+  const RowScale s = row_scale<T>(top, bad);
+  const u32x2 o = quant8<T>(y, s);
+  int8_t* q = p.q + (size_t)row * p.ldq;
+#pragma unroll
+  for (int k = 0; k < 7; ++k)
+    if (k < p.K) q[k] = (int8_t)(o[k >> 2] >> (8 * (k & 3)));
+  p.scale[row] = s.unit == 0.0f ? 0.0f : rstd * s.unit;
 }
 
 // y = q * scale, sixteen values a thread (K >= 16: the last vector of a row
@@ -355,37 +422,50 @@ dequant_kernel(const int8_t* __restrict__ q, long long ldq, const float* __restr
   }
 }
 
-template <class T, RowKind KIND, int WAVES, int VPT>
+template <class T, RowKind KIND, int TPR, int VPT>
 void launch_rows(const RowArgs& a, hipStream_t s) {
   static const std::string name = std::string("row_q8_kernel<") + (sizeof(T) == 2 ? "_Float16" : "float") + ", " +
-                                  std::to_string((int)KIND) + ", " + std::to_string(WAVES) + ", " +
+                                  std::to_string((int)KIND) + ", " + std::to_string(TPR) + ", " +
                                   std::to_string(VPT) + ">";
-  DLM_LAUNCH(name.c_str(), (row_q8_kernel<T, KIND, WAVES, VPT>), dim3(WAVES == 1 ? (a.rows + 3) / 4 : a.rows),
-             dim3(WAVES == 1 ? 256 : WAVES * 64), 0, s, a);
+  constexpr int ROWS = TPR < 256 ? 256 / TPR : 1;
+  DLM_LAUNCH(name.c_str(), (row_q8_kernel<T, KIND, TPR, VPT>), dim3((a.rows + ROWS - 1) / ROWS),
+             dim3(TPR < 256 ? 256 : TPR), 0, s, a);
 }
 
-// A wave holds rows of up to 1536 values (three vectors a lane), a workgroup
-// of four or eight waves up to 16384.
+// Threads a row by its length: each holds one to four vectors.  Rows of 1025-2048
+// values take a workgroup (8192x1280 quantise 8.2 us, RMS norm
+// 13.5; with a wave each 8.4 and 13.9, and 2.8 against 3.8 us for 256 rows),
+// but fp16 LayerNorms of many of them a wave: their third reduction weighs more
+// than the latency (8192x1280 13.6 -> 10.8 us, 2048x1280 5.9 -> 5.5; 1024 rows
+// the same either way; fp32 ones are slower with a wave).
 template <class T, RowKind KIND>
 void row_q8(const RowArgs& a, hipStream_t s) {
-  if (a.K < 8)
-    DLM_LAUNCH("row_q8_long_kernel<1>", (row_q8_long_kernel<T, KIND, 1>), dim3(a.rows), dim3(64), 0, s, a);
-  else if (a.K <= 512)
-    launch_rows<T, KIND, 1, 1>(a, s);
-  else if (a.K <= 1024)
-    launch_rows<T, KIND, 1, 2>(a, s);
-  else if (a.K <= 1536)
-    launch_rows<T, KIND, 1, 3>(a, s);
-  else if (a.K <= 2048)
-    launch_rows<T, KIND, 4, 1>(a, s);
-  else if (a.K <= 4096)
-    launch_rows<T, KIND, 4, 2>(a, s);
-  else if (a.K <= 8192)
-    launch_rows<T, KIND, 4, 4>(a, s);
-  else if (a.K <= 16384)
-    launch_rows<T, KIND, 8, 4>(a, s);
+  const int K = a.K;
+  if (K < 8)
+    DLM_LAUNCH("row_q8_short_kernel", (row_q8_short_kernel<T, KIND>), dim3((a.rows + 255) / 256), dim3(256), 0, s, a);
+  else if (K <= 64)
+    launch_rows<T, KIND, 8, 1>(a, s);
+  else if (K <= 128)
+    launch_rows<T, KIND, 16, 1>(a, s);
+  else if (K <= 256)
+    launch_rows<T, KIND, 32, 1>(a, s);
+  else if (K <= 512)
+    launch_rows<T, KIND, 64, 1>(a, s);
+  else if (K <= 1024)
+    launch_rows<T, KIND, 64, 2>(a, s);
+  else if (K <= 2048) {
+    if constexpr (KIND == kLayer && sizeof(T) == 2) {
+      if (a.rows >= 2048) return K <= 1536 ? launch_rows<T, KIND, 64, 3>(a, s) : launch_rows<T, KIND, 64, 4>(a, s);
+    }
+    launch_rows<T, KIND, 256, 1>(a, s);
+  } else if (K <= 4096)
+    launch_rows<T, KIND, 256, 2>(a, s);
+  else if (K <= 8192)
+    launch_rows<T, KIND, 512, 2>(a, s);
+  else if (K <= 16384)
+    launch_rows<T, KIND, 512, 4>(a, s);
   else
-    DLM_LAUNCH("row_q8_long_kernel<16>", (row_q8_long_kernel<T, KIND, 16>), dim3(a.rows), dim3(1024), 0, s, a);
+    DLM_LAUNCH("row_q8_long_kernel", (row_q8_long_kernel<T, KIND>), dim3(a.rows), dim3(1024), 0, s, a);
 }
 
 // A launch counts its threads in 32 bits: more rows than 2^21 go in parts.
@@ -484,7 +564,7 @@ extern "C" {
 int dlm_quantize_rows_fp16(const void* x, int ldx, void* q, int ldq, float* scale, int rows, int K, void* stream) {
   if (rows <= 0 || K <= 0) return DLM_OK;
   return row_entry<f16>(kQuant, __func__,
-                        RowArgs{x, nullptr, nullptr, nullptr, nullptr, (int8_t*)q, scale, ldx, 0, 0, ldq, rows, K, 0.0f},
+                        RowArgs{x, nullptr, nullptr, nullptr, nullptr, (int8_t*)q, scale, ldx, 0, 0, ldq, rows, K, 0.0f, 0.0f},
                         (hipStream_t)stream);
 }
 
@@ -492,7 +572,7 @@ int dlm_quantize_rows_f32(const float* x, int ldx, void* q, int ldq, float* scal
   if (rows <= 0 || K <= 0) return DLM_OK;
   return row_entry<float>(
       kQuant, __func__,
-      RowArgs{x, nullptr, nullptr, nullptr, nullptr, (int8_t*)q, scale, ldx, 0, 0, ldq, rows, K, 0.0f},
+      RowArgs{x, nullptr, nullptr, nullptr, nullptr, (int8_t*)q, scale, ldx, 0, 0, ldq, rows, K, 0.0f, 0.0f},
       (hipStream_t)stream);
 }
 
@@ -501,7 +581,7 @@ int dlm_rms_norm_q8_fp16(const void* x, int ldx, const void* R, int ldr, void* H
   if (rows <= 0 || K <= 0) return DLM_OK;
   return row_entry<f16>(
       kRms, __func__,
-      RowArgs{x, R, H, (const f16*)gamma, nullptr, (int8_t*)q, scale, ldx, ldr, ldh, ldq, rows, K, eps},
+      RowArgs{x, R, H, (const f16*)gamma, nullptr, (int8_t*)q, scale, ldx, ldr, ldh, ldq, rows, K, eps, 1.0f / (float)K},
       (hipStream_t)stream);
 }
 
@@ -510,7 +590,7 @@ int dlm_rms_norm_q8_f32(const float* x, int ldx, const float* R, int ldr, float*
   if (rows <= 0 || K <= 0) return DLM_OK;
   return row_entry<float>(
       kRms, __func__,
-      RowArgs{x, R, H, (const f16*)gamma, nullptr, (int8_t*)q, scale, ldx, ldr, ldh, ldq, rows, K, eps},
+      RowArgs{x, R, H, (const f16*)gamma, nullptr, (int8_t*)q, scale, ldx, ldr, ldh, ldq, rows, K, eps, 1.0f / (float)K},
       (hipStream_t)stream);
 }
 
@@ -520,7 +600,7 @@ int dlm_layer_norm_q8_fp16(const void* x, int ldx, const void* R, int ldr, void*
   if (rows <= 0 || K <= 0) return DLM_OK;
   return row_entry<f16>(
       kLayer, __func__,
-      RowArgs{x, R, H, (const f16*)gamma, (const f16*)beta, (int8_t*)q, scale, ldx, ldr, ldh, ldq, rows, K, eps},
+      RowArgs{x, R, H, (const f16*)gamma, (const f16*)beta, (int8_t*)q, scale, ldx, ldr, ldh, ldq, rows, K, eps, 1.0f / (float)K},
       (hipStream_t)stream);
 }
 
@@ -530,7 +610,7 @@ int dlm_layer_norm_q8_f32(const float* x, int ldx, const float* R, int ldr, floa
   if (rows <= 0 || K <= 0) return DLM_OK;
   return row_entry<float>(
       kLayer, __func__,
-      RowArgs{x, R, H, (const f16*)gamma, (const f16*)beta, (int8_t*)q, scale, ldx, ldr, ldh, ldq, rows, K, eps},
+      RowArgs{x, R, H, (const f16*)gamma, (const f16*)beta, (int8_t*)q, scale, ldx, ldr, ldh, ldq, rows, K, eps, 1.0f / (float)K},
       (hipStream_t)stream);
 }
 

@@ -181,6 +181,47 @@ def test_rms_norm_q8(gpu, K, residual, gamma, dtype):
     assert float(res[1][3]) == 0.0
 
 
+def test_norms_of_zero_rows_without_eps(gpu):
+    """0 / 0 is not formed: a row of zeros has scale 0 whatever eps is (RMS); of
+    equal values, a LayerNorm with eps > 0 has beta alone."""
+    announce("norms of rows without spread")
+    for K in (3, 64, 640, 1300, 5000, 17000):
+        z = torch.zeros(3, K, dtype=torch.float16, device="cuda")
+        q, s = ops.rms_norm_q8(z, eps=0.0)
+        assert (q == 0).all() and (s == 0).all()
+        b = cpu((K,), 3).cuda()
+        q, s = ops.layer_norm_q8(z + 5, None, b)
+        ref, rs = ops.quantize_rows(b[None].expand(3, K).contiguous())
+        assert torch.equal(q, ref) and torch.equal(s, rs)
+
+
+@pytest.mark.parametrize("rows,K", [(2048, 1100), (2050, 1283), (2048, 1536), (2049, 1800), (3000, 2048)])
+def test_layer_norm_q8_of_many_rows(gpu, rows, K):
+    """The kernel that many fp16 rows of 1025 to 2048 values take."""
+    announce(f"layer_norm_q8 {rows}x{K}")
+    x, g, b = spread(rows, K, K), cpu((K,), 3) * 0.3 + 1, cpu((K,), 4) * 0.2
+    whole, out = gpu_rows(rows, K, torch.int8)
+    q, s = ops.layer_norm_q8(x.cuda(), g.cuda(), b.cuda(), out=out)
+    assert untouched(whole, rows, K)
+    hd = x.double()
+    v = Q.layer_norm(hd, g.double(), b.double(), 1e-5)
+    check_rows(q.cpu(), s.cpu(), v, layer_error(hd, v, g, K, 1e-5), f"layer_norm {rows}x{K}")
+
+
+def layer_error(hd, v, g, K, eps):
+    """Per row, how far fp32 arithmetic may leave a LayerNorm's values from v.  The
+    mean is off by its sum's roundings of mean |h| at most, and shifts every value
+    by as much; the root's relative error as in the RMS norm; difference, product,
+    affine and its rounding: 4 more."""
+    gmax = 1.0 if g is None else float(g.double().abs().max())
+    d = hd - hd.mean(1, keepdim=True)
+    rs = 1.0 / torch.sqrt((d * d).mean(1) + eps)
+    n = sum_steps(K)
+    shift = U * (n + 3) * hd.abs().mean(1)
+    rel = U * (0.5 * (n + 5) + 7) + 0.5 * (shift * rs) ** 2
+    return gmax * rs * (shift + d.abs().amax(1) * rel + U * hd.abs().amax(1)) + U * v.abs().amax(1)
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 @pytest.mark.parametrize("residual,affine", [(False, False), (False, True), (True, True)])
 @pytest.mark.parametrize("K", WIDTHS)
