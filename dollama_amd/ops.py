@@ -730,11 +730,15 @@ _INT_MAX = 0x7fffffff
 def _rows(t: torch.Tensor, rows: int, K: int, name: str, dtypes, dev: int) -> int:
     """Row stride of t, which has to be [rows, K] of one of `dtypes` on device `dev`."""
     if t.dtype in dtypes and t.shape == (rows, K) and t.get_device() == dev:
-        ld, step = t.stride()
-        if rows <= 1:  # a single row's stride says nothing
-            ld = max(K, min(ld, _INT_MAX))
-        if (step == 1 or K == 1) and 1 <= K <= ld <= _INT_MAX and rows <= _INT_MAX:
-            return ld
+        if t.is_contiguous():
+            if 0 < K <= _INT_MAX and rows <= _INT_MAX:
+                return K
+        else:
+            ld, step = t.stride()
+            if rows <= 1:  # a single row's stride says nothing
+                ld = max(K, min(ld, _INT_MAX))
+            if (step == 1 or K == 1) and 1 <= K <= ld <= _INT_MAX and rows <= _INT_MAX:
+                return ld
     if t.dtype not in dtypes:
         raise ValueError(f"{name} must be {' or '.join(map(str, dtypes))}, got {t.dtype}")
     if t.shape != (rows, K):
@@ -759,10 +763,15 @@ def _vector(t: torch.Tensor, numel: int, name: str, dtype, dev: int) -> int:
 
 def _here(t: torch.Tensor, name: str) -> int:
     """The current device, whose current stream a call runs on; t has to be a matrix on it."""
-    dev = torch._C._cuda_getDevice() if t.is_cuda else -1
-    if t.dim() != 2 or dev != t.get_device() or dev < 0:
+    dev = t.get_device()
+    if dev < 0 or t.dim() != 2 or dev != torch._C._cuda_getDevice():
         raise ValueError(f"{name} must be a 2-D tensor on the current GPU")
     return dev
+
+
+def _stream_of(dev: int) -> int:
+    """Handle of a device's current stream."""
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _q8_out(rows: int, K: int, out, scale, like):
@@ -789,7 +798,7 @@ def quantize_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None,
     ldq = _rows(out, rows, K, "out", _INT8, dev)
     ps = _vector(scale, rows, "scale", torch.float32, dev)
     call("dlm_quantize_rows_fp16" if x.dtype == torch.float16 else "dlm_quantize_rows_f32", x.data_ptr(), ldx,
-         out.data_ptr(), ldq, ps, rows, K, _stream())
+         out.data_ptr(), ldq, ps, rows, K, _stream_of(dev))
     return out, scale
 
 
@@ -806,7 +815,7 @@ def dequantize_rows(q: torch.Tensor, scale: torch.Tensor, dtype=torch.float16,
         out = torch.empty(rows, K, dtype=dtype, device=q.device)
     ldy = _rows(out, rows, K, "out", _STREAM_TYPES, dev)
     call("dlm_dequantize_rows_fp16" if out.dtype == torch.float16 else "dlm_dequantize_rows_f32", q.data_ptr(), ldq,
-         ps, out.data_ptr(), ldy, rows, K, _stream())
+         ps, out.data_ptr(), ldy, rows, K, _stream_of(dev))
     return out
 
 
@@ -830,7 +839,7 @@ def _norm_q8(f16_entry, f32_entry, x, affine, residual, eps, sum_out, out, scale
     ldq = _rows(out, rows, K, "out", _INT8, dev)
     ps = _vector(scale, rows, "scale", torch.float32, dev)
     call(f16_entry if x.dtype == torch.float16 else f32_entry, x.data_ptr(), ldx, pr, ldr, ph, ldh, *pa,
-         out.data_ptr(), ldq, ps, rows, K, float(eps), _stream())
+         out.data_ptr(), ldq, ps, rows, K, float(eps), _stream_of(dev))
     return (out, scale) if residual is None else (out, scale, sum_out)
 
 
@@ -897,5 +906,5 @@ def linear_q8(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.Te
     if residual is not None:
         ldr, pr = _rows(residual, M, ncols, "residual", (out.dtype,), dev), residual.data_ptr()
     call("dlm_linear_q8_fp16" if out.dtype == torch.float16 else "dlm_linear_q8_f32out", xq.data_ptr(), ldx, psx,
-         wq.data_ptr(), ldw, psw, pb, pr, ldr, out.data_ptr(), ldy, M, N, K, float(beta), int(act), _stream())
+         wq.data_ptr(), ldw, psw, pb, pr, ldr, out.data_ptr(), ldy, M, N, K, float(beta), int(act), _stream_of(dev))
     return out
