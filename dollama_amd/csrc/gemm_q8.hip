@@ -340,14 +340,16 @@ q8_tile_kernel(Q8Gemm p, int tiles_m, int tiles_n) {
     if (IB * NW == GB || i + 1 < IB || wave < GB - (IB - 1) * NW)
       dma16(bl.rs, st + SA + (i * NW + wave) * 1024, bl.voff[i], bl.soff);
   };
+  if (ke > 0) {  // K < 16 has no slice
 #pragma unroll
-  for (int s = 0; s < NS - 1; ++s) {
-    al.prepare(min(s, ke - 1) * KG + kg);
-    bl.prepare(min(s, ke - 1) * KG + kg);
+    for (int s = 0; s < NS - 1; ++s) {
+      al.prepare(min(s, ke - 1) * KG + kg);
+      bl.prepare(min(s, ke - 1) * KG + kg);
 #pragma unroll
-    for (int i = 0; i < IA; ++i) dma_a(smem + s * STAGE, i);
+      for (int i = 0; i < IA; ++i) dma_a(smem + s * STAGE, i);
 #pragma unroll
-    for (int i = 0; i < IB; ++i) dma_b(smem + s * STAGE, i);
+      for (int i = 0; i < IB; ++i) dma_b(smem + s * STAGE, i);
+    }
   }
   // DMA instructions a slice that this wave leaves to others (0..2): its wait
   // for a slice allows P later slices of its own requests

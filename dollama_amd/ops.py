@@ -867,7 +867,7 @@ def _q8_operand(t: torch.Tensor, rows: int, K: int, name: str, dev: int) -> int:
     """Row stride of an int8 operand of the product: whole 16-byte vectors of every row."""
     ld = _rows(t, rows, K, name, _INT8, dev)
     k16 = (K + 15) // 16 * 16
-    if rows == 1:
+    if rows <= 1:
         ld = k16
     if ld < k16 or ld % 16 or t.data_ptr() % 16:
         raise ValueError(f"{name} needs 16-byte aligned rows: make it with quantize_rows or a norm")

@@ -536,3 +536,7 @@ def test_refusals(gpu):
     # no rows: empty results
     assert ops.linear_q8(q[:0], s[:0], w, sw).shape == (0, 32)
     assert ops.rms_norm_q8(x[:0], g)[0].shape == (0, 64)
+    q63, s63 = ops.quantize_rows(x[:, :63])
+    w63, sw63 = ops.quantize_rows(cpu((32, 63), 2).cuda())
+    assert ops.linear_q8(q63[:0], s63[:0], w63, sw63).shape == (0, 32)
+    assert ops.linear_q8(q63, s63, w63[:0], sw63[:0]).shape == (4, 0)
