@@ -124,18 +124,21 @@ struct Epilogue {
   static_assert(FIT >= 1, "a block's rows do not fit");
   static constexpr int CI = TM % 4 == 0 && FIT >= 4 ? 4 : TM % 2 == 0 && FIT >= 2 ? 2 : 1;
   static constexpr int V = 16 / sizeof(T), VR = WN / V, N_IT = (16 * CI * VR + 63) / 64;
-  static constexpr bool EARLY = TM * TN <= 8, EARLY_RES = TM * TN <= 4 && CI == TM;
+  static constexpr bool EARLY = TM * TN <= 8, EARLY_RES = TM * TN <= 4;
   typedef T VecT __attribute__((ext_vector_type(V)));
   const Q8Gemm& p;
   int m0, n0, lane;
   f32x4 cs[TN];
   f16x4 cb[TN];
   float sx[TM];
-  VecT rv[N_IT];
+  // a residual without an activation is requested ahead of the exchange, unless
+  // the accumulators leave no room (the 192x128 tile)
+  static constexpr bool AHEAD = TM * TN <= 10 || TM == CI;
+  VecT rv[AHEAD ? TM / CI : 1][N_IT];
 
   __device__ Epilogue(const Q8Gemm& p_, int m0_, int n0_, int lane_) : p(p_), m0(m0_), n0(n0_), lane(lane_) {
     if (EARLY) scales();
-    if (EARLY_RES) residual(0);
+    if (EARLY_RES) residual();
   }
   __device__ __forceinline__ void scales() {
 #pragma unroll
@@ -173,13 +176,17 @@ struct Epilogue {
     }
     return r;
   }
-  __device__ __forceinline__ void residual(int c) {
-    if (!p.res || p.act != DLM_ACT_NONE) return;
-    const bool whole = n0 + WN <= p.N;
+  __device__ __forceinline__ void residual() {
+    if constexpr (AHEAD) {
+      if (!p.res || p.act != DLM_ACT_NONE) return;
+      const bool whole = n0 + WN <= p.N;
 #pragma unroll
-    for (int it = 0; it < N_IT; ++it) {
-      const int idx = it * 64 + lane;
-      rv[it] = get_res(m0 + 16 * CI * c + idx / VR, n0 + idx % VR * V, p.N, whole);
+      for (int c = 0; c < TM / CI; ++c)
+#pragma unroll
+        for (int it = 0; it < N_IT; ++it) {
+          const int idx = it * 64 + lane;
+          rv[c][it] = get_res(m0 + 16 * CI * c + idx / VR, n0 + idx % VR * V, p.N, whole);
+        }
     }
   }
   // Stores a finished vector, columns col .. col + V - 1 of a row.
@@ -194,13 +201,53 @@ struct Epilogue {
         if (col + t < cols) y[t] = o[t];
     }
   }
+  // fp16 outputs with neither activation nor residual are rounded ahead of the
+  // exchange: half the bytes (2048x10240x1280 38.9 -> 36.4 us; GEGLU, whose
+  // outputs are half as many, gains nothing by being finished there).
+  __device__ __forceinline__ void finish_narrow(const i32x4 (&acc)[TM][TN], f16 DLM_LDS* st) {
+    constexpr int LDH = WN + 8, FITH = BYTES / (16 * LDH * 2);
+    constexpr int CH = TM % 4 == 0 && FITH >= 4 ? 4 : TM % 3 == 0 && FITH >= 3 ? 3 : TM % 2 == 0 && FITH >= 2 ? 2 : 1;
+    constexpr int ITH = (16 * CH * VR + 63) / 64;
+#pragma unroll
+    for (int c = 0; c < TM / CH; ++c) {
+#pragma unroll
+      for (int ii = 0; ii < CH; ++ii)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+          const i32x4& a = acc[c * CH + ii][j];
+          f16x4 o;
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            o[t] = (f16)__builtin_fmaf((float)a[t] * cs[j][t], sx[c * CH + ii], (float)cb[j][t]);
+          *reinterpret_cast<f16x4 DLM_LDS*>(st + (ii * 16 + (lane & 15)) * LDH + j * 16 + 4 * (lane >> 4)) = o;
+        }
+      __builtin_amdgcn_wave_barrier();
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int it = 0; it < ITH; ++it) {
+        const int idx = it * 64 + lane, r = idx / VR, col = idx % VR * V;
+        if ((16 * CH * VR) % 64 && idx >= 16 * CH * VR) break;
+        const VecT o = *reinterpret_cast<const VecT DLM_LDS*>(st + r * LDH + col);
+        put(m0 + 16 * CH * c + r, n0 + col, p.N, o);
+      }
+      __builtin_amdgcn_wave_barrier();
+      asm volatile("" ::: "memory");
+    }
+  }
   __device__ __forceinline__ void finish(const i32x4 (&acc)[TM][TN], float DLM_LDS* st) {
     const int l15 = lane & 15, c4 = 4 * (lane >> 4);
+    if (!EARLY_RES) residual();
+    if constexpr (sizeof(T) == 2) {
+      if (!p.res && p.act == DLM_ACT_NONE) {
+        if (!EARLY) scales();
+        finish_narrow(acc, (f16 DLM_LDS*)st);
+        return;
+      }
+    }
     if (!EARLY) scales();
 #pragma unroll
     for (int c = 0; c < TM / CI; ++c) {
       const int r0 = m0 + 16 * CI * c;
-      if (!EARLY_RES) residual(c);
 #pragma unroll
       for (int ii = 0; ii < CI; ++ii)
 #pragma unroll
@@ -220,13 +267,17 @@ struct Epilogue {
         for (int it = 0; it < N_IT; ++it) {
           const int idx = it * 64 + lane, r = idx / VR, col = idx % VR * V;
           if ((16 * CI * VR) % 64 && idx >= 16 * CI * VR) break;
-          VecT o;
+          VecT o, rg = {};
+          if constexpr (AHEAD)
+            rg = rv[c][it];
+          else if (p.res)
+            rg = get_res(r0 + r, n0 + col, p.N, n0 + WN <= p.N);
 #pragma unroll
           for (int u = 0; u < V / 4; ++u) {
             const f32x4 v = *reinterpret_cast<const f32x4 DLM_LDS*>(st + r * LD + col + 4 * u);
 #pragma unroll
             for (int t = 0; t < 4; ++t)
-              o[4 * u + t] = (T)(p.res ? __builtin_fmaf(p.beta, (float)rv[it][4 * u + t], v[t]) : v[t]);
+              o[4 * u + t] = (T)(p.res ? __builtin_fmaf(p.beta, (float)rg[4 * u + t], v[t]) : v[t]);
           }
           put(r0 + r, n0 + col, p.N, o);
         }
@@ -516,41 +567,46 @@ void launch_tile(const Q8Gemm& p, hipStream_t s) {
 thread_local int g_q8_tile = 0;
 
 // A launch's time is modelled as
-//   base + (fix + slices * slice) * (1 + more * (ceil(grid / 256) - 1))   [us]
-// grid: output tiles, slices: of 128 bytes of K, more: what each further
-// workgroup on a CU adds, relative to the first (over 1 where it queues for
-// the LDS).  The constants are fits to the launches of 503 shapes (1-8192 rows,
-// 16-12000 columns, K = 64-8192), graph-replayed; the modelled choice takes
-// 0.3% longer than the fastest of the eleven in the mean and 12% at worst
-// (829x1184x224, 4.6 us against 4.2).  Split K for few rows (us, without and
-// with K groups): 1x4096x4096 6.8 -> 5.9, 13x1280x5120 9.2 -> 6.2, 1x2560x8192
-// 12.5 -> 6.9.
+//   base + (fix + slices * slice) * (1 + more * (n - 1)) + io * words * n   [us]
+// n: output tiles a CU, rounded up; slices: of 128 bytes of K; more: what each
+// further workgroup on a CU adds, relative to the first (over 1 where it queues
+// for the LDS); words: 2-byte words that an output moves beyond the first (fp32,
+// a residual).  The constants are fits to 8200 launches of 1068 shapes (1-8192
+// rows, 16-12000 columns, K = 64-8192), graph-replayed; the modelled choice
+// takes 0.9% longer than the fastest of the twelve in the mean, and up to 30%
+// where rows are not 16-byte aligned (6957x96x176 with residual 5.2 us against
+// 4.0).  Split K for few rows (us, without and with K groups): 1x4096x4096 6.8 ->
+// 5.9, 13x1280x5120 9.2 -> 6.2, 1x2560x8192 12.5 -> 6.9.
 struct Q8Tile {
   int bm, bn;
-  float base, fix, slice, more;
+  float base, fix, slice, io, more;
 };
 constexpr Q8Tile kQ8Tiles[] = {
-    {16, 32, 1.91f, 1.53f, 0.064f, 1.30f},    // 1: four K groups
-    {16, 32, 2.48f, 0.49f, 0.095f, 0.77f},    // 2: two K groups
-    {32, 32, 2.29f, 0.61f, 0.149f, 0.68f},    // 3
-    {32, 32, 2.24f, 1.13f, 0.101f, 0.88f},    // 4: two K groups
-    {64, 32, 2.45f, 0.66f, 0.169f, 0.93f},    // 5
-    {64, 64, 2.23f, 1.42f, 0.216f, 0.88f},    // 6
-    {64, 128, 1.80f, 2.16f, 0.289f, 1.21f},   // 7
-    {128, 128, 1.50f, 3.85f, 0.467f, 1.09f},  // 8: four stages, one workgroup a CU
-    {128, 128, 1.50f, 2.84f, 0.796f, 0.64f},  // 9: two stages, two workgroups
-    {192, 128, 1.50f, 4.01f, 0.939f, 0.66f},  // 10: the same
-    {128, 256, 1.50f, 5.62f, 0.690f, 1.21f},  // 11: ping-pong
+    {16, 32, 1.91f, 1.48f, 0.065f, 0.08f, 1.26f},    // 1: four K groups
+    {16, 32, 2.29f, 0.59f, 0.099f, 0.06f, 0.67f},    // 2: two K groups
+    {32, 32, 2.17f, 0.66f, 0.149f, 0.05f, 0.64f},    // 3
+    {32, 32, 2.13f, 1.14f, 0.101f, 0.07f, 0.87f},    // 4: two K groups
+    {64, 32, 2.29f, 0.75f, 0.167f, 0.16f, 0.83f},    // 5
+    {64, 64, 2.38f, 1.27f, 0.207f, 0.33f, 0.92f},    // 6
+    {64, 128, 1.50f, 2.45f, 0.286f, 0.35f, 1.14f},   // 7
+    {128, 128, 1.50f, 3.61f, 0.458f, 0.73f, 1.11f},  // 8: four stages, one workgroup a CU
+    {128, 128, 1.50f, 2.81f, 0.799f, 0.74f, 0.64f},  // 9: two stages, two workgroups
+    {192, 128, 1.50f, 3.72f, 0.909f, 2.31f, 0.66f},  // 10: the same
+    {128, 256, 1.50f, 5.84f, 0.640f, 1.41f, 1.30f},  // 11: ping-pong
+    {128, 80, 2.97f, 2.32f, 0.417f, 1.03f, 0.77f},   // 12: four waves, two workgroups
 };
 
+template <class T>
 int plan_q8(const Q8Gemm& p) {
-  const int slices = (p.K + kSlice - 1) / kSlice;
+  const float slices = (float)((p.K + kSlice - 1) / kSlice);
+  const float words = (float)(sizeof(T) / 2 * (p.res ? 2 : 1) - 1);
   int best = 1;
   float best_us = 3e38f;
   for (const Q8Tile& t : kQ8Tiles) {
     const long long grid = (long long)((p.M + t.bm - 1) / t.bm) * ((p.N + t.bn - 1) / t.bn);
+    const float n = (float)((grid + 255) / 256);
     const float us =
-        t.base + (t.fix + (float)slices * t.slice) * (1.0f + t.more * (float)((grid + 255) / 256 - 1));
+        t.base + (t.fix + slices * t.slice) * (1.0f + t.more * (n - 1.0f)) + t.io * words * n;
     if (us < best_us) {
       best_us = us;
       best = (int)(&t - kQ8Tiles) + 1;
@@ -561,7 +617,7 @@ int plan_q8(const Q8Gemm& p) {
 
 template <class T>
 void q8_gemm(const Q8Gemm& p, hipStream_t s) {
-  switch (g_q8_tile > 0 ? g_q8_tile : plan_q8(p)) {
+  switch (g_q8_tile > 0 ? g_q8_tile : plan_q8<T>(p)) {
     case 1: return launch_tile<T, 16, 32, 16, 16, 4, kPlain, 4>(p, s);
     case 2: return launch_tile<T, 16, 32, 16, 16, 3, kPlain, 2>(p, s);
     case 3: return launch_tile<T, 32, 32, 16, 16, 4, kPlain>(p, s);
@@ -572,6 +628,7 @@ void q8_gemm(const Q8Gemm& p, hipStream_t s) {
     case 8: return launch_tile<T, 128, 128, 64, 32, 4, kPlain>(p, s);
     case 9: return launch_tile<T, 128, 128, 64, 32, 2, kPlain>(p, s);
     case 10: return launch_tile<T, 192, 128, 48, 64, 2, kPlain>(p, s);
+    case 12: return launch_tile<T, 128, 80, 32, 80, 3, kPlain>(p, s);
     default: return launch_tile<T, 128, 256, 64, 64, 3, kPingPong>(p, s);
   }
 }

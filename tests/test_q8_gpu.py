@@ -342,7 +342,7 @@ def test_linear_q8_activations(gpu, M, N, K, act, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
-@pytest.mark.parametrize("tile", range(1, 12))
+@pytest.mark.parametrize("tile", range(1, 13))
 def test_linear_q8_every_kernel(gpu, tile, dtype):
     """Every kernel and tile the plan chooses among (dlm_q8_force_tile), on shapes
     with ragged last tiles in both directions, K from less than a slice to more
