@@ -63,7 +63,7 @@ constexpr int kOOB = (int)0x80000000;      // any offset past the buffer reads 0
 constexpr int kPlain = 0, kPingPong = 1;   // main-loop schedules
 
 // DMA of one operand's tile: the lane's byte offsets, and the slice's.
-// K is a multiple of 16 here.
+// K is rounded up to a multiple of 16 here (rows have that room).
 template <int I>
 struct Q8Rows {
   i32x4 rs;
@@ -342,8 +342,6 @@ constexpr int waves_per_simd(int lds, int waves) { return (lds <= 80 * 1024 ? 2 
 // KG > 1 (few rows, where a grid of one workgroup a tile would leave most of
 // the chip waiting for one workgroup's slices): KG groups of waves take the
 // slices in turn, each with a ring of its own, and add their sums up in LDS.
-// The last 1 to 15 values of a K that is no multiple of 16 follow the loop:
-// one MFMA a block on fragments from memory, with what lies past K zeroed.
 template <class T, int BM, int BN, int WM, int WN, int NS, int SCH, int KG>
 __global__ void __launch_bounds__((BM / WM) * (BN / WN) * KG * 64,
                                   waves_per_simd(KG* NS* (BM + BN) * kSlice, (BM / WM) * (BN / WN) * KG))
@@ -369,7 +367,7 @@ q8_tile_kernel(Q8Gemm p, int tiles_m, int tiles_n) {
   int tmi, tni;
   tile_coords(blockIdx.x, tiles_m, tiles_n, tmi, tni);
   const int m0 = tmi * BM, n0 = tni * BN;
-  const int K16 = p.K & ~15;
+  const int K16 = (p.K + 15) & ~15;
   Q8Rows<IA> al(p.x + (size_t)m0 * p.ldx, p.ldx, min(BM, p.M - m0), K16, NW, wave, lane);
   Q8Rows<IB> bl(p.w + (size_t)n0 * p.ldw, p.ldw, min(BN, p.N - n0), K16, NW, wave, lane);
   constexpr int PART = (KG * NS * STAGE - (KG - 1) * BM * BN * 4) / NW & ~15;
@@ -391,17 +389,32 @@ q8_tile_kernel(Q8Gemm p, int tiles_m, int tiles_n) {
     if (IB * NW == GB || i + 1 < IB || wave < GB - (IB - 1) * NW)
       dma16(bl.rs, st + SA + (i * NW + wave) * 1024, bl.voff[i], bl.soff);
   };
-  if (ke > 0) {  // K < 16 has no slice
 #pragma unroll
-    for (int s = 0; s < NS - 1; ++s) {
-      al.prepare(min(s, ke - 1) * KG + kg);
-      bl.prepare(min(s, ke - 1) * KG + kg);
+  for (int s = 0; s < NS - 1; ++s) {
+    al.prepare(min(s, ke - 1) * KG + kg);
+    bl.prepare(min(s, ke - 1) * KG + kg);
 #pragma unroll
-      for (int i = 0; i < IA; ++i) dma_a(smem + s * STAGE, i);
+    for (int i = 0; i < IA; ++i) dma_a(smem + s * STAGE, i);
 #pragma unroll
-      for (int i = 0; i < IB; ++i) dma_b(smem + s * STAGE, i);
-    }
+    for (int i = 0; i < IB; ++i) dma_b(smem + s * STAGE, i);
   }
+  // The bytes of X past a K that is no multiple of 16 are cleared in LDS, by the
+  // lanes whose DMA brought them, between their wait for the last slice and the
+  // barrier that publishes it (W's then multiply zeros).
+  const int tail = p.K & 15, last = (K16 - 1) / kSlice;
+  auto clear_tail = [&](unsigned char DLM_LDS* st, int slice) {
+    if (tail == 0 || slice != last) return;  // uniform
+    if (al.kc == ((K16 - 16) & (kSlice - 1))) {
+#pragma unroll
+      for (int i = 0; i < IA; ++i) {
+        if (IA * NW == GA || i + 1 < IA || wave < GA - (IA - 1) * NW) {
+          i32x4 DLM_LDS* at = (i32x4 DLM_LDS*)(st + (i * NW + wave) * 1024 + lane * 16);
+          *at = keep_bytes(*at, tail);
+        }
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+  };
   // DMA instructions a slice that this wave leaves to others (0..2): its wait
   // for a slice allows P later slices of its own requests
   const int skips = ((IA * NW == GA || wave < GA - (IA - 1) * NW) ? 0 : 1) +
@@ -438,6 +451,7 @@ q8_tile_kernel(Q8Gemm p, int tiles_m, int tiles_n) {
   if constexpr (SCH == kPingPong) {
     const bool late = wave >= NW / 2;
     DLM_WAIT_SLICES(NS - 2);
+    clear_tail(smem, 0);
     __builtin_amdgcn_s_barrier();
     if (late) __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -458,7 +472,10 @@ q8_tile_kernel(Q8Gemm p, int tiles_m, int tiles_n) {
 #pragma unroll
         for (int i = 0; i < IB; ++i)
           if ((IA + i) % KS == ks) dma_b(nst, i);
-        if (ks == KS - 1) DLM_WAIT_SLICES(NS - 2);  // slice kt + 1
+        if (ks == KS - 1) {
+          DLM_WAIT_SLICES(NS - 2);  // slice kt + 1
+          clear_tail(smem + (slot + 1 == NS ? 0 : slot + 1) * STAGE, kt + 1);
+        }
         __builtin_amdgcn_s_waitcnt(0xC07F);         // lgkmcnt(0)
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
@@ -478,6 +495,7 @@ q8_tile_kernel(Q8Gemm p, int tiles_m, int tiles_n) {
   } else {
     for (int kt = 0; kt < ke; ++kt) {
       DLM_WAIT_SLICES(NS - 2);
+      clear_tail(smem + slot * STAGE, kt * KG + kg);
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
@@ -507,22 +525,6 @@ q8_tile_kernel(Q8Gemm p, int tiles_m, int tiles_n) {
   }
 #undef DLM_WAIT_SLICES
   DLM_WAIT_VM(0);  // no DMA may still be writing this workgroup's LDS at exit
-
-  if ((p.K & 15) && kg == 0) {
-    const bool mine = lane < 16;  // the first 16 values of the k-step
-    i32x4 fa[TM], fb[TN];
-#pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      const size_t r = min(m0 + wm * WM + 16 * i + l15, p.M - 1);
-      fa[i] = keep_bytes(*reinterpret_cast<const i32x4*>(p.x + r * p.ldx + K16), mine ? p.K & 15 : 0);
-    }
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const size_t r = min(n0 + wn * WN + 16 * j + l15, p.N - 1);
-      fb[j] = *reinterpret_cast<const i32x4*>(p.w + r * p.ldw + K16);
-    }
-    mma(fa, fb);
-  }
 
   __syncthreads();  // every wave is done with the ring
   if constexpr (KG > 1) {

@@ -775,9 +775,12 @@ def _stream_of(dev: int) -> int:
 
 
 def _q8_out(rows: int, K: int, out, scale, like):
-    """8-bit rows and scales: the caller's, or new ones whose rows `linear_q8` takes."""
+    """8-bit rows and scales: the caller's, or new ones whose rows `linear_q8` takes.
+    Long rows start on whole lines (at most an eighth more memory): 2048x1280x1296
+    with a residual 12.2 -> 11.0 us against rows that start every 16 bytes."""
     if out is None:
-        out = torch.empty(rows, (K + 15) // 16 * 16, dtype=torch.int8, device=like.device)[:, :K]
+        unit = 128 if K >= 1024 else 16
+        out = torch.empty(rows, (K + unit - 1) // unit * unit, dtype=torch.int8, device=like.device)[:, :K]
     if scale is None:
         scale = torch.empty(rows, dtype=torch.float32, device=like.device)
     return out, scale
@@ -788,8 +791,8 @@ def quantize_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None,
     """(q, scale) of fp16 or fp32 x [rows, K]: int8 q = round(127 x / max|x|) and
     fp32 scale = max|x| / 127 per row.  For activations the rows are tokens, for
     a weight [N, K] its output channels.  A row with an infinity or NaN gets
-    scale NaN.  New q rows start every K-rounded-up-to-16 bytes, as
-    ``linear_q8`` needs them."""
+    scale NaN.  New q is a view of rows that start every K rounded up to 16 bytes
+    (128 from K = 1024 on), as ``linear_q8`` needs them."""
     dev = _here(x, "x")
     rows, K = x.shape
     ldx = _rows(x, rows, K, "x", _STREAM_TYPES, dev)
