@@ -55,6 +55,17 @@ __device__ __forceinline__ float act_f(float v, int act) {
   return v;
 }
 
+// An fp32 result in the output's type.  The compiler may merge a multiply-add and
+// its conversion to fp16 into one instruction that rounds once (v_fma_mixlo_f16),
+// and does so in some instantiations: the same sums then differ by a unit in the
+// last place between tiles, where they lie close to a tie.  Opaque to it, every
+// result is rounded to fp32, then to T.
+template <class T>
+__device__ __forceinline__ T out_cast(float v) {
+  if constexpr (sizeof(T) == 2) asm("" : "+v"(v));
+  return (T)v;
+}
+
 // ---------------------------------------------------------------------------
 // Output tiles of BM x BN, operands through LDS.
 // ---------------------------------------------------------------------------
@@ -82,7 +93,7 @@ struct Q8Rows {
   }
   __device__ __forceinline__ void prepare(int kt) {
     soff = kt * kSlice;
-    if (kt * kSlice + kSlice > K) {  // uniform: the last slice, where it is not a whole one
+    if (kt * kSlice + kSlice > K) {  // uniform: a slice that K ends in or before
 #pragma unroll
       for (int i = 0; i < I; ++i) voff[i] = kt * kSlice + kc < K ? voff[i] : kOOB;
     }
@@ -109,17 +120,21 @@ __device__ __forceinline__ typename Vec4<T>::type load4(const T* p) {
 
 // Epilogue of a wave's TM x TN blocks at (m0, n0).  The blocks hold four columns
 // of a row a lane; stored from there, an instruction covers 32 bytes of each of
-// 16 rows, and the stores take longer than everything else (8192x1920x640:
-// QQ -> QQ us).  So the scaled sums go through the wave's part of the (now
-// free) operand ring, CI blocks' rows at a time, and are finished and stored
-// row by row, 16 bytes a lane.
-// v * sw * sx + bias is formed on the way in; activation, residual and the one
-// rounding to T on the way out.
-// Small wave tiles request the scales, bias and residual ahead of the main loop
-// (request), the others once their accumulators are done with.
+// 16 rows, which makes the stores the longest part of it (8192x1920x640 on
+// 128x128 tiles 25.3 us, through LDS 22.1; 2048x1280x128 with a residual 8.6,
+// 6.3).  So the scaled sums go through the wave's part of the (now free) operand
+// ring, CI blocks' rows at a time, and are finished and stored row by row, 16
+// bytes a lane (the hardware takes them at any alignment: off it they cost 1 us
+// of 14 at 1975x1283, where 4-byte stores cost 8).
+// Every tile forms an output by the same operations in the same order, so that
+// it does not depend on the tile that the shape selects:
+//   v = fma(float(sum) * sw, sx, bias) on the way in,
+//   act(v), fma(beta, R, .), rounding to T on the way out.
+// Small wave tiles request scales, bias and residual ahead of the main loop, the
+// others once their accumulators are done with.
 template <class T, int TM, int TN, int BYTES>
 struct Epilogue {
-  static constexpr int WN = TN * 16, LD = WN + 4;  // rows 4 (2 WN + 1) banks apart: writes touch each bank once
+  static constexpr int WN = TN * 16, LD = WN + 4;  // 16 rows' 16-byte writes touch each bank once
   static constexpr int FIT = BYTES / (16 * LD * 4);
   static_assert(FIT >= 1, "a block's rows do not fit");
   static constexpr int CI = TM % 4 == 0 && FIT >= 4 ? 4 : TM % 2 == 0 && FIT >= 2 ? 2 : 1;
@@ -218,7 +233,7 @@ struct Epilogue {
           f16x4 o;
 #pragma unroll
           for (int t = 0; t < 4; ++t)
-            o[t] = (f16)__builtin_fmaf((float)a[t] * cs[j][t], sx[c * CH + ii], (float)cb[j][t]);
+            o[t] = out_cast<f16>(__builtin_fmaf((float)a[t] * cs[j][t], sx[c * CH + ii], (float)cb[j][t]));
           *reinterpret_cast<f16x4 DLM_LDS*>(st + (ii * 16 + (lane & 15)) * LDH + j * 16 + 4 * (lane >> 4)) = o;
         }
       __builtin_amdgcn_wave_barrier();
@@ -277,7 +292,7 @@ struct Epilogue {
             const f32x4 v = *reinterpret_cast<const f32x4 DLM_LDS*>(st + r * LD + col + 4 * u);
 #pragma unroll
             for (int t = 0; t < 4; ++t)
-              o[4 * u + t] = (T)(p.res ? __builtin_fmaf(p.beta, (float)rg[4 * u + t], v[t]) : v[t]);
+              o[4 * u + t] = out_cast<T>(p.res ? __builtin_fmaf(p.beta, (float)rg[4 * u + t], v[t]) : v[t]);
           }
           put(r0 + r, n0 + col, p.N, o);
         }
@@ -296,7 +311,7 @@ struct Epilogue {
             const f32x4 g = *reinterpret_cast<const f32x4 DLM_LDS*>(q + 4);
 #pragma unroll
             for (int t = 0; t < 4; ++t)
-              o[4 * u + t] = (T)__builtin_fmaf(p.beta, (float)rg[4 * u + t], v[t] * gelu_erf_fast(g[t]));
+              o[4 * u + t] = out_cast<T>(__builtin_fmaf(p.beta, (float)rg[4 * u + t], v[t] * gelu_erf_fast(g[t])));
           }
           put(r0 + r, (n0 >> 1) + col, p.N >> 1, o);
         }
@@ -311,7 +326,7 @@ struct Epilogue {
             const f32x4 v = *reinterpret_cast<const f32x4 DLM_LDS*>(st + r * LD + col + 4 * u);
 #pragma unroll
             for (int t = 0; t < 4; ++t)
-              o[4 * u + t] = (T)__builtin_fmaf(p.beta, (float)rg[4 * u + t], act_f(v[t], p.act));
+              o[4 * u + t] = out_cast<T>(__builtin_fmaf(p.beta, (float)rg[4 * u + t], act_f(v[t], p.act)));
           }
           put(r0 + r, n0 + col, p.N, o);
         }

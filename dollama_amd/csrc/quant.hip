@@ -191,7 +191,10 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) row_q8_kernel(RowArgs p
 #pragma unroll
     for (int j = 0; j < VPT; ++j) h[j] = h[j] + r[j];
   }
-  // sum of f(j, i) over the row's values, each once
+  // sum over the row's values, each once: f(sum, j, i) adds value i of vector j.
+  // A wave that holds the vectors of several (LayerNorms of many rows) adds
+  // them up as those would, so that the sum does not depend on the kernel.
+  constexpr bool APART = TPR == 64 && VPT > 2;
   auto row_sum = [&](auto f, float* lds) {
     float sum = 0.0f;
 #pragma unroll
@@ -200,13 +203,16 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) row_q8_kernel(RowArgs p
       if (ragged) {
         const int skip = (t + TPR * j) * 8 - at[j];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) part += i >= skip ? f(j, i) : 0.0f;
+        for (int i = 0; i < 8; ++i) part = i >= skip ? f(part, j, i) : part;
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) part += f(j, i);
+        for (int i = 0; i < 8; ++i) part = f(part, j, i);
       }
-      sum += t + TPR * j < S ? part : 0.0f;
+      part = t + TPR * j < S ? part : 0.0f;
+      if constexpr (APART) part = row_reduce<TPR>(part, kSum, lds);
+      sum = j == 0 ? part : sum + part;
     }
+    if constexpr (APART) return sum;
     return row_reduce<TPR>(sum, kSum, lds);
   };
   f32x8 y[VPT];
@@ -220,16 +226,17 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) row_q8_kernel(RowArgs p
     for (int j = 0; j < VPT; ++j)
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[j][i] = p.gamma ? (float)h[j][i] * (float)g[j][i] : (float)h[j][i];
-    const float ss = row_sum([&](int j, int i) { return (float)h[j][i] * (float)h[j][i]; }, red[0]);
+    const float ss = row_sum(
+        [&](float s, int j, int i) { return __builtin_fmaf((float)h[j][i], (float)h[j][i], s); }, red[0]);
     bad = !(ss < INFINITY);
     rstd = rsqrtf(ss * p.inv_k + p.eps);
   } else {
-    const float mean = row_sum([&](int j, int i) { return (float)h[j][i]; }, red[0]) / (float)K;
+    const float mean = row_sum([&](float s, int j, int i) { return s + (float)h[j][i]; }, red[0]) / (float)K;
 #pragma unroll
     for (int j = 0; j < VPT; ++j)
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[j][i] = (float)h[j][i] - mean;
-    const float sq = row_sum([&](int j, int i) { return y[j][i] * y[j][i]; }, red[1]);
+    const float sq = row_sum([&](float s, int j, int i) { return __builtin_fmaf(y[j][i], y[j][i], s); }, red[1]);
     bad = !(sq < INFINITY);
     const float rs = rsqrtf(sq * p.inv_k + p.eps);
 #pragma unroll
@@ -321,7 +328,7 @@ __global__ void __launch_bounds__(1024) row_q8_long_kernel(RowArgs p) {
     mean = row_reduce<NT>(sum, kSum, red[0]) / (float)K;
     each([&](const f32x8& v, const f32x8&, const f32x8&, int n, int) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sq += i < n ? (v[i] - mean) * (v[i] - mean) : 0.0f;
+      for (int i = 0; i < 8; ++i) sq = i < n ? __builtin_fmaf(v[i] - mean, v[i] - mean, sq) : sq;
     });
     sq = row_reduce<NT>(sq, kSum, red[1]);
     bad = !(sq < INFINITY);
@@ -335,7 +342,7 @@ __global__ void __launch_bounds__(1024) row_q8_long_kernel(RowArgs p) {
     each([&](const f32x8& v, const f32x8& g, const f32x8& b, int n, int) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        ss += v[i] * v[i];
+        ss = __builtin_fmaf(v[i], v[i], ss);
         top = max_abs(top, value(v[i], g[i], b[i]));  // past n: zeros
       }
     });
@@ -417,7 +424,11 @@ dequant_kernel(const int8_t* __restrict__ q, long long ldq, const float* __restr
     const float s = scale[row];
     T o[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = (T)((float)b[e] * s);
+    for (int e = 0; e < V; ++e) {
+      float v = (float)b[e] * s;
+      asm("" : "+v"(v));  // rounded to fp32 before T, not merged into one instruction
+      o[e] = (T)v;
+    }
     __builtin_memcpy(y + (size_t)row * ldy + at, o, sizeof(o));
   }
 }

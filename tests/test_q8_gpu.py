@@ -399,6 +399,93 @@ def test_linear_q8_row_results_do_not_depend_on_the_batch(gpu):
         assert torch.equal(y, out[lo:lo + n]), f"rows {lo}..{lo + n}"
 
 
+@pytest.mark.parametrize("act,residual,dtype", [("none", False, torch.float16), ("none", True, torch.float16),
+                                                ("geglu", False, torch.float16), ("silu", True, torch.float16),
+                                                ("gelu", False, torch.float32), ("none", True, torch.float32)])
+def test_linear_q8_is_the_same_on_every_tile(gpu, act, residual, dtype):
+    """Four million outputs of each form: among so many, some lie so close to a tie
+    that one rounding more or less shows."""
+    from dollama_amd import _lib
+    announce(f"linear_q8 on every tile: {act} residual={residual} {dtype}")
+    M, N, K = 1024, 4096, 48
+    xg, _ = int8_rows(M, K, 3)
+    wg, _ = int8_rows(N, K, 4)
+    torch.manual_seed(5)
+    sx, sw = torch.rand(M, device="cuda") * 1e-2, torch.rand(N, device="cuda") * 1e-2
+    b = torch.randn(N, device="cuda").half()
+    cols = N // 2 if act == "geglu" else N
+    r = torch.randn(M, cols, device="cuda").to(dtype) if residual else None
+    code = {"none": ops.ACT_NONE, "silu": ops.ACT_SILU, "gelu": ops.ACT_GELU, "geglu": ops.ACT_GEGLU}[act]
+    run = lambda: ops.linear_q8(xg, sx, wg, sw, bias=b, residual=r, act=code, beta=0.7, dtype=dtype)  # noqa: E731
+    ref = run()
+    try:
+        for tile in range(1, 13):
+            _lib.call("dlm_q8_force_tile", tile)
+            assert torch.equal(run(), ref), f"tile {tile}"
+    finally:
+        _lib.call("dlm_q8_force_tile", 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("K", [48, 100, 640, 1031, 1280, 1501, 1536, 1800, 2048, 3000])
+def test_row_results_do_not_depend_on_the_number_of_rows(gpu, K, dtype):
+    announce(f"rows alone and among 4096, K={K} {dtype}")
+    torch.manual_seed(K)
+    x = torch.randn(4096, K, device="cuda").to(dtype) + 3
+    r = torch.randn(4096, K, device="cuda").to(dtype)
+    g, b = torch.randn(K, device="cuda").half(), torch.randn(K, device="cuda").half()
+    for call in (lambda v, w: ops.quantize_rows(v), lambda v, w: ops.rms_norm_q8(v, g, residual=w),
+                 lambda v, w: ops.layer_norm_q8(v, g, b, residual=w)):
+        whole = call(x, r)
+        for lo, n in ((0, 1), (17, 5), (1000, 1100), (0, 2047), (0, 2048)):
+            for a, c in zip(whole, call(x[lo:lo + n], r[lo:lo + n])):
+                assert torch.equal(a[lo:lo + n], c), f"rows {lo}..{lo + n}"
+
+
+# ------------------------------------------------------------- large sizes ---
+def test_rows_past_32_bit_offsets(gpu):
+    """Tensors of more than 2^31 elements, and more rows than one launch takes
+    (2^21): rows at the ends and at the launches' borders equal the same rows alone."""
+    for rows, K, dtype in ((70000, 32768, torch.float16), ((1 << 21) + 77, 24, torch.float32)):
+        announce(f"quantize, norms, dequantize {rows}x{K} {dtype}")
+        torch.manual_seed(K)
+        x = torch.randn(rows, K, device="cuda", dtype=dtype)
+        g = torch.rand(K, device="cuda").half() + 0.5
+        pick = torch.tensor([0, 1, rows // 2, min(rows - 1, (1 << 21) - 1), min(rows - 1, 1 << 21), rows - 2, rows - 1])
+        for name, call in (("quantize", lambda v: ops.quantize_rows(v)), ("rms", lambda v: ops.rms_norm_q8(v, g)),
+                           ("layer", lambda v: ops.layer_norm_q8(v, g, g))):
+            q, s = call(x)
+            q1, s1 = call(x[pick])
+            assert torch.equal(q[pick], q1) and torch.equal(s[pick], s1), name
+        y = ops.dequantize_rows(q, s)
+        assert torch.equal(y[pick], ops.dequantize_rows(q1, s1))
+        del x, y, q, s
+
+
+def test_linear_q8_past_32_bit_offsets(gpu):
+    """Operands and outputs of more than 4 GiB, and more rows than one launch takes."""
+    for M, N, K in ((40000, 60000, 16), (36000, 16, 131071), ((1 << 24) + 300, 16, 16)):
+        announce(f"linear_q8 {M}x{N}x{K}")
+        torch.manual_seed(N)
+        ld = (K + 15) // 16 * 16
+        x = torch.randint(-128, 128, (M, ld), device="cuda", dtype=torch.int8)[:, :K]
+        w = torch.randint(-128, 128, (N, ld), device="cuda", dtype=torch.int8)[:, :K]
+        sx, sw = torch.rand(M, device="cuda") * 1e-3, torch.rand(N, device="cuda") * 1e-2
+        b = torch.randn(N, device="cuda").half()
+        y = ops.linear_q8(x, sx, w, sw, bias=b)
+        pick = torch.tensor([0, M // 2, min(M - 1, (1 << 24) - 1), min(M - 1, 1 << 24), M - 1], device="cuda")
+        rows = x.new_zeros(len(pick), ld)
+        rows[:, :K] = x[pick]
+        assert torch.equal(y[pick], ops.linear_q8(rows[:, :K], sx[pick], w, sw, bias=b))
+        part = slice(max(0, N - 9), N)  # the last columns against float64
+        ref = (rows[:, :K].double().cpu() @ w[part].double().cpu().t()) * sx[pick].double().cpu()[:, None]
+        ref = ref * sw[part].double().cpu() + b[part].double().cpu()
+        mag = ref.abs() + 2 * b[part].double().cpu().abs()
+        off = (y[pick][:, part].cpu().double() - ref).abs()
+        assert bool((off <= 8 * U * mag + 2.0 ** -11 * ref.abs() * 1.001 + 2.0 ** -25).all())
+        del x, w, y
+
+
 # --------------------------------------------------------------- together ---
 class Block:
     """Norm, gated projection, row quantisation, projection back and residual:
