@@ -25,7 +25,7 @@
 // statistics and its output, in 8 to 512 threads by its length.  Measured (graph
 // replays, inputs that no cache holds): quantise 8192x1280 fp16 8.2 us (3.8 TB/s,
 // of which the launch is 2 us), RMS norm with residual 13.5 us (5.4 TB/s; fp32
-// 26.7 us, 5.1), LayerNorm 10.8 us (2.9 TB/s, three reductions in a chain); a 1 GiB
+// 26.7 us, 5.1), LayerNorm 12.5 us (2.5 TB/s, three reductions in a chain); a 1 GiB
 // copy reaches 5.15 TB/s.  One row: 2.3 us, 2.9 and 3.2.
 #include <algorithm>
 
@@ -444,11 +444,11 @@ void launch_rows(const RowArgs& a, hipStream_t s) {
 }
 
 // Threads a row by its length: each holds one to four vectors.  Rows of 1025-2048
-// values take a workgroup (8192x1280 quantise 8.2 us, RMS norm
-// 13.5; with a wave each 8.4 and 13.9, and 2.8 against 3.8 us for 256 rows),
-// but fp16 LayerNorms of many of them a wave: their third reduction weighs more
-// than the latency (8192x1280 13.6 -> 10.8 us, 2048x1280 5.9 -> 5.5; 1024 rows
-// the same either way; fp32 ones are slower with a wave).
+// values take a workgroup (8192x1280 quantise 8.2 us, RMS norm 13.5; with a wave
+// each 8.4 and 13.9, and 2.8 against 3.8 us for 256 rows), but fp16 LayerNorms of
+// many of them a wave, which has no barrier in its three reductions (8192x1280
+// 13.6 -> 12.5 us, 16384x2048 33 -> 26.5; 2048 rows take the same either way, fp32
+// rows are slower with a wave).
 template <class T, RowKind KIND>
 void row_q8(const RowArgs& a, hipStream_t s) {
   const int K = a.K;
@@ -466,7 +466,7 @@ void row_q8(const RowArgs& a, hipStream_t s) {
     launch_rows<T, KIND, 64, 2>(a, s);
   else if (K <= 2048) {
     if constexpr (KIND == kLayer && sizeof(T) == 2) {
-      if (a.rows >= 2048) return K <= 1536 ? launch_rows<T, KIND, 64, 3>(a, s) : launch_rows<T, KIND, 64, 4>(a, s);
+      if (a.rows >= 4096) return K <= 1536 ? launch_rows<T, KIND, 64, 3>(a, s) : launch_rows<T, KIND, 64, 4>(a, s);
     }
     launch_rows<T, KIND, 256, 1>(a, s);
   } else if (K <= 4096)

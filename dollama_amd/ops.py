@@ -774,6 +774,17 @@ def _stream_of(dev: int) -> int:
     return torch._C._cuda_getCurrentRawStream(dev)
 
 
+_entries = {}
+
+
+def _entry(name: str):
+    """The library's entry point `name`, looked up once."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(_lib.hip_lib(), name)
+    return fn
+
+
 def _q8_out(rows: int, K: int, out, scale, like):
     """8-bit rows and scales: the caller's, or new ones whose rows `linear_q8` takes.
     Long rows start on whole lines (at most an eighth more memory): 2048x1280x1296
@@ -800,8 +811,8 @@ def quantize_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None,
         out, scale = _q8_out(rows, K, out, scale, x)
     ldq = _rows(out, rows, K, "out", _INT8, dev)
     ps = _vector(scale, rows, "scale", torch.float32, dev)
-    call("dlm_quantize_rows_fp16" if x.dtype == torch.float16 else "dlm_quantize_rows_f32", x.data_ptr(), ldx,
-         out.data_ptr(), ldq, ps, rows, K, _stream_of(dev))
+    fn = _entry("dlm_quantize_rows_fp16" if x.dtype == torch.float16 else "dlm_quantize_rows_f32")
+    _lib.check(fn(x.data_ptr(), ldx, out.data_ptr(), ldq, ps, rows, K, _stream_of(dev)))
     return out, scale
 
 
@@ -817,16 +828,16 @@ def dequantize_rows(q: torch.Tensor, scale: torch.Tensor, dtype=torch.float16,
             raise ValueError(f"dtype must be float16 or float32, got {dtype}")
         out = torch.empty(rows, K, dtype=dtype, device=q.device)
     ldy = _rows(out, rows, K, "out", _STREAM_TYPES, dev)
-    call("dlm_dequantize_rows_fp16" if out.dtype == torch.float16 else "dlm_dequantize_rows_f32", q.data_ptr(), ldq,
-         ps, out.data_ptr(), ldy, rows, K, _stream_of(dev))
+    fn = _entry("dlm_dequantize_rows_fp16" if out.dtype == torch.float16 else "dlm_dequantize_rows_f32")
+    _lib.check(fn(q.data_ptr(), ldq, ps, out.data_ptr(), ldy, rows, K, _stream_of(dev)))
     return out
 
 
-def _norm_q8(f16_entry, f32_entry, x, affine, residual, eps, sum_out, out, scale):
+def _norm_q8(layer, x, gamma, beta, residual, eps, sum_out, out, scale):
     dev = _here(x, "x")
     rows, K = x.shape
     ldx = _rows(x, rows, K, "x", _STREAM_TYPES, dev)
-    pr = ph = None
+    pr = ph = pb = None
     ldr = ldh = 0
     if residual is not None:
         same = (x.dtype,)
@@ -836,13 +847,20 @@ def _norm_q8(f16_entry, f32_entry, x, affine, residual, eps, sum_out, out, scale
         ldh, ph = _rows(sum_out, rows, K, "sum_out", same, dev), sum_out.data_ptr()
     elif sum_out is not None:
         raise ValueError("sum_out needs a residual")
-    pa = [None if t is None else _vector(t, K, name, torch.float16, dev) for t, name in affine]
+    pg = None if gamma is None else _vector(gamma, K, "gamma", torch.float16, dev)
     if out is None or scale is None:
         out, scale = _q8_out(rows, K, out, scale, x)
     ldq = _rows(out, rows, K, "out", _INT8, dev)
     ps = _vector(scale, rows, "scale", torch.float32, dev)
-    call(f16_entry if x.dtype == torch.float16 else f32_entry, x.data_ptr(), ldx, pr, ldr, ph, ldh, *pa,
-         out.data_ptr(), ldq, ps, rows, K, float(eps), _stream_of(dev))
+    half = x.dtype == torch.float16
+    if layer:
+        pb = None if beta is None else _vector(beta, K, "beta", torch.float16, dev)
+        fn = _entry("dlm_layer_norm_q8_fp16" if half else "dlm_layer_norm_q8_f32")
+        st = fn(x.data_ptr(), ldx, pr, ldr, ph, ldh, pg, pb, out.data_ptr(), ldq, ps, rows, K, eps, _stream_of(dev))
+    else:
+        fn = _entry("dlm_rms_norm_q8_fp16" if half else "dlm_rms_norm_q8_f32")
+        st = fn(x.data_ptr(), ldx, pr, ldr, ph, ldh, pg, out.data_ptr(), ldq, ps, rows, K, eps, _stream_of(dev))
+    _lib.check(st)
     return (out, scale) if residual is None else (out, scale, sum_out)
 
 
@@ -853,8 +871,7 @@ def rms_norm_q8(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, residual:
     h / sqrt(mean(h^2) + eps) * gamma, as ``quantize_rows`` forms them, and h
     too where there is a residual.  x, residual and h are fp16 or fp32; sum_out
     receives h and may be x or residual itself."""
-    return _norm_q8("dlm_rms_norm_q8_fp16", "dlm_rms_norm_q8_f32", x, ((gamma, "gamma"),), residual, eps, sum_out,
-                    out, scale)
+    return _norm_q8(False, x, gamma, None, residual, eps, sum_out, out, scale)
 
 
 def layer_norm_q8(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, beta: Optional[torch.Tensor] = None,
@@ -862,8 +879,7 @@ def layer_norm_q8(x: torch.Tensor, gamma: Optional[torch.Tensor] = None, beta: O
                   sum_out: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
                   scale: Optional[torch.Tensor] = None):
     """``rms_norm_q8`` with a LayerNorm: rows of (h - mean) / sqrt(var + eps) * gamma + beta."""
-    return _norm_q8("dlm_layer_norm_q8_fp16", "dlm_layer_norm_q8_f32", x, ((gamma, "gamma"), (beta, "beta")), residual,
-                    eps, sum_out, out, scale)
+    return _norm_q8(True, x, gamma, beta, residual, eps, sum_out, out, scale)
 
 
 def _q8_operand(t: torch.Tensor, rows: int, K: int, name: str, dev: int) -> int:
@@ -908,6 +924,7 @@ def linear_q8(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.Te
     ldr, pr = 0, None
     if residual is not None:
         ldr, pr = _rows(residual, M, ncols, "residual", (out.dtype,), dev), residual.data_ptr()
-    call("dlm_linear_q8_fp16" if out.dtype == torch.float16 else "dlm_linear_q8_f32out", xq.data_ptr(), ldx, psx,
-         wq.data_ptr(), ldw, psw, pb, pr, ldr, out.data_ptr(), ldy, M, N, K, float(beta), int(act), _stream_of(dev))
+    fn = _entry("dlm_linear_q8_fp16" if out.dtype == torch.float16 else "dlm_linear_q8_f32out")
+    _lib.check(fn(xq.data_ptr(), ldx, psx, wq.data_ptr(), ldw, psw, pb, pr, ldr, out.data_ptr(), ldy, M, N, K, beta,
+                  act, _stream_of(dev)))
     return out

@@ -195,7 +195,7 @@ def test_norms_of_zero_rows_without_eps(gpu):
         assert torch.equal(q, ref) and torch.equal(s, rs)
 
 
-@pytest.mark.parametrize("rows,K", [(2048, 1100), (2050, 1283), (2048, 1536), (2049, 1800), (3000, 2048)])
+@pytest.mark.parametrize("rows,K", [(4096, 1100), (4098, 1283), (4096, 1536), (4097, 1800), (5000, 2048)])
 def test_layer_norm_q8_of_many_rows(gpu, rows, K):
     """The kernel that many fp16 rows of 1025 to 2048 values take."""
     announce(f"layer_norm_q8 {rows}x{K}")
@@ -429,15 +429,15 @@ def test_linear_q8_is_the_same_on_every_tile(gpu, act, residual, dtype):
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 @pytest.mark.parametrize("K", [48, 100, 640, 1031, 1280, 1501, 1536, 1800, 2048, 3000])
 def test_row_results_do_not_depend_on_the_number_of_rows(gpu, K, dtype):
-    announce(f"rows alone and among 4096, K={K} {dtype}")
+    announce(f"rows alone and among 5000, K={K} {dtype}")
     torch.manual_seed(K)
-    x = torch.randn(4096, K, device="cuda").to(dtype) + 3
-    r = torch.randn(4096, K, device="cuda").to(dtype)
+    x = torch.randn(5000, K, device="cuda").to(dtype) + 3
+    r = torch.randn(5000, K, device="cuda").to(dtype)
     g, b = torch.randn(K, device="cuda").half(), torch.randn(K, device="cuda").half()
     for call in (lambda v, w: ops.quantize_rows(v), lambda v, w: ops.rms_norm_q8(v, g, residual=w),
                  lambda v, w: ops.layer_norm_q8(v, g, b, residual=w)):
         whole = call(x, r)
-        for lo, n in ((0, 1), (17, 5), (1000, 1100), (0, 2047), (0, 2048)):
+        for lo, n in ((0, 1), (17, 5), (1000, 1100), (0, 4095), (0, 4096)):
             for a, c in zip(whole, call(x[lo:lo + n], r[lo:lo + n])):
                 assert torch.equal(a[lo:lo + n], c), f"rows {lo}..{lo + n}"
 
