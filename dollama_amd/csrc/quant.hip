@@ -16,10 +16,11 @@
 //
 // Rounding.  127 v / a is formed as v * (127 * rcp(a)) in fp32, which is off by
 // 2.3e-5 at most (relative errors of 2^-23 and 2^-24 on values up to 127).
-// Quotients within 2^-15 of a half (one in 16,000) are decided again by comparing 254 v with (2k + 1) a in fp64, where both
-// products are exact.  So q is the quotient's nearest integer whatever the
-// launch looks like; for fp16 rows (and fp16 gamma) of the first two kinds,
-// where v is exact in fp32, that is the mathematically exact result.
+// Quotients within 2^-15 of a half (one in 16,000) are decided again by comparing
+// 254 v with (2k + 1) a in fp64, where both products are exact.  So q is the
+// quotient's nearest integer whatever the launch looks like; for fp16 rows (and
+// fp16 gamma) of the first two kinds, where v is exact in fp32, that is the
+// mathematically exact result.
 //
 // What bounds them: memory, one pass.  A row stays in registers between its
 // statistics and its output, in 8 to 512 threads by its length.  Measured (graph
