@@ -289,3 +289,26 @@ inline void launch(void (*kernel)(F...), const dim3& grid, const dim3& block, ui
   } while (0)
 
 static inline bool dlm_aligned16(const void* p) { return (((uintptr_t)p) & 15) == 0; }
+
+namespace dlm {
+// An operand's rows in memory, for checks of what a call writes against what it
+// reads.
+struct Span {
+  const char* name;
+  const void* p;  // may be NULL: no operand
+  long long ld;   // elements
+  int rows, cols, elem;
+  uintptr_t lo() const { return (uintptr_t)p; }
+  uintptr_t hi() const { return (uintptr_t)p + ((uintptr_t)(rows - 1) * ld + cols) * elem; }
+};
+// Whether two operands share a byte.  Columns side by side in rows of one stride
+// (slices of a wider tensor) do not; rows of different strides count by their
+// whole extent.
+inline bool overlap(const Span& a, const Span& b) {
+  if (!a.p || !b.p || a.lo() >= b.hi() || b.lo() >= a.hi()) return false;
+  const uintptr_t stride = (uintptr_t)a.ld * a.elem;
+  if (a.rows < 2 || b.rows < 2 || stride != (uintptr_t)b.ld * b.elem) return true;
+  const uintptr_t at = b.lo() >= a.lo() ? (b.lo() - a.lo()) % stride : (stride - (a.lo() - b.lo()) % stride) % stride;
+  return at < (uintptr_t)a.cols * a.elem || at + (uintptr_t)b.cols * b.elem > stride;
+}
+}  // namespace dlm

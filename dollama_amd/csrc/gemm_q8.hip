@@ -675,21 +675,14 @@ int linear_q8(const char* fn, Q8Gemm p, hipStream_t s) {
       (uintptr_t)p.sw % 4)
     return bad("pointer not aligned to its element");
   if (!p.res) p.beta = 0.0f;  // kernels that add beta times nothing stay clear of infinities
-  const uintptr_t y0 = (uintptr_t)p.y, y1 = y0 + ((uintptr_t)(p.M - 1) * p.ldy + cols) * sizeof(T);
-  struct {
-    const char* name;
-    const void* p;
-    uintptr_t bytes;
-  } in[] = {{"X", p.x, (uintptr_t)(p.M - 1) * p.ldx + k16},
-            {"W", p.w, (uintptr_t)(p.N - 1) * p.ldw + k16},
-            {"sx", p.sx, (uintptr_t)p.M * 4},
-            {"sw", p.sw, (uintptr_t)p.N * 4},
-            {"bias", p.bias, (uintptr_t)p.N * 2},
-            {"R", p.res, ((uintptr_t)(p.M - 1) * p.ldr + cols) * sizeof(T)}};
-  for (const auto& i : in) {
-    if (!i.p || (uintptr_t)i.p >= y1 || (uintptr_t)i.p + i.bytes <= y0) continue;
-    if (i.p == p.res && p.res == p.y && p.ldr == p.ldy) continue;  // added in place
-    return bad(std::string("Y overlaps ") + i.name);
+  const int e = (int)sizeof(T);
+  const Span y{"Y", p.y, p.ldy, p.M, cols, e};
+  for (const Span& in : {Span{"X", p.x, p.ldx, p.M, k16, 1}, Span{"W", p.w, p.ldw, p.N, k16, 1},
+                         Span{"sx", p.sx, p.M, 1, p.M, 4}, Span{"sw", p.sw, p.N, 1, p.N, 4},
+                         Span{"bias", p.bias, p.N, 1, p.N, 2}, Span{"R", p.res, p.ldr, p.M, cols, e}}) {
+    if (!overlap(y, in)) continue;
+    if (in.p == p.res && p.res == p.y && p.ldr == p.ldy) continue;  // added in place
+    return bad(std::string("Y overlaps ") + in.name);
   }
   // rows of one launch: at most 2^28 outputs (2^28 threads of the smallest tile)
   const int part = std::max(1 << 8, std::min(1 << 24, (1 << 28) / p.N & ~255));

@@ -504,18 +504,8 @@ int row_parts(RowKind kind, RowArgs a, hipStream_t s) {
 // ---------------------------------------------------------------------------
 // Argument checks shared by the entry points.
 // ---------------------------------------------------------------------------
-// Bytes [p, p + n) of two operands: an output may be an input where it is the
-// same tensor (same address and row stride, elements of one size), and not
-// overlap it otherwise.
-struct Span {
-  const char* name;
-  const void* p;
-  long long ld;
-  int rows, cols, elem;
-  uintptr_t lo() const { return (uintptr_t)p; }
-  uintptr_t hi() const { return (uintptr_t)p + ((uintptr_t)(rows - 1) * ld + cols) * elem; }
-};
-bool overlap(const Span& a, const Span& b) { return a.p && b.p && a.lo() < b.hi() && b.lo() < a.hi(); }
+// An output may be an input where it is the same tensor (same address and row
+// stride, elements of one size), and not overlap it otherwise.
 bool same(const Span& a, const Span& b) { return a.p == b.p && a.ld == b.ld && a.elem == b.elem && a.cols == b.cols; }
 
 template <class T>

@@ -492,7 +492,8 @@ int dlm_linear_small_fp16(const void* X, int ldx, const void* W, const void* bia
  * x [rows, K] with row stride ldx (elements, >= K; any alignment of an
  * element); q has row stride ldq >= K bytes, of which K are written; a stride
  * of K rounded up to 16 on a 16-byte aligned q makes it an operand of
- * dlm_linear_q8_fp16.  Outputs may not overlap inputs.
+ * dlm_linear_q8_fp16.  Outputs may not overlap inputs; columns side by side in
+ * rows of one stride (slices of a wider tensor) do not.
  * No counterpart in the reference, whose transformer is fp16 throughout
  * (src/infer/unet.cu:677-802). */
 int dlm_quantize_rows_fp16(const void* x, int ldx, void* q, int ldq, float* scale, int rows, int K,

@@ -87,6 +87,23 @@ def test_linear_entries_refuse(lib):
         assert call(R=6 * A, ldr=48) == INVALID and "Y overlaps R" in err()
 
 
+def test_interleaved_slices_that_share_a_column_are_refused(lib):
+    for t, e in (("fp16", 2), ("f32", 4)):
+        # rows of 64 columns: x and the sum take 40 each, from column 0 and from 24 or 39
+        for at in (24, 39):
+            st = getattr(lib, f"dlm_rms_norm_q8_{t}")(A, 64, 2 * A, 64, A + at * e, 64, None, 5 * A, 64, 6 * A, 4, 40,
+                                                      1e-5, None)
+            assert st == INVALID and "sum overlaps x" in err()
+            # ... the sum first, and x wrapping into the row after it
+            st = getattr(lib, f"dlm_rms_norm_q8_{t}")(A + at * e, 64, 2 * A, 64, A, 64, None, 5 * A, 64, 6 * A, 4, 40,
+                                                      1e-5, None)
+            assert st == INVALID and "sum overlaps x" in err()
+        f = lib.dlm_linear_q8_fp16 if e == 2 else lib.dlm_linear_q8_f32out
+        for at in (1, 31, 33, 63):
+            assert f(A, 64, 2 * A, 3 * A, 64, 4 * A, None, 6 * A + at * e, 64, 6 * A, 64, 4, 32, 64, 1.0, 0,
+                     None) == INVALID and "Y overlaps R" in err()
+
+
 def test_wrappers_refuse_host_tensors():
     x, s = torch.zeros(4, 64, dtype=torch.float16), torch.ones(4)
     q = torch.zeros(4, 64, dtype=torch.int8)

@@ -281,6 +281,23 @@ def test_norms_write_the_sum_in_place_and_read_strided_rows(gpu):
                 assert torch.equal(q1, q[4:5]) and torch.equal(s1, s[4:5]) and torch.equal(h1, h[4:5])
 
 
+@pytest.mark.parametrize("K", [5, 40, 643, 2052, 17000])
+def test_norms_between_column_slices_of_one_tensor(gpu, K):
+    announce(f"norms: x, residual and sum side by side in the rows of one tensor, K {K}")
+    for dtype in (torch.float16, torch.float32):
+        x, r = spread(9, K, 1, dtype).cuda(), cpu((9, K), 2, dtype).cuda()
+        for norm in (ops.rms_norm_q8, ops.layer_norm_q8):
+            q, s, h = norm(x, residual=r)
+            for order in ((0, 1, 2), (2, 0, 1), (1, 2, 0)):
+                whole = torch.full((9, 3 * K), 77, dtype=dtype, device="cuda")
+                xs, rs, hs = (whole[:, c * K:(c + 1) * K] for c in order)
+                xs.copy_(x)
+                rs.copy_(r)
+                qs, ss, _ = norm(xs, residual=rs, sum_out=hs)
+                assert torch.equal(hs, h) and torch.equal(qs, q) and torch.equal(ss, s)
+                assert torch.equal(xs, x) and torch.equal(rs, r)
+
+
 # ----------------------------------------------------------------- linear ---
 def int8_rows(rows, K, seed, low=-127):
     """Random 8-bit rows at a 16-byte row stride whose padding holds garbage."""
@@ -387,6 +404,19 @@ def test_linear_q8_in_place_residual_and_nan_rows(gpu):
         assert torch.isnan(y[M // 2]).all()
         rest = [i for i in range(M) if i != M // 2]
         assert torch.equal(y[rest], out[rest])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_linear_q8_between_column_slices_of_one_tensor(gpu, dtype):
+    for M, N, K in ((3, 33, 100), (70, 200, 640), (300, 645, 256)):
+        xg, sx, wg, sw, b, r, out = check_linear(M, N, K, dtype=dtype)
+        for first in (0, 1):
+            whole = torch.full((M, 2 * N + 3), 77, dtype=dtype, device="cuda")
+            rs = whole[:, first * N:(first + 1) * N]
+            y = whole[:, (1 - first) * N:(2 - first) * N]
+            rs.copy_(r)
+            ops.linear_q8(xg, sx.cuda(), wg, sw.cuda(), bias=b.cuda(), residual=rs, out=y)
+            assert torch.equal(y, out) and torch.equal(rs, r.cuda()) and (whole[:, 2 * N:] == 77).all()
 
 
 def test_linear_q8_row_results_do_not_depend_on_the_batch(gpu):
