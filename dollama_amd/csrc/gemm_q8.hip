@@ -49,9 +49,26 @@ __device__ __forceinline__ i32x4 keep_bytes(i32x4 v, int n) {
   return v;
 }
 
+// x Phi(x) = max(x, 0) - |x| Q(|x|) with the upper tail Q(z) = erfc(z / sqrt 2) / 2
+// by Abramowitz & Stegun 7.1.26 (its coefficients halved, p and the exponent
+// scaled by 1 / sqrt 2; |error of Q| <= 7.5e-8).  Two VALU instructions fewer than
+// 0.5 x (1 + erf), where they bound the epilogue (GEGLU 2048x10240x1280 39.0 ->
+// 38.4 us), and no cancellation at negative x.  Past 16 the tail is 0 in fp32, so
+// that infinities keep to their limits; NaN stays NaN.
+__device__ __forceinline__ float gelu_tail(float x) {
+  const float z = __builtin_elementwise_minimum(fabsf(x), 16.0f);
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.231641888f, z, 1.0f));
+  float q = __builtin_fmaf(0.5307027145f, t, -0.7265760135f);
+  q = __builtin_fmaf(q, t, 0.7107068705f);
+  q = __builtin_fmaf(q, t, -0.142248368f);
+  q = __builtin_fmaf(q, t, 0.127414796f);
+  q *= t * __builtin_amdgcn_exp2f(z * z * -0.72134752f);
+  return __builtin_fmaf(-z, q, __builtin_elementwise_maximum(x, 0.0f));
+}
+
 __device__ __forceinline__ float act_f(float v, int act) {
   if (act == DLM_ACT_SILU) return silu_f(v);
-  if (act == DLM_ACT_GELU) return gelu_erf_fast(v);
+  if (act == DLM_ACT_GELU) return gelu_tail(v);
   return v;
 }
 
@@ -311,7 +328,7 @@ struct Epilogue {
             const f32x4 g = *reinterpret_cast<const f32x4 DLM_LDS*>(q + 4);
 #pragma unroll
             for (int t = 0; t < 4; ++t)
-              o[4 * u + t] = out_cast<T>(__builtin_fmaf(p.beta, (float)rg[4 * u + t], v[t] * gelu_erf_fast(g[t])));
+              o[4 * u + t] = out_cast<T>(__builtin_fmaf(p.beta, (float)rg[4 * u + t], v[t] * gelu_tail(g[t])));
           }
           put(r0 + r, (n0 >> 1) + col, p.N >> 1, o);
         }

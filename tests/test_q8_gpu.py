@@ -419,6 +419,24 @@ def test_linear_q8_between_column_slices_of_one_tensor(gpu, dtype):
             assert torch.equal(y, out) and torch.equal(rs, r.cuda()) and (whole[:, 2 * N:] == 77).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_linear_q8_activations_of_infinities_and_nan(gpu, dtype):
+    announce(f"linear_q8 activations of infinities and NaN {dtype}")
+    x = torch.ones(5, 64, dtype=torch.int8, device="cuda")
+    w = torch.ones(32, 64, dtype=torch.int8, device="cuda")
+    sx, sw = torch.ones(5, device="cuda"), torch.full((32,), 2.0 ** -6, device="cuda")  # sums of 1
+    b = torch.zeros(32, dtype=torch.float16, device="cuda")
+    b[4], b[5], b[6], b[7] = float("inf"), float("-inf"), float("nan"), -60000.0
+    for act in (ops.ACT_SILU, ops.ACT_GELU):
+        y = ops.linear_q8(x, sx, w, sw, bias=b, act=act, dtype=dtype)
+        assert (y[:, 4] == float("inf")).all() and torch.isnan(y[:, 6]).all() and (y[:, 7] == 0).all()
+        assert torch.isfinite(y[:, :4]).all() and torch.isfinite(y[:, 8:]).all()
+    # GEGLU: columns 4-7 are the gates of outputs 0-3
+    y = ops.linear_q8(x, sx, w, sw, bias=b, act=ops.ACT_GEGLU, dtype=dtype)
+    assert (y[:, 0] == float("inf")).all() and torch.isnan(y[:, 2]).all() and (y[:, 3] == 0).all()
+    assert torch.isfinite(y[:, 4:]).all()
+
+
 def test_linear_q8_row_results_do_not_depend_on_the_batch(gpu):
     announce("linear_q8: a row alone, in small batches and in a large one")
     M, N, K = 700, 640, 1280
