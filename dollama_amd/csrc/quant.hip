@@ -193,11 +193,12 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) row_q8_kernel(RowArgs p
     for (int j = 0; j < VPT; ++j) h[j] = h[j] + r[j];
   }
   // sum over the row's values, each once: f(sum, j, i) adds value i of vector j.
-  // A wave that holds the vectors of several (LayerNorms of many rows) adds
-  // them up as those would, so that the sum does not depend on the kernel.
-  constexpr bool APART = TPR == 64 && VPT > 2;
+  // Threads that hold the vectors of twice or four times as many (LayerNorms of
+  // many rows) add them up as those would, so that the sum does not depend on the
+  // kernel: a wave as a workgroup's waves, half a wave as the halves of a wave.
+  constexpr bool APART = TPR == 64 && VPT > 2, HALVES = TPR == 32 && VPT > 1;
   auto row_sum = [&](auto f, float* lds) {
-    float sum = 0.0f;
+    float sum = 0.0f, odd = 0.0f;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       float part = 0.0f;
@@ -211,9 +212,13 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) row_q8_kernel(RowArgs p
       }
       part = t + TPR * j < S ? part : 0.0f;
       if constexpr (APART) part = row_reduce<TPR>(part, kSum, lds);
-      sum = j == 0 ? part : sum + part;
+      if (HALVES && (j & 1))
+        odd = j == 1 ? part : odd + part;
+      else
+        sum = j == 0 ? part : sum + part;
     }
     if constexpr (APART) return sum;
+    if constexpr (HALVES) return row_reduce<TPR>(sum, kSum, lds) + row_reduce<TPR>(odd, kSum, lds);
     return row_reduce<TPR>(sum, kSum, lds);
   };
   f32x8 y[VPT];
@@ -449,7 +454,10 @@ void launch_rows(const RowArgs& a, hipStream_t s) {
 // each 8.4 and 13.9, and 2.8 against 3.8 us for 256 rows), but fp16 LayerNorms of
 // many of them a wave, which has no barrier in its three reductions (8192x1280
 // 13.6 -> 12.5 us, 16384x2048 33 -> 26.5; 2048 rows take the same either way, fp32
-// rows are slower with a wave).
+// rows are slower with a wave).  Their rows of 513-768 values take half a wave,
+// whose lanes are then all in use, and reduce two rows at a time (8192x640 8.5 ->
+// 7.3 us, 32768x640 22.2 -> 17.7; up to 512 and over 768 values nothing is
+// gained, the other kinds lose 2-6%).
 template <class T, RowKind KIND>
 void row_q8(const RowArgs& a, hipStream_t s) {
   const int K = a.K;
@@ -463,9 +471,12 @@ void row_q8(const RowArgs& a, hipStream_t s) {
     launch_rows<T, KIND, 32, 1>(a, s);
   else if (K <= 512)
     launch_rows<T, KIND, 64, 1>(a, s);
-  else if (K <= 1024)
+  else if (K <= 1024) {
+    if constexpr (KIND == kLayer && sizeof(T) == 2) {
+      if (a.rows >= 4096 && K <= 768) return launch_rows<T, KIND, 32, 3>(a, s);
+    }
     launch_rows<T, KIND, 64, 2>(a, s);
-  else if (K <= 2048) {
+  } else if (K <= 2048) {
     if constexpr (KIND == kLayer && sizeof(T) == 2) {
       if (a.rows >= 4096) return K <= 1536 ? launch_rows<T, KIND, 64, 3>(a, s) : launch_rows<T, KIND, 64, 4>(a, s);
     }

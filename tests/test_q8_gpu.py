@@ -195,9 +195,10 @@ def test_norms_of_zero_rows_without_eps(gpu):
         assert torch.equal(q, ref) and torch.equal(s, rs)
 
 
-@pytest.mark.parametrize("rows,K", [(4096, 1100), (4098, 1283), (4096, 1536), (4097, 1800), (5000, 2048)])
+@pytest.mark.parametrize("rows,K", [(4099, 513), (4096, 640), (4103, 701), (5001, 768), (4096, 1100), (4098, 1283),
+                                    (4096, 1536), (4097, 1800), (5000, 2048)])
 def test_layer_norm_q8_of_many_rows(gpu, rows, K):
-    """The kernel that many fp16 rows of 1025 to 2048 values take."""
+    """The kernels that many fp16 rows of 513 to 768 and of 1025 to 2048 values take."""
     announce(f"layer_norm_q8 {rows}x{K}")
     x, g, b = spread(rows, K, K), cpu((K,), 3) * 0.3 + 1, cpu((K,), 4) * 0.2
     whole, out = gpu_rows(rows, K, torch.int8)
@@ -475,7 +476,7 @@ def test_linear_q8_is_the_same_on_every_tile(gpu, act, residual, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
-@pytest.mark.parametrize("K", [48, 100, 640, 1031, 1280, 1501, 1536, 1800, 2048, 3000])
+@pytest.mark.parametrize("K", [48, 100, 320, 513, 640, 701, 768, 769, 1031, 1280, 1501, 1536, 1800, 2048, 3000])
 def test_row_results_do_not_depend_on_the_number_of_rows(gpu, K, dtype):
     announce(f"rows alone and among 5000, K={K} {dtype}")
     torch.manual_seed(K)
