@@ -26,9 +26,9 @@
 // statistics and its output, in 8 to 512 threads by its length.  Measured (graph
 // replays, inputs that no cache holds): quantise 8192x1280 fp16 8.2 us (3.8 TB/s,
 // of which the launch is 2 us), RMS norm with residual 13.5 us (5.4 TB/s; fp32
-// 26.7 us, 5.1), LayerNorm 12.5 us (2.5 TB/s: some 13 VALU instructions a value
-// and three reductions in a chain; 32768x640 3.6 TB/s); a 1 GiB
-// copy reaches 5.15 TB/s.  One row: 2.3 us, 2.9 and 3.2.
+// 26.7 us, 5.1), LayerNorm 12.5 us (2.5 TB/s: some 15 VALU instructions a value
+// and three reductions in a chain; 32768x640 3.6 TB/s); a 1 GiB copy reaches
+// 5.15 TB/s.  One row: 2.3 us, 2.9 and 3.2.
 #include <algorithm>
 
 #include "common.hpp"
