@@ -605,11 +605,13 @@ thread_local int g_q8_tile = 0;
 // n: output tiles a CU, rounded up; slices: of 128 bytes of K; more: what each
 // further workgroup on a CU adds, relative to the first (over 1 where it queues
 // for the LDS); words: 2-byte words that an output moves beyond the first (fp32,
-// a residual).  The constants are fits to 8200 launches of 1068 shapes (1-8192
+// a residual).  The constants are fits to 9400 launches of 1062 shapes (1-8192
 // rows, 16-12000 columns, K = 64-8192), graph-replayed; the modelled choice
-// takes 0.9% longer than the fastest of the twelve in the mean, and up to 30%
+// takes 0.7% longer than the fastest of the thirteen in the mean, and up to 30%
 // where rows are not 16-byte aligned (6957x96x176 with residual 5.2 us against
-// 4.0).  Split K for few rows (us, without and with K groups): 1x4096x4096 6.8 ->
+// 4.0).  128x160 is there for products whose outputs it cuts into one round
+// of 256 (us, without and with it: 8192x640x2560 22.5 -> 19.1, 4096x1280x5120 with
+// a residual 45.7 -> 35.9, 8192x640x640 10.6 -> 9.6).  Split K for few rows (us, without and with K groups): 1x4096x4096 6.8 ->
 // 5.9, 13x1280x5120 9.2 -> 6.2, 1x2560x8192 12.5 -> 6.9.
 struct Q8Tile {
   int bm, bn;
@@ -625,9 +627,10 @@ constexpr Q8Tile kQ8Tiles[] = {
     {64, 128, 1.50f, 2.45f, 0.286f, 0.35f, 1.14f},   // 7
     {128, 128, 1.50f, 3.61f, 0.458f, 0.73f, 1.11f},  // 8: four stages, one workgroup a CU
     {128, 128, 1.50f, 2.81f, 0.799f, 0.74f, 0.64f},  // 9: two stages, two workgroups
-    {192, 128, 1.50f, 3.72f, 0.909f, 2.31f, 0.66f},  // 10: the same
+    {192, 128, 1.50f, 3.72f, 0.909f, 1.80f, 0.66f},  // 10: the same
     {128, 256, 1.50f, 5.84f, 0.640f, 1.41f, 1.30f},  // 11: ping-pong
     {128, 80, 2.97f, 2.32f, 0.417f, 1.03f, 0.77f},   // 12: four waves, two workgroups
+    {128, 160, 2.20f, 4.37f, 0.566f, 1.40f, 1.14f},  // 13: three stages, one workgroup
 };
 
 template <class T>
@@ -663,6 +666,7 @@ void q8_gemm(const Q8Gemm& p, hipStream_t s) {
     case 9: return launch_tile<T, 128, 128, 64, 32, 2, kPlain>(p, s);
     case 10: return launch_tile<T, 192, 128, 48, 64, 2, kPlain>(p, s);
     case 12: return launch_tile<T, 128, 80, 32, 80, 3, kPlain>(p, s);
+    case 13: return launch_tile<T, 128, 160, 32, 80, 3, kPlain>(p, s);
     default: return launch_tile<T, 128, 256, 64, 64, 3, kPingPong>(p, s);
   }
 }
