@@ -49,7 +49,8 @@ int dlm_gemm_set_variant(int variant);
 /* The same for the 8-bit linears (dlm_linear_q8_*), 0 = automatic: 1 16x32 with
  * four K groups, 2 16x32 with two, 3 32x32, 4 32x32 with two K groups, 5 64x32,
  * 6 64x64, 7 64x128, 8 128x128 (four stages), 9 128x128 (two stages),
- * 10 192x128, 11 128x256 in ping-pong, 12 128x80, 13 128x160. */
+ * 10 192x128, 11 128x256 in ping-pong, 12 128x80, 13 128x160,
+ * 14 64x32 with two K groups. */
 int dlm_q8_force_tile(int tile_id);
 
 /* Counter calibration: `blocks` workgroups of 4 waves, each wave `iters`

@@ -605,14 +605,15 @@ thread_local int g_q8_tile = 0;
 // n: output tiles a CU, rounded up; slices: of 128 bytes of K; more: what each
 // further workgroup on a CU adds, relative to the first (over 1 where it queues
 // for the LDS); words: 2-byte words that an output moves beyond the first (fp32,
-// a residual).  The constants are fits to 9400 launches of 1062 shapes (1-8192
-// rows, 16-12000 columns, K = 64-8192), graph-replayed; the modelled choice
-// takes 0.7% longer than the fastest of the thirteen in the mean, and up to 30%
+// a residual).  The constants are fits to 11200 launches of 1165 shapes (1-8192
+// rows, 16-14336 columns, K = 64-14336), graph-replayed; the modelled choice
+// takes 0.6% longer than the fastest of the fourteen in the mean, and up to 30%
 // where rows are not 16-byte aligned (6957x96x176 with residual 5.2 us against
-// 4.0).  128x160 is there for products whose outputs it cuts into one round
-// of 256 (us, without and with it: 8192x640x2560 22.5 -> 19.1, 4096x1280x5120 with
-// a residual 45.7 -> 35.9, 8192x640x640 10.6 -> 9.6).  Split K for few rows (us, without and with K groups): 1x4096x4096 6.8 ->
-// 5.9, 13x1280x5120 9.2 -> 6.2, 1x2560x8192 12.5 -> 6.9.
+// 4.0).  K groups serve few rows and long K (us, without and with them:
+// 1x4096x4096 6.8 -> 5.9, 13x1280x5120 9.2 -> 6.2, 48x8192x8192 22.8 -> 17.8,
+// 100x4096x14336 31.0 -> 24.3, 256x2048x8192 14.8 -> 12.3), 128x160 the outputs
+// that it cuts into one round of 256 (8192x640x2560 22.5 -> 19.1,
+// 4096x1280x5120 with a residual 45.7 -> 35.9, 8192x640x640 10.6 -> 9.6).
 struct Q8Tile {
   int bm, bn;
   float base, fix, slice, io, more;
@@ -631,6 +632,7 @@ constexpr Q8Tile kQ8Tiles[] = {
     {128, 256, 1.50f, 5.84f, 0.640f, 1.41f, 1.30f},  // 11: ping-pong
     {128, 80, 2.97f, 2.32f, 0.417f, 1.03f, 0.77f},   // 12: four waves, two workgroups
     {128, 160, 2.20f, 4.37f, 0.566f, 1.40f, 1.14f},  // 13: three stages, one workgroup
+    {64, 32, 1.96f, 1.64f, 0.133f, 0.17f, 1.30f},    // 14: two K groups
 };
 
 template <class T>
@@ -667,6 +669,7 @@ void q8_gemm(const Q8Gemm& p, hipStream_t s) {
     case 10: return launch_tile<T, 192, 128, 48, 64, 2, kPlain>(p, s);
     case 12: return launch_tile<T, 128, 80, 32, 80, 3, kPlain>(p, s);
     case 13: return launch_tile<T, 128, 160, 32, 80, 3, kPlain>(p, s);
+    case 14: return launch_tile<T, 64, 32, 32, 16, 4, kPlain, 2>(p, s);
     default: return launch_tile<T, 128, 256, 64, 64, 3, kPingPong>(p, s);
   }
 }

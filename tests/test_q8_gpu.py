@@ -360,7 +360,7 @@ def test_linear_q8_activations(gpu, M, N, K, act, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
-@pytest.mark.parametrize("tile", range(1, 14))
+@pytest.mark.parametrize("tile", range(1, 15))
 def test_linear_q8_every_kernel(gpu, tile, dtype):
     """Every kernel and tile the plan chooses among (dlm_q8_force_tile), on shapes
     with ragged last tiles in both directions, K from less than a slice to more
@@ -468,7 +468,7 @@ def test_linear_q8_is_the_same_on_every_tile(gpu, act, residual, dtype):
     run = lambda: ops.linear_q8(xg, sx, wg, sw, bias=b, residual=r, act=code, beta=0.7, dtype=dtype)  # noqa: E731
     ref = run()
     try:
-        for tile in range(1, 14):
+        for tile in range(1, 15):
             _lib.call("dlm_q8_force_tile", tile)
             assert torch.equal(run(), ref), f"tile {tile}"
     finally:
