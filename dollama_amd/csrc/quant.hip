@@ -20,15 +20,20 @@
 // 254 v with (2k + 1) a in fp64, where both products are exact.  So q is the
 // quotient's nearest integer whatever the launch looks like; for fp16 rows (and
 // fp16 gamma) of the first two kinds, where v is exact in fp32, that is the
-// mathematically exact result.
+// mathematically exact result.  LayerNorm's v is not: statistics and values are
+// fp64 there, and quotients come out to 2^-40 (in fp32 about one integer in a
+// million fell on the other side of a half, 15 in a million where the mean is 40
+// times the spread, and the variance of rows beyond 1e19 or below 1e-19 was lost).
+// fp64 instructions run at fp32's rate here; the values take twice the registers,
+// which many rows notice (8192x1280 11.8 us with fp32, 8192x640 7.3 against 7.7).
 //
 // What bounds them: memory, one pass.  A row stays in registers between its
 // statistics and its output, in 8 to 512 threads by its length.  Measured (graph
 // replays, inputs that no cache holds): quantise 8192x1280 fp16 8.2 us (3.8 TB/s,
 // of which the launch is 2 us), RMS norm with residual 13.5 us (5.4 TB/s; fp32
-// 26.7 us, 5.1), LayerNorm 12.5 us (2.5 TB/s: some 15 VALU instructions a value
-// and three reductions in a chain; 32768x640 3.6 TB/s); a 1 GiB copy reaches
-// 5.15 TB/s.  One row: 2.3 us, 2.9 and 3.2.
+// 26.7 us, 5.1), LayerNorm 13.4 us (2.3 TB/s: some 16 VALU instructions a value
+// and three reductions in a chain; with residual 15.3 us, 4.8 TB/s; fp32 14.9 and
+// 27.5); a 1 GiB copy reaches 5.15 TB/s.  One row: 2.3 us, 2.9 and 3.2.
 #include <algorithm>
 
 #include "common.hpp"
@@ -48,10 +53,18 @@ struct RowArgs {
   float* scale;
   long long ldx, ldr, ldh, ldq;
   int rows, K;
-  float eps, inv_k;
+  float eps;
+  double inv_k;
 };
 
+// What a row's statistics, and its values on their way to q, are held in.
+template <class T, RowKind KIND>
+using Stat = std::conditional_t<KIND == kLayer, double, float>;
+template <class T, RowKind KIND>
+using Wide = std::conditional_t<KIND == kLayer, double, float>;
+
 typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef double f64x8 __attribute__((ext_vector_type(8)));
 template <class T>
 using Vec8 = T __attribute__((ext_vector_type(8)));
 
@@ -71,19 +84,34 @@ __device__ __forceinline__ void store8(T* p, const Vec8<T>& v) {
 // values at a time).
 __device__ __forceinline__ float max_abs(float m, float v) { return __builtin_elementwise_maximum(m, fabsf(v)); }
 __device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+// fp64 has no such instruction: these pass NaN over, and `Top` remembers it.
+__device__ __forceinline__ double max_abs(double m, double v) { return __builtin_fmax(m, __builtin_fabs(v)); }
+__device__ __forceinline__ double max_nan(double a, double b) { return __builtin_fmax(a, b); }
+
+// Running maximum of |v|; infinite or NaN once a value was.
+template <class W>
+struct Top {
+  W top = 0, zero = 0;  // zero: 0 times every value
+  __device__ __forceinline__ void add(W v) {
+    top = max_abs(top, v);
+    if constexpr (sizeof(W) == 8) zero = __builtin_fma(v, 0.0, zero);
+  }
+  __device__ __forceinline__ W get() const { return sizeof(W) == 8 && !(zero == 0) ? (W)INFINITY : top; }
+};
 
 // What a row's values are multiplied by on their way to q.
+template <class W>
 struct RowScale {
-  float r;     // 127 / (a m), 0 for rows without a finite positive maximum
-  float a;     // a m
+  W r;         // 127 / (a m), 0 for rows without a finite positive maximum
+  W a;         // a m
   float m;     // fp32 rows: a power of two that keeps 127 / a and its reciprocal normal numbers; else 1
-  float unit;  // a / 127, NaN for a row that holds an infinity or NaN
+  W unit;      // a / 127, NaN for a row that holds an infinity or NaN
 };
-// a: max |v|, NaN if there is one.  Values of fp16 rows are no smaller than
-// 2^-48 where they are not 0 (LayerNorm's 2^-112).
+// a: max |v|, not finite if a value is not.  Values of fp16 rows are no smaller
+// than 2^-48 where they are not 0.
 template <class T>
-__device__ __forceinline__ RowScale row_scale(float a, bool bad) {
-  RowScale s;
+__device__ __forceinline__ RowScale<float> row_scale(float a, bool bad) {
+  RowScale<float> s;
   bad = bad || !(a < INFINITY);
   s.m = sizeof(T) == 2 ? 1.0f : a < 0x1p-100f ? 0x1p100f : a > 0x1p100f ? 0x1p-100f : 1.0f;
   s.a = a * s.m;
@@ -91,12 +119,36 @@ __device__ __forceinline__ RowScale row_scale(float a, bool bad) {
   s.unit = bad ? __uint_as_float(0x7fc00000u) : a / 127.0f;
   return s;
 }
+// fp64 values, of at least 2^-240 where they are not 0 (2^-149 over the root of
+// the largest eps, times fp16's least gamma).  v_rcp_f64 and one step of Newton's
+// iteration, 1 / a to 2^-48.
+template <class T>
+__device__ __forceinline__ RowScale<double> row_scale(double a, bool bad) {
+  RowScale<double> s;
+  bad = bad || !(a < INFINITY);
+  s.a = a;
+  const double r = __builtin_amdgcn_rcp(a);
+  s.r = bad || a == 0.0 ? 0.0 : 127.0 * __builtin_fma(__builtin_fma(-a, r, 1.0), r, r);
+  const double unit = a * (1.0 / 127.0);
+  s.unit = bad ? __builtin_nan("") : __builtin_fma(__builtin_fma(-unit, 127.0, a), 1.0 / 127.0, unit);
+  return s;
+}
 
 // Eight values to eight bytes.  Adding 1.5 * 2^23 rounds to an integer (ties
 // to even) and leaves it in the low byte.
 constexpr float kRound = 12582912.0f;
+__device__ __forceinline__ u32x2 pack8(const unsigned (&u)[8], bool none) {
+  u32x2 o;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const unsigned lo = __builtin_amdgcn_perm(u[4 * j + 1], u[4 * j], 0x0c0c0400u);
+    const unsigned hi = __builtin_amdgcn_perm(u[4 * j + 3], u[4 * j + 2], 0x04000c0cu);
+    o[j] = none ? 0u : lo | hi;  // zeros, or a row with an infinity or NaN
+  }
+  return o;
+}
 template <class T>
-__device__ __forceinline__ u32x2 quant8(const f32x8& v, const RowScale& s) {
+__device__ __forceinline__ u32x2 quant8(const f32x8& v, const RowScale<float>& s) {
   float far = 0.0f, x[8];
   unsigned u[8];
 #pragma unroll
@@ -119,35 +171,72 @@ __device__ __forceinline__ u32x2 quant8(const f32x8& v, const RowScale& s) {
       }
     }
   }
-  u32x2 o;
+  return pack8(u, s.r == 0.0f);
+}
+// The same from fp64 values, whose quotients come out to 2^-40: adding 1.5 * 2^52
+// leaves the nearest integer.  Quotients that are halves exactly take a maximum of
+// few bits, as rows have whose values are beta's alone; those are decided by the
+// products (of 24 and 8 bits, exact).
+constexpr double kRound64 = 6755399441055744.0;
+template <class T>
+__device__ __forceinline__ u32x2 quant8(const f64x8& v, const RowScale<double>& s) {
+  unsigned u[8];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const unsigned lo = __builtin_amdgcn_perm(u[4 * j + 1], u[4 * j], 0x0c0c0400u);
-    const unsigned hi = __builtin_amdgcn_perm(u[4 * j + 3], u[4 * j + 2], 0x04000c0cu);
-    o[j] = s.r == 0.0f ? 0u : lo | hi;  // zeros, or a row with an infinity or NaN
+  for (int i = 0; i < 8; ++i) u[i] = (unsigned)__double2loint(__builtin_fma(v[i], s.r, kRound64));
+  if ((__double2loint(s.a) & 0x1fffffff) == 0) {  // uniform in a row: the maximum is an fp32 value
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const double n = (double)(int)u[i], d = __builtin_fma(v[i], s.r, -n);
+      if (__builtin_fabs(d) > 0.5 - 0x1p-36) {
+        const double k = d > 0.0 ? n : n - 1.0;  // between k and k + 1
+        const double e = 254.0 * v[i] - (2.0 * k + 1.0) * s.a;
+        u[i] = (unsigned)(int)(e > 0.0 || (e == 0.0 && ((int)k & 1)) ? k + 1.0 : k);
+      }
+    }
   }
-  return o;
+  return pack8(u, s.r == 0.0);
 }
 
 // Reductions over the TPR threads of a row: 8, 16 or 32 lanes of a wave, a wave,
 // or the waves of a workgroup through LDS (`lds`: another part of it for each
 // use).  All lanes have to take part.
-template <int TPR, typename Op>
-__device__ __forceinline__ float row_reduce(float v, Op op, float* lds) {
-  if constexpr (TPR >= 64) {
+template <int TPR, typename V, typename Op>
+__device__ __forceinline__ V row_reduce(V v, Op op, V* lds) {
+  if constexpr (TPR >= 64 && sizeof(V) == 4) {
     v = wave_reduce(v, op);
   } else {
+    // the same steps; of what fp64 has no DPP form, the moves need no old value
+    constexpr int W = sizeof(V) / 4;
     auto dpp = [&](auto ctrl) {
-      v = op(v, __uint_as_float(dpp_u32<decltype(ctrl)::value>(__float_as_uint(v))));
+      unsigned w[W];
+      V o;
+      __builtin_memcpy(w, &v, sizeof(V));
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        w[i] = (unsigned)__builtin_amdgcn_mov_dpp((int)w[i], decltype(ctrl)::value, 0xF, 0xF, true);
+      __builtin_memcpy(&o, w, sizeof(V));
+      v = op(v, o);
+    };
+    auto swap = [&](auto sw) {
+      unsigned w[W], x[W], y[W];
+      V a, b;
+      __builtin_memcpy(w, &v, sizeof(V));
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const auto s = sw(w[i]);
+        x[i] = s[0];
+        y[i] = s[1];
+      }
+      __builtin_memcpy(&a, x, sizeof(V));
+      __builtin_memcpy(&b, y, sizeof(V));
+      v = op(a, b);
     };
     dpp(std::integral_constant<int, kDppXor1>{});
     dpp(std::integral_constant<int, kDppXor2>{});
     dpp(std::integral_constant<int, kDppHalfMirror>{});
     if constexpr (TPR > 8) dpp(std::integral_constant<int, kDppMirror>{});
-    if constexpr (TPR == 32) {
-      const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-      v = op(__uint_as_float(s[0]), __uint_as_float(s[1]));
-    }
+    if constexpr (TPR >= 32) swap([](unsigned u) { return __builtin_amdgcn_permlane16_swap(u, u, false, false); });
+    if constexpr (TPR >= 64) swap([](unsigned u) { return __builtin_amdgcn_permlane32_swap(u, u, false, false); });
   }
   if constexpr (TPR > 64) {
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
@@ -158,8 +247,20 @@ __device__ __forceinline__ float row_reduce(float v, Op op, float* lds) {
   }
   return v;
 }
-constexpr auto kSum = [](float a, float b) { return a + b; };
-constexpr auto kMax = [](float a, float b) { return max_nan(a, b); };
+constexpr auto kSum = [](auto a, auto b) { return a + b; };
+constexpr auto kMax = [](auto a, auto b) { return max_nan(a, b); };
+
+// sum / K: the product with 1 / K and one step of Newton's division, so that the
+// mean of equal values is that value.
+__device__ __forceinline__ double mean_of(double sum, int K, double inv_k) {
+  const double m = sum * inv_k;
+  return __builtin_fma(__builtin_fma(-m, (double)K, sum), inv_k, m);
+}
+// 1 / sqrt(mean of squares + eps)
+__device__ __forceinline__ float root_of(float sq, const RowArgs& p) { return rsqrtf(sq * (float)p.inv_k + p.eps); }
+__device__ __forceinline__ double root_of(double sq, const RowArgs& p) {
+  return rsqrt(__builtin_fma(sq, p.inv_k, (double)p.eps));
+}
 
 // A row in the registers of TPR threads, VPT vectors of eight values each
 // (K >= 8).  Vector j of a thread starts at 8 (thread + TPR j); the row's last
@@ -167,10 +268,15 @@ constexpr auto kMax = [](float a, float b) { return max_nan(a, b); };
 // out and whose results are the same bytes.  All loads are issued before any
 // is used, at addresses inside the row.
 template <class T, RowKind KIND, int TPR, int VPT>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) row_q8_kernel(RowArgs p) {
-  constexpr int ROWS = TPR < 256 ? 256 / TPR : 1;  // of a workgroup
-  __shared__ float red[3][TPR > 64 ? TPR / 64 : 1];
-  const int t = threadIdx.x & (TPR - 1);
+__global__ void __launch_bounds__(TPR < 128 ? 256 : TPR) row_q8_kernel(RowArgs p) {
+  constexpr int ROWS = TPR < 128 ? 256 / TPR : 1;  // of a workgroup
+  typedef Stat<T, KIND> S1;
+  typedef Wide<T, KIND> W;
+  constexpr int WAVES = TPR > 64 ? TPR / 64 : 1;  // of a row
+  constexpr bool APART = KIND == kLayer && (TPR == 64 ? VPT > 2 : TPR == 128), HALVES = TPR == 32 && VPT > 1;
+  __shared__ S1 red[2][WAVES * (APART ? VPT : 1)];
+  __shared__ W red_top[WAVES];
+  const int t = ROWS == 1 ? threadIdx.x : threadIdx.x & (TPR - 1);
   const int row_at = ROWS == 1 ? (int)blockIdx.x : (int)blockIdx.x * ROWS + (int)threadIdx.x / TPR;
   const int row = min(row_at, p.rows - 1);  // lanes past the last row repeat it, and store nothing
   const int K = p.K, S = (K + 7) >> 3;
@@ -185,6 +291,10 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) row_q8_kernel(RowArgs p
     at[j] = min(min(t + TPR * j, S - 1) * 8, K - 8);
     h[j] = load8(x + at[j]);
     if (KIND != kQuant && p.res) r[j] = load8(res + at[j]);
+    if (KIND == kLayer) {
+      g[j] = (f16)1.0f;
+      b[j] = (f16)0.0f;
+    }
     if (KIND != kQuant && p.gamma) g[j] = load8(p.gamma + at[j]);
     if (KIND == kLayer && p.beta) b[j] = load8(p.beta + at[j]);
   }
@@ -194,15 +304,15 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) row_q8_kernel(RowArgs p
     for (int j = 0; j < VPT; ++j) h[j] = h[j] + r[j];
   }
   // sum over the row's values, each once: f(sum, j, i) adds value i of vector j.
-  // Threads that hold the vectors of twice or four times as many (LayerNorms of
+  // Threads that hold the vectors of twice to four times as many (LayerNorms of
   // many rows) add them up as those would, so that the sum does not depend on the
-  // kernel: a wave as a workgroup's waves, half a wave as the halves of a wave.
-  constexpr bool APART = TPR == 64 && VPT > 2, HALVES = TPR == 32 && VPT > 1;
-  auto row_sum = [&](auto f, float* lds) {
-    float sum = 0.0f, odd = 0.0f;
+  // kernel: a wave as several waves, each of which adds 64 vectors in a row, half
+  // a wave as the halves of a wave.
+  auto row_sum = [&](auto f, S1* lds) {
+    S1 sum = 0, odd = 0, parts[VPT];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-      float part = 0.0f;
+      S1 part = 0;
       if (ragged) {
         const int skip = (t + TPR * j) * 8 - at[j];
 #pragma unroll
@@ -211,19 +321,34 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) row_q8_kernel(RowArgs p
 #pragma unroll
         for (int i = 0; i < 8; ++i) part = f(part, j, i);
       }
-      part = t + TPR * j < S ? part : 0.0f;
-      if constexpr (APART) part = row_reduce<TPR>(part, kSum, lds);
+      part = t + TPR * j < S ? part : (S1)0;
+      if constexpr (APART) parts[j] = row_reduce<64>(part, kSum, lds);
       if (HALVES && (j & 1))
         odd = j == 1 ? part : odd + part;
       else
         sum = j == 0 ? part : sum + part;
     }
-    if constexpr (APART) return sum;
+    if constexpr (APART) {
+      if constexpr (TPR > 64) {
+        if ((t & 63) == 0) {
+#pragma unroll
+          for (int j = 0; j < VPT; ++j) lds[j * WAVES + (t >> 6)] = parts[j];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < VPT * WAVES; ++i) sum = i == 0 ? lds[0] : sum + lds[i];
+      } else {
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) sum = j == 0 ? parts[0] : sum + parts[j];
+      }
+      return sum;
+    }
     if constexpr (HALVES) return row_reduce<TPR>(sum, kSum, lds) + row_reduce<TPR>(odd, kSum, lds);
     return row_reduce<TPR>(sum, kSum, lds);
   };
-  f32x8 y[VPT];
-  float rstd = 1.0f;
+  typedef W W8 __attribute__((ext_vector_type(8)));
+  W8 y[VPT];
+  S1 rstd = 1;
   bool bad = false;
   if constexpr (KIND == kQuant) {
 #pragma unroll
@@ -236,28 +361,30 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) row_q8_kernel(RowArgs p
     const float ss = row_sum(
         [&](float s, int j, int i) { return __builtin_fmaf((float)h[j][i], (float)h[j][i], s); }, red[0]);
     bad = !(ss < INFINITY);
-    rstd = rsqrtf(ss * p.inv_k + p.eps);
+    rstd = root_of(ss, p);
   } else {
-    const float mean = row_sum([&](float s, int j, int i) { return s + (float)h[j][i]; }, red[0]) / (float)K;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) y[j] = __builtin_convertvector(h[j], f64x8);
+    const double mean = mean_of(row_sum([&](double s, int j, int i) { return s + y[j][i]; }, red[0]), K, p.inv_k);
 #pragma unroll
     for (int j = 0; j < VPT; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[j][i] = (float)h[j][i] - mean;
-    const float sq = row_sum([&](float s, int j, int i) { return __builtin_fmaf(y[j][i], y[j][i], s); }, red[1]);
+      for (int i = 0; i < 8; ++i) y[j][i] = y[j][i] - mean;
+    const double sq = row_sum([&](double s, int j, int i) { return __builtin_fma(y[j][i], y[j][i], s); }, red[1]);
     bad = !(sq < INFINITY);
-    const float rs = rsqrtf(sq * p.inv_k + p.eps);
+    const double rs = root_of(sq, p);
 #pragma unroll
     for (int j = 0; j < VPT; ++j)
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        y[j][i] = __builtin_fmaf(y[j][i] * rs, p.gamma ? (float)g[j][i] : 1.0f, p.beta ? (float)b[j][i] : 0.0f);
+        y[j][i] = __builtin_fma(y[j][i], rs * (double)g[j][i], (double)b[j][i]);
   }
-  float top = 0.0f;
+  Top<W> top;
 #pragma unroll
   for (int j = 0; j < VPT; ++j)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max_abs(top, y[j][i]);
-  const RowScale s = row_scale<T>(row_reduce<TPR>(top, kMax, red[2]), bad);
+    for (int i = 0; i < 8; ++i) top.add(y[j][i]);
+  const RowScale<W> s = row_scale<T>(row_reduce<TPR>(top.get(), kMax, red_top), bad);
   if (ROWS > 1 && row_at >= p.rows) return;
   int8_t* q = p.q + (size_t)row * p.ldq;
   T* ho = (T*)p.h + (size_t)row * p.ldh;
@@ -268,7 +395,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) row_q8_kernel(RowArgs p
     const u32x2 o = quant8<T>(y[j], s);
     __builtin_memcpy(q + at[j], &o, 8);
   }
-  if (t == 0) p.scale[row] = s.unit == 0.0f ? 0.0f : rstd * s.unit;
+  if (t == 0) p.scale[row] = s.unit == 0 ? 0.0f : (float)(rstd * s.unit);
 }
 
 // Rows of more values than the registers of a workgroup hold: one workgroup a
@@ -280,7 +407,11 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) row_q8_kernel(RowArgs p
 template <class T, RowKind KIND>
 __global__ void __launch_bounds__(1024) row_q8_long_kernel(RowArgs p) {
   constexpr int NT = 1024;
-  __shared__ float red[3][NT / 64];
+  typedef Stat<T, KIND> S1;
+  typedef Wide<T, KIND> W;
+  typedef W W8 __attribute__((ext_vector_type(8)));
+  __shared__ S1 red[2][NT / 64];
+  __shared__ W red_top[NT / 64];
   const int row = blockIdx.x, t = threadIdx.x;
   const int K = p.K, S = K >> 3, tail = S * 8 + t;
   const T* x = (const T*)p.x + (size_t)row * p.ldx;
@@ -298,7 +429,7 @@ __global__ void __launch_bounds__(1024) row_q8_long_kernel(RowArgs p) {
         v = v + load8(res + k);
         if (p.h) store8(ho + k, v);
       }
-      f16x8 g{}, b{};
+      f16x8 g = (f16)1.0f, b = (f16)0.0f;
       if (KIND != kQuant && p.gamma) g = load8(p.gamma + k);
       if (KIND == kLayer && p.beta) b = load8(p.beta + k);
       f(__builtin_convertvector(v, f32x8), __builtin_convertvector(g, f32x8), __builtin_convertvector(b, f32x8), 8, k);
@@ -310,7 +441,7 @@ __global__ void __launch_bounds__(1024) row_q8_long_kernel(RowArgs p) {
         v = v + res[tail];
         if (p.h) ho[tail] = v;
       }
-      f32x8 v8{}, g{}, b{};
+      f32x8 v8{}, g = 1.0f, b = 0.0f;
       v8[0] = (float)v;
       if (KIND != kQuant && p.gamma) g[0] = (float)p.gamma[tail];
       if (KIND == kLayer && p.beta) b[0] = (float)p.beta[tail];
@@ -318,51 +449,61 @@ __global__ void __launch_bounds__(1024) row_q8_long_kernel(RowArgs p) {
     }
     first = false;
   };
-  float rstd = 1.0f, mean = 0.0f, rs = 1.0f;
+  S1 rstd = 1, mean = 0, rs = 1;
   bool bad = false;
-  auto value = [&](float v, float g, float b) {
-    if constexpr (KIND == kRms) return p.gamma ? v * g : v;
-    if constexpr (KIND == kLayer) return __builtin_fmaf((v - mean) * rs, p.gamma ? g : 1.0f, p.beta ? b : 0.0f);
+  auto value = [&](float v, float g, float b) -> W {
+    if constexpr (KIND == kRms) return v * g;
+    if constexpr (KIND == kLayer) return __builtin_fma(v - mean, rs * g, (double)b);
     return v;
   };
-  float top = 0.0f;
+  Top<W> top;
   if constexpr (KIND == kLayer) {
-    float sum = 0.0f, sq = 0.0f;
+    // Both sums in one pass, over the differences from the row's first value: its
+    // own square is among those that the variance sums, so that taking
+    // K (mean difference)^2 away again leaves the variance to 2 K 2^-53.
+    float v0 = (float)(T)(add ? x[0] + res[0] : x[0]);
+    asm volatile("" : "+v"(v0));  // here by now: behind the barrier the sum may replace it
+    __syncthreads();
+    const double first_value = v0;
+    double sum = 0.0, sq = 0.0;
     each([&](const f32x8& v, const f32x8&, const f32x8&, int n, int) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += i < n ? v[i] : 0.0f;
+      for (int i = 0; i < 8; ++i) {
+        const double d = i < n ? v[i] - first_value : 0.0;
+        sum += d;
+        sq = __builtin_fma(d, d, sq);
+      }
     });
-    mean = row_reduce<NT>(sum, kSum, red[0]) / (float)K;
-    each([&](const f32x8& v, const f32x8&, const f32x8&, int n, int) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sq = i < n ? __builtin_fmaf(v[i] - mean, v[i] - mean, sq) : sq;
-    });
+    sum = row_reduce<NT>(sum, kSum, red[0]);
     sq = row_reduce<NT>(sq, kSum, red[1]);
     bad = !(sq < INFINITY);
-    rs = rsqrtf(sq * p.inv_k + p.eps);
+    mean = sum * p.inv_k;
+    rs = root_of(__builtin_fmax(__builtin_fma(-sum, mean, sq), 0.0), p);
+    mean += first_value;
     each([&](const f32x8& v, const f32x8& g, const f32x8& b, int n, int) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = i < n ? max_abs(top, value(v[i], g[i], b[i])) : top;
+      for (int i = 0; i < 8; ++i)
+        if (i < n) top.add(value(v[i], g[i], b[i]));
     });
   } else {
-    float ss = 0.0f;
+    S1 ss = 0;
     each([&](const f32x8& v, const f32x8& g, const f32x8& b, int n, int) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         ss = __builtin_fmaf(v[i], v[i], ss);
-        top = max_abs(top, value(v[i], g[i], b[i]));  // past n: zeros
+        top.add(value(v[i], g[i], b[i]));  // past n: zeros
       }
     });
     if constexpr (KIND == kRms) {
       ss = row_reduce<NT>(ss, kSum, red[0]);
       bad = !(ss < INFINITY);
-      rstd = rsqrtf(ss * p.inv_k + p.eps);
+      rstd = root_of(ss, p);
     }
   }
-  const RowScale s = row_scale<T>(row_reduce<NT>(top, kMax, red[2]), bad);
+  const RowScale<W> s = row_scale<T>(row_reduce<NT>(top.get(), kMax, red_top), bad);
   int8_t* q = p.q + (size_t)row * p.ldq;
   each([&](const f32x8& v, const f32x8& g, const f32x8& b, int n, int k) {
-    f32x8 y;
+    W8 y;
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = value(v[i], g[i], b[i]);
     const u32x2 o = quant8<T>(y, s);
@@ -371,7 +512,7 @@ __global__ void __launch_bounds__(1024) row_q8_long_kernel(RowArgs p) {
     else
       q[k] = (int8_t)(o[0] & 0xff);
   });
-  if (t == 0) p.scale[row] = s.unit == 0.0f ? 0.0f : rstd * s.unit;
+  if (t == 0) p.scale[row] = s.unit == 0 ? 0.0f : (float)(rstd * s.unit);
 }
 
 // Rows of fewer than eight values: a thread a row.
@@ -380,38 +521,42 @@ __global__ void __launch_bounds__(256) row_q8_short_kernel(RowArgs p) {
   const int row = blockIdx.x * 256 + threadIdx.x;
   if (row >= p.rows) return;
   const T* x = (const T*)p.x + (size_t)row * p.ldx;
-  f32x8 y{};
-  float sum = 0.0f, sq = 0.0f, top = 0.0f, rstd = 1.0f;
+  typedef Stat<T, KIND> S1;
+  typedef Wide<T, KIND> W;
+  typedef W W8 __attribute__((ext_vector_type(8)));
+  W8 y{};
+  S1 sum = 0, sq = 0, rstd = 1, mean = 0;
+  Top<W> top;
 #pragma unroll
   for (int k = 0; k < 7; ++k) {
     if (k >= p.K) break;
     T v = x[k];
     if (KIND != kQuant && p.res) v = v + ((const T*)p.res)[(size_t)row * p.ldr + k];
     if (KIND != kQuant && p.h) ((T*)p.h)[(size_t)row * p.ldh + k] = v;
-    y[k] = (float)v;
+    y[k] = (W)v;
     sum += y[k];
   }
-  const float mean = KIND == kLayer ? sum / (float)p.K : 0.0f;
+  if constexpr (KIND == kLayer) mean = mean_of(sum, p.K, p.inv_k);
 #pragma unroll
-  for (int k = 0; k < 7; ++k) sq += k < p.K ? (y[k] - mean) * (y[k] - mean) : 0.0f;
+  for (int k = 0; k < 7; ++k) sq += k < p.K ? (y[k] - mean) * (y[k] - mean) : (S1)0;
   const bool bad = KIND != kQuant && !(sq < INFINITY);
-  const float rs = rsqrtf(sq * p.inv_k + p.eps);
+  const S1 rs = root_of(sq, p);
   if (KIND == kRms) rstd = rs;
 #pragma unroll
   for (int k = 0; k < 7; ++k) {
     if (k >= p.K) break;
     const float g = KIND != kQuant && p.gamma ? (float)p.gamma[k] : 1.0f;
-    if (KIND == kRms) y[k] = y[k] * g;
-    if (KIND == kLayer) y[k] = __builtin_fmaf((y[k] - mean) * rs, g, p.beta ? (float)p.beta[k] : 0.0f);
-    top = max_abs(top, y[k]);
+    if constexpr (KIND == kRms) y[k] = y[k] * g;
+    if constexpr (KIND == kLayer) y[k] = __builtin_fma(y[k] - mean, rs * g, p.beta ? (double)p.beta[k] : 0.0);
+    top.add(y[k]);
   }
-  const RowScale s = row_scale<T>(top, bad);
+  const RowScale<W> s = row_scale<T>(top.get(), bad);
   const u32x2 o = quant8<T>(y, s);
   int8_t* q = p.q + (size_t)row * p.ldq;
 #pragma unroll
   for (int k = 0; k < 7; ++k)
     if (k < p.K) q[k] = (int8_t)(o[k >> 2] >> (8 * (k & 3)));
-  p.scale[row] = s.unit == 0.0f ? 0.0f : rstd * s.unit;
+  p.scale[row] = s.unit == 0 ? 0.0f : (float)(rstd * s.unit);
 }
 
 // y = q * scale, sixteen values a thread (K >= 16: the last vector of a row
@@ -445,20 +590,41 @@ void launch_rows(const RowArgs& a, hipStream_t s) {
   static const std::string name = std::string("row_q8_kernel<") + (sizeof(T) == 2 ? "_Float16" : "float") + ", " +
                                   std::to_string((int)KIND) + ", " + std::to_string(TPR) + ", " +
                                   std::to_string(VPT) + ">";
-  constexpr int ROWS = TPR < 256 ? 256 / TPR : 1;
+  constexpr int ROWS = TPR < 128 ? 256 / TPR : 1;
   DLM_LAUNCH(name.c_str(), (row_q8_kernel<T, KIND, TPR, VPT>), dim3((a.rows + ROWS - 1) / ROWS),
-             dim3(TPR < 256 ? 256 : TPR), 0, s, a);
+             dim3(TPR < 128 ? 256 : TPR), 0, s, a);
+}
+
+// LayerNorms of 1025-16384 values, whose fp64 instructions are the longest part,
+// take as many threads as leave few of them idle: 192 or 384 with one vector each,
+// 256 or 512 with three (975x1283 5.1 -> 4.8 us against 256, 2048x5120 16.9 -> 12.6
+// and 1024x12000 20.3 -> 13.6 against 512 with two and four).  Many rows share what a
+// row has to do once among fewer threads: a wave with three vectors (fp16 3000x1280
+// 7.4 -> 6.6 us, 1536 rows the same, fp32 rows 7.6 -> 7.8) or four (16384x2048 36 ->
+// 31; below 4096 rows nothing), two waves with three (2048x2560 10.0 -> 8.5; 512 rows
+// 4.4 -> 5.0).
+template <class T>
+void layer_rows(const RowArgs& a, hipStream_t s) {
+  const int K = a.K;
+  if (K <= 2048) {
+    if constexpr (sizeof(T) == 2) {
+      if (a.rows >= 2048 && K <= 1536) return launch_rows<T, kLayer, 64, 3>(a, s);
+      if (a.rows >= 4096) return launch_rows<T, kLayer, 64, 4>(a, s);
+    }
+    return K <= 1536 ? launch_rows<T, kLayer, 192, 1>(a, s) : launch_rows<T, kLayer, 256, 1>(a, s);
+  }
+  if (K <= 3072) return a.rows >= 1024 ? launch_rows<T, kLayer, 128, 3>(a, s) : launch_rows<T, kLayer, 384, 1>(a, s);
+  if (K <= 4096) return launch_rows<T, kLayer, 256, 2>(a, s);
+  if (K <= 6144) return launch_rows<T, kLayer, 256, 3>(a, s);
+  if (K <= 8192) return launch_rows<T, kLayer, 512, 2>(a, s);
+  return K <= 12288 ? launch_rows<T, kLayer, 512, 3>(a, s) : launch_rows<T, kLayer, 512, 4>(a, s);
 }
 
 // Threads a row by its length: each holds one to four vectors.  Rows of 1025-2048
 // values take a workgroup (8192x1280 quantise 8.2 us, RMS norm 13.5; with a wave
-// each 8.4 and 13.9, and 2.8 against 3.8 us for 256 rows), but fp16 LayerNorms of
-// many of them a wave, which has no barrier in its three reductions (8192x1280
-// 13.6 -> 12.5 us, 16384x2048 33 -> 26.5; 2048 rows take the same either way, fp32
-// rows are slower with a wave).  Their rows of 513-768 values take half a wave,
-// whose lanes are then all in use, and reduce two rows at a time (8192x640 8.5 ->
-// 7.3 us, 32768x640 22.2 -> 17.7; up to 512 and over 768 values nothing is
-// gained, the other kinds lose 2-6%).
+// each 8.4 and 13.9, and 2.8 against 3.8 us for 256 rows).  Many fp16 LayerNorms of
+// 513-768 values take half a wave each (8192x640 9.2 -> 7.7 us; the other kinds lose
+// 2-6%).
 template <class T, RowKind KIND>
 void row_q8(const RowArgs& a, hipStream_t s) {
   const int K = a.K;
@@ -477,19 +643,18 @@ void row_q8(const RowArgs& a, hipStream_t s) {
       if (a.rows >= 4096 && K <= 768) return launch_rows<T, KIND, 32, 3>(a, s);
     }
     launch_rows<T, KIND, 64, 2>(a, s);
-  } else if (K <= 2048) {
-    if constexpr (KIND == kLayer && sizeof(T) == 2) {
-      if (a.rows >= 4096) return K <= 1536 ? launch_rows<T, KIND, 64, 3>(a, s) : launch_rows<T, KIND, 64, 4>(a, s);
-    }
+  } else if (K > 16384)
+    DLM_LAUNCH("row_q8_long_kernel", (row_q8_long_kernel<T, KIND>), dim3(a.rows), dim3(1024), 0, s, a);
+  else if constexpr (KIND == kLayer)
+    layer_rows<T>(a, s);
+  else if (K <= 2048)
     launch_rows<T, KIND, 256, 1>(a, s);
-  } else if (K <= 4096)
+  else if (K <= 4096)
     launch_rows<T, KIND, 256, 2>(a, s);
   else if (K <= 8192)
     launch_rows<T, KIND, 512, 2>(a, s);
-  else if (K <= 16384)
-    launch_rows<T, KIND, 512, 4>(a, s);
   else
-    DLM_LAUNCH("row_q8_long_kernel", (row_q8_long_kernel<T, KIND>), dim3(a.rows), dim3(1024), 0, s, a);
+    launch_rows<T, KIND, 512, 4>(a, s);
 }
 
 // A launch counts its threads in 32 bits: more rows than 2^21 go in parts.
@@ -578,7 +743,7 @@ extern "C" {
 int dlm_quantize_rows_fp16(const void* x, int ldx, void* q, int ldq, float* scale, int rows, int K, void* stream) {
   if (rows <= 0 || K <= 0) return DLM_OK;
   return row_entry<f16>(kQuant, __func__,
-                        RowArgs{x, nullptr, nullptr, nullptr, nullptr, (int8_t*)q, scale, ldx, 0, 0, ldq, rows, K, 0.0f, 0.0f},
+                        RowArgs{x, nullptr, nullptr, nullptr, nullptr, (int8_t*)q, scale, ldx, 0, 0, ldq, rows, K, 0.0f, 0.0},
                         (hipStream_t)stream);
 }
 
@@ -586,7 +751,7 @@ int dlm_quantize_rows_f32(const float* x, int ldx, void* q, int ldq, float* scal
   if (rows <= 0 || K <= 0) return DLM_OK;
   return row_entry<float>(
       kQuant, __func__,
-      RowArgs{x, nullptr, nullptr, nullptr, nullptr, (int8_t*)q, scale, ldx, 0, 0, ldq, rows, K, 0.0f, 0.0f},
+      RowArgs{x, nullptr, nullptr, nullptr, nullptr, (int8_t*)q, scale, ldx, 0, 0, ldq, rows, K, 0.0f, 0.0},
       (hipStream_t)stream);
 }
 
@@ -595,7 +760,7 @@ int dlm_rms_norm_q8_fp16(const void* x, int ldx, const void* R, int ldr, void* H
   if (rows <= 0 || K <= 0) return DLM_OK;
   return row_entry<f16>(
       kRms, __func__,
-      RowArgs{x, R, H, (const f16*)gamma, nullptr, (int8_t*)q, scale, ldx, ldr, ldh, ldq, rows, K, eps, 1.0f / (float)K},
+      RowArgs{x, R, H, (const f16*)gamma, nullptr, (int8_t*)q, scale, ldx, ldr, ldh, ldq, rows, K, eps, 1.0 / K},
       (hipStream_t)stream);
 }
 
@@ -604,7 +769,7 @@ int dlm_rms_norm_q8_f32(const float* x, int ldx, const float* R, int ldr, float*
   if (rows <= 0 || K <= 0) return DLM_OK;
   return row_entry<float>(
       kRms, __func__,
-      RowArgs{x, R, H, (const f16*)gamma, nullptr, (int8_t*)q, scale, ldx, ldr, ldh, ldq, rows, K, eps, 1.0f / (float)K},
+      RowArgs{x, R, H, (const f16*)gamma, nullptr, (int8_t*)q, scale, ldx, ldr, ldh, ldq, rows, K, eps, 1.0 / K},
       (hipStream_t)stream);
 }
 
@@ -614,7 +779,7 @@ int dlm_layer_norm_q8_fp16(const void* x, int ldx, const void* R, int ldr, void*
   if (rows <= 0 || K <= 0) return DLM_OK;
   return row_entry<f16>(
       kLayer, __func__,
-      RowArgs{x, R, H, (const f16*)gamma, (const f16*)beta, (int8_t*)q, scale, ldx, ldr, ldh, ldq, rows, K, eps, 1.0f / (float)K},
+      RowArgs{x, R, H, (const f16*)gamma, (const f16*)beta, (int8_t*)q, scale, ldx, ldr, ldh, ldq, rows, K, eps, 1.0 / K},
       (hipStream_t)stream);
 }
 
@@ -624,7 +789,7 @@ int dlm_layer_norm_q8_f32(const float* x, int ldx, const float* R, int ldr, floa
   if (rows <= 0 || K <= 0) return DLM_OK;
   return row_entry<float>(
       kLayer, __func__,
-      RowArgs{x, R, H, (const f16*)gamma, (const f16*)beta, (int8_t*)q, scale, ldx, ldr, ldh, ldq, rows, K, eps, 1.0f / (float)K},
+      RowArgs{x, R, H, (const f16*)gamma, (const f16*)beta, (int8_t*)q, scale, ldx, ldr, ldh, ldq, rows, K, eps, 1.0 / K},
       (hipStream_t)stream);
 }
 

@@ -259,6 +259,61 @@ def test_layer_norm_q8(gpu, K, residual, affine, dtype):
     check_rows(out.cpu(), res[1].cpu(), v, err, f"layer_norm {K}")
 
 
+def same_rows(q, scale, v, tol, what):
+    """q and scale of the oracle's rows v (float64), each integer the nearest one
+    unless its quotient lies within tol (per row) of a half; the scale rounded once."""
+    t, ref, s = Q.rows(v)
+    off = q.double() != ref
+    near = (t - torch.floor(t) - 0.5).abs() <= tol[:, None]
+    assert not bool((off & ~near).any()), f"{what}: {int((off & ~near).sum())} integers differ"
+    # from fp64 that is off by 2^-45 or so, to fp32
+    assert bool(((scale.double() - s).abs() <= U * (1 + 2.0 ** -20) * s + 2.0 ** -149).all()), f"{what}: scale"
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("mean", [0, 40])
+@pytest.mark.parametrize("rows,K", [(300000, 5), (30000, 60), (20000, 77), (10000, 200), (8000, 320), (1000, 640),
+                                    (8192, 640), (4099, 701), (1500, 1031), (5000, 1283), (4096, 1800), (1024, 2500),
+                                    (512, 5000), (256, 12000), (150, 20000)])
+def test_layer_norm_q8_integers_are_those_of_64_bits(gpu, rows, K, mean, dtype):
+    """Millions of values, some of whose quotients lie as close to a half as fp32
+    statistics are to the real ones."""
+    announce(f"layer_norm_q8 {rows}x{K} around {mean} against float64, {dtype}")
+    x = (spread(rows, K, K).cuda().float() + mean).to(dtype)
+    g, b = (cpu((K,), 3) * 0.3 + 1).cuda(), (cpu((K,), 4) * 0.2).cuda()
+    eps = torch.tensor(1e-5).double().cuda()  # as the entry points take it
+    h = x.double()
+    v = Q.layer_norm(h, g.double(), b.double(), eps)
+    # sums of K values in fp64, in any order, in kernel and oracle: (K + 8) 2^-53 of the
+    # largest |h| each, which shifts v by as much over the spread; 127 / top of it twice
+    rs = 1.0 / torch.sqrt((h - h.mean(1, keepdim=True)).square().mean(1) + eps)
+    tol = 4 * 127 * (K + 8) * 2.0 ** -53 * h.abs().amax(1) * rs * float(g.abs().max()) / v.abs().amax(1)
+    q, s = ops.layer_norm_q8(x, g, b)
+    same_rows(q, s, v, tol, f"layer_norm {rows}x{K}")
+
+
+@pytest.mark.parametrize("K", [5, 77, 640, 1283, 5000, 20000])
+def test_layer_norm_q8_of_tiny_and_huge_fp32_without_eps(gpu, K):
+    """The squares of these pass fp32's range in either direction."""
+    announce(f"layer_norm_q8 of fp32 rows near the ends of the range, K={K}")
+    f = torch.tensor([1e-36, 1e-30, 1e-23, 1e-20, 1.0, 1e18, 1e25, 1e34])
+    x = spread(8, K, K, torch.float32) * f[:, None]
+    g = cpu((K,), 3) * 0.3 + 1
+    v = Q.layer_norm(x.double(), g.double(), None, 0.0)
+    q, s = ops.layer_norm_q8(x.cuda(), g.cuda(), eps=0.0)
+    tol = torch.full((8,), 4 * 127 * (K + 8) * 2.0 ** -53 * math.sqrt(K) * float(g.abs().max()), dtype=torch.float64)
+    same_rows(q.cpu(), s.cpu(), v, tol, f"layer_norm {K}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("K", [3, 7, 77, 640, 1283, 5000, 20000])
+def test_layer_norm_q8_of_equal_values_is_zero(gpu, K, dtype):
+    announce(f"layer_norm_q8 of rows of one value, K={K} {dtype}")
+    x = torch.tensor([0.3, -1.7, 1234.5, 1e-3]).to(dtype).cuda()[:, None].expand(4, K).contiguous()
+    q, s = ops.layer_norm_q8(x)
+    assert (q == 0).all() and (s == 0).all()
+
+
 def test_norms_write_the_sum_in_place_and_read_strided_rows(gpu):
     announce("norms: sum over x or over the residual, rows inside wider tensors")
     for K in (40, 640, 2052, 5000, 17000):
@@ -473,6 +528,20 @@ def test_linear_q8_is_the_same_on_every_tile(gpu, act, residual, dtype):
             assert torch.equal(run(), ref), f"tile {tile}"
     finally:
         _lib.call("dlm_q8_force_tile", 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,K", [(2300, 1100), (2300, 1536), (4200, 1537), (4200, 2048), (1100, 2049), (1500, 2560),
+                                    (1024, 2901)])
+def test_layer_norm_rows_do_not_depend_on_their_number(gpu, rows, K, dtype):
+    announce(f"layer_norm_q8 rows alone and among {rows}, K={K} {dtype}")
+    x = (spread(rows, K, K).cuda().float() + 3).to(dtype)
+    g, b = (cpu((K,), 3) * 0.3 + 1).cuda(), (cpu((K,), 4) * 0.2).cuda()
+    # eps makes the variance count: a sum in another order shows in the scales
+    q, s = ops.layer_norm_q8(x, g, b, eps=0.5)
+    for lo, n in ((0, 1), (17, 5), (100, 900)):
+        q1, s1 = ops.layer_norm_q8(x[lo:lo + n], g, b, eps=0.5)
+        assert torch.equal(q1, q[lo:lo + n]) and torch.equal(s1, s[lo:lo + n]), f"rows {lo}..{lo + n}"
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
