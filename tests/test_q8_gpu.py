@@ -181,6 +181,23 @@ def test_rms_norm_q8(gpu, K, residual, gamma, dtype):
     assert float(res[1][3]) == 0.0
 
 
+@pytest.mark.parametrize("K", [5, 77, 640, 1283, 5000, 20000])
+def test_rms_norm_q8_of_tiny_and_huge_fp32_without_eps(gpu, K):
+    """The squares of these pass fp32's range in either direction."""
+    announce(f"rms_norm_q8 of fp32 rows near the ends of the range, K={K}")
+    f = torch.tensor([1e-41, 1e-36, 1e-30, 1e-23, 1e-20, 1.0, 1e18, 1e25, 1e35])
+    x = spread(9, K, K, torch.float32).clamp(-99, 99) * f[:, None]
+    g = cpu((K,), 3) * 0.3 + 1
+    for gamma in (None, g):
+        q, s = ops.rms_norm_q8(x.cuda(), None if gamma is None else gamma.cuda(), eps=0.0)
+        prod = x if gamma is None else x * gamma.float()
+        _, ref, top = Q.rows(prod.double())
+        ref_s = top / x.double().square().mean(1).sqrt()
+        assert torch.equal(q.cpu().double(), ref)
+        # the product's rounding is in ref_s; the scale's own from fp64
+        assert bool(((s.cpu().double() - ref_s).abs() <= U * (1 + 2.0 ** -20) * ref_s).all())
+
+
 def test_norms_of_zero_rows_without_eps(gpu):
     """0 / 0 is not formed: a row of zeros has scale 0 whatever eps is (RMS); of
     equal values, a LayerNorm with eps > 0 has beta alone."""
