@@ -703,11 +703,11 @@ int linear_q8(const char* fn, Q8Gemm p, hipStream_t s) {
   const Span y{"Y", p.y, p.ldy, p.M, cols, e};
   for (const Span& in : {Span{"X", p.x, p.ldx, p.M, k16, 1}, Span{"W", p.w, p.ldw, p.N, k16, 1},
                          Span{"sx", p.sx, p.M, 1, p.M, 4}, Span{"sw", p.sw, p.N, 1, p.N, 4},
-                         Span{"bias", p.bias, p.N, 1, p.N, 2}, Span{"R", p.res, p.ldr, p.M, cols, e}}) {
-    if (!overlap(y, in)) continue;
-    if (in.p == p.res && p.res == p.y && p.ldr == p.ldy) continue;  // added in place
-    return bad(std::string("Y overlaps ") + in.name);
-  }
+                         Span{"bias", p.bias, p.N, 1, p.N, 2}})
+    if (overlap(y, in)) return bad(std::string("Y overlaps ") + in.name);
+  // R alone may be Y: an output's residual is read by the lane that replaces it
+  if (!(p.res == p.y && p.ldr == p.ldy) && overlap(y, Span{"R", p.res, p.ldr, p.M, cols, e}))
+    return bad("Y overlaps R");
   // rows of one launch: at most 2^28 outputs (2^28 threads of the smallest tile)
   const int part = std::max(1 << 8, std::min(1 << 24, (1 << 28) / p.N & ~255));
   for (int left = p.M; left > 0; left -= part) {

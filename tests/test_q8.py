@@ -87,6 +87,17 @@ def test_linear_entries_refuse(lib):
         assert call(R=6 * A, ldr=48) == INVALID and "Y overlaps R" in err()
 
 
+def test_only_the_residual_may_be_the_output(lib):
+    for f, e in ((lib.dlm_linear_q8_fp16, 2), (lib.dlm_linear_q8_f32out, 4)):
+        def call(X=A, sx=2 * A, W=3 * A, sw=4 * A, bias=None, act=0):
+            # R is Y, with the same row stride; the operand named below is there too
+            return f(X, 64, sx, W, 64, sw, bias, 6 * A, 64, 6 * A, 64, 4, 32, 64, 1.0, act, None)
+
+        for k in ("X", "W", "sx", "sw", "bias"):
+            for act in (0, 2):
+                assert call(**{k: 6 * A}, act=act) == INVALID and "Y overlaps " + k in err()
+
+
 def test_interleaved_slices_that_share_a_column_are_refused(lib):
     for t, e in (("fp16", 2), ("f32", 4)):
         # rows of 64 columns: x and the sum take 40 each, from column 0 and from 24 or 39
