@@ -687,10 +687,8 @@ int row_parts(RowKind kind, RowArgs a, hipStream_t s) {
 // ---------------------------------------------------------------------------
 // Argument checks shared by the entry points.
 // ---------------------------------------------------------------------------
-// An output may be an input where it is the same tensor (same address and row
-// stride, elements of one size), and not overlap it otherwise.
-bool same(const Span& a, const Span& b) { return a.p == b.p && a.ld == b.ld && a.elem == b.elem && a.cols == b.cols; }
-
+// The sum may be x or the residual where it is the same tensor (same address and
+// row stride); otherwise an output overlaps neither inputs nor other outputs.
 template <class T>
 int row_entry(RowKind kind, const char* fn, const RowArgs& a, hipStream_t s) {
   auto bad = [&](const std::string& m) { return fail(DLM_ERR_INVALID_ARG, std::string(fn) + ": " + m); };
@@ -710,9 +708,10 @@ int row_entry(RowKind kind, const char* fn, const RowArgs& a, hipStream_t s) {
                       {"scale", a.scale, 1, a.rows, 1, 4},
                       {"sum", a.h, a.ldh, a.rows, a.K, e}};
   for (int o = 0; o < 3; ++o) {
-    for (const Span& i : in)
-      if (overlap(out[o], i) && !(o == 2 && same(out[o], i)))
-        return bad(std::string(out[o].name) + " overlaps " + i.name);
+    for (int i = 0; i < 4; ++i) {
+      const bool in_place = o == 2 && i < 2 && in[i].p == a.h && in[i].ld == a.ldh;
+      if (!in_place && overlap(out[o], in[i])) return bad(std::string(out[o].name) + " overlaps " + in[i].name);
+    }
     for (int u = 0; u < o; ++u)
       if (overlap(out[o], out[u])) return bad(std::string(out[o].name) + " overlaps " + out[u].name);
   }

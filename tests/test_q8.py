@@ -87,6 +87,16 @@ def test_linear_entries_refuse(lib):
         assert call(R=6 * A, ldr=48) == INVALID and "Y overlaps R" in err()
 
 
+def test_the_sum_may_be_neither_gamma_nor_beta(lib):
+    for t in ("fp16", "f32"):
+        for rows, K, ldh in ((4, 64, 64), (1, 64, 64), (4, 64, 128), (1, 128, 128)):
+            rms, layer = getattr(lib, f"dlm_rms_norm_q8_{t}"), getattr(lib, f"dlm_layer_norm_q8_{t}")
+            H, tail = 3 * A, (5 * A, K, 6 * A, rows, K, 1e-5, None)
+            assert rms(A, K, 2 * A, K, H, ldh, H, *tail) == INVALID and "sum overlaps gamma" in err()
+            assert layer(A, K, 2 * A, K, H, ldh, H, None, *tail) == INVALID and "sum overlaps gamma" in err()
+            assert layer(A, K, 2 * A, K, H, ldh, None, H, *tail) == INVALID and "sum overlaps beta" in err()
+
+
 def test_only_the_residual_may_be_the_output(lib):
     for f, e in ((lib.dlm_linear_q8_fp16, 2), (lib.dlm_linear_q8_f32out, 4)):
         def call(X=A, sx=2 * A, W=3 * A, sw=4 * A, bias=None, act=0):
