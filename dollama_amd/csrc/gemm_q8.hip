@@ -51,10 +51,12 @@ __device__ __forceinline__ i32x4 keep_bytes(i32x4 v, int n) {
 
 // x Phi(x) = max(x, 0) - |x| Q(|x|) with the upper tail Q(z) = erfc(z / sqrt 2) / 2
 // by Abramowitz & Stegun 7.1.26 (its coefficients halved, p and the exponent
-// scaled by 1 / sqrt 2; |error of Q| <= 7.5e-8).  Two VALU instructions fewer than
-// 0.5 x (1 + erf), where they bound the epilogue (GEGLU 2048x10240x1280 39.0 ->
-// 38.4 us), and no cancellation at negative x.  Past 16 the tail is 0 in fp32, so
-// that infinities keep to their limits; NaN stays NaN.
+// scaled by 1 / sqrt 2; |error of Q| <= 7.5e-8, with the roundings 3.1e-7).  Two VALU
+// instructions fewer than 0.5 x (1 + erf), where they bound the epilogue (GEGLU
+// 2048x10240x1280 39.0 -> 38.4 us), and no cancellation at negative x.  Relative to
+// the result that is 6e-7 for |x| < 1 (fp32's erf would give 1.5e-7) and 1.6e-3 at
+// -5, where 0.5 x (1 + erf) has lost all but two digits.  Past 16 the tail is 0 in
+// fp32, so that infinities keep to their limits; NaN stays NaN.
 __device__ __forceinline__ float gelu_tail(float x) {
   const float z = __builtin_elementwise_minimum(fabsf(x), 16.0f);
   const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.231641888f, z, 1.0f));

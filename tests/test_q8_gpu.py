@@ -371,6 +371,43 @@ def test_norms_between_column_slices_of_one_tensor(gpu, K):
                 assert torch.equal(xs, x) and torch.equal(rs, r)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("K", [5, 60, 77, 200, 640, 1283, 2052, 5000, 9000, 17000])
+def test_norms_with_a_non_finite_gamma_or_beta(gpu, K, dtype):
+    """v is not finite in any row then, rows of zeros included (0 times infinity)."""
+    announce(f"norms with infinities and NaN in gamma and beta, K={K} {dtype}")
+    x, g, b = spread(4, K, 1, dtype).cuda(), (cpu((K,), 3) + 1).cuda(), cpu((K,), 4).cuda()
+    x[2] = 0
+    for value in (float("inf"), float("-inf"), float("nan")):
+        for at in (0, K // 2, K - 1):
+            h = g.clone()
+            h[at] = value
+            for q, s in (ops.rms_norm_q8(x, h), ops.layer_norm_q8(x, h, b), ops.layer_norm_q8(x, None, h)):
+                assert (q == 0).all() and torch.isnan(s).all(), f"{value} at {at}"
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("K", [5, 40, 640, 643, 1283, 2052, 5000, 17000])
+def test_norms_that_do_not_write_their_sum(gpu, K, dtype):
+    """A residual with no place for the sum, which the C entries take: the same
+    rows as with one, and x and the residual as they were."""
+    from dollama_amd import _lib
+    announce(f"norms of a sum that is not written, K={K} {dtype}")
+    rows, t = 9, "fp16" if dtype == torch.float16 else "f32"
+    x, r = spread(rows, K, 1, dtype).cuda(), cpu((rows, K), 2, dtype).cuda()
+    g, b = (cpu((K,), 3) + 1).cuda(), (cpu((K,), 4) * 0.2).cuda()
+    x0, r0 = x.clone(), r.clone()
+    stream = torch.cuda.current_stream().cuda_stream
+    for name, norm, extra in (("rms", ops.rms_norm_q8, ()), ("layer", ops.layer_norm_q8, (b,))):
+        q, s, _ = norm(x, g, *extra, residual=r, eps=1e-5)
+        whole, out = gpu_rows(rows, K, torch.int8)
+        scale = torch.full((rows,), 77.0, device="cuda")
+        _lib.call(f"dlm_{name}_norm_q8_{t}", x.data_ptr(), K, r.data_ptr(), K, None, 0, g.data_ptr(),
+                  *(e.data_ptr() for e in extra), out.data_ptr(), K + 24, scale.data_ptr(), rows, K, 1e-5, stream)
+        assert torch.equal(out, q) and torch.equal(scale, s) and untouched(whole, rows, K), name
+        assert torch.equal(x, x0) and torch.equal(r, r0), name
+
+
 # ----------------------------------------------------------------- linear ---
 def int8_rows(rows, K, seed, low=-127):
     """Random 8-bit rows at a 16-byte row stride whose padding holds garbage."""
@@ -508,6 +545,48 @@ def test_linear_q8_activations_of_infinities_and_nan(gpu, dtype):
     y = ops.linear_q8(x, sx, w, sw, bias=b, act=ops.ACT_GEGLU, dtype=dtype)
     assert (y[:, 0] == float("inf")).all() and torch.isnan(y[:, 2]).all() and (y[:, 3] == 0).all()
     assert torch.isfinite(y[:, 4:]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_linear_q8_activations_at_minus_infinity(gpu, dtype):
+    """GELU takes its limit, 0, as a gate too; SiLU is the quotient x / (1 + exp(-x)),
+    NaN there."""
+    announce(f"linear_q8 activations at -infinity {dtype}")
+    x = torch.ones(5, 64, dtype=torch.int8, device="cuda")
+    w = torch.ones(32, 64, dtype=torch.int8, device="cuda")
+    sx, sw = torch.ones(5, device="cuda"), torch.full((32,), 2.0 ** -6, device="cuda")  # sums of 1
+    b = torch.zeros(32, dtype=torch.float16, device="cuda")
+    b[5] = float("-inf")
+    y = ops.linear_q8(x, sx, w, sw, bias=b, act=ops.ACT_GELU, dtype=dtype)
+    assert (y[:, 5] == 0).all()
+    y = ops.linear_q8(x, sx, w, sw, bias=b, act=ops.ACT_SILU, dtype=dtype)
+    assert torch.isnan(y[:, 5]).all() and torch.isfinite(y[:, 6:]).all()
+    # columns 4-7 are the gates of outputs 0-3
+    y = ops.linear_q8(x, sx, w, sw, bias=b, act=ops.ACT_GEGLU, dtype=dtype)
+    assert (y[:, 1] == 0).all() and torch.isfinite(y).all()
+
+
+def test_linear_q8_activations_over_their_range(gpu):
+    """Each activation of 400,000 values of either sign from 1e-6 to 30, one product
+    each: GELU within 4e-7 |x| (7.5e-8 of its tail's approximation, 5 roundings and
+    the reciprocal's of a tail of at most 1/2), SiLU within |x| 2^-24 relative (the
+    exponent's rounding) and 6 roundings."""
+    announce("linear_q8 activations against float64")
+    g = torch.Generator().manual_seed(3)
+    z = torch.exp(torch.rand(400000, generator=g, dtype=torch.float64) * math.log(3e7) + math.log(1e-6)).float()
+    z = torch.cat([z, -z, torch.zeros(8)])
+    N = z.numel()
+    w = torch.zeros(N, 16, dtype=torch.int8, device="cuda")
+    w[:, 0] = 1
+    x = torch.zeros(1, 16, dtype=torch.int8, device="cuda")
+    x[0, 0] = 1
+    run = lambda act: ops.linear_q8(x, torch.ones(1, device="cuda"), w, z.cuda(), act=act,  # noqa: E731
+                                    dtype=torch.float32)[0].cpu().double()
+    zd = z.double()
+    ref = zd * torch.special.ndtr(zd)
+    assert bool(((run(ops.ACT_GELU) - ref).abs() <= 4e-7 * zd.abs()).all())
+    ref = zd * torch.sigmoid(zd)
+    assert bool(((run(ops.ACT_SILU) - ref).abs() <= (6 + zd.abs()) * 2.0 ** -24 * ref.abs()).all())
 
 
 def test_linear_q8_row_results_do_not_depend_on_the_batch(gpu):
