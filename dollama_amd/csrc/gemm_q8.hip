@@ -710,8 +710,9 @@ int linear_q8(const char* fn, Q8Gemm p, hipStream_t s) {
   // R alone may be Y: an output's residual is read by the lane that replaces it
   if (!(p.res == p.y && p.ldr == p.ldy) && overlap(y, Span{"R", p.res, p.ldr, p.M, cols, e}))
     return bad("Y overlaps R");
-  // rows of one launch: at most 2^28 outputs (2^28 threads of the smallest tile)
-  const int part = std::max(1 << 8, std::min(1 << 24, (1 << 28) / p.N & ~255));
+  // rows of one launch: at most 2^31 outputs, of which the smallest tile has one a
+  // thread (a launch counts threads in 32 bits), and 64 rows at least, as N <= 2^25
+  const int part = (int)std::min(1LL << 24, (1LL << 31) / p.N & ~63LL);
   for (int left = p.M; left > 0; left -= part) {
     p.M = std::min(left, part);
     q8_gemm<T>(p, s);

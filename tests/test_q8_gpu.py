@@ -700,6 +700,29 @@ def test_linear_q8_past_32_bit_offsets(gpu):
         del x, w, y
 
 
+def test_linear_q8_of_most_columns_on_every_tile(gpu):
+    """The largest N with more rows than the smallest tile's launch takes."""
+    from dollama_amd import _lib
+    M, N, K = 130, 1 << 25, 16
+    announce(f"linear_q8 {M}x{N}x{K} on every tile")
+    torch.manual_seed(1)
+    x = torch.randint(-128, 128, (M, K), device="cuda", dtype=torch.int8)
+    w = torch.randint(-128, 128, (N, K), device="cuda", dtype=torch.int8)
+    sx, sw = torch.rand(M, device="cuda") * 1e-2, torch.rand(N, device="cuda") * 1e-2
+    ref, y = ops.linear_q8(x, sx, w, sw), torch.empty(M, N, dtype=torch.float16, device="cuda")
+    cols = torch.tensor([0, 1, N // 2, N - 33, N - 1], device="cuda")
+    z = (x.double().cpu() @ w[cols].double().cpu().t()) * sx.double().cpu()[:, None] * sw[cols].double().cpu()
+    assert bool(((ref[:, cols].cpu().double() - z).abs() <= (2.0 ** -11 + 2.0 ** -20) * z.abs() + 2.0 ** -25).all())
+    try:
+        for tile in range(1, 15):
+            print(f"[case] tile {tile}", flush=True)
+            _lib.call("dlm_q8_force_tile", tile)
+            y.zero_()
+            assert torch.equal(ops.linear_q8(x, sx, w, sw, out=y), ref), f"tile {tile}"
+    finally:
+        _lib.call("dlm_q8_force_tile", 0)
+
+
 # --------------------------------------------------------------- together ---
 class Block:
     """Norm, gated projection, row quantisation, projection back and residual:
