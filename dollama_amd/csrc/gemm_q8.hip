@@ -672,7 +672,7 @@ void q8_gemm(const Q8Gemm& p, hipStream_t s) {
     case 12: return launch_tile<T, 128, 80, 32, 80, 3, kPlain>(p, s);
     case 13: return launch_tile<T, 128, 160, 32, 80, 3, kPlain>(p, s);
     case 14: return launch_tile<T, 64, 32, 32, 16, 4, kPlain, 2>(p, s);
-    default: return launch_tile<T, 128, 256, 64, 64, 3, kPingPong>(p, s);
+    default: return launch_tile<T, 128, 256, 64, 64, 3, kPingPong>(p, s);  // 11
   }
 }
 
@@ -733,6 +733,7 @@ using namespace dlm;
 extern "C" {
 
 int dlm_q8_force_tile(int tile) {
+  DLM_REQUIRE(tile >= 0 && tile <= 14, "tile must be in [0, 14]");
   dlm::g_q8_tile = tile;
   return DLM_OK;
 }

@@ -125,6 +125,12 @@ def test_interleaved_slices_that_share_a_column_are_refused(lib):
                      None) == INVALID and "Y overlaps R" in err()
 
 
+def test_forced_tiles_are_those_there_are(lib):
+    for tile in (-1, 15, 1 << 20):
+        assert lib.dlm_q8_force_tile(tile) == INVALID and "[0, 14]" in err()
+    assert lib.dlm_q8_force_tile(14) == 0 and lib.dlm_q8_force_tile(0) == 0
+
+
 def test_wrappers_refuse_host_tensors():
     x, s = torch.zeros(4, 64, dtype=torch.float16), torch.ones(4)
     q = torch.zeros(4, 64, dtype=torch.int8)
