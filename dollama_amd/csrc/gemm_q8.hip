@@ -607,11 +607,10 @@ thread_local int g_q8_tile = 0;
 // n: output tiles a CU, rounded up; slices: of 128 bytes of K; more: what each
 // further workgroup on a CU adds, relative to the first (over 1 where it queues
 // for the LDS); words: 2-byte words that an output moves beyond the first (fp32,
-// a residual).  The constants are fits to 11200 launches of 1165 shapes (1-8192
-// rows, 16-14336 columns, K = 64-14336), graph-replayed; the modelled choice
-// takes 0.6% longer than the fastest of the fourteen in the mean, and up to 30%
-// where rows are not 16-byte aligned (6957x96x176 with residual 5.2 us against
-// 4.0).  K groups serve few rows and long K (us, without and with them:
+// a residual).  The constants are fits to 11240 launches of 1165 shapes (1-8192
+// rows, 16-14336 columns, K = 64-14336) on 7 to 14 of the tiles each, graph-replayed;
+// the modelled choice takes 0.6% longer than the fastest timed in the mean, and up to
+// 30% (5517x1155x234 13.7 us against 10.5).  K groups serve few rows and long K (us, without and with them:
 // 1x4096x4096 6.8 -> 5.9, 13x1280x5120 9.2 -> 6.2, 48x8192x8192 22.8 -> 17.8,
 // 100x4096x14336 31.0 -> 24.3, 256x2048x8192 14.8 -> 12.3), 128x160 the outputs
 // that it cuts into one round of 256 (8192x640x2560 22.5 -> 19.1,

@@ -512,11 +512,11 @@ int dlm_dequantize_rows_f32(const void* q, int ldq, const float* scale, float* y
  *   RMS norm:  v = h gamma / sqrt(mean(h^2) + eps)
  *   LayerNorm: v = (h - mean) / sqrt(var + eps) gamma + beta
  * with the statistics over the stored h, in fp64 (in fp32 for the RMS norm of
- * fp16 rows), so that eps may be 0 for rows of any magnitude; the RMS norm's
- * products h gamma are fp32.  H (may be NULL; only with R) receives h and may be
- * x or R itself (same pointer and row stride), but not overlap them otherwise.
- * gamma and beta are fp16 [K] and may be NULL (1 and 0).  x, R, H are fp16 or,
- * in the _f32 forms, fp32. */
+ * fp16 rows), so that eps may be 0 for rows of any magnitude (but a LayerNorm of
+ * equal values is NaN then); the RMS norm's products h gamma are fp32.  H (may be
+ * NULL; only with R) receives h and may be x or R itself (same pointer and row
+ * stride), but not overlap them otherwise.  gamma and beta are fp16 [K] and may
+ * be NULL (1 and 0).  x, R, H are fp16 or, in the _f32 forms, fp32. */
 int dlm_rms_norm_q8_fp16(const void* x, int ldx, const void* R, int ldr, void* H, int ldh,
                          const void* gamma, void* q, int ldq, float* scale, int rows, int K, float eps,
                          void* stream);

@@ -329,6 +329,8 @@ def test_layer_norm_q8_of_equal_values_is_zero(gpu, K, dtype):
     x = torch.tensor([0.3, -1.7, 1234.5, 1e-3]).to(dtype).cuda()[:, None].expand(4, K).contiguous()
     q, s = ops.layer_norm_q8(x)
     assert (q == 0).all() and (s == 0).all()
+    q, s = ops.layer_norm_q8(x, eps=0.0)  # 0 / 0
+    assert (q == 0).all() and torch.isnan(s).all()
 
 
 def test_norms_write_the_sum_in_place_and_read_strided_rows(gpu):
