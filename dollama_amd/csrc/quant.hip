@@ -611,19 +611,19 @@ void launch_rows(const RowArgs& a, hipStream_t s) {
 // 4.4 -> 5.0).
 template <class T>
 void layer_rows(const RowArgs& a, hipStream_t s) {
-  const int K = a.K;
-  if (K <= 2048) {
+  const int S = (a.K + 7) / 8;  // vectors a row
+  if (S <= 256) {
     if constexpr (sizeof(T) == 2) {
-      if (a.rows >= 2048 && K <= 1536) return launch_rows<T, kLayer, 64, 3>(a, s);
+      if (a.rows >= 2048 && S <= 192) return launch_rows<T, kLayer, 64, 3>(a, s);
       if (a.rows >= 4096) return launch_rows<T, kLayer, 64, 4>(a, s);
     }
-    return K <= 1536 ? launch_rows<T, kLayer, 192, 1>(a, s) : launch_rows<T, kLayer, 256, 1>(a, s);
+    return S <= 192 ? launch_rows<T, kLayer, 192, 1>(a, s) : launch_rows<T, kLayer, 256, 1>(a, s);
   }
-  if (K <= 3072) return a.rows >= 1024 ? launch_rows<T, kLayer, 128, 3>(a, s) : launch_rows<T, kLayer, 384, 1>(a, s);
-  if (K <= 4096) return launch_rows<T, kLayer, 256, 2>(a, s);
-  if (K <= 6144) return launch_rows<T, kLayer, 256, 3>(a, s);
-  if (K <= 8192) return launch_rows<T, kLayer, 512, 2>(a, s);
-  return K <= 12288 ? launch_rows<T, kLayer, 512, 3>(a, s) : launch_rows<T, kLayer, 512, 4>(a, s);
+  if (S <= 384) return a.rows >= 1024 ? launch_rows<T, kLayer, 128, 3>(a, s) : launch_rows<T, kLayer, 384, 1>(a, s);
+  if (S <= 512) return launch_rows<T, kLayer, 256, 2>(a, s);
+  if (S <= 768) return launch_rows<T, kLayer, 256, 3>(a, s);
+  if (S <= 1024) return launch_rows<T, kLayer, 512, 2>(a, s);
+  return S <= 1536 ? launch_rows<T, kLayer, 512, 3>(a, s) : launch_rows<T, kLayer, 512, 4>(a, s);
 }
 
 // Threads a row by its length: each holds one to four vectors.  Rows of 1025-2048
