@@ -18,20 +18,22 @@
 // 2.3e-5 at most (relative errors of 2^-23 and 2^-24 on values up to 127).
 // Quotients within 2^-15 of a half (one in 16,000) are decided again by comparing
 // 254 v with (2k + 1) a in fp64, where both products are exact.  So q is the
-// quotient's nearest integer whatever the launch looks like; for fp16 rows (and
-// fp16 gamma) of the first two kinds, where v is exact in fp32, that is the
-// mathematically exact result.  LayerNorm's v is not: statistics and values are
-// fp64 there, and quotients come out to 2^-40 (in fp32 about one integer in a
-// million fell on the other side of a half, 15 in a million where the mean is 40
-// times the spread, and the variance of rows beyond 1e19 or below 1e-19 was lost).
-// fp64 instructions run at fp32's rate here; the values take twice the registers,
-// which many rows notice (8192x1280 11.8 us with fp32, 8192x640 7.3 against 7.7).
+// quotient's nearest integer whatever the launch looks like: exactly for fp16 rows
+// (and fp16 gamma) of the first two kinds and for fp32 rows of the first, where v is
+// exact in fp32.  An fp32 row's products with gamma are exact in fp64, and are that;
+// so are LayerNorm's statistics and values, whose quotients come out to 2^-38.  (In
+// fp32 one integer in 8 million of the former fell on the other side of a half, one in
+// a million of the latter, 15 in a million where the mean is 40 times the spread; and
+// the squares of rows beyond 1e19 or below 1e-19 were lost.)  fp64 instructions run at
+// fp32's rate here; the values take twice the registers, which many rows notice:
+// LayerNorm 8192x1280 11.8 -> 13.3 us, 8192x640 7.3 -> 7.7, RMS norm of 8192x640 in
+// fp32 7.4 -> 8.6, with residual 12.2 -> 12.3.
 //
 // What bounds them: memory, one pass.  A row stays in registers between its
 // statistics and its output, in 8 to 512 threads by its length.  Measured (graph
 // replays, inputs that no cache holds): quantise 8192x1280 fp16 8.2 us (3.8 TB/s,
 // of which the launch is 2 us), RMS norm with residual 13.5 us (5.4 TB/s; fp32
-// 26.7 us, 5.1), LayerNorm 13.4 us (2.3 TB/s: some 16 VALU instructions a value
+// 27.2 us, 5.0), LayerNorm 13.4 us (2.3 TB/s: some 16 VALU instructions a value
 // and three reductions in a chain; with residual 15.3 us, 4.8 TB/s; fp32 14.9 and
 // 27.5); a 1 GiB copy reaches 5.15 TB/s.  One row: 2.3 us, 2.9 and 3.2.
 #include <algorithm>
@@ -57,13 +59,10 @@ struct RowArgs {
   double inv_k;
 };
 
-// What a row's statistics, and its values on their way to q, are held in.  The
-// squares of fp32 rows pass fp32's range at either end (8192x1280 RMS norm 10.9 ->
-// 11.6 us, with residual 26.7 -> 26.8).
+// What a row's statistics, and its values on their way to q, are held in: fp64
+// where fp32 would round them.
 template <class T, RowKind KIND>
-using Stat = std::conditional_t<KIND == kLayer || (KIND == kRms && sizeof(T) == 4), double, float>;
-template <class T, RowKind KIND>
-using Wide = std::conditional_t<KIND == kLayer, double, float>;
+using Wide = std::conditional_t<KIND == kLayer || (KIND == kRms && sizeof(T) == 4), double, float>;
 
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef double f64x8 __attribute__((ext_vector_type(8)));
@@ -102,35 +101,35 @@ struct Top {
 };
 
 // What a row's values are multiplied by on their way to q.
-template <class W, class S1>
+template <class W>
 struct RowScale {
   W r;         // 127 / (a m), 0 for rows without a finite positive maximum
   W a;         // a m
   float m;     // fp32 rows: a power of two that keeps 127 / a and its reciprocal normal numbers; else 1
-  S1 unit;     // a / 127, NaN for a row that holds an infinity or NaN
+  W unit;      // a / 127, NaN for a row that holds an infinity or NaN
 };
 // a: max |v|, not finite if a value is not.  Values of fp16 rows are no smaller
 // than 2^-48 where they are not 0.
-template <class T, class S1>
-__device__ __forceinline__ RowScale<float, S1> row_scale(float a, bool bad) {
-  RowScale<float, S1> s;
+template <class T>
+__device__ __forceinline__ RowScale<float> row_scale(float a, bool bad) {
+  RowScale<float> s;
   bad = bad || !(a < INFINITY);
   s.m = sizeof(T) == 2 ? 1.0f : a < 0x1p-100f ? 0x1p100f : a > 0x1p100f ? 0x1p-100f : 1.0f;
   s.a = a * s.m;
   s.r = bad || a == 0.0f ? 0.0f : 127.0f * __builtin_amdgcn_rcpf(s.a);
-  s.unit = bad ? (S1)__builtin_nanf("") : sizeof(S1) == 8 ? (S1)a * (S1)(1.0 / 127.0) : (S1)(a / 127.0f);
+  s.unit = bad ? __uint_as_float(0x7fc00000u) : a / 127.0f;
   return s;
 }
 // fp64 values, of at least 2^-240 where they are not 0 (2^-149 over the root of
 // the largest eps, times fp16's least gamma).  v_rcp_f64 and one step of Newton's
-// iteration, 1 / a to 2^-48.
-template <class T, class S1>
-__device__ __forceinline__ RowScale<double, S1> row_scale(double a, bool bad) {
-  RowScale<double, S1> s;
+// iteration, 1 / a to 2^-48, and 127 2^-45 more (see quant8).
+template <class T>
+__device__ __forceinline__ RowScale<double> row_scale(double a, bool bad) {
+  RowScale<double> s;
   bad = bad || !(a < INFINITY);
   s.a = a;
   const double r = __builtin_amdgcn_rcp(a);
-  s.r = bad || a == 0.0 ? 0.0 : 127.0 * __builtin_fma(__builtin_fma(-a, r, 1.0), r, r);
+  s.r = bad || a == 0.0 ? 0.0 : (127.0 + 127.0 * 0x1p-45) * __builtin_fma(__builtin_fma(-a, r, 1.0), r, r);
   const double unit = a * (1.0 / 127.0);
   s.unit = bad ? __builtin_nan("") : __builtin_fma(__builtin_fma(-unit, 127.0, a), 1.0 / 127.0, unit);
   return s;
@@ -149,8 +148,8 @@ __device__ __forceinline__ u32x2 pack8(const unsigned (&u)[8], bool none) {
   }
   return o;
 }
-template <class T, class S1>
-__device__ __forceinline__ u32x2 quant8(const f32x8& v, const RowScale<float, S1>& s) {
+template <class T, RowKind KIND>
+__device__ __forceinline__ u32x2 quant8(const f32x8& v, const RowScale<float>& s) {
   float far = 0.0f, x[8];
   unsigned u[8];
 #pragma unroll
@@ -175,21 +174,25 @@ __device__ __forceinline__ u32x2 quant8(const f32x8& v, const RowScale<float, S1
   }
   return pack8(u, s.r == 0.0f);
 }
-// The same from fp64 values, whose quotients come out to 2^-40: adding 1.5 * 2^52
-// leaves the nearest integer.  Quotients that are halves exactly take a maximum of
-// few bits, as rows have whose values are beta's alone; those are decided by the
-// products (of 24 and 8 bits, exact).
+// The same from fp64 values, whose quotients come out to 2^-38 and a little large:
+// adding 1.5 * 2^52 leaves the nearest integer.  What is half an integer exactly,
+// 254 v = (2k + 1) a, takes k = 63 or an a that 127 divides: either v = a / 2, and
+// 63.5 goes to the even 64 as a little more than it does, or a / 127 is exact, and
+// the products decide (exact for the RMS norm's 35 bits).  LayerNorms, of whose
+// values only beta alone is exact, ask whether a is an fp32 value, which is known
+// earlier (5% at 512x16384).
 constexpr double kRound64 = 6755399441055744.0;
-template <class T, class S1>
-__device__ __forceinline__ u32x2 quant8(const f64x8& v, const RowScale<double, S1>& s) {
+template <class T, RowKind KIND>
+__device__ __forceinline__ u32x2 quant8(const f64x8& v, const RowScale<double>& s) {
   unsigned u[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) u[i] = (unsigned)__double2loint(__builtin_fma(v[i], s.r, kRound64));
-  if ((__double2loint(s.a) & 0x1fffffff) == 0) {  // uniform in a row: the maximum is an fp32 value
+  const bool ties = KIND == kLayer ? (__double2loint(s.a) & 0x1fffffff) == 0 : __builtin_fma(s.unit, -127.0, s.a) == 0.0;
+  if (ties) {  // uniform in a row
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const double n = (double)(int)u[i], d = __builtin_fma(v[i], s.r, -n);
-      if (__builtin_fabs(d) > 0.5 - 0x1p-36) {
+      if (__builtin_fabs(d) > 0.5 - 0x1p-34) {
         const double k = d > 0.0 ? n : n - 1.0;  // between k and k + 1
         const double e = 254.0 * v[i] - (2.0 * k + 1.0) * s.a;
         u[i] = (unsigned)(int)(e > 0.0 || (e == 0.0 && ((int)k & 1)) ? k + 1.0 : k);
@@ -277,11 +280,10 @@ __device__ __forceinline__ double root_of(double sq, const RowArgs& p) {
 template <class T, RowKind KIND, int TPR, int VPT>
 __global__ void __launch_bounds__(TPR < 128 ? 256 : TPR) row_q8_kernel(RowArgs p) {
   constexpr int ROWS = TPR < 128 ? 256 / TPR : 1;  // of a workgroup
-  typedef Stat<T, KIND> S1;
   typedef Wide<T, KIND> W;
   constexpr int WAVES = TPR > 64 ? TPR / 64 : 1;  // of a row
   constexpr bool APART = KIND == kLayer && (TPR == 64 ? VPT > 2 : TPR == 128), HALVES = TPR == 32 && VPT > 1;
-  __shared__ S1 red[2][WAVES * (APART ? VPT : 1)];
+  __shared__ W red[2][WAVES * (APART ? VPT : 1)];
   __shared__ W red_top[WAVES];
   const int t = ROWS == 1 ? threadIdx.x : threadIdx.x & (TPR - 1);
   const int row_at = ROWS == 1 ? (int)blockIdx.x : (int)blockIdx.x * ROWS + (int)threadIdx.x / TPR;
@@ -298,10 +300,8 @@ __global__ void __launch_bounds__(TPR < 128 ? 256 : TPR) row_q8_kernel(RowArgs p
     at[j] = min(min(t + TPR * j, S - 1) * 8, K - 8);
     h[j] = load8(x + at[j]);
     if (KIND != kQuant && p.res) r[j] = load8(res + at[j]);
-    if (KIND == kLayer) {
-      g[j] = (f16)1.0f;
-      b[j] = (f16)0.0f;
-    }
+    if (KIND != kQuant) g[j] = (f16)1.0f;
+    if (KIND == kLayer) b[j] = (f16)0.0f;
     if (KIND != kQuant && p.gamma) g[j] = load8(p.gamma + at[j]);
     if (KIND == kLayer && p.beta) b[j] = load8(p.beta + at[j]);
   }
@@ -315,11 +315,11 @@ __global__ void __launch_bounds__(TPR < 128 ? 256 : TPR) row_q8_kernel(RowArgs p
   // many rows) add them up as those would, so that the sum does not depend on the
   // kernel: a wave as several waves, each of which adds 64 vectors in a row, half
   // a wave as the halves of a wave.
-  auto row_sum = [&](auto f, S1* lds) {
-    S1 sum = 0, odd = 0, parts[VPT];
+  auto row_sum = [&](auto f, W* lds) {
+    W sum = 0, odd = 0, parts[VPT];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-      S1 part = 0;
+      W part = 0;
       if (ragged) {
         const int skip = (t + TPR * j) * 8 - at[j];
 #pragma unroll
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 256 : TPR) row_q8_kernel(RowArgs p
 #pragma unroll
         for (int i = 0; i < 8; ++i) part = f(part, j, i);
       }
-      part = t + TPR * j < S ? part : (S1)0;
+      part = t + TPR * j < S ? part : (W)0;
       if constexpr (APART) parts[j] = row_reduce<64>(part, kSum, lds);
       if (HALVES && (j & 1))
         odd = j == 1 ? part : odd + part;
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 256 : TPR) row_q8_kernel(RowArgs p
   };
   typedef W W8 __attribute__((ext_vector_type(8)));
   W8 y[VPT];
-  S1 rstd = 1;
+  W rstd = 1;
   bool bad = false;
   if constexpr (KIND == kQuant) {
 #pragma unroll
@@ -364,8 +364,8 @@ __global__ void __launch_bounds__(TPR < 128 ? 256 : TPR) row_q8_kernel(RowArgs p
 #pragma unroll
     for (int j = 0; j < VPT; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[j][i] = p.gamma ? (float)h[j][i] * (float)g[j][i] : (float)h[j][i];
-    const S1 ss = row_sum([&](S1 s, int j, int i) { return add_square<S1>(s, h[j][i]); }, red[0]);
+      for (int i = 0; i < 8; ++i) y[j][i] = (W)h[j][i] * (W)g[j][i];
+    const W ss = row_sum([&](W s, int j, int i) { return add_square<W>(s, h[j][i]); }, red[0]);
     bad = !(ss < INFINITY);
     rstd = root_of(ss, p);
   } else {
@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 256 : TPR) row_q8_kernel(RowArgs p
   for (int j = 0; j < VPT; ++j)
 #pragma unroll
     for (int i = 0; i < 8; ++i) top.add(y[j][i]);
-  const RowScale<W, S1> s = row_scale<T, S1>(row_reduce<TPR>(top.get(), kMax, red_top), bad);
+  const RowScale<W> s = row_scale<T>(row_reduce<TPR>(top.get(), kMax, red_top), bad);
   if (ROWS > 1 && row_at >= p.rows) return;
   int8_t* q = p.q + (size_t)row * p.ldq;
   T* ho = (T*)p.h + (size_t)row * p.ldh;
@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 256 : TPR) row_q8_kernel(RowArgs p
   for (int j = 0; j < VPT; ++j) {
     if (t + TPR * j >= S) continue;
     if (KIND != kQuant && p.h) store8(ho + at[j], h[j]);
-    const u32x2 o = quant8<T>(y[j], s);
+    const u32x2 o = quant8<T, KIND>(y[j], s);
     __builtin_memcpy(q + at[j], &o, 8);
   }
   if (t == 0) p.scale[row] = s.unit == 0 ? 0.0f : (float)(rstd * s.unit);
@@ -413,10 +413,9 @@ __global__ void __launch_bounds__(TPR < 128 ? 256 : TPR) row_q8_kernel(RowArgs p
 template <class T, RowKind KIND>
 __global__ void __launch_bounds__(1024) row_q8_long_kernel(RowArgs p) {
   constexpr int NT = 1024;
-  typedef Stat<T, KIND> S1;
   typedef Wide<T, KIND> W;
   typedef W W8 __attribute__((ext_vector_type(8)));
-  __shared__ S1 red[2][NT / 64];
+  __shared__ W red[2][NT / 64];
   __shared__ W red_top[NT / 64];
   const int row = blockIdx.x, t = threadIdx.x;
   const int K = p.K, S = K >> 3, tail = S * 8 + t;
@@ -455,10 +454,10 @@ __global__ void __launch_bounds__(1024) row_q8_long_kernel(RowArgs p) {
     }
     first = false;
   };
-  S1 rstd = 1, mean = 0, rs = 1;
+  W rstd = 1, mean = 0, rs = 1;
   bool bad = false;
   auto value = [&](float v, float g, float b) -> W {
-    if constexpr (KIND == kRms) return v * g;
+    if constexpr (KIND == kRms) return (W)v * (W)g;
     if constexpr (KIND == kLayer) return __builtin_fma(v - mean, rs * g, (double)b);
     return v;
   };
@@ -492,11 +491,11 @@ __global__ void __launch_bounds__(1024) row_q8_long_kernel(RowArgs p) {
         if (i < n) top.add(value(v[i], g[i], b[i]));
     });
   } else {
-    S1 ss = 0;
+    W ss = 0;
     each([&](const f32x8& v, const f32x8& g, const f32x8& b, int n, int) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        ss = add_square<S1>(ss, v[i]);
+        ss = add_square<W>(ss, v[i]);
         top.add(value(v[i], g[i], b[i]));  // past n: zeros
       }
     });
@@ -506,13 +505,13 @@ __global__ void __launch_bounds__(1024) row_q8_long_kernel(RowArgs p) {
       rstd = root_of(ss, p);
     }
   }
-  const RowScale<W, S1> s = row_scale<T, S1>(row_reduce<NT>(top.get(), kMax, red_top), bad);
+  const RowScale<W> s = row_scale<T>(row_reduce<NT>(top.get(), kMax, red_top), bad);
   int8_t* q = p.q + (size_t)row * p.ldq;
   each([&](const f32x8& v, const f32x8& g, const f32x8& b, int n, int k) {
     W8 y;
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = value(v[i], g[i], b[i]);
-    const u32x2 o = quant8<T>(y, s);
+    const u32x2 o = quant8<T, KIND>(y, s);
     if (n == 8)
       __builtin_memcpy(q + k, &o, 8);
     else
@@ -527,11 +526,10 @@ __global__ void __launch_bounds__(256) row_q8_short_kernel(RowArgs p) {
   const int row = blockIdx.x * 256 + threadIdx.x;
   if (row >= p.rows) return;
   const T* x = (const T*)p.x + (size_t)row * p.ldx;
-  typedef Stat<T, KIND> S1;
   typedef Wide<T, KIND> W;
   typedef W W8 __attribute__((ext_vector_type(8)));
   W8 y{};
-  S1 sum = 0, sq = 0, rstd = 1, mean = 0;
+  W sum = 0, sq = 0, rstd = 1, mean = 0;
   Top<W> top;
 #pragma unroll
   for (int k = 0; k < 7; ++k) {
@@ -544,9 +542,9 @@ __global__ void __launch_bounds__(256) row_q8_short_kernel(RowArgs p) {
   }
   if constexpr (KIND == kLayer) mean = mean_of(sum, p.K, p.inv_k);
 #pragma unroll
-  for (int k = 0; k < 7; ++k) sq += k < p.K ? ((S1)y[k] - mean) * ((S1)y[k] - mean) : (S1)0;
+  for (int k = 0; k < 7; ++k) sq += k < p.K ? ((W)y[k] - mean) * ((W)y[k] - mean) : (W)0;
   const bool bad = KIND != kQuant && !(sq < INFINITY);
-  const S1 rs = root_of(sq, p);
+  const W rs = root_of(sq, p);
   if (KIND == kRms) rstd = rs;
 #pragma unroll
   for (int k = 0; k < 7; ++k) {
@@ -556,8 +554,8 @@ __global__ void __launch_bounds__(256) row_q8_short_kernel(RowArgs p) {
     if constexpr (KIND == kLayer) y[k] = __builtin_fma(y[k] - mean, rs * g, p.beta ? (double)p.beta[k] : 0.0);
     top.add(y[k]);
   }
-  const RowScale<W, S1> s = row_scale<T, S1>(top.get(), bad);
-  const u32x2 o = quant8<T>(y, s);
+  const RowScale<W> s = row_scale<T>(top.get(), bad);
+  const u32x2 o = quant8<T, KIND>(y, s);
   int8_t* q = p.q + (size_t)row * p.ldq;
 #pragma unroll
   for (int k = 0; k < 7; ++k)
@@ -601,29 +599,37 @@ void launch_rows(const RowArgs& a, hipStream_t s) {
              dim3(TPR < 128 ? 256 : TPR), 0, s, a);
 }
 
-// LayerNorms of 1025-16384 values, whose fp64 instructions are the longest part,
-// take as many threads as leave few of them idle: 192 or 384 with one vector each,
-// 256 or 512 with three (975x1283 5.1 -> 4.8 us against 256, 2048x5120 16.9 -> 12.6
-// and 1024x12000 20.3 -> 13.6 against 512 with two and four).  Many rows share what a
-// row has to do once among fewer threads: a wave with three vectors (fp16 3000x1280
-// 7.4 -> 6.6 us, 1536 rows the same, fp32 rows 7.6 -> 7.8) or four (16384x2048 36 ->
-// 31; below 4096 rows nothing), two waves with three (2048x2560 10.0 -> 8.5; 512 rows
-// 4.4 -> 5.0).
-template <class T>
-void layer_rows(const RowArgs& a, hipStream_t s) {
+// Rows of 1025-16384 values that are fp64 on their way.  Their instructions are the
+// longest part, or nearly, so they take as many threads as leave few of them idle:
+// 192 or 384 with one vector each, 256 or 512 with three (LayerNorm 975x1283 5.1 ->
+// 4.8 us against 256, 2048x5120 16.9 -> 12.6 and 1024x12000 20.3 -> 13.6 against 512
+// with two and four; RMS norm 8192x1280 13.3 -> 11.7, with residual 26.9 -> 27.2, and
+// 1024x12000 18.0 -> 13.1).  LayerNorms of many rows share what a row has to do once
+// among fewer threads: a wave with three vectors (fp16 3000x1280 7.4 -> 6.6 us, 1536
+// rows the same, fp32 rows 7.6 -> 7.8) or four (16384x2048 36 -> 31; below 4096 rows
+// nothing), two waves with three (2048x2560 10.0 -> 8.5; 512 rows 4.4 -> 5.0).  RMS
+// norms do not take 256 with three: 2048x5120 12.7 -> 12.1, but 28.2 -> 29.7 with a
+// residual.
+template <class T, RowKind KIND>
+void wide_rows(const RowArgs& a, hipStream_t s) {
+  constexpr bool LAYER = KIND == kLayer;
   const int S = (a.K + 7) / 8;  // vectors a row
-  if (S <= 256) {
-    if constexpr (sizeof(T) == 2) {
-      if (a.rows >= 2048 && S <= 192) return launch_rows<T, kLayer, 64, 3>(a, s);
-      if (a.rows >= 4096) return launch_rows<T, kLayer, 64, 4>(a, s);
-    }
-    return S <= 192 ? launch_rows<T, kLayer, 192, 1>(a, s) : launch_rows<T, kLayer, 256, 1>(a, s);
+  if constexpr (LAYER && sizeof(T) == 2) {
+    if (a.rows >= 2048 && S <= 192) return launch_rows<T, KIND, 64, 3>(a, s);
+    if (a.rows >= 4096 && S <= 256) return launch_rows<T, KIND, 64, 4>(a, s);
   }
-  if (S <= 384) return a.rows >= 1024 ? launch_rows<T, kLayer, 128, 3>(a, s) : launch_rows<T, kLayer, 384, 1>(a, s);
-  if (S <= 512) return launch_rows<T, kLayer, 256, 2>(a, s);
-  if (S <= 768) return launch_rows<T, kLayer, 256, 3>(a, s);
-  if (S <= 1024) return launch_rows<T, kLayer, 512, 2>(a, s);
-  return S <= 1536 ? launch_rows<T, kLayer, 512, 3>(a, s) : launch_rows<T, kLayer, 512, 4>(a, s);
+  if (S <= 192) return launch_rows<T, KIND, 192, 1>(a, s);
+  if (S <= 256) return launch_rows<T, KIND, 256, 1>(a, s);
+  if constexpr (LAYER) {
+    if (a.rows >= 1024 && S <= 384) return launch_rows<T, KIND, 128, 3>(a, s);
+  }
+  if (S <= 384) return launch_rows<T, KIND, 384, 1>(a, s);
+  if (S <= 512) return launch_rows<T, KIND, 256, 2>(a, s);
+  if constexpr (LAYER) {
+    if (S <= 768) return launch_rows<T, KIND, 256, 3>(a, s);
+  }
+  if (S <= 1024) return launch_rows<T, KIND, 512, 2>(a, s);
+  return S <= 1536 ? launch_rows<T, KIND, 512, 3>(a, s) : launch_rows<T, KIND, 512, 4>(a, s);
 }
 
 // Threads a row by its length: each holds one to four vectors.  Rows of 1025-2048
@@ -651,8 +657,8 @@ void row_q8(const RowArgs& a, hipStream_t s) {
     launch_rows<T, KIND, 64, 2>(a, s);
   } else if (K > 16384)
     DLM_LAUNCH("row_q8_long_kernel", (row_q8_long_kernel<T, KIND>), dim3(a.rows), dim3(1024), 0, s, a);
-  else if constexpr (KIND == kLayer)
-    layer_rows<T>(a, s);
+  else if constexpr (sizeof(Wide<T, KIND>) == 8)
+    wide_rows<T, KIND>(a, s);
   else if (K <= 2048)
     launch_rows<T, KIND, 256, 1>(a, s);
   else if (K <= 4096)

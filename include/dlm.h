@@ -485,11 +485,9 @@ int dlm_linear_small_fp16(const void* X, int ldx, const void* W, const void* bia
  *   a = max |v|,  q[k] = round(127 v[k] / a) (halves to the even integer),
  *   scale = a / 127,  so v[k] ~ q[k] * scale and |q| <= 127.
  * A row of zeros has scale 0 and q 0.  A row that holds an infinity or NaN
- * (or, in the RMS norm, whose product with gamma overflows fp32) has scale NaN
- * and q 0, so that everything computed from it is NaN.  A row's result depends on
- * that row alone.  Where v is exact in fp32 (fp16 rows; their products with an
- * fp16 gamma), and in the LayerNorm, whose v is fp64, q is the quotient's
- * nearest integer.
+ * has scale NaN and q 0, so that everything computed from it is NaN.  A row's
+ * result depends on that row alone.  q is the exact quotient's nearest integer
+ * (the LayerNorm's v is fp64, everything else exact).
  * x [rows, K] with row stride ldx (elements, >= K; any alignment of an
  * element); q has row stride ldq >= K bytes, of which K are written; a stride
  * of K rounded up to 16 on a 16-byte aligned q makes it an operand of
@@ -513,10 +511,10 @@ int dlm_dequantize_rows_f32(const void* q, int ldq, const float* scale, float* y
  *   LayerNorm: v = (h - mean) / sqrt(var + eps) gamma + beta
  * with the statistics over the stored h, in fp64 (in fp32 for the RMS norm of
  * fp16 rows), so that eps may be 0 for rows of any magnitude (but a LayerNorm of
- * equal values is NaN then); the RMS norm's products h gamma are fp32.  H (may be
- * NULL; only with R) receives h and may be x or R itself (same pointer and row
- * stride), but not overlap them otherwise.  gamma and beta are fp16 [K] and may
- * be NULL (1 and 0).  x, R, H are fp16 or, in the _f32 forms, fp32. */
+ * equal values is NaN then).  H (may be NULL; only with R) receives h and may be
+ * x or R itself (same pointer and row stride), but not overlap them otherwise.
+ * gamma and beta are fp16 [K] and may be NULL (1 and 0).  x, R, H are fp16 or,
+ * in the _f32 forms, fp32. */
 int dlm_rms_norm_q8_fp16(const void* x, int ldx, const void* R, int ldr, void* H, int ldh,
                          const void* gamma, void* q, int ldq, float* scale, int rows, int K, float eps,
                          void* stream);

@@ -188,14 +188,60 @@ def test_rms_norm_q8_of_tiny_and_huge_fp32_without_eps(gpu, K):
     f = torch.tensor([1e-41, 1e-36, 1e-30, 1e-23, 1e-20, 1.0, 1e18, 1e25, 1e35])
     x = spread(9, K, K, torch.float32).clamp(-99, 99) * f[:, None]
     g = cpu((K,), 3) * 0.3 + 1
-    for gamma in (None, g):
+    for gamma in (None, g, g * 1000, g / 1000):
         q, s = ops.rms_norm_q8(x.cuda(), None if gamma is None else gamma.cuda(), eps=0.0)
-        prod = x if gamma is None else x * gamma.float()
-        _, ref, top = Q.rows(prod.double())
+        prod = x.double() if gamma is None else x.double() * gamma.double()
+        _, ref, top = Q.rows(prod)
         ref_s = top / x.double().square().mean(1).sqrt()
         assert torch.equal(q.cpu().double(), ref)
-        # the product's rounding is in ref_s; the scale's own from fp64
+        # one rounding from fp64
         assert bool(((s.cpu().double() - ref_s).abs() <= U * (1 + 2.0 ** -20) * ref_s).all())
+
+
+@pytest.mark.parametrize("rows,K", [(300000, 5), (30000, 60), (20000, 77), (10000, 200), (8000, 320), (8192, 640),
+                                    (4099, 701), (8192, 1280), (5000, 1283), (4096, 1800), (1024, 2500), (512, 5000),
+                                    (300, 8192), (256, 12000), (150, 16384), (150, 20000)])
+def test_rms_norm_q8_integers_of_fp32_rows_are_those_of_64_bits(gpu, rows, K):
+    """Millions of products with gamma, some of whose quotients lie as close to a
+    half as the products' fp32 rounding is to them."""
+    announce(f"rms_norm_q8 {rows}x{K} against float64, fp32")
+    x = spread(rows, K, K, torch.float32).cuda()
+    r = cpu((rows, K), 2, torch.float32).cuda()
+    g = (cpu((K,), 3) * 0.3 + 1).cuda()
+    eps = torch.tensor(1e-5).double().cuda()
+    q, s, h = ops.rms_norm_q8(x, g, residual=r, eps=1e-5)
+    hd = h.double()
+    _, ref, top = Q.rows(hd * g.double())  # exact: 24 and 11 bits
+    assert int((q.double() != ref).sum()) == 0
+    ref = top / torch.sqrt(hd.square().mean(1) + eps)
+    assert bool(((s.double() - ref).abs() <= U * (1 + 2.0 ** -20) * ref).all())
+
+
+@pytest.mark.parametrize("K", [5, 77, 640, 1283, 5000, 20000])
+def test_norms_round_exact_halves_to_the_even_integer(gpu, K):
+    """Rows of small integers whose maximum makes many quotients half an integer
+    exactly: 254 v = (2k + 1) a for v = a / 2 and where 127 divides a."""
+    announce(f"norms of rows with exact halves, K={K}")
+    gen = torch.Generator().manual_seed(K)
+    top = torch.tensor([254, 2, 127 * 6, 127 * 16, 2046, 10, 127 * 14, 508])
+    x = torch.round((torch.rand(8, K, generator=gen) * 2 - 1).double() * top[:, None])
+    x[:, 0], x[:, 1] = top.double(), -(top // 2).double()
+    halves = (x * 254).remainder(top[:, None]) == 0
+    assert bool(((halves & ((x * 254 / top[:, None]).remainder(2) == 1)).sum(1) >= 1).all())
+    for dtype in (torch.float16, torch.float32):
+        for scale in (1.0, 2.0 ** -9):
+            h = (x * scale).to(dtype)
+            assert torch.equal(h.double(), x * scale)
+            _, ref, _ = Q.rows(x)
+            for gamma in (None, 1.0, 1.2998046875, -0.0625):
+                g = None if gamma is None else torch.full((K,), gamma, dtype=torch.float16, device="cuda")
+                q, _ = ops.rms_norm_q8(h.cuda(), g)
+                sign = -1.0 if gamma is not None and gamma < 0 else 1.0
+                assert torch.equal(q.cpu().double(), sign * ref), f"rms {dtype} {scale} {gamma}"
+            # beta alone: rows of equal values
+            for row in range(8):
+                q, _ = ops.layer_norm_q8(torch.ones(2, K, dtype=dtype, device="cuda"), None, h[row].half().cuda())
+                assert torch.equal(q.cpu().double(), ref[row].expand(2, K)), f"layer {dtype} {scale} {row}"
 
 
 def test_norms_of_zero_rows_without_eps(gpu):
