@@ -67,6 +67,37 @@ class AttentionVtArgs(ctypes.Structure):
     ]
 
 
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", P), ("k", P), ("q_out", P), ("k_out", P),
+        ("q_sb", LL), ("q_ss", LL), ("q_sh", LL),
+        ("k_sb", LL), ("k_ss", LL), ("k_sh", LL),
+        ("qo_sb", LL), ("qo_ss", LL), ("qo_sh", LL),
+        ("ko_sb", LL), ("ko_ss", LL), ("ko_sh", LL),
+        ("q_gamma", P), ("k_gamma", P), ("pos", P), ("pos_sb", LL), ("pos_ss", LL), ("freqs", P),
+        ("pos_type", I), ("axes", I), ("sections", I * 4), ("interleaved", I), ("norm", I),
+        ("eps", F), ("dtype", I), ("B", I), ("S", I), ("H", I), ("Hkv", I), ("Dh", I),
+    ]
+
+
+class AttentionMaskedArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", P), ("k", P), ("v", P), ("o", P),
+        ("q_sb", LL), ("q_ss", LL), ("q_sh", LL),
+        ("k_sb", LL), ("k_ss", LL), ("k_sh", LL),
+        ("v_sb", LL), ("v_ss", LL), ("v_sh", LL),
+        ("o_sb", LL), ("o_ss", LL), ("o_sh", LL),
+        ("key_range", P), ("kr_sb", LL), ("q_pos", P), ("qp_sb", LL), ("slopes", P), ("rel_bias", P),
+        ("R", I), ("scale", F), ("cap", F), ("causal", I), ("dtype", I),
+        ("B", I), ("Sq", I), ("Sk", I), ("H", I), ("Hkv", I), ("Dh", I),
+    ]
+
+
+# The same two as formats of the struct module: packing one is one call, against a
+# store per field (40 of them: 6 us of a one-token call).
+ROTARY_FORMAT = "@4P12q3P2qP2i4i2ifi5i0P"
+ATTENTION_MASKED_FORMAT = "@4P12qPqPqPPiffii6i0P"
+
 # name -> (restype, argtypes); every int-returning entry point is a status.
 HIP_SIGNATURES = {
     "dlm_last_error": (c_char_p, []),
@@ -135,6 +166,11 @@ HIP_SIGNATURES = {
     "dlm_layer_norm_q8_f32": (I, [P, I, P, I, P, I, P, P, P, I, P, I, I, F, P]),
     "dlm_linear_q8_fp16": (I, [P, I, P, P, I, P, P, P, I, P, I, I, I, I, F, I, P]),
     "dlm_linear_q8_f32out": (I, [P, I, P, P, I, P, P, P, I, P, I, I, I, I, F, I, P]),
+    # their argument structures as addresses: packed bytes or byref() of the classes above
+    "dlm_rotary_axes": (I, [P, P]),
+    "dlm_qk_norm_rotary": (I, [P, P]),
+    "dlm_attention_masked_workspace_bytes": (c_size_t, [P]),
+    "dlm_attention_masked": (I, [P, P, c_size_t, P]),
     "dlm_euler_cfg_step": (I, [P, P, P, I, F, F, F, F, P]),
     "dlm_euler_step": (I, [P, P, P, I, F, F, F, P]),
     "dlm_scale_latent_fp16": (I, [P, P, I, F, I, P]),

@@ -1,0 +1,859 @@
+// Attention with masks, capped scores and biases of distance, for fp16 and bf16,
+// grouped heads, from one query to long prompts.  No counterpart in the reference
+// (src/kernels/attention.cuh:53-73 has neither masks nor biases).
+//
+//   s = scale q.k;  s = cap tanh(s / cap);  s += bias(j - p);  o = softmax(s) v
+//
+// Every mask here is an interval of keys per query (documents, prefixes, lengths,
+// causal order, windows), so whole key tiles are left out, whole ones run without
+// mask code, and only those an interval ends in compare keys.
+//
+// Formulation (wave64, v_mfma_f32_32x32x16): a wave owns 32 rows, a row being a query
+// of one of the G heads that share a key head (row = query * G + head), so K and V are
+// read once for the group.  Scores are computed transposed, S^T = K Q^T, so that a lane
+// owns one row and every other four of its keys; exponentiated they are the B operand of O^T = V^T P^T
+// as they stand.  V stays [key][d] in LDS: ds_read_b64_tr_b16 hands a lane four keys of
+// its d.  K and V tiles come by DMA, 16-byte chunks of a row swizzled so that both kinds
+// of read touch every bank once.
+//
+// The softmax keeps a base m per row, moved only when a tile's maximum passes it by
+// 2^8: p = 2^((s - m) c + SH) stays far from fp16's ends (SH = 7: the row's largest p is
+// at least 2^7 times the smallest normal number's 2^14), and the accumulators are rescaled rarely.
+#include <cfloat>
+#include <climits>
+
+#include "dma.hpp"
+
+namespace dlm {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x8 __attribute__((ext_vector_type(8)));
+
+template <typename T> struct Half;
+template <> struct Half<f16> {
+  typedef f16x8 x8;
+  static constexpr float shift = 7.0f;
+  static constexpr unsigned inf = 0x7c00;
+  static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) { return mfma32x32x16(a, b, c); }
+  static __device__ __forceinline__ float dot2(f16x2 p, float c) {
+    return __builtin_amdgcn_fdot2(p, f16x2{(f16)1.0f, (f16)1.0f}, c, false);
+  }
+  typedef f16x2 x2;
+};
+template <> struct Half<__bf16> {
+  typedef bf16x8 x8;
+  static constexpr float shift = 0.0f;  // fp32's range: no p is too small
+  static constexpr unsigned inf = 0x7f80;
+  static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float dot2(bf16x2 p, float c) {
+    return __builtin_amdgcn_fdot2_f32_bf16(p, bf16x2{(__bf16)1.0f, (__bf16)1.0f}, c, false);
+  }
+  typedef bf16x2 x2;
+};
+
+struct AmParams {
+  const char* q;
+  const char* k;
+  const char* v;
+  char* o;
+  long long q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh, o_sb, o_ss, o_sh;  // elements
+  const int* key_range;
+  long long kr_sb;
+  const int* q_pos;
+  long long qp_sb;
+  const float* slopes;
+  const float* table;
+  int R;
+  int Sq, Sk, Hkv, G, Dh, rows;  // rows = Sq * G
+  int causal, nrb, heads, splits;  // row blocks, B * Hkv, parts of the keys
+  float scale, c, thr, cap;        // c: to powers of two; thr: 8 / c
+  float* part;                     // [splits][heads][rows][Dh], then [splits][heads][rows][2]
+};
+
+#define AM_WAIT_ALL() __builtin_amdgcn_s_waitcnt(0x70)  // vmcnt(0) lgkmcnt(0)
+#define AM_WAIT_LGKM() __builtin_amdgcn_s_waitcnt(0xC07F)
+
+__device__ __forceinline__ float am_max_halves(float x) {
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float am_sum_halves(float x) {
+  const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+__device__ __forceinline__ int am_wave_min(int v) {
+  return __builtin_amdgcn_readfirstlane(wave_reduce(v, [](int a, int b) { return a < b ? a : b; }));
+}
+__device__ __forceinline__ int am_wave_max(int v) {
+  return __builtin_amdgcn_readfirstlane(wave_reduce(v, [](int a, int b) { return a > b ? a : b; }));
+}
+
+// tanh(t) / t in u = t^2 on [0, 1/4]: Chebyshev fit of degree 4, relative error 1.4e-8
+__device__ __forceinline__ float tanh_ratio(float u) {
+  float r = __builtin_fmaf(0.017141319047f, u, -0.052989241175f);
+  r = __builtin_fmaf(r, u, 0.133248289977f);
+  r = __builtin_fmaf(r, u, -0.333330718942f);
+  return __builtin_fmaf(r, u, 0.999999987069f);
+}
+
+// A row's place and what it sees; all of it lives in the row's two lanes.
+struct Row {
+  int i, h;          // query, head
+  bool live, empty;  // a row of the call; one that sees no key
+  int lo, hi, p;
+  int tlo, thi;  // the wave's keys: from the first to behind the last that a row sees
+  int flo, fhi;  // keys that all its rows see
+  int pmin, pmax;
+};
+
+__device__ __forceinline__ Row am_row(const AmParams& p, int b, int hk, int r) {
+  Row w;
+  w.live = r < p.rows;
+  const int rc = w.live ? r : p.rows - 1;
+  w.i = rc / p.G;
+  w.h = hk * p.G + rc - w.i * p.G;
+  w.lo = 0;
+  w.hi = p.Sk;
+  if (p.key_range) {
+    const int2 x = *reinterpret_cast<const int2*>(p.key_range + b * p.kr_sb + 2LL * w.i);
+    w.lo = max(x.x, 0);
+    w.hi = min(x.y, p.Sk);
+  }
+  w.p = w.i + p.Sk - p.Sq;
+  if (p.q_pos) w.p = max(-(1 << 30), min(1 << 30, p.q_pos[b * p.qp_sb + w.i]));
+  if (p.causal && w.p < p.Sk) w.hi = min(w.hi, w.p + 1);
+  w.empty = w.lo >= w.hi;
+  // rows that see nothing, and those behind the last, run along unmasked: what they
+  // compute is never stored
+  const bool on = w.live && !w.empty;
+  w.tlo = am_wave_min(on ? w.lo : INT_MAX);
+  w.thi = am_wave_max(on ? w.hi : 0);
+  w.flo = am_wave_max(on ? w.lo : 0);
+  w.fhi = am_wave_min(on ? w.hi : INT_MAX);
+  w.pmin = am_wave_min(w.p);
+  w.pmax = am_wave_max(w.p);
+  if (!on) {
+    w.lo = INT_MIN;
+    w.hi = INT_MAX;
+  }
+  return w;
+}
+
+// What a wave does with tiles of KB * 32 keys.  PB: bytes of a key's row in LDS, DK:
+// steps of 16 dims, DV: blocks of 32 dims; NW: waves that fill a tile together.
+template <typename T, int PB, int DK, int DV, bool MOD, int KB, int NW>
+struct Core {
+  using Hf = Half<T>;
+  using x8 = typename Hf::x8;
+  static constexpr int BK = KB * 32;
+  static constexpr int TILE = BK * PB;       // bytes of the K (or V) tile
+  static constexpr int STAGE = 2 * TILE;
+  static constexpr int RPI = 1024 / PB;      // rows of one DMA instruction
+  static constexpr int NI = BK / RPI / NW;   // instructions of a wave and operand
+  static constexpr int CH = PB / 16;
+  // distinct swizzles among a wave's instructions
+  static constexpr int NKV = std::max(1, 16 / (NW * RPI));
+  static constexpr int NVV = std::max(1, 4 / (NW * RPI));
+  static_assert(NI * RPI * NW == BK && NI % NKV == 0 && NI % NVV == 0, "whole instructions");
+
+  const AmParams& p;
+  const Row& row;
+  const int lane, g;
+  const char* kbase;
+  const char* vbase;
+  unsigned koff[NKV], voff[NVV];
+  x8 qf[DK];
+  f32x16 o[DV];
+  float m, l, mref;
+  float slope, tabl, tabr;
+  const float* tab;
+
+  static __device__ __forceinline__ int kswz(int r) { return PB == 128 ? (r >> 1) & 7 : r & 15; }
+  static __device__ __forceinline__ int vswz(int r) { return PB == 128 ? (r & 2) << 1 : (r & 3) << 2; }
+
+  __device__ __forceinline__ Core(const AmParams& p_, const Row& row_, int b, int hk, int lane_, int wave)
+      : p(p_), row(row_), lane(lane_), g(lane_ >> 5) {
+    kbase = p.k + (b * p.k_sb + hk * p.k_sh) * 2;
+    vbase = p.v + (b * p.v_sb + hk * p.v_sh) * 2;
+    const int r0 = wave * RPI + lane / CH, phys = lane % CH;
+#pragma unroll
+    for (int i = 0; i < NKV; ++i) {
+      const int r = i * NW * RPI + r0, c = phys ^ kswz(r);
+      koff[i] = c * 8 < p.Dh ? (unsigned)(r * (int)p.k_ss * 2 + c * 16) : 0x80000000u;
+    }
+#pragma unroll
+    for (int i = 0; i < NVV; ++i) {
+      const int r = i * NW * RPI + r0, c = phys ^ vswz(r);
+      voff[i] = c * 8 < p.Dh ? (unsigned)(r * (int)p.v_ss * 2 + c * 16) : 0x80000000u;
+    }
+  }
+
+  __device__ __forceinline__ void load_q(int b) {
+    const T* qp = (const T*)p.q + b * p.q_sb + row.i * p.q_ss + row.h * p.q_sh + g * 8;
+#pragma unroll
+    for (int ds = 0; ds < DK; ++ds) {
+      const bool in = ds * 16 + g * 8 < p.Dh;
+      const x8 v = *reinterpret_cast<const x8*>(in ? qp + ds * 16 : qp - g * 8);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) qf[ds][e] = in ? v[e] : (T)0.0f;
+    }
+#pragma unroll
+    for (int dt = 0; dt < DV; ++dt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[dt][e] = 0.0f;
+    m = -INFINITY;
+    mref = 0.0f;
+    l = 0.0f;
+    if constexpr (MOD) {
+      slope = p.slopes ? p.slopes[row.h] : 0.0f;
+      tab = nullptr;
+      tabl = tabr = 0.0f;
+      if (p.table) {
+        tab = p.table + (long long)row.h * (2 * p.R + 1) + p.R;
+        tabl = tab[-p.R];
+        tabr = tab[p.R];
+      }
+    }
+  }
+
+  // Copies tile t into LDS: a buffer that starts at the tile's first row, so offsets stay
+  // small however long the cache, and ends with the last key's row (what lies past it, and
+  // dims past Dh, are zeros).
+  __device__ __forceinline__ void issue(unsigned char DLM_LDS* st, int t, int wave) const {
+    const int k0 = t * BK, n = min(BK, p.Sk - k0);
+    const i32x4 rk = dma_rsrc(kbase + (long long)k0 * p.k_ss * 2, (unsigned)(((n - 1) * (int)p.k_ss + p.Dh) * 2));
+    const i32x4 rv = dma_rsrc(vbase + (long long)k0 * p.v_ss * 2, (unsigned)(((n - 1) * (int)p.v_ss + p.Dh) * 2));
+    const unsigned ks = NKV * NW * RPI * (int)p.k_ss * 2, vs = NVV * NW * RPI * (int)p.v_ss * 2;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) dma16(rk, st + (i * NW + wave) * 1024, (int)(koff[i % NKV] + (i / NKV) * ks), 0);
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      dma16(rv, st + TILE + (i * NW + wave) * 1024, (int)(voff[i % NVV] + (i / NVV) * vs), 0);
+  }
+
+  __device__ __forceinline__ void scores(const unsigned char DLM_LDS* st, f32x16 (&s)[KB]) const {
+    const int base = (lane & 31) * PB + ((g ^ kswz(lane & 31)) * 16);
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[kb][e] = 0.0f;
+#pragma unroll
+    for (int ds = 0; ds < DK; ++ds)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const x8 kf = *reinterpret_cast<const x8 DLM_LDS*>(st + (base ^ (32 * ds)) + kb * 32 * PB);
+        s[kb] = Hf::mfma(kf, qf[ds], s[kb]);
+      }
+  }
+
+  // key of element e of block kb, against the tile's first key and without the lane's 4 g
+  static constexpr __device__ int key_of(int kb, int e) { return kb * 32 + 8 * (e >> 2) + (e & 3); }
+
+  // Cap and bias: s becomes the score itself (without them it stays q.k)
+  __device__ __forceinline__ void modify(f32x16 (&s)[KB], int k0) const {
+    if (p.cap > 0.0f) {
+      const float ic = p.scale / p.cap;
+      float top = 0.0f;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          s[kb][e] *= ic;
+          top = fmaxf(top, fabsf(s[kb][e]));
+        }
+      if (__builtin_amdgcn_ballot_w64(!(top <= 0.5f)) == 0) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float t = s[kb][e];
+            s[kb][e] = t * p.cap * tanh_ratio(t * t);
+          }
+      } else {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float x = __builtin_amdgcn_exp2f(s[kb][e] * 2.8853900817779268f);  // e^2t
+            s[kb][e] = __builtin_fmaf(-2.0f * p.cap, __builtin_amdgcn_rcpf(1.0f + x), p.cap);
+          }
+      }
+    } else {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[kb][e] *= p.scale;
+    }
+    const int d0 = k0 + 4 * g - row.p;
+    if (p.slopes) {
+      const float f0 = (float)d0;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          s[kb][e] = __builtin_fmaf(-slope, fabsf(f0 + (float)key_of(kb, e)), s[kb][e]);
+    }
+    if (p.table) {
+      if (k0 + BK - 1 - row.pmin <= -p.R || k0 - row.pmax >= p.R) {
+        const float left = tabl, right = tabr, t = k0 - row.pmax >= p.R ? right : left;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[kb][e] += t;
+      } else {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[kb][e] += tab[max(-p.R, min(p.R, d0 + key_of(kb, e)))];
+      }
+    }
+  }
+
+  __device__ __forceinline__ x8 vfrag(const unsigned char DLM_LDS* st, int j, int dt) const {
+    const int r4 = (lane & 15) >> 2;
+    const int base = (4 * g + r4) * PB + vswz(r4) * 16 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+    const unsigned char DLM_LDS* a = st + TILE + (base ^ (64 * dt)) + 16 * j * PB;
+    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 DLM_LDS*)a);
+    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 DLM_LDS*)(a + 8 * PB));
+    return __builtin_bit_cast(x8, i16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+  }
+
+  static __device__ __forceinline__ bool not_finite(short x) { return ((unsigned short)x & Hf::inf) == Hf::inf; }
+
+  // O^T += V^T P^T of a tile whose V holds infinities or NaN, where 0 * V would spoil
+  // rows that do not see them: the finite values by the product, and for each kind of the
+  // others the count of those that a row sees.
+  static __device__ __forceinline__ void pv_special(f32x16 (&o)[DV], const x8 (&pf)[2 * KB], unsigned seen,
+                                                              const Core& c, const unsigned char DLM_LDS* st) {
+#pragma unroll
+    for (int dt = 0; dt < DV; ++dt) {
+      f32x16 n[3];
+#pragma unroll
+      for (int w = 0; w < 3; ++w)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) n[w][e] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 2 * KB; ++j) {
+        const i16x8 v = __builtin_bit_cast(i16x8, c.vfrag(st, j, dt));
+        x8 fin, k[3], one;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const short bits = v[e];  // (an element itself is no operand of bit_cast)
+          const unsigned short x = (unsigned short)bits;
+          const bool odd = not_finite(bits), nan = odd && (x & 0x7fff) != Hf::inf;
+          fin[e] = odd ? (T)0.0f : __builtin_bit_cast(T, bits);
+          k[0][e] = odd && !nan && !(x & 0x8000) ? (T)1.0f : (T)0.0f;
+          k[1][e] = odd && !nan && (x & 0x8000) ? (T)1.0f : (T)0.0f;
+          k[2][e] = nan ? (T)1.0f : (T)0.0f;
+          one[e] = seen >> (8 * j + e) & 1 ? (T)1.0f : (T)0.0f;
+        }
+        o[dt] = Hf::mfma(fin, pf[j], o[dt]);
+#pragma unroll
+        for (int w = 0; w < 3; ++w) n[w] = Hf::mfma(k[w], one, n[w]);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if (n[0][e] > 0.0f) o[dt][e] += INFINITY;
+        if (n[1][e] > 0.0f) o[dt][e] -= INFINITY;
+        if (n[2][e] > 0.0f) o[dt][e] = NAN;
+      }
+    }
+  }
+
+  // One tile in LDS at st
+  __device__ __forceinline__ void tile(const unsigned char DLM_LDS* st, int t) {
+    const int k0 = t * BK;
+    f32x16 s[KB];
+    scores(st, s);
+    if constexpr (MOD) modify(s, k0);
+    bool guard = false;
+    if (k0 < row.flo || k0 + BK > row.fhi) {
+      guard = true;
+      // in 32 bits whatever the bounds: lo and hi against the tile's first key
+      const int lo = max(row.lo, k0) - k0 - 4 * g, hi = min(row.hi, k0 + BK) - k0 - 4 * g;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (key_of(kb, e) < lo || key_of(kb, e) >= hi) s[kb][e] = -INFINITY;
+    }
+    float mt = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[kb][e]);
+    mt = am_max_halves(mt);
+    if constexpr (MOD) {
+      if (p.table && !guard) {  // an entry of -infinity masks its distance
+        float low = s[0][0];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) low = fminf(low, s[kb][e]);
+        guard = __builtin_amdgcn_ballot_w64(low == -INFINITY) != 0;
+      }
+    }
+    if (__builtin_amdgcn_ballot_w64(mt > m + p.thr)) {
+      const bool move = mt > m + p.thr;
+      const float alpha = move ? __builtin_amdgcn_exp2f((m - mt) * p.c) : 1.0f;
+      m = move ? mt : m;
+      mref = m == -INFINITY ? 0.0f : MOD ? m : __builtin_fmaf(m, p.c, -Hf::shift);
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DV; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+    }
+    unsigned seen = 0;
+    bool special = false;
+    if (guard) {
+      unsigned bad = 0;
+#pragma unroll
+      for (int j = 0; j < 2 * KB; ++j)
+#pragma unroll
+        for (int dt = 0; dt < DV; ++dt) {
+          const i16x8 v = __builtin_bit_cast(i16x8, vfrag(st, j, dt));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) bad |= not_finite(v[e]);
+        }
+      special = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+      if (special) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) seen |= (s[kb][e] != -INFINITY ? 1u : 0u) << (16 * kb + e);
+      }
+    }
+    x8 pf[2 * KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        // without cap and bias (scale and log2 e in one): one multiply-add; else the
+        // difference first, which scores of the largest magnitude survive
+        const float x = MOD ? __builtin_fmaf(s[kb][e] - mref, p.c, Hf::shift) : __builtin_fmaf(s[kb][e], p.c, -mref);
+        pf[2 * kb + (e >> 3)][e & 7] = (T)__builtin_amdgcn_exp2f(x);
+      }
+#pragma unroll
+    for (int j = 0; j < 2 * KB; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) l = Hf::dot2(typename Hf::x2{pf[j][e], pf[j][e + 1]}, l);
+    if (special) {
+      pv_special(o, pf, seen, *this, st);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 2 * KB; ++j)
+#pragma unroll
+      for (int dt = 0; dt < DV; ++dt) o[dt] = Hf::mfma(vfrag(st, j, dt), pf[j], o[dt]);
+  }
+};
+
+// d of element e of output block dt, without the lane's 4 g
+__device__ __forceinline__ int am_dim(int dt, int e4) { return dt * 32 + 8 * e4; }
+
+__device__ __forceinline__ float* am_part_o(const AmParams& p, int split, int head, int r) {
+  return p.part + (((long long)split * p.heads + head) * p.rows + r) * p.Dh;
+}
+__device__ __forceinline__ float* am_part_ml(const AmParams& p, int split, int head, int r) {
+  return p.part + (long long)p.splits * p.heads * p.rows * p.Dh +
+         (((long long)split * p.heads + head) * p.rows + r) * 2;
+}
+
+template <typename T>
+__device__ __forceinline__ void am_store4(const AmParams& p, int b, int i, int h, int d, float x0, float x1, float x2,
+                                          float x3) {
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<t4*>((T*)p.o + b * p.o_sb + i * p.o_ss + h * p.o_sh + d) = t4{(T)x0, (T)x1, (T)x2, (T)x3};
+}
+
+// Tiles of part `split` of the keys [lo, hi).
+__device__ __forceinline__ void am_span(int lo, int hi, int bk, int splits, int split, int& t0, int& t1) {
+  if (lo >= hi) {
+    t0 = t1 = 0;
+    return;
+  }
+  const int a = lo / bk, b = (hi - 1) / bk + 1;
+  const int per = (b - a + splits - 1) / splits;
+  t0 = min(b, a + split * per);
+  t1 = min(b, t0 + per);
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: 4 waves of 32 rows share tiles of 64 keys.
+// ---------------------------------------------------------------------------
+template <typename T, int PB, int DK, int DV, bool MOD>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PB == 512 ? 1 : 2)))
+attn_masked_kernel(AmParams p) {
+  using C = Core<T, PB, DK, DV, MOD, 2, 4>;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem_g[2 * C::STAGE];
+  __shared__ int span[8];
+  unsigned char DLM_LDS* smem = (unsigned char DLM_LDS*)smem_g;
+  // consecutive blocks (the row blocks of one key head, then the next head) on one XCD,
+  // whose L2 then holds the K and V of its own heads; the last row blocks, which see the most
+  // keys where the mask is causal, first
+  int split, head, rb;
+  {
+    const int total = p.nrb * p.heads * p.splits;
+    const int q8 = total >> 3, r8 = total & 7;
+    const int x = blockIdx.x & 7, slot = blockIdx.x >> 3;
+    const int logical = x * q8 + (x < r8 ? x : r8) + slot;
+    const int u = logical / p.splits;
+    split = logical - u * p.splits;
+    head = u / p.nrb;
+    rb = p.nrb - 1 - (u - head * p.nrb);
+  }
+  const int b = head / p.Hkv, hk = head - b * p.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = rb * 128 + wave * 32 + (lane & 31);
+  const Row row = am_row(p, b, hk, r);
+  if (lane == 0) {
+    span[2 * wave] = row.tlo;
+    span[2 * wave + 1] = row.thi;
+  }
+  C c(p, row, b, hk, lane, wave);
+  c.load_q(b);
+  __syncthreads();
+  const int lo = __builtin_amdgcn_readfirstlane(min(min(span[0], span[2]), min(span[4], span[6])));
+  const int hi = __builtin_amdgcn_readfirstlane(max(max(span[1], span[3]), max(span[5], span[7])));
+  int t0, t1;
+  am_span(lo, hi, C::BK, p.splits, split, t0, t1);
+  if (t0 < t1) c.issue(smem, t0, wave);
+  int buf = 0;
+  for (int t = t0; t < t1; ++t) {
+    // tile t has arrived (this wave's part, then everyone's), and all are done with t - 1
+    AM_WAIT_ALL();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    if (t + 1 < t1) c.issue(smem + (buf ^ 1) * C::STAGE, t + 1, wave);
+    const int k0 = t * C::BK;
+    if (k0 < row.thi && k0 + C::BK > row.tlo) c.tile(smem + buf * C::STAGE, t);
+    buf ^= 1;
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  const float l = am_sum_halves(c.l);
+  if (!row.live) return;
+  if (p.splits > 1) {
+    float* po = am_part_o(p, split, head, r);
+#pragma unroll
+    for (int dt = 0; dt < DV; ++dt)
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        const int d = am_dim(dt, e4) + 4 * c.g;
+        if (d < p.Dh)
+          *reinterpret_cast<f32x4*>(po + d) =
+              f32x4{c.o[dt][4 * e4], c.o[dt][4 * e4 + 1], c.o[dt][4 * e4 + 2], c.o[dt][4 * e4 + 3]};
+      }
+    if (c.g == 0) {
+      float* ml = am_part_ml(p, split, head, r);
+      ml[0] = row.empty ? -INFINITY : c.m;
+      ml[1] = row.empty ? 0.0f : l;
+    }
+    return;
+  }
+  const bool none = row.empty || l == 0.0f;
+  const float inv = 1.0f / l;
+#pragma unroll
+  for (int dt = 0; dt < DV; ++dt)
+#pragma unroll
+    for (int e4 = 0; e4 < 4; ++e4) {
+      const int d = am_dim(dt, e4) + 4 * c.g;
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = none ? 0.0f : c.o[dt][4 * e4 + e] * inv;
+      if (d < p.Dh) am_store4<T>(p, b, row.i, row.h, d, x[0], x[1], x[2], x[3]);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: every wave of a workgroup holds the same 32 rows and takes every NW-th tile of
+// 32 keys through a ring of its own, without barriers; the waves' parts meet in LDS.  Bound
+// by K and V from memory, two tiles a wave in flight.
+// ---------------------------------------------------------------------------
+template <typename T, int PB, int DK, int DV, bool MOD>
+__global__ void __launch_bounds__(PB == 512 ? 128 : 256) __attribute__((amdgpu_waves_per_eu(1)))
+attn_masked_rows_kernel(AmParams p) {
+  constexpr int NW = PB == 512 ? 2 : 4;
+  using C = Core<T, PB, DK, DV, MOD, 1, 1>;
+  constexpr int RING = 2 * C::STAGE;
+  constexpr int D = DV * 32;
+  static_assert(NW * 32 * D * 4 <= NW * RING, "the waves' parts fit the rings");
+  __shared__ __attribute__((aligned(1024))) unsigned char smem_g[NW * RING];
+  __shared__ float ml[NW][32][2];
+  const int rb = blockIdx.x, head = blockIdx.y, split = blockIdx.z;
+  const int b = head / p.Hkv, hk = head - b * p.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  unsigned char DLM_LDS* smem = (unsigned char DLM_LDS*)smem_g + wave * RING;
+  const Row row = am_row(p, b, hk, rb * 32 + (lane & 31));
+  C c(p, row, b, hk, lane, 0);
+  int t0, t1;
+  am_span(row.tlo, row.thi, C::BK, p.splits, split, t0, t1);
+  int t = t0 + wave;
+  if (t < t1) c.issue(smem, t, 0);
+  if (t + NW < t1) c.issue(smem + C::STAGE, t + NW, 0);
+  c.load_q(b);
+  int buf = 0;
+  for (; t < t1; t += NW) {
+    if (t + NW < t1) {
+      DLM_WAIT_VM(2 * C::NI);  // the next tile's requests may be in flight
+    } else {
+      DLM_WAIT_VM(0);
+    }
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    c.tile(smem + buf * C::STAGE, t);
+    __builtin_amdgcn_sched_barrier(0);
+    AM_WAIT_LGKM();  // this tile's fragments are read
+    asm volatile("" ::: "memory");
+    if (t + 2 * NW < t1) c.issue(smem + buf * C::STAGE, t + 2 * NW, 0);
+    buf ^= 1;
+  }
+  const float l = am_sum_halves(c.l);
+  if (lane < 32) {
+    ml[wave][lane][0] = c.m;
+    ml[wave][lane][1] = l;
+  }
+  __syncthreads();
+  // this wave's sums in the units of the largest base, then all waves' together
+  float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) top = fmaxf(top, ml[w][lane & 31][0]);
+  auto weight = [&](float m) { return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - top) * p.c); };
+#pragma unroll
+  for (int w = 0; w < NW; ++w) sum += ml[w][lane & 31][1] * weight(ml[w][lane & 31][0]);
+  const float mine = weight(c.m);
+  float DLM_LDS* part = (float DLM_LDS*)smem_g;  // [wave][d][row]
+#pragma unroll
+  for (int dt = 0; dt < DV; ++dt)
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      part[(wave * D + am_dim(dt, e >> 2) + 4 * c.g + (e & 3)) * 32 + (lane & 31)] =
+          c.m == -INFINITY ? 0.0f : c.o[dt][e] * mine;
+  __syncthreads();
+  if (!row.live) return;
+  const int r = rb * 32 + (lane & 31);
+  const bool none = row.empty || sum == 0.0f;
+  const float inv = 1.0f / sum;
+  for (int d = (tid >> 5) * 4; d < p.Dh; d += NW * 8) {
+    float x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float a = 0.0f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) a += part[(w * D + d + e) * 32 + (lane & 31)];
+      x[e] = a;
+    }
+    if (p.splits > 1) {
+      *reinterpret_cast<f32x4*>(am_part_o(p, split, head, r) + d) = f32x4{x[0], x[1], x[2], x[3]};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = none ? 0.0f : x[e] * inv;
+      am_store4<T>(p, b, row.i, row.h, d, x[0], x[1], x[2], x[3]);
+    }
+  }
+  if (p.splits > 1 && tid < 32) {
+    float* q = am_part_ml(p, split, head, r);
+    q[0] = row.empty ? -INFINITY : top;
+    q[1] = row.empty ? 0.0f : sum;
+  }
+}
+
+// Joins the parts of every row; a thread takes four dims.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_masked_join_kernel(AmParams p) {
+  const int per = p.Dh / 4;
+  const long long at = blockIdx.x * 256LL + threadIdx.x;
+  const long long total = (long long)p.heads * p.rows;
+  const long long hr = at / per;
+  if (hr >= total) return;
+  const int d = (int)(at - hr * per) * 4;
+  const int head = (int)(hr / p.rows), r = (int)(hr - (long long)head * p.rows);
+  float top = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) top = fmaxf(top, am_part_ml(p, s, head, r)[0]);
+  float sum = 0.0f;
+  f32x4 a{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 ml = *reinterpret_cast<const float2*>(am_part_ml(p, s, head, r));
+    const f32x4 x = *reinterpret_cast<const f32x4*>(am_part_o(p, s, head, r) + d);
+    if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // saw no key
+    const float w = __builtin_amdgcn_exp2f((ml.x - top) * p.c);
+    sum = __builtin_fmaf(ml.y, w, sum);
+    a += x * w;
+  }
+  const float inv = 1.0f / sum;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) a[e] = sum == 0.0f ? 0.0f : a[e] * inv;
+  const int b = head / p.Hkv, hk = head - b * p.Hkv, i = r / p.G;
+  am_store4<T>(p, b, i, hk * p.G + r - i * p.G, d, a[0], a[1], a[2], a[3]);
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+// Which kernel, and over how many parts of the keys: by the sizes alone, since what the
+// masks leave is known on the device only.
+struct AmPlan {
+  bool few;
+  int nrb, splits;
+};
+static AmPlan am_plan(const dlm_attention_masked_args* a) {
+  const long long heads = (long long)a->B * a->Hkv, rows = (long long)a->Sq * (a->H / a->Hkv);
+  AmPlan pl;
+  pl.few = rows <= 64;
+  pl.nrb = (int)((rows + (pl.few ? 31 : 127)) / (pl.few ? 32 : 128));
+  const long long blocks = heads * pl.nrb;
+  const long long want = pl.few ? 256 : 512, unit = pl.few ? 512 : 256;
+  pl.splits = (int)std::max<long long>(1, std::min({(want + blocks - 1) / blocks, (long long)(a->Sk + unit - 1) / unit, 64LL}));
+  return pl;
+}
+
+static size_t am_workspace(const dlm_attention_masked_args* a, const AmPlan& pl) {
+  if (pl.splits == 1) return 0;
+  return (size_t)pl.splits * a->B * a->H * a->Sq * (a->Dh + 2) * 4;
+}
+
+template <typename T, int PB, int DK, int DV, bool MOD>
+static int am_launch(const AmParams& p, const AmPlan& pl, hipStream_t s) {
+  if (pl.few)
+    DLM_LAUNCH("attn_masked_rows_kernel", (attn_masked_rows_kernel<T, PB, DK, DV, MOD>),
+               dim3(pl.nrb, p.heads, pl.splits), dim3(PB == 512 ? 128 : 256), 0, s, p);
+  else
+    DLM_LAUNCH("attn_masked_kernel", (attn_masked_kernel<T, PB, DK, DV, MOD>), dim3(pl.nrb * p.heads * pl.splits),
+               dim3(256), 0, s, p);
+  DLM_LAUNCH_CHECK();
+  if (pl.splits > 1) {
+    const long long n = (long long)p.heads * p.rows * (p.Dh / 4);
+    DLM_LAUNCH("attn_masked_join_kernel", attn_masked_join_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s,
+               p);
+    DLM_LAUNCH_CHECK();
+  }
+  return DLM_OK;
+}
+
+template <typename T, bool MOD>
+static int am_by_head(const AmParams& p, const AmPlan& pl, hipStream_t s) {
+  if (p.Dh <= 64) return am_launch<T, 128, 4, 2, MOD>(p, pl, s);
+  if (p.Dh <= 96) return am_launch<T, 256, 6, 3, MOD>(p, pl, s);
+  if (p.Dh <= 128) return am_launch<T, 256, 8, 4, MOD>(p, pl, s);
+  return am_launch<T, 512, 16, 8, MOD>(p, pl, s);
+}
+
+static int am_check(const char* fn, const dlm_attention_masked_args* a) {
+  auto bad = [&](const std::string& m) { return fail(DLM_ERR_INVALID_ARG, std::string(fn) + ": " + m); };
+  if (!a->q || !a->o || (a->Sk > 0 && (!a->k || !a->v))) return bad("NULL operand");
+  if (a->dtype != DLM_DTYPE_F16 && a->dtype != DLM_DTYPE_BF16) return bad("unknown dtype");
+  if (a->Sk < 0) return bad("negative number of keys");
+  if (a->Dh % 8 != 0 || a->Dh > 256) return bad("Dh must be a multiple of 8 and at most 256");
+  if (a->Hkv <= 0 || a->H % a->Hkv != 0) return bad("H must be a multiple of Hkv");
+  if (!(a->scale > 0.0f && a->scale < INFINITY)) return bad("scale must be positive and finite");
+  if (!(a->cap >= 0.0f && a->cap < INFINITY)) return bad("cap must be finite and not negative");
+  if (a->slopes && a->rel_bias) return bad("one bias of distance, slopes or a table");
+  if (a->rel_bias && (a->R < 0 || a->R > (1 << 24))) return bad("R must be 0 to 2^24");
+  if (a->Sq > (1 << 28) || a->Sk > (1 << 28)) return bad("more than 2^28 queries or keys");
+  const long long G = a->H / a->Hkv;
+  if (a->Sq * G >= (1LL << 30) || (long long)a->B * a->Hkv > 65535) return bad("more rows or heads than a grid takes");
+  if ((long long)a->B * a->Hkv * ((a->Sq * G + 31) / 32) >= (1LL << 24)) return bad("more rows than a grid takes");
+  struct Op {
+    const char* name;
+    const void* p;
+    long long sb, ss, sh;
+    int S, H, unit, align;
+  };
+  Op ops[4] = {{"q", a->q, a->q_sb, a->q_ss, a->q_sh, a->Sq, a->H, 8, 16},
+               {"k", a->k, a->k_sb, a->k_ss, a->k_sh, a->Sk, a->Hkv, 8, 16},
+               {"v", a->v, a->v_sb, a->v_ss, a->v_sh, a->Sk, a->Hkv, 8, 16},
+               {"o", a->o, a->o_sb, a->o_ss, a->o_sh, a->Sq, a->H, 4, 8}};
+  uintptr_t lo[4], hi[4];
+  for (int i = 0; i < 4; ++i) {
+    Op& x = ops[i];
+    if (a->B == 1) x.sb = 0;  // a dimension of one has no stride
+    if (x.S <= 1) x.ss = 0;
+    if (x.H == 1) x.sh = 0;
+    if (x.sb < 0 || x.ss < 0 || x.sh < 0) return bad(std::string(x.name) + ": negative stride");
+    if ((uintptr_t)x.p % x.align != 0 || x.sb % x.unit != 0 || x.ss % x.unit != 0 || x.sh % x.unit != 0)
+      return bad(std::string(x.name) + (i < 3 ? ": address and strides must keep 16-byte alignment"
+                                              : ": address and strides must keep 8-byte alignment"));
+    const double last = (double)(a->B - 1) * (double)x.sb + (double)(std::max(x.S, 1) - 1) * (double)x.ss +
+                        (double)(x.H - 1) * (double)x.sh + a->Dh;
+    if (last > 0x1p46) return bad(std::string(x.name) + " spans more than 2^46 elements");
+    if ((i == 1 || i == 2) && x.S > 1 && (x.ss < a->Dh || x.ss >= (1 << 23)))
+      return bad(std::string(x.name) + ": a key row's stride must be Dh to 2^23");
+    lo[i] = (uintptr_t)x.p;
+    hi[i] = lo[i] + (uintptr_t)last * 2;
+  }
+  // an output's own elements have to lie apart
+  {
+    struct Dim {
+      long long st;
+      int n;
+    } d[3] = {{ops[3].sb, a->B}, {ops[3].ss, a->Sq}, {ops[3].sh, a->H}};
+    std::sort(d, d + 3, [](const Dim& x, const Dim& y) { return x.st < y.st; });
+    long long inner = a->Dh;
+    for (const Dim& x : d) {
+      if (x.n <= 1) continue;
+      if (x.st < inner) return bad("o overlaps itself");
+      inner += (x.n - 1) * x.st;
+    }
+  }
+  for (int i = 0; i < 3; ++i)
+    if (ops[i].S > 0 && lo[3] < hi[i] && lo[i] < hi[3]) return bad(std::string("o overlaps ") + ops[i].name);
+  if ((uintptr_t)a->key_range % 8 != 0 || (uintptr_t)a->q_pos % 4 != 0 || (uintptr_t)a->slopes % 4 != 0 ||
+      (uintptr_t)a->rel_bias % 4 != 0)
+    return bad("key_range must be 8-byte, q_pos, slopes and rel_bias 4-byte aligned");
+  if (a->kr_sb < 0 || a->kr_sb % 2 != 0 || a->qp_sb < 0) return bad("batch strides of the masks must be whole and not negative");
+  return DLM_OK;
+}
+
+}  // namespace dlm
+
+using namespace dlm;
+
+extern "C" {
+
+size_t dlm_attention_masked_workspace_bytes(const dlm_attention_masked_args* a) {
+  if (!a || a->B <= 0 || a->Sq <= 0 || a->H <= 0 || a->Dh <= 0 || a->Hkv <= 0 || a->H % a->Hkv != 0) return 0;
+  return am_workspace(a, am_plan(a));
+}
+
+int dlm_attention_masked(const dlm_attention_masked_args* a, void* workspace, size_t workspace_bytes, void* stream) {
+  DLM_REQUIRE(a != nullptr, "args is NULL");
+  if (a->B <= 0 || a->Sq <= 0 || a->H <= 0 || a->Dh <= 0) return DLM_OK;
+  if (const int st = am_check(__func__, a)) return st;
+  const AmPlan pl = am_plan(a);
+  const size_t need = am_workspace(a, pl);
+  if (need > 0) {
+    DLM_REQUIRE(workspace != nullptr && workspace_bytes >= need, "the workspace is too small");
+    DLM_REQUIRE(dlm_aligned16(workspace), "the workspace must be 16-byte aligned");
+  }
+  AmParams p{};
+  p.q = (const char*)a->q, p.k = (const char*)a->k, p.v = (const char*)a->v, p.o = (char*)a->o;
+  p.q_sb = a->q_sb, p.q_ss = a->q_ss, p.q_sh = a->q_sh;
+  p.k_sb = a->k_sb, p.k_ss = a->Sk > 1 ? a->k_ss : a->Dh, p.k_sh = a->k_sh;
+  p.v_sb = a->v_sb, p.v_ss = a->Sk > 1 ? a->v_ss : a->Dh, p.v_sh = a->v_sh;
+  p.o_sb = a->o_sb, p.o_ss = a->o_ss, p.o_sh = a->o_sh;
+  p.key_range = a->key_range, p.kr_sb = a->kr_sb;
+  p.q_pos = a->q_pos, p.qp_sb = a->qp_sb;
+  p.slopes = a->slopes, p.table = a->rel_bias, p.R = a->R;
+  p.Sq = a->Sq, p.Sk = a->Sk, p.Hkv = a->Hkv, p.G = a->H / a->Hkv, p.Dh = a->Dh;
+  p.rows = a->Sq * p.G;
+  p.causal = a->causal != 0, p.nrb = pl.nrb, p.heads = a->B * a->Hkv, p.splits = pl.splits;
+  p.scale = a->scale, p.cap = a->cap;
+  p.part = (float*)workspace;
+  const float log2e = 1.4426950408889634f;
+  // (a scale past ln 2 could carry the largest of scores past fp32 on the short path)
+  const bool mod = a->cap > 0.0f || a->slopes || a->rel_bias || a->scale * log2e > 1.0f;
+  p.c = mod ? log2e : a->scale * log2e;
+  p.thr = std::min(8.0f / p.c, 1e38f);
+  hipStream_t s = (hipStream_t)stream;
+  if (a->dtype == DLM_DTYPE_F16) return mod ? am_by_head<f16, true>(p, pl, s) : am_by_head<f16, false>(p, pl, s);
+  return mod ? am_by_head<__bf16, true>(p, pl, s) : am_by_head<__bf16, false>(p, pl, s);
+}
+
+}  // extern "C"

@@ -19,7 +19,8 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import Optional
+import struct
+from typing import Optional, Sequence
 
 import torch
 
@@ -35,7 +36,8 @@ __all__ = [
     "launch_conv_bias_residual", "launch_timestep_embedding", "linear", "pack_conv_weight",
     "conv2d_nhwc", "group_norm_nhwc", "attention_strided", "pack_geglu", "nchw_to_nhwc",
     "nhwc_to_nchw", "linear_small", "sdxl_embed_inputs", "quantize_rows", "dequantize_rows",
-    "rms_norm_q8", "layer_norm_q8", "linear_q8",
+    "rms_norm_q8", "layer_norm_q8", "linear_q8", "rotary_freqs", "rotary_axes", "qk_norm_rotary",
+    "document_ranges", "prefix_ranges", "attention_masked",
     "ACT_NONE", "ACT_SILU", "ACT_GEGLU", "ACT_GELU",
 ]
 
@@ -927,4 +929,233 @@ def linear_q8(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.Te
     fn = _entry("dlm_linear_q8_fp16" if out.dtype == torch.float16 else "dlm_linear_q8_f32out")
     _lib.check(fn(xq.data_ptr(), ldx, psx, wq.data_ptr(), ldw, psw, pb, pr, ldr, out.data_ptr(), ldy, M, N, K, beta,
                   act, _stream_of(dev)))
+    return out
+
+
+# ---------------------------------------------------------------------------
+# Attention with positions, masks and biases.  Operands are [batch, token, head, Dh] or
+# [token, head, Dh] views, fp16 or bf16, with any strides as long as a head's values are
+# consecutive: slices of a fused projection, a cache's used part, head-major layouts
+# seen through transpose.
+# ---------------------------------------------------------------------------
+_HALF = {torch.float16: 0, torch.bfloat16: 1}
+_POS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+_pack_rotary = struct.Struct(_lib.ROTARY_FORMAT).pack
+_pack_attention = struct.Struct(_lib.ATTENTION_MASKED_FORMAT).pack
+
+
+def _heads_dev(t: torch.Tensor, name: str) -> int:
+    """The current device, whose current stream a call runs on; t has to be on it."""
+    dev = t.get_device()
+    if dev < 0 or dev != torch._C._cuda_getDevice():
+        raise ValueError(f"{name} must be on the current GPU, got {t.device}")
+    if t.dtype not in _HALF:
+        raise ValueError(f"{name} must be float16 or bfloat16, got {t.dtype}")
+    if t.dim() not in (3, 4):
+        raise ValueError(f"{name} must be [batch, token, head, Dh] or [token, head, Dh], got {list(t.shape)}")
+    return dev
+
+
+def _heads(t: torch.Tensor, shape, dtype, name: str, dev: int):
+    """(batch, token, head) strides of t, which has to be `shape` of `dtype` on device `dev`."""
+    if t.dtype == dtype and t.shape == shape and t.get_device() == dev:
+        st = t.stride()
+        if st[-1] == 1 or shape[-1] == 1:
+            return st[:3] if len(st) == 4 else (0, st[0], st[1])
+        raise ValueError(f"{name} must have consecutive values in a head")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    raise ValueError(f"{name} must be on the current device, cuda:{dev}, got {t.device}")
+
+
+def rotary_freqs(sections: Sequence[int], theta: float = 10000.0, shared: bool = False, device="cuda") -> torch.Tensor:
+    """Frequencies (fp64, radians per position) of sum(sections) pairs: every axis runs
+    through theta^(-i / n) over its own n pairs, or, where shared, the axes take
+    consecutive parts of one such run over all pairs."""
+    if any(n < 0 for n in sections):
+        raise ValueError("a section has a negative number of pairs")
+    if shared:
+        n = sum(sections)
+        f = [theta ** (-i / n) for i in range(n)]
+    else:
+        f = [theta ** (-i / n) for n in sections for i in range(n)]
+    return torch.tensor(f, dtype=torch.float64).to(device)
+
+
+def _rotary(name, q, k, q_gamma, k_gamma, positions, freqs, sections, interleaved, norm, eps, q_out, k_out):
+    dev = _heads_dev(q, "q")
+    shape, dt = q.shape, q.dtype
+    B, (S, H, Dh) = (shape[0] if len(shape) == 4 else 1), shape[-3:]
+    sq = _heads(q, shape, dt, "q", dev)
+    if q_out is None:
+        q_out = torch.empty(shape, dtype=dt, device=q.device)
+    so = _heads(q_out, shape, dt, "q_out", dev)
+    sk = sko = (0, 0, 0)
+    pk = pko = Hkv = 0
+    if k is not None:
+        if k.dim() != len(shape) or k.shape[-2] < 1:
+            raise ValueError(f"k must have q's dimensions and a head at least, got {list(k.shape)}")
+        Hkv = k.shape[-2]
+        kshape = (*shape[:-2], Hkv, Dh)
+        sk = _heads(k, kshape, dt, "k", dev)
+        if k_out is None:
+            k_out = torch.empty(kshape, dtype=dt, device=q.device)
+        sko = _heads(k_out, kshape, dt, "k_out", dev)
+        pk, pko = k.data_ptr(), k_out.data_ptr()
+    elif k_out is not None or k_gamma is not None:
+        raise ValueError("k_out and k_gamma need k")
+    gq = 0 if q_gamma is None else _vector(q_gamma, Dh, "q_gamma", dt, dev)
+    gk = 0 if k_gamma is None else _vector(k_gamma, Dh, "k_gamma", dt, dev)
+    axes = len(sections)
+    if axes > 4:
+        raise ValueError("at most four axes")
+    if any(n < 0 for n in sections):
+        raise ValueError("a section has a negative number of pairs")
+    P = sum(sections)
+    pp = pf = pt = 0
+    sp = (0, 0)
+    if P > 0:
+        if positions is None or freqs is None:
+            raise ValueError("sections need positions and freqs")
+        if positions.dtype not in _POS or positions.get_device() != dev:
+            raise ValueError(f"positions must be int32, int64 or float32 on the current device, got "
+                             f"{positions.dtype} on {positions.device}")
+        pshape = positions.shape
+        if pshape != (S, axes) and pshape != (*shape[:-2], axes):
+            raise ValueError(f"positions must be {[*shape[:-2], axes]} or {[S, axes]}, got {list(pshape)}")
+        st = positions.stride()
+        if axes > 1 and st[-1] != 1:
+            raise ValueError("positions must have consecutive axes")
+        sp = st[:2] if len(st) == 3 else (0, st[0])
+        pp, pt = positions.data_ptr(), _POS[positions.dtype]
+        pf = _vector(freqs, P, "freqs", torch.float64, dev)
+    elif positions is not None or freqs is not None:
+        raise ValueError("positions and freqs need sections")
+    if not q.numel():
+        return q_out, k_out
+    args = _pack_rotary(q.data_ptr(), pk, q_out.data_ptr(), pko, *sq, *sk, *so, *sko, gq, gk, pp, *sp, pf, pt, axes,
+                        *sections, *(0,) * (4 - axes), interleaved, norm, eps, _HALF[dt], B, S, H, Hkv, Dh)
+    _lib.check(_entry(name)(args, _stream_of(dev)))
+    return q_out, k_out
+
+
+def rotary_axes(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, sections: Sequence[int],
+                interleaved: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotary positions with up to four axes: pair i of every head of x
+    [(batch,) token, head, Dh] is turned by positions[token, axis(i)] * freqs[i] radians.
+    The first sections[0] pairs go by axis 0, the next sections[1] by axis 1 and so
+    on; with P pairs in all, a pair is elements (i, i + P), or (2i, 2i + 1) where
+    interleaved, and elements from 2P on stay as they are.  positions [(batch,)
+    token, axis] are int32, int64 or float32; freqs [P] are float64 (``rotary_freqs``),
+    as is the angle, so far positions lose nothing.  out may be x."""
+    return _rotary("dlm_rotary_axes", x, None, None, None, positions, freqs, sections, bool(interleaved), 0, 0.0, out,
+                   None)[0]
+
+
+def qk_norm_rotary(q: torch.Tensor, k: Optional[torch.Tensor] = None, q_gamma: Optional[torch.Tensor] = None,
+                   k_gamma: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                   freqs: Optional[torch.Tensor] = None, sections: Sequence[int] = (), interleaved: bool = False,
+                   eps: float = 1e-6, q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None):
+    """(q, k) with every head's RMS norm, x / sqrt(mean(x^2) + eps) * gamma (gammas [Dh],
+    None: ones), and then ``rotary_axes``, in one pass and with one rounding; without
+    sections the norm alone.  q [(batch,) token, head, Dh] and k (or None) may
+    differ in heads.  q_out may be q and k_out k."""
+    return _rotary("dlm_qk_norm_rotary", q, k, q_gamma, k_gamma, positions, freqs, sections, bool(interleaved), 1, eps,
+                   q_out, k_out)
+
+
+def document_ranges(lengths: Sequence[int], tokens: Optional[int] = None, device="cuda") -> torch.Tensor:
+    """key_range [tokens, 2] of ``attention_masked`` for documents of these lengths packed
+    one behind the other: a token sees its document's.  Tokens behind the last
+    document (padding up to `tokens`) see nothing."""
+    if any(n < 0 for n in lengths):
+        raise ValueError("a document has a negative length")
+    n = torch.tensor(list(lengths), dtype=torch.int64)
+    end = torch.cumsum(n, 0)
+    used = int(end[-1]) if len(end) else 0
+    tokens = used if tokens is None else tokens
+    if tokens < used:
+        raise ValueError(f"{used} tokens of documents in {tokens}")
+    r = torch.zeros(tokens, 2, dtype=torch.int32)
+    r[:used, 0] = torch.repeat_interleave(end - n, n).to(torch.int32)
+    r[:used, 1] = torch.repeat_interleave(end, n).to(torch.int32)
+    return r.to(device)
+
+
+def prefix_ranges(prefixes: Sequence[int], queries: int, keys: Optional[int] = None, device="cuda") -> torch.Tensor:
+    """key_range [batch, queries, 2] of ``attention_masked`` for sequences that begin with a
+    prefix every query sees whole (its length per batch), in order behind it; the
+    queries are the last of the keys (as many as there are queries if None)."""
+    keys = queries if keys is None else keys
+    p = torch.arange(keys - queries, keys)
+    hi = torch.maximum((p + 1)[None], torch.tensor(list(prefixes), dtype=torch.int64)[:, None]).clamp(0, keys)
+    return torch.stack([torch.zeros_like(hi), hi], 2).to(torch.int32).to(device)
+
+
+def _batch_ints(t, B, inner, name, dev):
+    """(address, batch stride) of int32 [B, *inner] or [*inner]."""
+    if t.dtype != torch.int32 or t.get_device() != dev:
+        raise ValueError(f"{name} must be int32 on the current device, got {t.dtype} on {t.device}")
+    if t.shape != inner and t.shape != (B, *inner):
+        raise ValueError(f"{name} must be {[B, *inner]} or {list(inner)}, got {list(t.shape)}")
+    if t.is_contiguous():
+        return t.data_ptr(), (t.stride(0) if len(t.shape) > len(inner) else 0)
+    if len(t.shape) > len(inner) and t.shape[0] > 0 and t[0].is_contiguous():
+        return t.data_ptr(), t.stride(0)
+    raise ValueError(f"{name} must be contiguous within a batch")
+
+
+def attention_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_range: Optional[torch.Tensor] = None,
+                     q_pos: Optional[torch.Tensor] = None, causal: bool = False, scale: Optional[float] = None,
+                     cap: float = 0.0, slopes: Optional[torch.Tensor] = None,
+                     rel_bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(s) v for q [(batch,) Sq, H, Dh] and k, v [(batch,) Sk, Hkv, Dh], query head h
+    reading key head h // (H / Hkv); Dh a multiple of 8 up to 256.
+
+    s = scale q.k (scale None: Dh^-0.5), capped by cap tanh(s / cap) where cap > 0, plus
+    -slopes[h] |j - p| (slopes fp32 [H]) or rel_bias[h, clip(j - p, -R, R) + R]
+    (fp32 [H, 2R + 1]) for key j and a query at place p among the keys: q_pos int32
+    [(batch,) Sq], or the last Sq of the Sk places if None.
+
+    A query sees the keys lo <= j < hi of its key_range (int32 [(batch,) Sq, 2]:
+    ``document_ranges``, ``prefix_ranges``, lengths, windows; None: all) and, where
+    causal, only j <= p.  So a cache in use up to n keys is q_pos = n - 1 with causal.
+    A query that sees nothing gives 0; what masked keys hold has no effect."""
+    dev = _heads_dev(q, "q")
+    shape, dt = q.shape, q.dtype
+    if k.dim() != len(shape) or k.shape[-2] < 1:
+        raise ValueError(f"k must have q's dimensions and a head at least, got {list(k.shape)}")
+    B, (Sq, H, Dh) = (shape[0] if len(shape) == 4 else 1), shape[-3:]
+    Sk, Hkv = k.shape[-3:-1]
+    kshape = (*shape[:-3], Sk, Hkv, Dh)
+    sq = _heads(q, shape, dt, "q", dev)
+    sk = _heads(k, kshape, dt, "k", dev)
+    sv = _heads(v, kshape, dt, "v", dev)
+    if out is None:
+        out = torch.empty(shape, dtype=dt, device=q.device)
+    so = _heads(out, shape, dt, "out", dev)
+    kr = qp = ps = pb = 0
+    krb = qpb = R = 0
+    if key_range is not None:
+        kr, krb = _batch_ints(key_range, B, (Sq, 2), "key_range", dev)
+    if q_pos is not None:
+        qp, qpb = _batch_ints(q_pos, B, (Sq,), "q_pos", dev)
+    if slopes is not None:
+        ps = _vector(slopes, H, "slopes", torch.float32, dev)
+    if rel_bias is not None:
+        R = rel_bias.shape[-1] // 2
+        if rel_bias.shape != (H, 2 * R + 1):
+            raise ValueError(f"rel_bias must be [{H}, 2R + 1], got {list(rel_bias.shape)}")
+        pb = _vector(rel_bias, H * (2 * R + 1), "rel_bias", torch.float32, dev)
+    if scale is None:
+        scale = Dh ** -0.5 if Dh else 1.0
+    if not q.numel():
+        return out
+    args = _pack_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *sq, *sk, *sv, *so, kr, krb, qp, qpb,
+                           ps, pb, R, scale, cap, bool(causal), _HALF[dt], B, Sq, Sk, H, Hkv, Dh)
+    n = _entry("dlm_attention_masked_workspace_bytes")(args)
+    ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+    _lib.check(_entry("dlm_attention_masked")(args, _p(ws), n, _stream_of(dev)))
     return out

@@ -553,6 +553,111 @@ int dlm_linear_q8_f32out(const void* X, int ldx, const float* sx, const void* W,
                          const float* sw, const void* bias, const float* R, int ldr, float* Y, int ldy,
                          int M, int N, int K, float beta, int act, void* stream);
 
+/* ------------------------------------------------------------------ */
+/* Rotary positions, query / key norms and masked attention            */
+/* ------------------------------------------------------------------ */
+
+#define DLM_DTYPE_F16 0
+#define DLM_DTYPE_BF16 1
+#define DLM_POS_I32 0
+#define DLM_POS_I64 1
+#define DLM_POS_F32 2
+
+/* Rotary positions with several axes, of queries and (k may be NULL) keys:
+ * pair i of a head, (x1, x2) = elements (i, i + P), or (2i, 2i + 1) where
+ * interleaved, becomes (x1 cos a - x2 sin a, x2 cos a + x1 sin a) with the angle
+ * a = pos[b, s, axis(i)] * freqs[i] in radians.  The first sections[0] pairs go
+ * by axis 0, the next sections[1] by axis 1 and so on (a section may be empty);
+ * P is their sum, 2P <= Dh, and elements from 2P on stay as they are.
+ * Element (b, s, h, d) of an operand is at b sb + s ss + h sh + d; positions are
+ * at b pos_sb + s pos_ss + axis (pos_sb = 0: one line of positions for every
+ * batch), int32, int64 or fp32 (DLM_POS_*).  freqs are fp64, and so is the
+ * angle, reduced to a turn before its sine; all else is fp32, rounded once.
+ *
+ * dlm_qk_norm_rotary (norm = 1) first makes every head of q and of k
+ * x / sqrt(mean(x^2) + eps) * gamma, with q_gamma and k_gamma [Dh] of the
+ * operands' type or NULL (ones); with axes = 0 it is the norm alone.
+ * dlm_rotary_axes (norm = 0, gammas NULL) is the rotation alone.
+ *
+ * dtype is fp16 or bf16 (DLM_DTYPE_*) for every operand but positions and
+ * frequencies.  Dh is even and at most 256.  Any alignment of an element is
+ * taken; 16-byte aligned heads are fastest.  An output may be its own input
+ * (same pointer and strides) and overlap nothing else; slices of one tensor do
+ * not overlap.  Uses no workspace.  No counterpart in the reference
+ * (src/infer/unet.cu:677-802: no positions, no norm of queries and keys). */
+typedef struct dlm_rotary_args {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  long long q_sb, q_ss, q_sh;
+  long long k_sb, k_ss, k_sh;
+  long long qo_sb, qo_ss, qo_sh;
+  long long ko_sb, ko_ss, ko_sh;
+  const void* q_gamma;
+  const void* k_gamma;
+  const void* pos;
+  long long pos_sb, pos_ss;
+  const double* freqs;
+  int pos_type, axes;
+  int sections[4];
+  int interleaved, norm;
+  float eps;
+  int dtype;
+  int B, S, H, Hkv, Dh;
+} dlm_rotary_args;
+int dlm_rotary_axes(const dlm_rotary_args* args, void* stream);
+int dlm_qk_norm_rotary(const dlm_rotary_args* args, void* stream);
+
+/* Attention with masks, capped scores and a bias of distance:
+ *   s = scale q.k;  s = cap tanh(s / cap) where cap > 0
+ *   s -= slopes[h] |j - p_i|  or  s += rel_bias[h][clip(j - p_i, -R, R) + R]
+ *   o_i = sum_j softmax_j(s) v_j  over the keys j that query i sees
+ * Query i of batch b sees key j when lo <= j < hi of its interval
+ * key_range[b, i] = (lo, hi) (NULL: every key; hi past Sk counts as Sk), and,
+ * where causal, j <= p_i.  p_i = q_pos[b, i] is the query's place among the keys
+ * (NULL: i + Sk - Sq), within +-2^30.  A query that sees no key, or whose scores
+ * are all -infinity, is 0.  What masked keys hold, infinities and NaN too, has
+ * no effect.
+ * Query head h reads key / value head h / (H / Hkv).  Element (b, s, h, d) of an
+ * operand is at b sb + s ss + h sh + d.  Dh is a multiple of 8 up to 256.  q, k
+ * and v start at 16-byte aligned addresses and have strides that are multiples
+ * of 8, o at an 8-byte aligned one with strides that are multiples of 4; a key
+ * row's stride is at least Dh and below 2^23.  key_range is int32 [.., Sq, 2] with
+ * batch stride kr_sb (elements, 0: one for every batch), 8-byte aligned; q_pos
+ * int32 [.., Sq] with batch stride qp_sb; slopes fp32 [H]; rel_bias fp32 [H][2R + 1].
+ * scale > 0 and cap >= 0 are finite.  dtype is that of q, k, v and o; scores, softmax and sums are
+ * fp32, the probabilities are rounded to dtype for the product with v.
+ * Few queries against many keys are split over the keys; the parts meet in the
+ * workspace, of dlm_attention_masked_workspace_bytes(args) bytes (may be 0; it
+ * goes by sizes alone), 16-byte aligned, which no other call may use until this one's work is
+ * done.  o may not overlap q, k or v.  A query's result is reproducible bit for bit.
+ * No counterpart in the reference (src/kernels/attention.cuh:53-73 has neither
+ * masks nor biases). */
+typedef struct dlm_attention_masked_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  long long q_sb, q_ss, q_sh;
+  long long k_sb, k_ss, k_sh;
+  long long v_sb, v_ss, v_sh;
+  long long o_sb, o_ss, o_sh;
+  const int* key_range;
+  long long kr_sb;
+  const int* q_pos;
+  long long qp_sb;
+  const float* slopes;
+  const float* rel_bias;
+  int R;
+  float scale, cap;
+  int causal, dtype;
+  int B, Sq, Sk, H, Hkv, Dh;
+} dlm_attention_masked_args;
+size_t dlm_attention_masked_workspace_bytes(const dlm_attention_masked_args* args);
+int dlm_attention_masked(const dlm_attention_masked_args* args, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
 /* Euler step fused with classifier-free guidance (reference
  * src/infer/diffusion.cu:968-973 and src/infer/scheduler.hpp:112-143):
  * eps = u + g (c - u) from noise [2, n] (cond slice first, uncond second),
