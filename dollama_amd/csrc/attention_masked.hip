@@ -30,11 +30,13 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef short i16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
 
 template <typename T> struct Half;
 template <> struct Half<f16> {
   typedef f16x8 x8;
   static constexpr float shift = 7.0f;
+  static constexpr float limit = 3.0e6f;  // 32 finite values sum to less
   static constexpr unsigned inf = 0x7c00;
   static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) { return mfma32x32x16(a, b, c); }
   static __device__ __forceinline__ float dot2(f16x2 p, float c) {
@@ -45,6 +47,7 @@ template <> struct Half<f16> {
 template <> struct Half<__bf16> {
   typedef bf16x8 x8;
   static constexpr float shift = 0.0f;  // fp32's range: no p is too small
+  static constexpr float limit = 0x1p40f;
   static constexpr unsigned inf = 0x7f80;
   static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -70,7 +73,7 @@ struct AmParams {
   int R;
   int Sq, Sk, Hkv, G, Dh, rows;  // rows = Sq * G
   int causal, nrb, heads, splits;  // row blocks, B * Hkv, parts of the keys
-  float scale, c, thr, cap;        // c: to powers of two; thr: 8 / c
+  float scale, c, cap;             // c: to powers of two
   float* part;                     // [splits][heads][rows][Dh], then [splits][heads][rows][2]
 };
 
@@ -143,6 +146,22 @@ __device__ __forceinline__ Row am_row(const AmParams& p, int b, int hk, int r) {
   return w;
 }
 
+// A row's bias of distance.
+struct Bias {
+  float slope, left, right;  // the table's ends
+  const float* table;        // its middle
+};
+__device__ __forceinline__ Bias am_bias(const AmParams& p, const Row& row) {
+  Bias b{0.0f, 0.0f, 0.0f, nullptr};
+  if (p.slopes) b.slope = p.slopes[row.h];
+  if (p.table) {
+    b.table = p.table + (long long)row.h * (2 * p.R + 1) + p.R;
+    b.left = b.table[-p.R];
+    b.right = b.table[p.R];
+  }
+  return b;
+}
+
 // What a wave does with tiles of KB * 32 keys.  PB: bytes of a key's row in LDS, DK:
 // steps of 16 dims, DV: blocks of 32 dims; NW: waves that fill a tile together.
 template <typename T, int PB, int DK, int DV, bool MOD, int KB, int NW>
@@ -151,7 +170,6 @@ struct Core {
   using x8 = typename Hf::x8;
   static constexpr int BK = KB * 32;
   static constexpr int TILE = BK * PB;       // bytes of the K (or V) tile
-  static constexpr int STAGE = 2 * TILE;
   static constexpr int RPI = 1024 / PB;      // rows of one DMA instruction
   static constexpr int NI = BK / RPI / NW;   // instructions of a wave and operand
   static constexpr int CH = PB / 16;
@@ -160,39 +178,46 @@ struct Core {
   static constexpr int NVV = std::max(1, 4 / (NW * RPI));
   static_assert(NI * RPI * NW == BK && NI % NKV == 0 && NI % NVV == 0, "whole instructions");
 
-  const AmParams& p;
-  const Row& row;
-  const int lane, g;
-  const char* kbase;
-  const char* vbase;
+  const int lane, g, wave;
+  // the next tile of either operand that is copied: its first row, and the keys from it on
+  const char* kptr;
+  const char* vptr;
+  int kleft, vleft, kss, vss, dh;
   unsigned koff[NKV], voff[NVV];
   x8 qf[DK];
   f32x16 o[DV];
-  float m, l, mref;
-  float slope, tabl, tabr;
-  const float* tab;
+  float m, l, mref, lim, c;
+  bool special = false;  // some tile's V was not finite where a row does not see it
 
   static __device__ __forceinline__ int kswz(int r) { return PB == 128 ? (r >> 1) & 7 : r & 15; }
   static __device__ __forceinline__ int vswz(int r) { return PB == 128 ? (r & 2) << 1 : (r & 3) << 2; }
 
-  __device__ __forceinline__ Core(const AmParams& p_, const Row& row_, int b, int hk, int lane_, int wave)
-      : p(p_), row(row_), lane(lane_), g(lane_ >> 5) {
-    kbase = p.k + (b * p.k_sb + hk * p.k_sh) * 2;
-    vbase = p.v + (b * p.v_sb + hk * p.v_sh) * 2;
+  __device__ __forceinline__ Core(const AmParams& p, int lane_, int wave_) : lane(lane_), g(lane_ >> 5), wave(wave_) {
+    kss = (int)p.k_ss * 2;
+    vss = (int)p.v_ss * 2;
+    dh = p.Dh * 2;
+    c = p.c;
     const int r0 = wave * RPI + lane / CH, phys = lane % CH;
 #pragma unroll
     for (int i = 0; i < NKV; ++i) {
-      const int r = i * NW * RPI + r0, c = phys ^ kswz(r);
-      koff[i] = c * 8 < p.Dh ? (unsigned)(r * (int)p.k_ss * 2 + c * 16) : 0x80000000u;
+      const int r = i * NW * RPI + r0, ch = phys ^ kswz(r);
+      koff[i] = ch * 16 < dh ? (unsigned)(r * kss + ch * 16) : 0x80000000u;
     }
 #pragma unroll
     for (int i = 0; i < NVV; ++i) {
-      const int r = i * NW * RPI + r0, c = phys ^ vswz(r);
-      voff[i] = c * 8 < p.Dh ? (unsigned)(r * (int)p.v_ss * 2 + c * 16) : 0x80000000u;
+      const int r = i * NW * RPI + r0, ch = phys ^ vswz(r);
+      voff[i] = ch * 16 < dh ? (unsigned)(r * vss + ch * 16) : 0x80000000u;
     }
   }
 
-  __device__ __forceinline__ void load_q(int b) {
+  // The next tile is t; `step` tiles lie between one copy and the next
+  __device__ __forceinline__ void start(const AmParams& p, int b, int hk, int t) {
+    kptr = p.k + (b * p.k_sb + hk * p.k_sh) * 2 + (long long)t * BK * kss;
+    vptr = p.v + (b * p.v_sb + hk * p.v_sh) * 2 + (long long)t * BK * vss;
+    kleft = vleft = p.Sk - t * BK;
+  }
+
+  __device__ __forceinline__ void load_q(const AmParams& p, const Row& row, int b) {
     const T* qp = (const T*)p.q + b * p.q_sb + row.i * p.q_ss + row.h * p.q_sh + g * 8;
 #pragma unroll
     for (int ds = 0; ds < DK; ++ds) {
@@ -208,31 +233,27 @@ struct Core {
     m = -INFINITY;
     mref = 0.0f;
     l = 0.0f;
-    if constexpr (MOD) {
-      slope = p.slopes ? p.slopes[row.h] : 0.0f;
-      tab = nullptr;
-      tabl = tabr = 0.0f;
-      if (p.table) {
-        tab = p.table + (long long)row.h * (2 * p.R + 1) + p.R;
-        tabl = tab[-p.R];
-        tabr = tab[p.R];
-      }
-    }
+    lim = -1.0f;  // no key seen: the first tile's sum moves the base
   }
 
-  // Copies tile t into LDS: a buffer that starts at the tile's first row, so offsets stay
-  // small however long the cache, and ends with the last key's row (what lies past it, and
-  // dims past Dh, are zeros).
-  __device__ __forceinline__ void issue(unsigned char DLM_LDS* st, int t, int wave) const {
-    const int k0 = t * BK, n = min(BK, p.Sk - k0);
-    const i32x4 rk = dma_rsrc(kbase + (long long)k0 * p.k_ss * 2, (unsigned)(((n - 1) * (int)p.k_ss + p.Dh) * 2));
-    const i32x4 rv = dma_rsrc(vbase + (long long)k0 * p.v_ss * 2, (unsigned)(((n - 1) * (int)p.v_ss + p.Dh) * 2));
-    const unsigned ks = NKV * NW * RPI * (int)p.k_ss * 2, vs = NVV * NW * RPI * (int)p.v_ss * 2;
-#pragma unroll
-    for (int i = 0; i < NI; ++i) dma16(rk, st + (i * NW + wave) * 1024, (int)(koff[i % NKV] + (i / NKV) * ks), 0);
+  // Copies the next tile of an operand into LDS: a buffer that starts at the tile's first row, so
+  // offsets stay small however long the cache, and ends with the last key's row (what lies
+  // past it, and dims past Dh, are zeros).
+  __device__ __forceinline__ void issue_k(unsigned char DLM_LDS* st, int step = 1) {
+    const i32x4 r = dma_rsrc(kptr, (unsigned)((min(BK, kleft) - 1) * kss + dh));
 #pragma unroll
     for (int i = 0; i < NI; ++i)
-      dma16(rv, st + TILE + (i * NW + wave) * 1024, (int)(voff[i % NVV] + (i / NVV) * vs), 0);
+      dma16(r, st + (i * NW + wave) * 1024, (int)(koff[i % NKV] + (unsigned)(i / NKV * NKV * NW * RPI * kss)), 0);
+    kptr += (long long)step * BK * kss;
+    kleft -= step * BK;
+  }
+  __device__ __forceinline__ void issue_v(unsigned char DLM_LDS* st, int step = 1) {
+    const i32x4 r = dma_rsrc(vptr, (unsigned)((min(BK, vleft) - 1) * vss + dh));
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      dma16(r, st + (i * NW + wave) * 1024, (int)(voff[i % NVV] + (unsigned)(i / NVV * NVV * NW * RPI * vss)), 0);
+    vptr += (long long)step * BK * vss;
+    vleft -= step * BK;
   }
 
   __device__ __forceinline__ void scores(const unsigned char DLM_LDS* st, f32x16 (&s)[KB]) const {
@@ -254,7 +275,7 @@ struct Core {
   static constexpr __device__ int key_of(int kb, int e) { return kb * 32 + 8 * (e >> 2) + (e & 3); }
 
   // Cap and bias: s becomes the score itself (without them it stays q.k)
-  __device__ __forceinline__ void modify(f32x16 (&s)[KB], int k0) const {
+  __device__ __forceinline__ void modify(const AmParams& p, const Row& row, const Bias& bias, f32x16 (&s)[KB], int k0) const {
     if (p.cap > 0.0f) {
       const float ic = p.scale / p.cap;
       float top = 0.0f;
@@ -295,11 +316,11 @@ struct Core {
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          s[kb][e] = __builtin_fmaf(-slope, fabsf(f0 + (float)key_of(kb, e)), s[kb][e]);
+          s[kb][e] = __builtin_fmaf(-bias.slope, fabsf(f0 + (float)key_of(kb, e)), s[kb][e]);
     }
     if (p.table) {
       if (k0 + BK - 1 - row.pmin <= -p.R || k0 - row.pmax >= p.R) {
-        const float left = tabl, right = tabr, t = k0 - row.pmax >= p.R ? right : left;
+        const float left = bias.left, right = bias.right, t = k0 - row.pmax >= p.R ? right : left;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -308,7 +329,7 @@ struct Core {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[kb][e] += tab[max(-p.R, min(p.R, d0 + key_of(kb, e)))];
+          for (int e = 0; e < 16; ++e) s[kb][e] += bias.table[max(-p.R, min(p.R, d0 + key_of(kb, e)))];
       }
     }
   }
@@ -316,77 +337,150 @@ struct Core {
   __device__ __forceinline__ x8 vfrag(const unsigned char DLM_LDS* st, int j, int dt) const {
     const int r4 = (lane & 15) >> 2;
     const int base = (4 * g + r4) * PB + vswz(r4) * 16 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
-    const unsigned char DLM_LDS* a = st + TILE + (base ^ (64 * dt)) + 16 * j * PB;
+    const unsigned char DLM_LDS* a = st + (base ^ (64 * dt)) + 16 * j * PB;
     const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 DLM_LDS*)a);
     const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 DLM_LDS*)(a + 8 * PB));
     return __builtin_bit_cast(x8, i16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
   }
 
-  static __device__ __forceinline__ bool not_finite(short x) { return ((unsigned short)x & Hf::inf) == Hf::inf; }
-
-  // O^T += V^T P^T of a tile whose V holds infinities or NaN, where 0 * V would spoil
-  // rows that do not see them: the finite values by the product, and for each kind of the
-  // others the count of those that a row sees.
-  static __device__ __forceinline__ void pv_special(f32x16 (&o)[DV], const x8 (&pf)[2 * KB], unsigned seen,
-                                                              const Core& c, const unsigned char DLM_LDS* st) {
+  // p = 2^((s - m) c + shift) in the operands' type, and this lane's sum of them
+  __device__ __forceinline__ float exponentials(const f32x16 (&s)[KB], x8 (&pf)[2 * KB]) const {
 #pragma unroll
-    for (int dt = 0; dt < DV; ++dt) {
-      f32x16 n[3];
-#pragma unroll
-      for (int w = 0; w < 3; ++w)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) n[w][e] = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 2 * KB; ++j) {
-        const i16x8 v = __builtin_bit_cast(i16x8, c.vfrag(st, j, dt));
-        x8 fin, k[3], one;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const short bits = v[e];  // (an element itself is no operand of bit_cast)
-          const unsigned short x = (unsigned short)bits;
-          const bool odd = not_finite(bits), nan = odd && (x & 0x7fff) != Hf::inf;
-          fin[e] = odd ? (T)0.0f : __builtin_bit_cast(T, bits);
-          k[0][e] = odd && !nan && !(x & 0x8000) ? (T)1.0f : (T)0.0f;
-          k[1][e] = odd && !nan && (x & 0x8000) ? (T)1.0f : (T)0.0f;
-          k[2][e] = nan ? (T)1.0f : (T)0.0f;
-          one[e] = seen >> (8 * j + e) & 1 ? (T)1.0f : (T)0.0f;
-        }
-        o[dt] = Hf::mfma(fin, pf[j], o[dt]);
-#pragma unroll
-        for (int w = 0; w < 3; ++w) n[w] = Hf::mfma(k[w], one, n[w]);
-      }
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        if (n[0][e] > 0.0f) o[dt][e] += INFINITY;
-        if (n[1][e] > 0.0f) o[dt][e] -= INFINITY;
-        if (n[2][e] > 0.0f) o[dt][e] = NAN;
+        // without cap and bias (scale and log2 e in one): one multiply-add; else the
+        // difference first, which scores of the largest magnitude survive
+        const float x = MOD ? __builtin_fmaf(s[kb][e] - mref, c, Hf::shift) : __builtin_fmaf(s[kb][e], c, -mref);
+        pf[2 * kb + (e >> 3)][e & 7] = (T)__builtin_amdgcn_exp2f(x);
+      }
+    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < 2 * KB; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) sum[j & 1] = Hf::dot2(typename Hf::x2{pf[j][e], pf[j][e + 1]}, sum[j & 1]);
+    return sum[0] + sum[1];
+  }
+
+  // The weights of a tile against the row's base.  No maximum is taken: the sum, which is
+  // needed anyway, tells when some p came near the end of its type; only then (and at a row's first keys)
+  // the base moves to the tile's maximum and the weights are made again.  That a row moves goes
+  // by its own values, so its result depends on no other row.
+  template <typename Order>
+  __device__ __forceinline__ void softmax(const f32x16 (&s)[KB], x8 (&pf)[2 * KB], Order order) {
+    float sum = exponentials(s, pf);
+    order();
+    const bool past = !(sum <= lim);
+    if (__builtin_amdgcn_ballot_w64(past) != 0) {
+      asm volatile("" ::: "memory");  // a real branch
+      float mt = s[0][0];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[kb][e]);
+      mt = am_max_halves(mt);
+      const bool move = am_max_halves(past ? 1.0f : 0.0f) > 0.0f && mt > m;
+      const float alpha = move ? __builtin_amdgcn_exp2f((m - mt) * c) : 1.0f;
+      m = move ? mt : m;
+      lim = move ? Hf::limit : lim;
+      mref = m == -INFINITY ? 0.0f : MOD ? m : __builtin_fmaf(m, c, -Hf::shift);
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DV; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+      sum = exponentials(s, pf);
+    }
+    l += sum;
+  }
+
+  // O^T += V^T P^T
+  __device__ __forceinline__ void pv(const unsigned char DLM_LDS* st, const x8 (&pf)[2 * KB]) {
+#pragma unroll
+    for (int j = 0; j < 2 * KB; ++j)
+#pragma unroll
+      for (int dt = 0; dt < DV; ++dt) o[dt] = Hf::mfma(vfrag(st, j, dt), pf[j], o[dt]);
+  }
+
+  // The same of a tile whose V holds infinities or NaN, where 0 * V would spoil rows that
+  // do not see them: the finite values alone.
+  __device__ __forceinline__ void pv_finite(const unsigned char DLM_LDS* st, const x8 (&pf)[2 * KB]) {
+#pragma unroll
+    for (int j = 0; j < 2 * KB; ++j)
+#pragma unroll
+      for (int dt = 0; dt < DV; ++dt) {
+        u16x8 v = __builtin_bit_cast(u16x8, vfrag(st, j, dt));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (v[e] & Hf::inf) == Hf::inf ? 0 : v[e];
+        o[dt] = Hf::mfma(__builtin_bit_cast(x8, v), pf[j], o[dt]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  }
+
+  // ... and behind the loop over tiles (first, first + step, ... below last) the others, read from
+  // memory again: a second product counts those that a row sees, 1 for infinity, 128 for
+  // -infinity, both for NaN (whole numbers up to 64 * 129, exact in either type and in the sums).
+  __device__ __forceinline__ void add_special(const AmParams& p, const Row& row, const Bias& bias, int b, int hk,
+                                              int first, int last, int step) {
+    const T* v = (const T*)p.v + b * p.v_sb + hk * p.v_sh;
+    for (int t = first; t < last; t += step) {
+      const int k0 = t * BK;
+      if (k0 >= row.thi || k0 + BK <= row.tlo || (k0 >= row.flo && k0 + BK <= row.fhi && !p.table)) continue;
+#pragma unroll
+      for (int dt = 0; dt < DV; ++dt) {
+        const int d = dt * 32 + (lane & 31);
+        f32x16 n;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) n[e] = 0.0f;
+#pragma unroll 1
+        for (int j = 0; j < 2 * KB; ++j) {
+          x8 kind, one;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int key = k0 + 16 * j + 4 * g + (e & 3) + 8 * (e >> 2);
+            unsigned short x = 0;
+            if (key < p.Sk && d < p.Dh) x = __builtin_bit_cast(unsigned short, v[key * p.v_ss + d]);
+            const bool odd = (x & Hf::inf) == Hf::inf, nan = (x & 0x7fff) != Hf::inf;
+            bool sees = key >= row.lo && key < row.hi;
+            if (MOD && p.table) sees = sees && bias.table[max(-p.R, min(p.R, key - row.p))] != -INFINITY;
+            kind[e] = (T)(!odd ? 0.0f : nan ? 129.0f : x & 0x8000 ? 128.0f : 1.0f);
+            one[e] = (T)(sees ? 1.0f : 0.0f);
+          }
+          n = Hf::mfma(kind, one, n);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int count = (int)n[e];
+          if (count & 127) o[dt][e] += INFINITY;
+          if (count >> 7) o[dt][e] -= INFINITY;
+        }
       }
     }
   }
 
-  // One tile in LDS at st
-  __device__ __forceinline__ void tile(const unsigned char DLM_LDS* st, int t) {
+  // Softmax and product of tile t, whose scores are in s and whose V is in LDS at st; any mask
+  __device__ __forceinline__ void finish(const AmParams& p, const Row& row, const Bias& bias, f32x16 (&s)[KB],
+                                         const unsigned char DLM_LDS* st, int t) {
     const int k0 = t * BK;
-    f32x16 s[KB];
-    scores(st, s);
-    if constexpr (MOD) modify(s, k0);
+    if constexpr (MOD) modify(p, row, bias, s, k0);
     bool guard = false;
     if (k0 < row.flo || k0 + BK > row.fhi) {
       guard = true;
       // in 32 bits whatever the bounds: lo and hi against the tile's first key
       const int lo = max(row.lo, k0) - k0 - 4 * g, hi = min(row.hi, k0 + BK) - k0 - 4 * g;
+      if (k0 < row.flo) {
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (key_of(kb, e) < lo || key_of(kb, e) >= hi) s[kb][e] = -INFINITY;
+          for (int e = 0; e < 16; ++e) s[kb][e] = key_of(kb, e) < lo ? -INFINITY : s[kb][e];
+      }
+      if (k0 + BK > row.fhi) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[kb][e] = key_of(kb, e) >= hi ? -INFINITY : s[kb][e];
+      }
     }
-    float mt = s[0][0];
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[kb][e]);
-    mt = am_max_halves(mt);
     if constexpr (MOD) {
       if (p.table && !guard) {  // an entry of -infinity masks its distance
         float low = s[0][0];
@@ -397,59 +491,32 @@ struct Core {
         guard = __builtin_amdgcn_ballot_w64(low == -INFINITY) != 0;
       }
     }
-    if (__builtin_amdgcn_ballot_w64(mt > m + p.thr)) {
-      const bool move = mt > m + p.thr;
-      const float alpha = move ? __builtin_amdgcn_exp2f((m - mt) * p.c) : 1.0f;
-      m = move ? mt : m;
-      mref = m == -INFINITY ? 0.0f : MOD ? m : __builtin_fmaf(m, p.c, -Hf::shift);
-      l *= alpha;
-#pragma unroll
-      for (int dt = 0; dt < DV; ++dt)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
-    }
-    unsigned seen = 0;
-    bool special = false;
+    x8 pf[2 * KB];
     if (guard) {
-      unsigned bad = 0;
+      // V times zeros: NaN where V is not finite (the matrix pipe has room here, the vector pipe
+      // has not)
+      f32x16 n;
+      x8 zero;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) n[e] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) zero[e] = (T)0.0f;
 #pragma unroll
       for (int j = 0; j < 2 * KB; ++j)
 #pragma unroll
-        for (int dt = 0; dt < DV; ++dt) {
-          const i16x8 v = __builtin_bit_cast(i16x8, vfrag(st, j, dt));
+        for (int dt = 0; dt < DV; ++dt) n = Hf::mfma(vfrag(st, j, dt), zero, n);
+      float sum = 0.0f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) bad |= not_finite(v[e]);
-        }
-      special = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
-      if (special) {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) seen |= (s[kb][e] != -INFINITY ? 1u : 0u) << (16 * kb + e);
+      for (int e = 0; e < 16; ++e) sum += n[e];
+      if (__builtin_amdgcn_ballot_w64(sum != 0.0f) != 0) {
+        special = true;
+        softmax(s, pf, [] {});
+        pv_finite(st, pf);
+        return;
       }
     }
-    x8 pf[2 * KB];
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        // without cap and bias (scale and log2 e in one): one multiply-add; else the
-        // difference first, which scores of the largest magnitude survive
-        const float x = MOD ? __builtin_fmaf(s[kb][e] - mref, p.c, Hf::shift) : __builtin_fmaf(s[kb][e], p.c, -mref);
-        pf[2 * kb + (e >> 3)][e & 7] = (T)__builtin_amdgcn_exp2f(x);
-      }
-#pragma unroll
-    for (int j = 0; j < 2 * KB; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) l = Hf::dot2(typename Hf::x2{pf[j][e], pf[j][e + 1]}, l);
-    if (special) {
-      pv_special(o, pf, seen, *this, st);
-      return;
-    }
-#pragma unroll
-    for (int j = 0; j < 2 * KB; ++j)
-#pragma unroll
-      for (int dt = 0; dt < DV; ++dt) o[dt] = Hf::mfma(vfrag(st, j, dt), pf[j], o[dt]);
+    softmax(s, pf, [] {});
+    pv(st, pf);
   }
 };
 
@@ -484,14 +551,17 @@ __device__ __forceinline__ void am_span(int lo, int hi, int bk, int splits, int 
 }
 
 // ---------------------------------------------------------------------------
-// Many rows: 4 waves of 32 rows share tiles of 64 keys.
+// Many rows: 4 waves of 32 rows share tiles of 64 keys.  The scores of tile t + 1 are
+// issued ahead of tile t's softmax, so a wave's matrix and vector instructions overlap;
+// K therefore runs a tile ahead of V, and two buffers of each suffice: the barrier
+// that shows K of t + 1 and V of t to all also proves K of t and V of t - 1 read.
 // ---------------------------------------------------------------------------
 template <typename T, int PB, int DK, int DV, bool MOD>
 __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PB == 512 ? 1 : 2)))
 attn_masked_kernel(AmParams p) {
   using C = Core<T, PB, DK, DV, MOD, 2, 4>;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem_g[2 * C::STAGE];
-  __shared__ int span[8];
+  __shared__ __attribute__((aligned(1024))) unsigned char smem_g[4 * C::TILE];
+  __shared__ int span[16];
   unsigned char DLM_LDS* smem = (unsigned char DLM_LDS*)smem_g;
   // consecutive blocks (the row blocks of one key head, then the next head) on one XCD,
   // whose L2 then holds the K and V of its own heads; the last row blocks, which see the most
@@ -507,51 +577,155 @@ attn_masked_kernel(AmParams p) {
     head = u / p.nrb;
     rb = p.nrb - 1 - (u - head * p.nrb);
   }
-  const int b = head / p.Hkv, hk = head - b * p.Hkv;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = rb * 128 + wave * 32 + (lane & 31);
-  const Row row = am_row(p, b, hk, r);
-  if (lane == 0) {
-    span[2 * wave] = row.tlo;
-    span[2 * wave + 1] = row.thi;
+  Row row;
+  Bias bias{};
+  int hidden = 0;
+  C c(p, lane, wave);
+  {
+    const int b = head / p.Hkv, hk = head - b * p.Hkv;
+    row = am_row(p, b, hk, r);
+    if (lane == 0) {
+      span[4 * wave] = row.tlo;
+      span[4 * wave + 1] = row.thi;
+      span[4 * wave + 2] = row.flo;
+      span[4 * wave + 3] = row.fhi;
+    }
+    c.load_q(p, row, b);
+    if constexpr (MOD) {
+      bias = am_bias(p, row);
+      // a table's entries of -infinity are looked for once; a long table counts as having some
+      if (p.table) {
+        const long long n = (2LL * p.R + 1) * p.G;
+        bool none = n <= 8192;
+        const float* tab = p.table + hk * n;
+        if (none)
+          for (int i = tid; i < n; i += 256) none &= tab[i] != -INFINITY;
+        hidden = __syncthreads_or(!none);
+      }
+    }
+    __syncthreads();
   }
-  C c(p, row, b, hk, lane, wave);
-  c.load_q(b);
-  __syncthreads();
-  const int lo = __builtin_amdgcn_readfirstlane(min(min(span[0], span[2]), min(span[4], span[6])));
-  const int hi = __builtin_amdgcn_readfirstlane(max(max(span[1], span[3]), max(span[5], span[7])));
-  int t0, t1;
-  am_span(lo, hi, C::BK, p.splits, split, t0, t1);
-  if (t0 < t1) c.issue(smem, t0, wave);
-  int buf = 0;
-  for (int t = t0; t < t1; ++t) {
-    // tile t has arrived (this wave's part, then everyone's), and all are done with t - 1
-    AM_WAIT_ALL();
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-    if (t + 1 < t1) c.issue(smem + (buf ^ 1) * C::STAGE, t + 1, wave);
-    const int k0 = t * C::BK;
-    if (k0 < row.thi && k0 + C::BK > row.tlo) c.tile(smem + buf * C::STAGE, t);
-    buf ^= 1;
-    __builtin_amdgcn_sched_barrier(0);
+  // Tiles [t0, t1) hold the block's keys; [f0, f1) of them, an even number of tiles and an even
+  // number after t0, are seen whole by every row
+  int t0, t1, f0, f1;
+  {
+    auto all = [&](int i, auto op) {
+      return __builtin_amdgcn_readfirstlane(op(op(span[i], span[4 + i]), op(span[8 + i], span[12 + i])));
+    };
+    auto least = [](int x, int y) { return x < y ? x : y; };
+    auto most = [](int x, int y) { return x > y ? x : y; };
+    am_span(all(0, least), all(1, most), C::BK, p.splits, split, t0, t1);
+    const int flo = all(2, most), fhi = all(3, least);
+    f0 = max(t0, (flo + C::BK - 1) / C::BK);
+    f0 += (f0 - t0) & 1;
+    f1 = min(t1, fhi / C::BK);
+    f1 -= (f1 - f0) & 1;
+    if (MOD && hidden) f1 = f0;
+  }
+  if (t0 < t1) {
+    unsigned char DLM_LDS* const vmem = smem + 2 * C::TILE;
+    auto arrive = [&] {
+      AM_WAIT_ALL();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    {
+      const int b = head / p.Hkv;
+      c.start(p, b, head - b * p.Hkv, t0);
+    }
+    f32x16 sa[2], sb[2];
+    c.issue_k(smem);
+    c.issue_v(vmem);
+    if (t0 + 1 < t1) c.issue_k(smem + C::TILE);
+    arrive();
+    c.scores(smem, sa);
+    // tile t is in buffers `par`, its scores in sc; the next tile's go to sn (behind the last tile
+    // they are made of whatever the buffer holds and not used)
+    auto weigh = [&](int par, f32x16 (&sc)[2], f32x16 (&sn)[2], int t) {
+      typename C::x8 pf[4];
+      c.scores(smem + (par ^ 1) * C::TILE, sn);
+      if constexpr (MOD) c.modify(p, row, bias, sc, t * C::BK);
+      c.softmax(sc, pf, [] {
+        // the order of the block up to the branch: a score product, its share of the
+        // exponentials, the next fragment of K
+        if constexpr (!MOD) {
+          __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+          for (int i = 0; i < 2 * DK; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x2, 32 / DK, 0);
+            __builtin_amdgcn_sched_group_barrier(0x400, 16 / DK, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          }
+        }
+      });
+      c.pv(vmem + par * C::TILE, pf);
+      __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+      for (int i = 0; i < 4 * DV; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      }
+    };
+    auto whole = [&](int t, int par, f32x16 (&sc)[2], f32x16 (&sn)[2]) {
+      arrive();
+      if (t + 2 < t1) c.issue_k(smem + par * C::TILE);
+      if (t + 1 < t1) c.issue_v(vmem + (par ^ 1) * C::TILE);
+      weigh(par, sc, sn, t);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    int t = t0;
+    while (t < t1) {
+      if (t == f0) {
+        for (; t < f1; t += 2) {
+          whole(t, 0, sa, sb);
+          whole(t + 1, 1, sb, sa);
+        }
+        f0 = -1;
+        if (t == t1) break;
+      }
+      // a tile that some row does not see, or not whole: its scores are not needed any more when the next
+      // tile's are made, which leaves registers for the masks
+      const int par = (t - t0) & 1;
+      arrive();
+      if (t + 2 < t1) c.issue_k(smem + par * C::TILE);
+      if (t + 1 < t1) c.issue_v(vmem + (par ^ 1) * C::TILE);
+      const int k0 = t * C::BK;
+      if (k0 < row.thi && k0 + C::BK > row.tlo) c.finish(p, row, bias, sa, vmem + par * C::TILE, t);
+      if (k0 + C::BK < row.thi && k0 + 2 * C::BK > row.tlo) c.scores(smem + (par ^ 1) * C::TILE, sa);
+      __builtin_amdgcn_sched_barrier(0);
+      ++t;
+    }
+    if (c.special) {
+      const int b = head / p.Hkv;
+      c.add_special(p, row, bias, b, head - b * p.Hkv, t0, t1, 1);
+    }
   }
   const float l = am_sum_halves(c.l);
   if (!row.live) return;
-  if (p.splits > 1) {
-    float* po = am_part_o(p, split, head, r);
+  // the arguments are read again here rather than kept in scalar registers through the loop
+  const AmParams __attribute__((address_space(4)))* q =
+      (const AmParams __attribute__((address_space(4)))*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(q));
+  const int Dh = q->Dh;
+  if (q->splits > 1) {
+    const long long at = ((long long)split * q->heads + head) * q->rows + r;
+    float* po = q->part + at * Dh;
 #pragma unroll
     for (int dt = 0; dt < DV; ++dt)
 #pragma unroll
       for (int e4 = 0; e4 < 4; ++e4) {
         const int d = am_dim(dt, e4) + 4 * c.g;
-        if (d < p.Dh)
+        if (d < Dh)
           *reinterpret_cast<f32x4*>(po + d) =
               f32x4{c.o[dt][4 * e4], c.o[dt][4 * e4 + 1], c.o[dt][4 * e4 + 2], c.o[dt][4 * e4 + 3]};
       }
     if (c.g == 0) {
-      float* ml = am_part_ml(p, split, head, r);
+      float* ml = q->part + (long long)q->splits * q->heads * q->rows * Dh + at * 2;
       ml[0] = row.empty ? -INFINITY : c.m;
       ml[1] = row.empty ? 0.0f : l;
     }
@@ -559,15 +733,17 @@ attn_masked_kernel(AmParams p) {
   }
   const bool none = row.empty || l == 0.0f;
   const float inv = 1.0f / l;
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  T* po = (T*)q->o + (head / q->Hkv) * q->o_sb + row.i * q->o_ss + row.h * q->o_sh;
 #pragma unroll
   for (int dt = 0; dt < DV; ++dt)
 #pragma unroll
     for (int e4 = 0; e4 < 4; ++e4) {
       const int d = am_dim(dt, e4) + 4 * c.g;
-      float x[4];
+      t4 x;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = none ? 0.0f : c.o[dt][4 * e4 + e] * inv;
-      if (d < p.Dh) am_store4<T>(p, b, row.i, row.h, d, x[0], x[1], x[2], x[3]);
+      for (int e = 0; e < 4; ++e) x[e] = (T)(none ? 0.0f : c.o[dt][4 * e4 + e] * inv);
+      if (d < Dh) *reinterpret_cast<t4*>(po + d) = x;
     }
 }
 
@@ -581,7 +757,7 @@ __global__ void __launch_bounds__(PB == 512 ? 128 : 256) __attribute__((amdgpu_w
 attn_masked_rows_kernel(AmParams p) {
   constexpr int NW = PB == 512 ? 2 : 4;
   using C = Core<T, PB, DK, DV, MOD, 1, 1>;
-  constexpr int RING = 2 * C::STAGE;
+  constexpr int STAGE = 2 * C::TILE, RING = 2 * STAGE;
   constexpr int D = DV * 32;
   static_assert(NW * 32 * D * 4 <= NW * RING, "the waves' parts fit the rings");
   __shared__ __attribute__((aligned(1024))) unsigned char smem_g[NW * RING];
@@ -592,13 +768,20 @@ attn_masked_rows_kernel(AmParams p) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   unsigned char DLM_LDS* smem = (unsigned char DLM_LDS*)smem_g + wave * RING;
   const Row row = am_row(p, b, hk, rb * 32 + (lane & 31));
-  C c(p, row, b, hk, lane, 0);
+  C c(p, lane, 0);
   int t0, t1;
   am_span(row.tlo, row.thi, C::BK, p.splits, split, t0, t1);
   int t = t0 + wave;
-  if (t < t1) c.issue(smem, t, 0);
-  if (t + NW < t1) c.issue(smem + C::STAGE, t + NW, 0);
-  c.load_q(b);
+  c.start(p, b, hk, t);
+  auto issue = [&](unsigned char DLM_LDS* st) {
+    c.issue_k(st, NW);
+    c.issue_v(st + C::TILE, NW);
+  };
+  if (t < t1) issue(smem);
+  if (t + NW < t1) issue(smem + STAGE);
+  c.load_q(p, row, b);
+  Bias bias{};
+  if constexpr (MOD) bias = am_bias(p, row);
   int buf = 0;
   for (; t < t1; t += NW) {
     if (t + NW < t1) {
@@ -608,13 +791,16 @@ attn_masked_rows_kernel(AmParams p) {
     }
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    c.tile(smem + buf * C::STAGE, t);
+    f32x16 s[1];
+    c.scores(smem + buf * STAGE, s);
+    c.finish(p, row, bias, s, smem + buf * STAGE + C::TILE, t);
     __builtin_amdgcn_sched_barrier(0);
     AM_WAIT_LGKM();  // this tile's fragments are read
     asm volatile("" ::: "memory");
-    if (t + 2 * NW < t1) c.issue(smem + buf * C::STAGE, t + 2 * NW, 0);
+    if (t + 2 * NW < t1) issue(smem + buf * STAGE);
     buf ^= 1;
   }
+  if (c.special) c.add_special(p, row, bias, b, hk, t0 + wave, t1, NW);
   const float l = am_sum_halves(c.l);
   if (lane < 32) {
     ml[wave][lane][0] = c.m;
@@ -850,7 +1036,6 @@ int dlm_attention_masked(const dlm_attention_masked_args* a, void* workspace, si
   // (a scale past ln 2 could carry the largest of scores past fp32 on the short path)
   const bool mod = a->cap > 0.0f || a->slopes || a->rel_bias || a->scale * log2e > 1.0f;
   p.c = mod ? log2e : a->scale * log2e;
-  p.thr = std::min(8.0f / p.c, 1e38f);
   hipStream_t s = (hipStream_t)stream;
   if (a->dtype == DLM_DTYPE_F16) return mod ? am_by_head<f16, true>(p, pl, s) : am_by_head<f16, false>(p, pl, s);
   return mod ? am_by_head<__bf16, true>(p, pl, s) : am_by_head<__bf16, false>(p, pl, s);
