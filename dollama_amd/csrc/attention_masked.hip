@@ -73,6 +73,7 @@ struct AmParams {
   int R;
   int Sq, Sk, Hkv, G, Dh, rows;  // rows = Sq * G
   int causal, nrb, heads, splits;  // row blocks, B * Hkv, parts of the keys
+  int parts;                       // workgroups that may share a block's rows
   float scale, c, cap;             // c: to powers of two
   float* part;                     // [splits][heads][rows][Dh], then [splits][heads][rows][2]
 };
@@ -130,20 +131,25 @@ __device__ __forceinline__ Row am_row(const AmParams& p, int b, int hk, int r) {
   if (p.q_pos) w.p = max(-(1 << 30), min(1 << 30, p.q_pos[b * p.qp_sb + w.i]));
   if (p.causal && w.p < p.Sk) w.hi = min(w.hi, w.p + 1);
   w.empty = w.lo >= w.hi;
-  // rows that see nothing, and those behind the last, run along unmasked: what they
-  // compute is never stored
+  w.pmin = am_wave_min(w.p);
+  w.pmax = am_wave_max(w.p);
+  return w;
+}
+
+// What the wave's rows see together.  Those that see nothing, and those that are not this
+// workgroup's, run along unmasked: what they compute is never stored.
+__device__ __forceinline__ void am_bounds(Row& w) {
   const bool on = w.live && !w.empty;
   w.tlo = am_wave_min(on ? w.lo : INT_MAX);
   w.thi = am_wave_max(on ? w.hi : 0);
   w.flo = am_wave_max(on ? w.lo : 0);
   w.fhi = am_wave_min(on ? w.hi : INT_MAX);
-  w.pmin = am_wave_min(w.p);
-  w.pmax = am_wave_max(w.p);
-  if (!on) {
+}
+__device__ __forceinline__ void am_unmask(Row& w) {
+  if (!w.live || w.empty) {
     w.lo = INT_MIN;
     w.hi = INT_MAX;
   }
-  return w;
 }
 
 // A row's bias of distance.
@@ -553,24 +559,31 @@ __device__ __forceinline__ void am_span(int lo, int hi, int bk, int splits, int 
 // ---------------------------------------------------------------------------
 // Many rows: 4 waves of 32 rows share tiles of 64 keys.  The scores of tile t + 1 are
 // issued ahead of tile t's softmax, so a wave's matrix and vector instructions overlap;
-// K therefore runs a tile ahead of V, and two buffers of each suffice: the barrier
-// that shows K of t + 1 and V of t to all also proves K of t and V of t - 1 read.
+// K therefore runs a tile ahead of V, and two buffers of each suffice: the barrier that
+// shows K of t + 1 and V of t to all also proves K of t and V of t - 1 read.  (A third buffer of
+// each changed nothing: 2x4096x10x64 130 us either way.)
 // ---------------------------------------------------------------------------
 template <typename T, int PB, int DK, int DV, bool MOD>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PB == 512 ? 1 : 2)))
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PB == 512 ? 1 : PB == 128 && !MOD ? 3 : 2)))
 attn_masked_kernel(AmParams p) {
   using C = Core<T, PB, DK, DV, MOD, 2, 4>;
   __shared__ __attribute__((aligned(1024))) unsigned char smem_g[4 * C::TILE];
-  __shared__ int span[16];
+  __shared__ int span[32];
   unsigned char DLM_LDS* smem = (unsigned char DLM_LDS*)smem_g;
   // consecutive blocks (the row blocks of one key head, then the next head) on one XCD,
   // whose L2 then holds the K and V of its own heads; the last row blocks, which see the most
   // keys where the mask is causal, first
-  int split, head, rb;
+  int split, head, rb, part;
   {
     const int total = p.nrb * p.heads * p.splits;
+    int at = blockIdx.x;
+    part = 0;
+    if (p.parts > 1) {  // the second parts, most of which have nothing to do, start first
+      part = at < total;
+      at -= part ? 0 : total;
+    }
     const int q8 = total >> 3, r8 = total & 7;
-    const int x = blockIdx.x & 7, slot = blockIdx.x >> 3;
+    const int x = at & 7, slot = at >> 3;
     const int logical = x * q8 + (x < r8 ? x : r8) + slot;
     const int u = logical / p.splits;
     split = logical - u * p.splits;
@@ -587,12 +600,6 @@ attn_masked_kernel(AmParams p) {
   {
     const int b = head / p.Hkv, hk = head - b * p.Hkv;
     row = am_row(p, b, hk, r);
-    if (lane == 0) {
-      span[4 * wave] = row.tlo;
-      span[4 * wave + 1] = row.thi;
-      span[4 * wave + 2] = row.flo;
-      span[4 * wave + 3] = row.fhi;
-    }
     c.load_q(p, row, b);
     if constexpr (MOD) {
       bias = am_bias(p, row);
@@ -606,17 +613,47 @@ attn_masked_kernel(AmParams p) {
         hidden = __syncthreads_or(!none);
       }
     }
-    __syncthreads();
   }
   // Tiles [t0, t1) hold the block's keys; [f0, f1) of them, an even number of tiles and an even
   // number after t0, are seen whole by every row
   int t0, t1, f0, f1;
   {
-    auto all = [&](int i, auto op) {
-      return __builtin_amdgcn_readfirstlane(op(op(span[i], span[4 + i]), op(span[8 + i], span[12 + i])));
-    };
     auto least = [](int x, int y) { return x < y ? x : y; };
     auto most = [](int x, int y) { return x > y ? x : y; };
+    auto share = [&](int longest) {
+      am_bounds(row);
+      if (lane == 0) {
+        int DLM_LDS* s = (int DLM_LDS*)span + 8 * wave;
+        s[0] = row.tlo;
+        s[1] = row.thi;
+        s[2] = row.flo;
+        s[3] = row.fhi;
+        s[4] = longest;
+      }
+      AM_WAIT_LGKM();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    };
+    auto all = [&](int i, auto op) {
+      return __builtin_amdgcn_readfirstlane(op(op(span[i], span[8 + i]), op(span[16 + i], span[24 + i])));
+    };
+    share(p.parts > 1 ? am_wave_max(row.live && !row.empty ? row.hi - row.lo : 0) : 0);
+    if (p.parts > 1) {
+      // Rows of two documents see twice the keys of one between them: then one workgroup takes the
+      // rows of the first half of those keys and a second one the others (2112 + 1984 tokens twice,
+      // x10x64: 104 -> XX us).  Where the rows see much the same the second one has nothing to do.
+      const int lo = all(0, least), hi = all(1, most), longest = all(4, most);
+      const bool apart = (hi - lo) / 2 >= longest / 4 * 3 && hi - lo > 4 * C::BK;
+      if (part == 1 && !apart) return;
+      if (apart) {
+        const bool second = !row.empty && (row.lo >> 1) + (row.hi >> 1) >= (lo >> 1) + (hi >> 1);
+        row.live = row.live && second == (part == 1);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        share(0);
+      }
+    }
+    am_unmask(row);
     am_span(all(0, least), all(1, most), C::BK, p.splits, split, t0, t1);
     const int flo = all(2, most), fhi = all(3, least);
     f0 = max(t0, (flo + C::BK - 1) / C::BK);
@@ -627,11 +664,18 @@ attn_masked_kernel(AmParams p) {
   }
   if (t0 < t1) {
     unsigned char DLM_LDS* const vmem = smem + 2 * C::TILE;
+    // K of t + 1 and V of t have arrived (this wave's part, then everyone's), and all are done with K
+    // of t and V of t - 1
     auto arrive = [&] {
       AM_WAIT_ALL();
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
+    };
+    // ... whose places the next copies take (tile t is in the buffers `par`)
+    auto copy = [&](int t, int par) {
+      if (t + 2 < t1) c.issue_k(smem + par * C::TILE);
+      if (t + 1 < t1) c.issue_v(vmem + (par ^ 1) * C::TILE);
     };
     {
       const int b = head / p.Hkv;
@@ -643,9 +687,11 @@ attn_masked_kernel(AmParams p) {
     if (t0 + 1 < t1) c.issue_k(smem + C::TILE);
     arrive();
     c.scores(smem, sa);
-    // tile t is in buffers `par`, its scores in sc; the next tile's go to sn (behind the last tile
-    // they are made of whatever the buffer holds and not used)
-    auto weigh = [&](int par, f32x16 (&sc)[2], f32x16 (&sn)[2], int t) {
+    // a tile that every row sees whole, its scores in sc; the next tile's go to sn (behind the
+    // last tile they are made of whatever the buffer holds and not used)
+    auto whole = [&](int t, int par, f32x16 (&sc)[2], f32x16 (&sn)[2]) {
+      arrive();
+      copy(t, par);
       typename C::x8 pf[4];
       c.scores(smem + (par ^ 1) * C::TILE, sn);
       if constexpr (MOD) c.modify(p, row, bias, sc, t * C::BK);
@@ -670,12 +716,6 @@ attn_masked_kernel(AmParams p) {
         __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
       }
-    };
-    auto whole = [&](int t, int par, f32x16 (&sc)[2], f32x16 (&sn)[2]) {
-      arrive();
-      if (t + 2 < t1) c.issue_k(smem + par * C::TILE);
-      if (t + 1 < t1) c.issue_v(vmem + (par ^ 1) * C::TILE);
-      weigh(par, sc, sn, t);
       __builtin_amdgcn_sched_barrier(0);
     };
     int t = t0;
@@ -686,14 +726,13 @@ attn_masked_kernel(AmParams p) {
           whole(t + 1, 1, sb, sa);
         }
         f0 = -1;
-        if (t == t1) break;
+        if (t >= t1) break;
       }
       // a tile that some row does not see, or not whole: its scores are not needed any more when the next
       // tile's are made, which leaves registers for the masks
       const int par = (t - t0) & 1;
       arrive();
-      if (t + 2 < t1) c.issue_k(smem + par * C::TILE);
-      if (t + 1 < t1) c.issue_v(vmem + (par ^ 1) * C::TILE);
+      copy(t, par);
       const int k0 = t * C::BK;
       if (k0 < row.thi && k0 + C::BK > row.tlo) c.finish(p, row, bias, sa, vmem + par * C::TILE, t);
       if (k0 + C::BK < row.thi && k0 + 2 * C::BK > row.tlo) c.scores(smem + (par ^ 1) * C::TILE, sa);
@@ -767,7 +806,9 @@ attn_masked_rows_kernel(AmParams p) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   unsigned char DLM_LDS* smem = (unsigned char DLM_LDS*)smem_g + wave * RING;
-  const Row row = am_row(p, b, hk, rb * 32 + (lane & 31));
+  Row row = am_row(p, b, hk, rb * 32 + (lane & 31));
+  am_bounds(row);
+  am_unmask(row);
   C c(p, lane, 0);
   int t0, t1;
   am_span(row.tlo, row.thi, C::BK, p.splits, split, t0, t1);
@@ -911,7 +952,7 @@ static int am_launch(const AmParams& p, const AmPlan& pl, hipStream_t s) {
     DLM_LAUNCH("attn_masked_rows_kernel", (attn_masked_rows_kernel<T, PB, DK, DV, MOD>),
                dim3(pl.nrb, p.heads, pl.splits), dim3(PB == 512 ? 128 : 256), 0, s, p);
   else
-    DLM_LAUNCH("attn_masked_kernel", (attn_masked_kernel<T, PB, DK, DV, MOD>), dim3(pl.nrb * p.heads * pl.splits),
+    DLM_LAUNCH("attn_masked_kernel", (attn_masked_kernel<T, PB, DK, DV, MOD>), dim3(pl.nrb * p.heads * pl.splits * p.parts),
                dim3(256), 0, s, p);
   DLM_LAUNCH_CHECK();
   if (pl.splits > 1) {
@@ -944,8 +985,8 @@ static int am_check(const char* fn, const dlm_attention_masked_args* a) {
   if (a->rel_bias && (a->R < 0 || a->R > (1 << 24))) return bad("R must be 0 to 2^24");
   if (a->Sq > (1 << 28) || a->Sk > (1 << 28)) return bad("more than 2^28 queries or keys");
   const long long G = a->H / a->Hkv;
-  if (a->Sq * G >= (1LL << 30) || (long long)a->B * a->Hkv > 65535) return bad("more rows or heads than a grid takes");
-  if ((long long)a->B * a->Hkv * ((a->Sq * G + 31) / 32) >= (1LL << 24)) return bad("more rows than a grid takes");
+  if (a->Sq * G >= (1LL << 29) || (long long)a->B * a->Hkv > 65535) return bad("more rows or heads than a grid takes");
+  if ((long long)a->B * a->Hkv * ((a->Sq * G + 31) / 32) >= (1LL << 23)) return bad("more rows than a grid takes");
   struct Op {
     const char* name;
     const void* p;
@@ -1030,6 +1071,7 @@ int dlm_attention_masked(const dlm_attention_masked_args* a, void* workspace, si
   p.Sq = a->Sq, p.Sk = a->Sk, p.Hkv = a->Hkv, p.G = a->H / a->Hkv, p.Dh = a->Dh;
   p.rows = a->Sq * p.G;
   p.causal = a->causal != 0, p.nrb = pl.nrb, p.heads = a->B * a->Hkv, p.splits = pl.splits;
+  p.parts = a->key_range ? 2 : 1;
   p.scale = a->scale, p.cap = a->cap;
   p.part = (float*)workspace;
   const float log2e = 1.4426950408889634f;
