@@ -104,18 +104,34 @@ __device__ __forceinline__ float tanh_ratio(float u) {
   return __builtin_fmaf(r, u, 0.999999987069f);
 }
 
-// A row's place and what it sees; all of it lives in the row's two lanes.
-struct Row {
-  int i, h;          // query, head
-  bool live, empty;  // a row of the call; one that sees no key
-  int lo, hi, p;
-  int tlo, thi;  // the wave's keys: from the first to behind the last that a row sees
-  int flo, fhi;  // keys that all its rows see
-  int pmin, pmax;
+// What a wave's rows see: keys from the first to behind the last that one of them sees, the
+// keys that all of them see, and their places.
+struct KeySpan {
+  int tlo, thi, flo, fhi, pmin, pmax;
+  __device__ __forceinline__ bool any(int k0, int n) const { return k0 < thi && k0 + n > tlo; }
+  __device__ __forceinline__ bool whole(int k0, int n) const { return k0 >= flo && k0 + n <= fhi; }
 };
 
-__device__ __forceinline__ Row am_row(const AmParams& p, int b, int hk, int r) {
-  Row w;
+// A row's place and what it sees, in LDS (an array of 64 per field and wave): the loop needs
+// little of it and rarely, and registers spilled to memory would be read back behind the copies
+// in flight.
+struct Row {
+  enum { LO, HI, P, FLAGS, HEAD, SLOPE, LEFT, RIGHT, N };
+  enum { LIVE = 1, EMPTY = 2 };  // a row that is stored; one that sees no key
+  int DLM_LDS* at;
+  __device__ __forceinline__ int get(int f) const { return at[f * 64]; }
+  __device__ __forceinline__ float num(int f) const { return __int_as_float(at[f * 64]); }
+  __device__ __forceinline__ void set(int f, int v) const { at[f * 64] = v; }
+};
+
+struct RowInit {
+  int i, h;  // query, head
+  bool live, empty;
+  int lo, hi, p;
+};
+
+__device__ __forceinline__ RowInit am_row(const AmParams& p, int b, int hk, int r) {
+  RowInit w;
   w.live = r < p.rows;
   const int rc = w.live ? r : p.rows - 1;
   w.i = rc / p.G;
@@ -131,41 +147,41 @@ __device__ __forceinline__ Row am_row(const AmParams& p, int b, int hk, int r) {
   if (p.q_pos) w.p = max(-(1 << 30), min(1 << 30, p.q_pos[b * p.qp_sb + w.i]));
   if (p.causal && w.p < p.Sk) w.hi = min(w.hi, w.p + 1);
   w.empty = w.lo >= w.hi;
-  w.pmin = am_wave_min(w.p);
-  w.pmax = am_wave_max(w.p);
   return w;
 }
 
-// What the wave's rows see together.  Those that see nothing, and those that are not this
-// workgroup's, run along unmasked: what they compute is never stored.
-__device__ __forceinline__ void am_bounds(Row& w) {
+// Rows that see nothing, and those that are not this workgroup's, run along unmasked: what
+// they compute is never stored.
+__device__ __forceinline__ void am_span(const RowInit& w, KeySpan& s) {
   const bool on = w.live && !w.empty;
-  w.tlo = am_wave_min(on ? w.lo : INT_MAX);
-  w.thi = am_wave_max(on ? w.hi : 0);
-  w.flo = am_wave_max(on ? w.lo : 0);
-  w.fhi = am_wave_min(on ? w.hi : INT_MAX);
-}
-__device__ __forceinline__ void am_unmask(Row& w) {
-  if (!w.live || w.empty) {
-    w.lo = INT_MIN;
-    w.hi = INT_MAX;
-  }
+  s.tlo = am_wave_min(on ? w.lo : INT_MAX);
+  s.thi = am_wave_max(on ? w.hi : 0);
+  s.flo = am_wave_max(on ? w.lo : 0);
+  s.fhi = am_wave_min(on ? w.hi : INT_MAX);
 }
 
-// A row's bias of distance.
-struct Bias {
-  float slope, left, right;  // the table's ends
-  const float* table;        // its middle
-};
-__device__ __forceinline__ Bias am_bias(const AmParams& p, const Row& row) {
-  Bias b{0.0f, 0.0f, 0.0f, nullptr};
-  if (p.slopes) b.slope = p.slopes[row.h];
-  if (p.table) {
-    b.table = p.table + (long long)row.h * (2 * p.R + 1) + p.R;
-    b.left = b.table[-p.R];
-    b.right = b.table[p.R];
+__device__ __forceinline__ const float* am_table(const AmParams& p, int h) {
+  return p.table + (long long)h * (2 * p.R + 1) + p.R;
+}
+
+template <bool MOD>
+__device__ __forceinline__ void am_keep(const AmParams& p, const RowInit& w, KeySpan& s, const Row& row) {
+  const bool on = w.live && !w.empty;
+  row.set(Row::LO, on ? w.lo : INT_MIN);
+  row.set(Row::HI, on ? w.hi : INT_MAX);
+  row.set(Row::FLAGS, (w.live ? Row::LIVE : 0) | (w.empty ? Row::EMPTY : 0));
+  if constexpr (MOD) {
+    s.pmin = am_wave_min(w.p);
+    s.pmax = am_wave_max(w.p);
+    row.set(Row::P, w.p);
+    row.set(Row::HEAD, w.h);
+    if (p.slopes) row.set(Row::SLOPE, __float_as_int(p.slopes[w.h]));
+    if (p.table) {
+      const float* tab = am_table(p, w.h);
+      row.set(Row::LEFT, __float_as_int(tab[-p.R]));
+      row.set(Row::RIGHT, __float_as_int(tab[p.R]));
+    }
   }
-  return b;
 }
 
 // What a wave does with tiles of KB * 32 keys.  PB: bytes of a key's row in LDS, DK:
@@ -223,7 +239,7 @@ struct Core {
     kleft = vleft = p.Sk - t * BK;
   }
 
-  __device__ __forceinline__ void load_q(const AmParams& p, const Row& row, int b) {
+  __device__ __forceinline__ void load_q(const AmParams& p, const RowInit& row, int b) {
     const T* qp = (const T*)p.q + b * p.q_sb + row.i * p.q_ss + row.h * p.q_sh + g * 8;
 #pragma unroll
     for (int ds = 0; ds < DK; ++ds) {
@@ -262,8 +278,16 @@ struct Core {
     vleft -= step * BK;
   }
 
-  __device__ __forceinline__ void scores(const unsigned char DLM_LDS* st, f32x16 (&s)[KB]) const {
-    const int base = (lane & 31) * PB + ((g ^ kswz(lane & 31)) * 16);
+  // A lane's number that the compiler cannot follow: addresses made of it are made where they are
+  // used (kept for all of the kernel they take registers that the main loop needs)
+  __device__ __forceinline__ int lane_here() const {
+    int x = lane;
+    asm volatile("" : "+v"(x));
+    return x;
+  }
+
+  __device__ __forceinline__ void scores(const unsigned char DLM_LDS* st, f32x16 (&s)[KB], int lane) const {
+    const int base = (lane & 31) * PB + (((lane >> 5) ^ kswz(lane & 31)) * 16);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -281,7 +305,8 @@ struct Core {
   static constexpr __device__ int key_of(int kb, int e) { return kb * 32 + 8 * (e >> 2) + (e & 3); }
 
   // Cap and bias: s becomes the score itself (without them it stays q.k)
-  __device__ __forceinline__ void modify(const AmParams& p, const Row& row, const Bias& bias, f32x16 (&s)[KB], int k0) const {
+  __device__ __forceinline__ void modify(const AmParams& p, const KeySpan& span, const Row& row, f32x16 (&s)[KB], int k0,
+                                         int g) const {
     if (p.cap > 0.0f) {
       const float ic = p.scale / p.cap;
       float top = 0.0f;
@@ -315,34 +340,35 @@ struct Core {
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[kb][e] *= p.scale;
     }
-    const int d0 = k0 + 4 * g - row.p;
+    const int d0 = k0 + 4 * g - row.get(Row::P);
     if (p.slopes) {
-      const float f0 = (float)d0;
+      const float f0 = (float)d0, slope = row.num(Row::SLOPE);
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          s[kb][e] = __builtin_fmaf(-bias.slope, fabsf(f0 + (float)key_of(kb, e)), s[kb][e]);
+          s[kb][e] = __builtin_fmaf(-slope, fabsf(f0 + (float)key_of(kb, e)), s[kb][e]);
     }
     if (p.table) {
-      if (k0 + BK - 1 - row.pmin <= -p.R || k0 - row.pmax >= p.R) {
-        const float left = bias.left, right = bias.right, t = k0 - row.pmax >= p.R ? right : left;
+      if (k0 + BK - 1 - span.pmin <= -p.R || k0 - span.pmax >= p.R) {
+        const float t = row.num(k0 - span.pmax >= p.R ? Row::RIGHT : Row::LEFT);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
           for (int e = 0; e < 16; ++e) s[kb][e] += t;
       } else {
+        const float* tab = am_table(p, row.get(Row::HEAD));
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[kb][e] += bias.table[max(-p.R, min(p.R, d0 + key_of(kb, e)))];
+          for (int e = 0; e < 16; ++e) s[kb][e] += tab[max(-p.R, min(p.R, d0 + key_of(kb, e)))];
       }
     }
   }
 
-  __device__ __forceinline__ x8 vfrag(const unsigned char DLM_LDS* st, int j, int dt) const {
+  static __device__ __forceinline__ x8 vfrag(const unsigned char DLM_LDS* st, int j, int dt, int lane) {
     const int r4 = (lane & 15) >> 2;
-    const int base = (4 * g + r4) * PB + vswz(r4) * 16 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+    const int base = (4 * (lane >> 5) + r4) * PB + vswz(r4) * 16 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
     const unsigned char DLM_LDS* a = st + (base ^ (64 * dt)) + 16 * j * PB;
     const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 DLM_LDS*)a);
     const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 DLM_LDS*)(a + 8 * PB));
@@ -401,21 +427,21 @@ struct Core {
   }
 
   // O^T += V^T P^T
-  __device__ __forceinline__ void pv(const unsigned char DLM_LDS* st, const x8 (&pf)[2 * KB]) {
+  __device__ __forceinline__ void pv(const unsigned char DLM_LDS* st, const x8 (&pf)[2 * KB], int lane) {
 #pragma unroll
     for (int j = 0; j < 2 * KB; ++j)
 #pragma unroll
-      for (int dt = 0; dt < DV; ++dt) o[dt] = Hf::mfma(vfrag(st, j, dt), pf[j], o[dt]);
+      for (int dt = 0; dt < DV; ++dt) o[dt] = Hf::mfma(vfrag(st, j, dt, lane), pf[j], o[dt]);
   }
 
   // The same of a tile whose V holds infinities or NaN, where 0 * V would spoil rows that
   // do not see them: the finite values alone.
-  __device__ __forceinline__ void pv_finite(const unsigned char DLM_LDS* st, const x8 (&pf)[2 * KB]) {
+  __device__ __forceinline__ void pv_finite(const unsigned char DLM_LDS* st, const x8 (&pf)[2 * KB], int lane) {
 #pragma unroll
     for (int j = 0; j < 2 * KB; ++j)
 #pragma unroll
       for (int dt = 0; dt < DV; ++dt) {
-        u16x8 v = __builtin_bit_cast(u16x8, vfrag(st, j, dt));
+        u16x8 v = __builtin_bit_cast(u16x8, vfrag(st, j, dt, lane));
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = (v[e] & Hf::inf) == Hf::inf ? 0 : v[e];
         o[dt] = Hf::mfma(__builtin_bit_cast(x8, v), pf[j], o[dt]);
@@ -426,12 +452,13 @@ struct Core {
   // ... and behind the loop over tiles (first, first + step, ... below last) the others, read from
   // memory again: a second product counts those that a row sees, 1 for infinity, 128 for
   // -infinity, both for NaN (whole numbers up to 64 * 129, exact in either type and in the sums).
-  __device__ __forceinline__ void add_special(const AmParams& p, const Row& row, const Bias& bias, int b, int hk,
+  __device__ __forceinline__ void add_special(const AmParams& p, const KeySpan& span, const Row& row, int b, int hk,
                                               int first, int last, int step) {
     const T* v = (const T*)p.v + b * p.v_sb + hk * p.v_sh;
+    const int lo = row.get(Row::LO), hi = row.get(Row::HI);
     for (int t = first; t < last; t += step) {
       const int k0 = t * BK;
-      if (k0 >= row.thi || k0 + BK <= row.tlo || (k0 >= row.flo && k0 + BK <= row.fhi && !p.table)) continue;
+      if (!span.any(k0, BK) || (span.whole(k0, BK) && !p.table)) continue;
 #pragma unroll
       for (int dt = 0; dt < DV; ++dt) {
         const int d = dt * 32 + (lane & 31);
@@ -447,8 +474,9 @@ struct Core {
             unsigned short x = 0;
             if (key < p.Sk && d < p.Dh) x = __builtin_bit_cast(unsigned short, v[key * p.v_ss + d]);
             const bool odd = (x & Hf::inf) == Hf::inf, nan = (x & 0x7fff) != Hf::inf;
-            bool sees = key >= row.lo && key < row.hi;
-            if (MOD && p.table) sees = sees && bias.table[max(-p.R, min(p.R, key - row.p))] != -INFINITY;
+            bool sees = key >= lo && key < hi;
+            if (MOD && p.table)
+              sees = sees && am_table(p, row.get(Row::HEAD))[max(-p.R, min(p.R, key - row.get(Row::P)))] != -INFINITY;
             kind[e] = (T)(!odd ? 0.0f : nan ? 129.0f : x & 0x8000 ? 128.0f : 1.0f);
             one[e] = (T)(sees ? 1.0f : 0.0f);
           }
@@ -465,22 +493,23 @@ struct Core {
   }
 
   // Softmax and product of tile t, whose scores are in s and whose V is in LDS at st; any mask
-  __device__ __forceinline__ void finish(const AmParams& p, const Row& row, const Bias& bias, f32x16 (&s)[KB],
+  __device__ __forceinline__ void finish(const AmParams& p, const KeySpan& span, const Row& row, f32x16 (&s)[KB],
                                          const unsigned char DLM_LDS* st, int t) {
-    const int k0 = t * BK;
-    if constexpr (MOD) modify(p, row, bias, s, k0);
+    const int k0 = t * BK, lane = lane_here(), g = lane >> 5;
+    if constexpr (MOD) modify(p, span, row, s, k0, g);
     bool guard = false;
-    if (k0 < row.flo || k0 + BK > row.fhi) {
+    if (!span.whole(k0, BK)) {
       guard = true;
       // in 32 bits whatever the bounds: lo and hi against the tile's first key
-      const int lo = max(row.lo, k0) - k0 - 4 * g, hi = min(row.hi, k0 + BK) - k0 - 4 * g;
-      if (k0 < row.flo) {
+      if (k0 < span.flo) {
+        const int lo = max(row.get(Row::LO), k0) - k0 - 4 * g;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
           for (int e = 0; e < 16; ++e) s[kb][e] = key_of(kb, e) < lo ? -INFINITY : s[kb][e];
       }
-      if (k0 + BK > row.fhi) {
+      if (k0 + BK > span.fhi) {
+        const int hi = min(row.get(Row::HI), k0 + BK) - k0 - 4 * g;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -510,19 +539,19 @@ struct Core {
 #pragma unroll
       for (int j = 0; j < 2 * KB; ++j)
 #pragma unroll
-        for (int dt = 0; dt < DV; ++dt) n = Hf::mfma(vfrag(st, j, dt), zero, n);
+        for (int dt = 0; dt < DV; ++dt) n = Hf::mfma(vfrag(st, j, dt, lane), zero, n);
       float sum = 0.0f;
 #pragma unroll
       for (int e = 0; e < 16; ++e) sum += n[e];
       if (__builtin_amdgcn_ballot_w64(sum != 0.0f) != 0) {
         special = true;
         softmax(s, pf, [] {});
-        pv_finite(st, pf);
+        pv_finite(st, pf, lane);
         return;
       }
     }
     softmax(s, pf, [] {});
-    pv(st, pf);
+    pv(st, pf, lane);
   }
 };
 
@@ -545,7 +574,7 @@ __device__ __forceinline__ void am_store4(const AmParams& p, int b, int i, int h
 }
 
 // Tiles of part `split` of the keys [lo, hi).
-__device__ __forceinline__ void am_span(int lo, int hi, int bk, int splits, int split, int& t0, int& t1) {
+__device__ __forceinline__ void am_tiles(int lo, int hi, int bk, int splits, int split, int& t0, int& t1) {
   if (lo >= hi) {
     t0 = t1 = 0;
     return;
@@ -568,7 +597,8 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PB == 
 attn_masked_kernel(AmParams p) {
   using C = Core<T, PB, DK, DV, MOD, 2, 4>;
   __shared__ __attribute__((aligned(1024))) unsigned char smem_g[4 * C::TILE];
-  __shared__ int span[32];
+  __shared__ int shared[32];
+  __shared__ int rows[4 * Row::N * 64];
   unsigned char DLM_LDS* smem = (unsigned char DLM_LDS*)smem_g;
   // consecutive blocks (the row blocks of one key head, then the next head) on one XCD,
   // whose L2 then holds the K and V of its own heads; the last row blocks, which see the most
@@ -593,16 +623,16 @@ attn_masked_kernel(AmParams p) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = rb * 128 + wave * 32 + (lane & 31);
-  Row row;
-  Bias bias{};
+  const Row row{(int DLM_LDS*)rows + wave * Row::N * 64 + lane};
+  KeySpan span{};
   int hidden = 0;
   C c(p, lane, wave);
+  RowInit init;
   {
     const int b = head / p.Hkv, hk = head - b * p.Hkv;
-    row = am_row(p, b, hk, r);
-    c.load_q(p, row, b);
+    init = am_row(p, b, hk, r);
+    c.load_q(p, init, b);
     if constexpr (MOD) {
-      bias = am_bias(p, row);
       // a table's entries of -infinity are looked for once; a long table counts as having some
       if (p.table) {
         const long long n = (2LL * p.R + 1) * p.G;
@@ -621,13 +651,13 @@ attn_masked_kernel(AmParams p) {
     auto least = [](int x, int y) { return x < y ? x : y; };
     auto most = [](int x, int y) { return x > y ? x : y; };
     auto share = [&](int longest) {
-      am_bounds(row);
+      am_span(init, span);
       if (lane == 0) {
-        int DLM_LDS* s = (int DLM_LDS*)span + 8 * wave;
-        s[0] = row.tlo;
-        s[1] = row.thi;
-        s[2] = row.flo;
-        s[3] = row.fhi;
+        int DLM_LDS* s = (int DLM_LDS*)shared + 8 * wave;
+        s[0] = span.tlo;
+        s[1] = span.thi;
+        s[2] = span.flo;
+        s[3] = span.fhi;
         s[4] = longest;
       }
       AM_WAIT_LGKM();
@@ -635,9 +665,9 @@ attn_masked_kernel(AmParams p) {
       asm volatile("" ::: "memory");
     };
     auto all = [&](int i, auto op) {
-      return __builtin_amdgcn_readfirstlane(op(op(span[i], span[8 + i]), op(span[16 + i], span[24 + i])));
+      return __builtin_amdgcn_readfirstlane(op(op(shared[i], shared[8 + i]), op(shared[16 + i], shared[24 + i])));
     };
-    share(p.parts > 1 ? am_wave_max(row.live && !row.empty ? row.hi - row.lo : 0) : 0);
+    share(p.parts > 1 ? am_wave_max(init.live && !init.empty ? init.hi - init.lo : 0) : 0);
     if (p.parts > 1) {
       // Rows of two documents see twice the keys of one between them: then one workgroup takes the
       // rows of the first half of those keys and a second one the others (2112 + 1984 tokens twice,
@@ -646,15 +676,15 @@ attn_masked_kernel(AmParams p) {
       const bool apart = (hi - lo) / 2 >= longest / 4 * 3 && hi - lo > 4 * C::BK;
       if (part == 1 && !apart) return;
       if (apart) {
-        const bool second = !row.empty && (row.lo >> 1) + (row.hi >> 1) >= (lo >> 1) + (hi >> 1);
-        row.live = row.live && second == (part == 1);
+        const bool second = !init.empty && (init.lo >> 1) + (init.hi >> 1) >= (lo >> 1) + (hi >> 1);
+        init.live = init.live && second == (part == 1);
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         share(0);
       }
     }
-    am_unmask(row);
-    am_span(all(0, least), all(1, most), C::BK, p.splits, split, t0, t1);
+    am_keep<MOD>(p, init, span, row);
+    am_tiles(all(0, least), all(1, most), C::BK, p.splits, split, t0, t1);
     const int flo = all(2, most), fhi = all(3, least);
     f0 = max(t0, (flo + C::BK - 1) / C::BK);
     f0 += (f0 - t0) & 1;
@@ -686,15 +716,15 @@ attn_masked_kernel(AmParams p) {
     c.issue_v(vmem);
     if (t0 + 1 < t1) c.issue_k(smem + C::TILE);
     arrive();
-    c.scores(smem, sa);
+    c.scores(smem, sa, c.lane_here());
     // a tile that every row sees whole, its scores in sc; the next tile's go to sn (behind the
     // last tile they are made of whatever the buffer holds and not used)
     auto whole = [&](int t, int par, f32x16 (&sc)[2], f32x16 (&sn)[2]) {
       arrive();
       copy(t, par);
       typename C::x8 pf[4];
-      c.scores(smem + (par ^ 1) * C::TILE, sn);
-      if constexpr (MOD) c.modify(p, row, bias, sc, t * C::BK);
+      c.scores(smem + (par ^ 1) * C::TILE, sn, lane);
+      if constexpr (MOD) c.modify(p, span, row, sc, t * C::BK, c.g);
       c.softmax(sc, pf, [] {
         // the order of the block up to the branch: a score product, its share of the
         // exponentials, the next fragment of K
@@ -709,7 +739,7 @@ attn_masked_kernel(AmParams p) {
           }
         }
       });
-      c.pv(vmem + par * C::TILE, pf);
+      c.pv(vmem + par * C::TILE, pf, lane);
       __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
 #pragma unroll
       for (int i = 0; i < 4 * DV; ++i) {
@@ -734,18 +764,20 @@ attn_masked_kernel(AmParams p) {
       arrive();
       copy(t, par);
       const int k0 = t * C::BK;
-      if (k0 < row.thi && k0 + C::BK > row.tlo) c.finish(p, row, bias, sa, vmem + par * C::TILE, t);
-      if (k0 + C::BK < row.thi && k0 + 2 * C::BK > row.tlo) c.scores(smem + (par ^ 1) * C::TILE, sa);
+      if (span.any(k0, C::BK)) c.finish(p, span, row, sa, vmem + par * C::TILE, t);
+      if (span.any(k0 + C::BK, C::BK)) c.scores(smem + (par ^ 1) * C::TILE, sa, c.lane_here());
       __builtin_amdgcn_sched_barrier(0);
       ++t;
     }
     if (c.special) {
       const int b = head / p.Hkv;
-      c.add_special(p, row, bias, b, head - b * p.Hkv, t0, t1, 1);
+      c.add_special(p, span, row, b, head - b * p.Hkv, t0, t1, 1);
     }
   }
   const float l = am_sum_halves(c.l);
-  if (!row.live) return;
+  const int flags = row.get(Row::FLAGS);
+  const bool empty = flags & Row::EMPTY;
+  if (!(flags & Row::LIVE)) return;
   // the arguments are read again here rather than kept in scalar registers through the loop
   const AmParams __attribute__((address_space(4)))* q =
       (const AmParams __attribute__((address_space(4)))*)__builtin_amdgcn_kernarg_segment_ptr();
@@ -765,15 +797,17 @@ attn_masked_kernel(AmParams p) {
       }
     if (c.g == 0) {
       float* ml = q->part + (long long)q->splits * q->heads * q->rows * Dh + at * 2;
-      ml[0] = row.empty ? -INFINITY : c.m;
-      ml[1] = row.empty ? 0.0f : l;
+      ml[0] = empty ? -INFINITY : c.m;
+      ml[1] = empty ? 0.0f : l;
     }
     return;
   }
-  const bool none = row.empty || l == 0.0f;
+  const bool none = empty || l == 0.0f;
   const float inv = 1.0f / l;
+  const int query = r / q->G, sub = r - query * q->G;
   typedef T t4 __attribute__((ext_vector_type(4)));
-  T* po = (T*)q->o + (head / q->Hkv) * q->o_sb + row.i * q->o_ss + row.h * q->o_sh;
+  const int batch = head / q->Hkv;
+  T* po = (T*)q->o + batch * q->o_sb + query * q->o_ss + ((head - batch * q->Hkv) * q->G + sub) * q->o_sh;
 #pragma unroll
   for (int dt = 0; dt < DV; ++dt)
 #pragma unroll
@@ -806,12 +840,14 @@ attn_masked_rows_kernel(AmParams p) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   unsigned char DLM_LDS* smem = (unsigned char DLM_LDS*)smem_g + wave * RING;
-  Row row = am_row(p, b, hk, rb * 32 + (lane & 31));
-  am_bounds(row);
-  am_unmask(row);
+  __shared__ int rows[NW * Row::N * 64];
+  const Row row{(int DLM_LDS*)rows + wave * Row::N * 64 + lane};
+  const RowInit init = am_row(p, b, hk, rb * 32 + (lane & 31));
+  KeySpan span{};
+  am_span(init, span);
   C c(p, lane, 0);
   int t0, t1;
-  am_span(row.tlo, row.thi, C::BK, p.splits, split, t0, t1);
+  am_tiles(span.tlo, span.thi, C::BK, p.splits, split, t0, t1);
   int t = t0 + wave;
   c.start(p, b, hk, t);
   auto issue = [&](unsigned char DLM_LDS* st) {
@@ -820,9 +856,8 @@ attn_masked_rows_kernel(AmParams p) {
   };
   if (t < t1) issue(smem);
   if (t + NW < t1) issue(smem + STAGE);
-  c.load_q(p, row, b);
-  Bias bias{};
-  if constexpr (MOD) bias = am_bias(p, row);
+  c.load_q(p, init, b);
+  am_keep<MOD>(p, init, span, row);
   int buf = 0;
   for (; t < t1; t += NW) {
     if (t + NW < t1) {
@@ -833,15 +868,15 @@ attn_masked_rows_kernel(AmParams p) {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
     f32x16 s[1];
-    c.scores(smem + buf * STAGE, s);
-    c.finish(p, row, bias, s, smem + buf * STAGE + C::TILE, t);
+    c.scores(smem + buf * STAGE, s, lane);
+    c.finish(p, span, row, s, smem + buf * STAGE + C::TILE, t);
     __builtin_amdgcn_sched_barrier(0);
     AM_WAIT_LGKM();  // this tile's fragments are read
     asm volatile("" ::: "memory");
     if (t + 2 * NW < t1) issue(smem + buf * STAGE);
     buf ^= 1;
   }
-  if (c.special) c.add_special(p, row, bias, b, hk, t0 + wave, t1, NW);
+  if (c.special) c.add_special(p, span, row, b, hk, t0 + wave, t1, NW);
   const float l = am_sum_halves(c.l);
   if (lane < 32) {
     ml[wave][lane][0] = c.m;
@@ -864,9 +899,9 @@ attn_masked_rows_kernel(AmParams p) {
       part[(wave * D + am_dim(dt, e >> 2) + 4 * c.g + (e & 3)) * 32 + (lane & 31)] =
           c.m == -INFINITY ? 0.0f : c.o[dt][e] * mine;
   __syncthreads();
-  if (!row.live) return;
+  if (!init.live) return;
   const int r = rb * 32 + (lane & 31);
-  const bool none = row.empty || sum == 0.0f;
+  const bool none = init.empty || sum == 0.0f;
   const float inv = 1.0f / sum;
   for (int d = (tid >> 5) * 4; d < p.Dh; d += NW * 8) {
     float x[4];
@@ -882,13 +917,13 @@ attn_masked_rows_kernel(AmParams p) {
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[e] = none ? 0.0f : x[e] * inv;
-      am_store4<T>(p, b, row.i, row.h, d, x[0], x[1], x[2], x[3]);
+      am_store4<T>(p, b, init.i, init.h, d, x[0], x[1], x[2], x[3]);
     }
   }
   if (p.splits > 1 && tid < 32) {
     float* q = am_part_ml(p, split, head, r);
-    q[0] = row.empty ? -INFINITY : top;
-    q[1] = row.empty ? 0.0f : sum;
+    q[0] = init.empty ? -INFINITY : top;
+    q[1] = init.empty ? 0.0f : sum;
   }
 }
 
