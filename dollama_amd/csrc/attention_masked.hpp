@@ -107,13 +107,13 @@ constexpr float AM_LOG2E = 1.4426950408889634f;
 // tanh(t) / t in u = t^2 on [0, 1/4]: Chebyshev fit of degree 4, relative error 1.4e-8
 constexpr double AM_TANH[5] = {0.9999999870693153, -0.3333307189419686, 0.13324828997687793, -0.052989241174895264,
                                0.017141319047070502};
-__device__ __forceinline__ float capped_small(const AmParams& p, float t, float ref) {
+__device__ __forceinline__ float capped_small(const AmParams& p, float t) {
   const float u = t * t;
   float r = __builtin_fmaf(p.ct[4], u, p.ct[3]);
   r = __builtin_fmaf(r, u, p.ct[2]);
   r = __builtin_fmaf(r, u, p.ct[1]);
   r = __builtin_fmaf(r, u, p.ct[0]);
-  return __builtin_fmaf(t, r, -ref);
+  return t * r;
 }
 // tanh(t) = 1 - 2 / (1 + e^2t)
 __device__ __forceinline__ float capped(const AmParams& p, float x) {
@@ -301,6 +301,14 @@ struct Core {
     lim = -1.0f;  // no key seen: the first tile's sum moves the base
   }
 
+  // A value that the compiler cannot follow: what is made of it is made where it is used (kept
+  // for all of the kernel, addresses take registers that the main loop needs, and come back from memory
+  // behind the copies in flight)
+  static __device__ __forceinline__ unsigned here(unsigned x) {
+    asm volatile("" : "+v"(x));
+    return x;
+  }
+
   // Copies the next tile of an operand into LDS: a buffer that starts at the tile's first row, so
   // offsets stay small however long the cache, and ends with the last key's row (what lies
   // past it, and dims past Dh, are zeros).
@@ -308,7 +316,7 @@ struct Core {
     const i32x4 r = dma_rsrc(kptr, (unsigned)((min(BK, kleft) - 1) * kss + dh));
 #pragma unroll
     for (int i = 0; i < NI; ++i)
-      dma16(r, st + (i * NW + wave) * 1024, (int)(koff[i % NKV] + (unsigned)(i / NKV * NKV * NW * RPI * kss)), 0);
+      dma16(r, st + (i * NW + wave) * 1024, (int)(here(koff[i % NKV]) + (unsigned)(i / NKV * NKV * NW * RPI * kss)), 0);
     kptr += (long long)step * BK * kss;
     kleft -= step * BK;
   }
@@ -316,17 +324,9 @@ struct Core {
     const i32x4 r = dma_rsrc(vptr, (unsigned)((min(BK, vleft) - 1) * vss + dh));
 #pragma unroll
     for (int i = 0; i < NI; ++i)
-      dma16(r, st + (i * NW + wave) * 1024, (int)(voff[i % NVV] + (unsigned)(i / NVV * NVV * NW * RPI * vss)), 0);
+      dma16(r, st + (i * NW + wave) * 1024, (int)(here(voff[i % NVV]) + (unsigned)(i / NVV * NVV * NW * RPI * vss)), 0);
     vptr += (long long)step * BK * vss;
     vleft -= step * BK;
-  }
-
-  // A lane's number that the compiler cannot follow: addresses made of it are made where they are
-  // used (kept for all of the kernel they take registers that the main loop needs)
-  __device__ __forceinline__ int lane_here() const {
-    int x = lane;
-    asm volatile("" : "+v"(x));
-    return x;
   }
 
   __device__ __forceinline__ void scores(const unsigned char DLM_LDS* st, f32x16 (&s)[KB], int lane) const {
@@ -347,18 +347,15 @@ struct Core {
   // key of element e of block kb, against the tile's first key and without the lane's 4 g
   static constexpr __device__ int key_of(int kb, int e) { return kb * 32 + 8 * (e >> 2) + (e & 3); }
 
-  // Calls f(z): z(x, kb, e, ref) is the score of element e of block kb in powers of two, less ref,
-  // made of its q.k x.
+  // Calls f(z): z(x, kb, e) is the score of element e of block kb in powers of two, made of
+  // its q.k x.  (Plain scores stay q.k: their scale goes into the exponent's one operation.)
   template <typename F>
   __device__ __forceinline__ void with_scores(const AmParams& p, const KeySpan& span, const Row& row,
                                               const f32x16 (&s)[KB], int k0, int g, F f) const {
-    if constexpr (MODE == AM_PLAIN) {
-      const float c = p.c;
-      f([&](float x, int, int, float ref) { return __builtin_fmaf(x, c, -ref); });
-    }
+    if constexpr (MODE == AM_PLAIN) f([](float x, int, int) { return x; });
     if constexpr (MODE == AM_CAP) {
       // c tanh(t), t = x ic: where no t of the wave passes a half, t times a polynomial in t^2 (7
-      // operations against two of a quarter of their rate and 5)
+      // operations against two of a quarter of their rate and 3)
       float top = 0.0f;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
@@ -366,23 +363,23 @@ struct Core {
         for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(s[kb][e]));
       const float ic = p.ic;
       if (__builtin_amdgcn_ballot_w64(!(top * ic <= 0.5f)) == 0)
-        f([&](float x, int, int, float ref) { return capped_small(p, x * ic, ref); });
+        f([&](float x, int, int) { return capped_small(p, x * ic); });
       else
-        f([&](float x, int, int, float ref) { return capped(p, x) - ref; });
+        f([&](float x, int, int) { return capped(p, x); });
     }
     if constexpr (MODE == AM_SLOPE) {
       // slopes are in powers of two.  Where every key of the tile lies on one side of every row, the
-      // distance is linear in the key: one operation for both
+      // distance is linear in the key
       const float c = p.c, f0 = (float)(k0 + 4 * g - row.get(Row::P)), slope = row.num(Row::SLOPE);
       const bool before = k0 + BK - 1 <= span.pmin;
       if (before || k0 >= span.pmax) {
         const float d = before ? slope : -slope;
-        f([&](float x, int kb, int e, float ref) {
-          return __builtin_fmaf(x, c, __builtin_fmaf(d, (float)key_of(kb, e), __builtin_fmaf(d, f0, -ref)));
+        f([&](float x, int kb, int e) {
+          return __builtin_fmaf(x, c, __builtin_fmaf(d, (float)key_of(kb, e), d * f0));
         });
       } else {
-        f([&](float x, int kb, int e, float ref) {
-          return __builtin_fmaf(x, c, __builtin_fmaf(-slope, fabsf(f0 + (float)key_of(kb, e)), -ref));
+        f([&](float x, int kb, int e) {
+          return __builtin_fmaf(-slope, fabsf(f0 + (float)key_of(kb, e)), x * c);
         });
       }
     }
@@ -390,28 +387,28 @@ struct Core {
       const float c = p.c;
       if (k0 + BK - 1 - span.pmin <= -p.R || k0 - span.pmax >= p.R) {
         const float t = row.num(k0 - span.pmax >= p.R ? Row::RIGHT : Row::LEFT);
-        f([&](float x, int, int, float ref) { return __builtin_fmaf(x, c, t) - ref; });
+        f([&](float x, int, int) { return __builtin_fmaf(x, c, t); });
       } else if (p.table_lds) {
         const int d0 = k0 + 4 * g - row.get(Row::P), R = p.R;
         const float DLM_LDS* tab = row.table + row.get(Row::SUB) * (2 * R + 1) + R;
-        f([&](float x, int kb, int e, float ref) {
-          return __builtin_fmaf(x, c, tab[max(-R, min(R, d0 + key_of(kb, e)))]) - ref;
+        f([&](float x, int kb, int e) {
+          return __builtin_fmaf(x, c, tab[max(-R, min(R, d0 + key_of(kb, e)))]);
         });
       } else {
-        f([&](float x, int kb, int e, float ref) {
-          return __builtin_fmaf(x, c, am_table(p, row, k0 + 4 * g + key_of(kb, e))) - ref;
+        f([&](float x, int kb, int e) {
+          return __builtin_fmaf(x, c, am_table(p, row, k0 + 4 * g + key_of(kb, e)));
         });
       }
     }
     if constexpr (MODE == AM_BOTH) {
       const float f0 = (float)(k0 + 4 * g - row.get(Row::P)), slope = p.slopes ? row.num(Row::SLOPE) : 0.0f;
       if (p.slopes)
-        f([&](float x, int kb, int e, float ref) {
-          return __builtin_fmaf(-slope, fabsf(f0 + (float)key_of(kb, e)), capped(p, x)) - ref;
+        f([&](float x, int kb, int e) {
+          return __builtin_fmaf(-slope, fabsf(f0 + (float)key_of(kb, e)), capped(p, x));
         });
       else
-        f([&](float x, int kb, int e, float ref) {
-          return capped(p, x) + am_table(p, row, k0 + 4 * g + key_of(kb, e)) - ref;
+        f([&](float x, int kb, int e) {
+          return capped(p, x) + am_table(p, row, k0 + 4 * g + key_of(kb, e));
         });
     }
   }
@@ -425,15 +422,17 @@ struct Core {
     return __builtin_bit_cast(x8, i16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
   }
 
-  // p = 2^(score - base) in the operands' type, and this lane's sum of them
-  template <typename Z>
-  __device__ __forceinline__ float exponentials(const f32x16 (&s)[KB], x8 (&pf)[2 * KB], Z z) const {
+  // 2^(score - base)
+  __device__ __forceinline__ T weight(const AmParams& p, float s) const {
+    return (T)__builtin_amdgcn_exp2f(MODE == AM_PLAIN ? __builtin_fmaf(s, p.c, -mref) : s - mref);
+  }
+  // ... of a tile, and this lane's sum of them
+  __device__ __forceinline__ float weights(const AmParams& p, const f32x16 (&s)[KB], x8 (&pf)[2 * KB]) const {
+    float sum[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        pf[2 * kb + (e >> 3)][e & 7] = (T)__builtin_amdgcn_exp2f(z(s[kb][e], kb, e, mref));
-    float sum[2] = {0.0f, 0.0f};
+      for (int e = 0; e < 16; ++e) pf[2 * kb + (e >> 3)][e & 7] = weight(p, s[kb][e]);
 #pragma unroll
     for (int j = 0; j < 2 * KB; ++j)
 #pragma unroll
@@ -441,23 +440,20 @@ struct Core {
     return sum[0] + sum[1];
   }
 
-  // The weights of a tile against the row's base.  No maximum is taken: the sum, which is
-  // needed anyway, tells when some p came near the end of its type; only then (and at a row's first keys)
-  // the base moves to the tile's maximum and the weights are made again.  That a row moves goes
+  // A tile's weights against the row's base, given their sum.  No maximum is taken: the sum, which is
+  // needed anyway, tells when some weight came near the end of its type; only then (and at a row's first
+  // keys) the base moves to the tile's maximum and the weights are made again.  That a row moves goes
   // by its own values, so its result depends on no other row.
-  template <typename Z, typename Order>
-  __device__ __forceinline__ void softmax(const f32x16 (&s)[KB], x8 (&pf)[2 * KB], Z z, Order order) {
-    float sum = exponentials(s, pf, z);
-    order();
+  __device__ __forceinline__ void settle(const AmParams& p, const f32x16 (&s)[KB], x8 (&pf)[2 * KB], float sum) {
     const bool past = !(sum <= lim);
     if (__builtin_amdgcn_ballot_w64(past) != 0) {
       asm volatile("" ::: "memory");  // a real branch
-      float mt = z(s[0][0], 0, 0, 0.0f);
+      float mt = s[0][0];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) mt = fmaxf(mt, z(s[kb][e], kb, e, 0.0f));
-      mt = am_max_halves(mt);
+        for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[kb][e]);
+      mt = am_max_halves(MODE == AM_PLAIN ? mt * p.c : mt);
       const bool move = am_max_halves(past ? 1.0f : 0.0f) > 0.0f && mt > m;
       const float alpha = move ? __builtin_amdgcn_exp2f(m - mt) : 1.0f;
       m = move ? mt : m;
@@ -468,9 +464,52 @@ struct Core {
       for (int dt = 0; dt < DV; ++dt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
-      sum = exponentials(s, pf, z);
+      sum = weights(p, s, pf);
     }
     l += sum;
+  }
+
+  // The weights of a tile (s: q.k, then scores) while the next tile's sn are made of K at st: step by
+  // step of 16 dims two products, a share of the exponentials, and the next step's fragments.  The
+  // steps are kept apart, or all fragments would be read ahead, into registers there are not.
+  template <typename Z>
+  __device__ __forceinline__ float look_ahead(const AmParams& p, const unsigned char DLM_LDS* st, f32x16 (&sn)[KB],
+                                              f32x16 (&s)[KB], x8 (&pf)[2 * KB], Z z, int lane) const {
+    const int base = (lane & 31) * PB + (((lane >> 5) ^ kswz(lane & 31)) * 16);
+    auto frag = [&](int ds, int kb) {
+      return *reinterpret_cast<const x8 DLM_LDS*>(st + (base ^ (32 * ds)) + kb * 32 * PB);
+    };
+    x8 k[2][KB];
+    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      k[0][kb] = frag(0, kb);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sn[kb][e] = 0.0f;
+    }
+#pragma unroll
+    for (int ds = 0; ds < DK; ++ds) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+        if (ds + 1 < DK) k[(ds + 1) & 1][kb] = frag(ds + 1, kb);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) sn[kb] = Hf::mfma(k[ds & 1][kb], qf[ds], sn[kb]);
+#pragma unroll
+      for (int i = 8 * KB * ds / DK; i < 8 * KB * (ds + 1) / DK; ++i) {  // pairs of elements
+        const int kb = i >> 3, e = 2 * (i & 7);
+        typename Hf::x2 w;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          s[kb][e + u] = z(s[kb][e + u], kb, e + u);
+          w[u] = weight(p, s[kb][e + u]);
+        }
+        pf[2 * kb + (e >> 3)][e & 7] = w[0];
+        pf[2 * kb + (e >> 3)][(e & 7) + 1] = w[1];
+        sum[i & 1] = Hf::dot2(w, sum[i & 1]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    return sum[0] + sum[1];
   }
 
   // O^T += V^T P^T
@@ -541,16 +580,15 @@ struct Core {
   // Softmax and product of tile t, whose scores are in s and whose V is in LDS at st; any mask
   __device__ __forceinline__ void finish(const AmParams& p, const KeySpan& span, const Row& row, f32x16 (&s)[KB],
                                          const unsigned char DLM_LDS* st, int t) {
-    const int k0 = t * BK, lane = lane_here(), g = lane >> 5;
+    const int k0 = t * BK, lane = (int)here(this->lane), g = lane >> 5;
     // (a cap takes even -infinity, which masks a key below, to a number)
     if constexpr (MODE != AM_PLAIN)
       with_scores(p, span, row, s, k0, g, [&](auto z) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[kb][e] = z(s[kb][e], kb, e, 0.0f);
+          for (int e = 0; e < 16; ++e) s[kb][e] = z(s[kb][e], kb, e);
       });
-    auto z = [&](float x, int, int, float ref) { return MODE == AM_PLAIN ? __builtin_fmaf(x, p.c, -ref) : x - ref; };
     bool guard = false;
     if (!span.whole(k0, BK)) {
       guard = true;
@@ -599,12 +637,12 @@ struct Core {
       for (int e = 0; e < 16; ++e) sum += n[e];
       if (__builtin_amdgcn_ballot_w64(sum != 0.0f) != 0) {
         special = true;
-        softmax(s, pf, z, [] {});
+        settle(p, s, pf, weights(p, s, pf));
         pv_finite(st, pf, lane);
         return;
       }
     }
-    softmax(s, pf, z, [] {});
+    settle(p, s, pf, weights(p, s, pf));
     pv(st, pf, lane);
   }
 };
@@ -762,30 +800,18 @@ attn_masked_kernel(AmParams p) {
     c.issue_v(vmem + ((t0 ^ even) & 1) * C::TILE);
     if (t0 + 1 < t1) c.issue_k(smem + ((t0 ^ even ^ 1) & 1) * C::TILE);
     arrive();
-    c.scores(smem + ((t0 ^ even) & 1) * C::TILE, sa, c.lane_here());
+    c.scores(smem + ((t0 ^ even) & 1) * C::TILE, sa, (int)C::here(lane));
     // a tile that every row sees whole, its scores in sc; the next tile's go to sn (behind the
     // last tile they are made of whatever the buffer holds and not used)
     auto whole = [&](int t, int par, f32x16 (&sc)[2], f32x16 (&sn)[2]) {
       arrive();
       copy(t, par);
       typename C::x8 pf[4];
+      float sum = 0.0f;
       c.with_scores(p, span, row, sc, t * C::BK, c.g, [&](auto z) {
-        c.scores(smem + (par ^ 1) * C::TILE, sn, lane);
-        c.softmax(sc, pf, z, [] {
-          // the order of the block up to the branch: a score product, its share of the
-          // exponentials, the next fragment of K
-          if constexpr (MODE == AM_PLAIN) {
-            __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
-#pragma unroll
-            for (int i = 0; i < 2 * DK; ++i) {
-              __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-              __builtin_amdgcn_sched_group_barrier(0x2, 32 / DK, 0);
-              __builtin_amdgcn_sched_group_barrier(0x400, 16 / DK, 0);
-              __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            }
-          }
-        });
+        sum = c.look_ahead(p, smem + (par ^ 1) * C::TILE, sn, sc, pf, z, lane);
       });
+      c.settle(p, sc, pf, sum);
       c.pv(vmem + par * C::TILE, pf, lane);
       __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
 #pragma unroll
@@ -812,7 +838,7 @@ attn_masked_kernel(AmParams p) {
       copy(t, par);
       const int k0 = t * C::BK;
       if (span.any(k0, C::BK)) c.finish(p, span, row, sa, vmem + par * C::TILE, t);
-      if (span.any(k0 + C::BK, C::BK)) c.scores(smem + (par ^ 1) * C::TILE, sa, c.lane_here());
+      if (span.any(k0 + C::BK, C::BK)) c.scores(smem + (par ^ 1) * C::TILE, sa, (int)C::here(lane));
       __builtin_amdgcn_sched_barrier(0);
       ++t;
     }
