@@ -127,7 +127,12 @@ int dlm_attention_masked(const dlm_attention_masked_args* a, void* workspace, si
   if (a->cap > 0.0f) {
     p.ic = a->scale / a->cap;
     p.cl = a->cap * AM_LOG2E;
-    for (int i = 0; i < 5; ++i) p.ct[i] = (float)(AM_TANH[i] * a->cap * 1.4426950408889634);
+    // tanh_ratio's coefficients for q.k itself; where their powers would leave fp32's range the
+    // polynomial is not used
+    const double ic = (double)a->scale / a->cap;
+    p.small = ic > 1e-4 && ic < 1e4 ? (float)(0.5 / ic) : -1.0f;
+    double f = (double)a->cap * 1.4426950408889634 * ic;
+    for (int i = 0; i < 5; ++i, f *= ic * ic) p.ct[i] = p.small > 0.0f ? (float)(AM_TANH[i] * f) : 0.0f;
   }
   p.table_lds = a->rel_bias && (2LL * a->R + 1) * p.G <= AM_TABLE_MAX;
   return a->dtype == DLM_DTYPE_F16 ? am_run_f16(p, pl, a->cap > 0.0f, (hipStream_t)stream)

@@ -77,7 +77,8 @@ struct AmParams {
   int causal, nrb, heads, splits;  // row blocks, B * Hkv, parts of the keys
   int parts;                       // workgroups that may share a block's rows
   float c;                         // scale, to powers of two
-  float ic, cl, ct[5];             // scale / cap; the cap, and it times tanh_ratio's coefficients, to powers of two
+  float ic, cl;                    // scale / cap; the cap, to powers of two
+  float small, ct[5];              // q.k up to which, and coefficients with which, the cap is a polynomial
   int table_lds;                   // the table's rows of a key head fit LDS
   float* part;                     // [splits][heads][rows][Dh], then [splits][heads][rows][2]
 };
@@ -107,13 +108,13 @@ constexpr float AM_LOG2E = 1.4426950408889634f;
 // tanh(t) / t in u = t^2 on [0, 1/4]: Chebyshev fit of degree 4, relative error 1.4e-8
 constexpr double AM_TANH[5] = {0.9999999870693153, -0.3333307189419686, 0.13324828997687793, -0.052989241174895264,
                                0.017141319047070502};
-__device__ __forceinline__ float capped_small(const AmParams& p, float t) {
-  const float u = t * t;
+__device__ __forceinline__ float capped_small(const AmParams& p, float x) {
+  const float u = x * x;
   float r = __builtin_fmaf(p.ct[4], u, p.ct[3]);
   r = __builtin_fmaf(r, u, p.ct[2]);
   r = __builtin_fmaf(r, u, p.ct[1]);
   r = __builtin_fmaf(r, u, p.ct[0]);
-  return t * r;
+  return x * r;
 }
 // tanh(t) = 1 - 2 / (1 + e^2t)
 __device__ __forceinline__ float capped(const AmParams& p, float x) {
@@ -354,16 +355,15 @@ struct Core {
                                               const f32x16 (&s)[KB], int k0, int g, F f) const {
     if constexpr (MODE == AM_PLAIN) f([](float x, int, int) { return x; });
     if constexpr (MODE == AM_CAP) {
-      // c tanh(t), t = x ic: where no t of the wave passes a half, t times a polynomial in t^2 (7
+      // c tanh(t), t = x ic: where no t of the wave passes a half, x times a polynomial in x^2 (6
       // operations against two of a quarter of their rate and 3)
       float top = 0.0f;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(s[kb][e]));
-      const float ic = p.ic;
-      if (__builtin_amdgcn_ballot_w64(!(top * ic <= 0.5f)) == 0)
-        f([&](float x, int, int) { return capped_small(p, x * ic); });
+      if (__builtin_amdgcn_ballot_w64(!(top <= p.small)) == 0)
+        f([&](float x, int, int) { return capped_small(p, x); });
       else
         f([&](float x, int, int) { return capped(p, x); });
     }
@@ -752,11 +752,12 @@ attn_masked_kernel(AmParams p) {
     };
     share(p.parts > 1 ? am_wave_max(init.live && !init.empty ? init.hi - init.lo : 0) : 0);
     if (p.parts > 1) {
-      // Rows of two documents see twice the keys of one between them: then one workgroup takes the
-      // rows of the first half of those keys and a second one the others (2112 + 1984 tokens twice,
-      // x10x64: 104 -> XX us).  Where the rows see much the same the second one has nothing to do.
+      // Rows of two documents see the keys of both between them: then one workgroup takes the
+      // rows that see the first half of those keys and a second one the others (documents of 2112 and
+      // 1984 tokens, x10x64: 104 -> 66 us).  Where the rows see much the same (less than four tiles and
+      // an eighth more than one of them) the second one has nothing to do.
       const int lo = all(0, least), hi = all(1, most), longest = all(4, most);
-      const bool apart = (hi - lo) / 2 >= longest / 4 * 3 && hi - lo > 4 * C::BK;
+      const bool apart = hi - lo - longest >= max(4 * C::BK, longest / 8);
       if (part == 1 && !apart) return;
       if (apart) {
         const bool second = !init.empty && (init.lo >> 1) + (init.hi >> 1) >= (lo >> 1) + (hi >> 1);
