@@ -20,23 +20,16 @@ struct RotaryParams {
   const char* gamma[2];
   long long xb[2], xs[2], xh[2];  // strides in elements: batch, token, head
   long long yb[2], ys[2], yh[2];
-  int heads[2], blocks[2];        // heads, and blocks of `hpg` heads along the grid's y
+  int heads[2], blocks[2], hpg[2];  // heads, and blocks of `hpg` heads along the grid's y
   const void* pos;
   long long pb, ps;
   int pos_type, axes;
   int ends[4];                    // pairs up to and with each axis
   const double* freqs;
-  int P, Dh, hpg, norm;
-  long long tokens;
-  int S;
+  int P, Dh, norm;
+  int tokens, S;
   float eps, inv_dh;
 };
-
-__device__ __forceinline__ double rot_pos(const RotaryParams& p, long long at) {
-  if (p.pos_type == DLM_POS_I32) return (double)((const int*)p.pos)[at];
-  if (p.pos_type == DLM_POS_I64) return (double)((const long long*)p.pos)[at];
-  return (double)((const float*)p.pos)[at];
-}
 
 // The sum over a group of W consecutive lanes (W a power of two), the same bits in
 // each of them.
@@ -58,67 +51,103 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
-// A group of W lanes takes one token and `hpg` heads of it: the angles are computed
-// once for all of them.  A lane holds two vectors of V elements of a head (C chunks
+// A group of W lanes takes one token and some heads of it: the angles are computed once for
+// all of them.  Groups side by side take tokens side by side (heads side by side, which makes a wave's
+// accesses longer, took 41 instead of 31 us for 8192x(32+8)x128 in place).  A lane holds two vectors of V elements of a head (C chunks
 // of them where a head has more lanes than a wave):
-//   halves:      8 pairs (i, i + P) as V at i and V at P + i; behind 2P, plain pairs
-//                of vectors
+//   halves:      V pairs (i, i + P) as V elements at i and V at P + i; behind 2P, any two vectors
 //   interleaved: V at i and V at Dh / 2 + i, V / 2 pairs in each (V = 1: elements 2i
 //                and 2i + 1)
-// Memory bounds it: U heads are requested ahead of the first one's arithmetic.
-template <typename T, int V, int W, int C, bool IL>
-__global__ void __launch_bounds__(256) rotary_kernel(RotaryParams p) {
+// Memory bounds it: U heads are requested at a time, the first ones ahead of the angles.  A few heads
+// of a few tokens (U = 1) are bound by the instructions' way to the CUs instead: 32 heads of one token 5.2 us with
+// the code for four heads at a time, the norm's among it, 3.3 us without.
+template <typename T, int V, int W, int C, bool IL, bool NORM, int U>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4)))
+rotary_kernel(RotaryParams p) {
   typedef T TV __attribute__((ext_vector_type(V)));
-  constexpr int U = C > 1 ? 1 : V == 8 ? 4 : 8;
   const int lane = threadIdx.x & (W - 1);
-  const long long token = (long long)blockIdx.x * (256 / W) + threadIdx.x / W;
+  const int token = (int)blockIdx.x * (256 / W) + threadIdx.x / W;
   const bool live = token < p.tokens;
-  const long long tok = live ? token : p.tokens - 1;  // dead groups follow along: the sums need whole waves
+  const unsigned tok = live ? token : p.tokens - 1;  // dead groups follow along: the sums need whole waves
   const int kv = (int)blockIdx.y >= p.blocks[0];
-  const int h0 = ((int)blockIdx.y - (kv ? p.blocks[0] : 0)) * p.hpg;
-  const int h1 = min(p.heads[kv], h0 + p.hpg);
-  const long long b = tok / p.S, s = tok - b * p.S;
+  const int h0 = ((int)blockIdx.y - (kv ? p.blocks[0] : 0)) * p.hpg[kv];
+  const int h1 = min(p.heads[kv], h0 + p.hpg[kv]);
+  const unsigned b = tok / (unsigned)p.S, s = tok - b * (unsigned)p.S;
 
-  // where this lane's two vectors start, whether they are in the head, and their pairs
+  // where this lane's two vectors start, and whether they are in the head
   int at[C][2];
   bool in[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int i = (c * W + lane) * V;
+    in[c] = 2 * i < p.Dh;
+    at[c][0] = IL ? (V == 1 ? 2 * i : i) : i < p.P ? i : 2 * i;
+    at[c][1] = IL ? (V == 1 ? 2 * i + 1 : p.Dh / 2 + i) : i < p.P ? p.P + i : 2 * i + V;
+  }
+  const T* src = (const T*)p.x[kv] + (long long)b * p.xb[kv] + (long long)s * p.xs[kv];
+  T* dst = (T*)p.y[kv] + (long long)b * p.yb[kv] + (long long)s * p.ys[kv];
+  TV r[U][C][2];
+  auto request = [&](int h) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          r[u][c][w] = TV{};
+          if (in[c] && h + u < h1)
+            r[u][c][w] = *reinterpret_cast<const TV*>(src + (h + u) * p.xh[kv] + at[c][w]);
+        }
+  };
+  int h = h0;
+  request(h);
+
+  // the token's places, the pairs' angles, gamma
+  double place[4] = {0.0, 0.0, 0.0, 0.0};
+  if (p.P > 0) {
+    const long long at0 = (long long)b * p.pb + (long long)s * p.ps;
+    auto places = [&](auto* q) {
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+        if (a < p.axes) place[a] = (double)q[at0 + a];
+    };
+    if (p.pos_type == DLM_POS_I32)
+      places((const int*)p.pos);
+    else if (p.pos_type == DLM_POS_I64)
+      places((const long long*)p.pos);
+    else
+      places((const float*)p.pos);
+  }
   float cs[C][V], sn[C][V];
   float gam[C][2][V];
   unsigned plain[C];  // pairs that stay as they are
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    plain[c] = 0;
     const int i = (c * W + lane) * V;
-    in[c] = 2 * i < p.Dh;
-    int pair[V];
-    if (IL) {
-      at[c][0] = V == 1 ? 2 * i : i;
-      at[c][1] = V == 1 ? 2 * i + 1 : p.Dh / 2 + i;
+    plain[c] = (1u << V) - 1;
+    if (p.P > 0) {
+      plain[c] = 0;
 #pragma unroll
-      for (int e = 0; e < V; ++e)
-        pair[e] = V == 1 ? i : e < V / 2 ? i / 2 + e : p.Dh / 4 + i / 2 + (e - V / 2);
-    } else {
-      at[c][0] = i < p.P ? i : 2 * i;
-      at[c][1] = i < p.P ? p.P + i : 2 * i + V;
+      for (int e = 0; e < V; ++e) {
+        const int pair = IL && V > 1 ? (e < V / 2 ? i / 2 + e : p.Dh / 4 + i / 2 + (e - V / 2)) : i + e;
+        const bool turns = pair < p.P;
+        double x = place[0];
 #pragma unroll
-      for (int e = 0; e < V; ++e) pair[e] = i + e;
-    }
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      cs[c][e] = 1.0f;
-      sn[c][e] = 0.0f;
-      if (in[c] && pair[e] < p.P) {
-        const int a = (pair[e] >= p.ends[0]) + (pair[e] >= p.ends[1]) + (pair[e] >= p.ends[2]);
-        constexpr double inv2pi = 0.15915494309189533577;
-        const double turns = rot_pos(p, b * p.pb + s * p.ps + a) * (p.freqs[pair[e]] * inv2pi);
-        const float f = (float)(turns - __builtin_floor(turns));
+        for (int a = 0; a < 3; ++a) x = pair >= p.ends[a] ? place[a + 1] : x;
+        x *= p.freqs[turns ? pair : 0] * 0.15915494309189533577;
+        const float f = (float)(x - __builtin_floor(x));
         cs[c][e] = __builtin_amdgcn_cosf(f);
         sn[c][e] = __builtin_amdgcn_sinf(f);
-      } else {
-        plain[c] |= 1u << e;
+        plain[c] |= turns ? 0 : 1u << e;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        cs[c][e] = 1.0f;
+        sn[c][e] = 0.0f;
       }
     }
-    if (p.norm) {
+    if constexpr (NORM) {
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         TV g;
@@ -131,22 +160,9 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryParams p) {
     }
   }
 
-  const T* src = (const T*)p.x[kv] + b * p.xb[kv] + s * p.xs[kv];
-  T* dst = (T*)p.y[kv] + b * p.yb[kv] + s * p.ys[kv];
-  for (int h = h0; h < h1; h += U) {
-    TV r[U][C][2];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int c = 0; c < C; ++c)
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          r[u][c][w] = TV{};
-          if (in[c] && h + u < h1) r[u][c][w] = *reinterpret_cast<const TV*>(src + (h + u) * p.xh[kv] + at[c][w]);
-        }
+  for (;;) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (h + u >= h1) break;
       float x[C][2][V];
 #pragma unroll
       for (int c = 0; c < C; ++c)
@@ -154,7 +170,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryParams p) {
         for (int w = 0; w < 2; ++w)
 #pragma unroll
           for (int e = 0; e < V; ++e) x[c][w][e] = (float)r[u][c][w][e];
-      if (p.norm) {
+      if constexpr (NORM) {
         auto squares = [&] {
           float q = 0.0f;
 #pragma unroll
@@ -200,15 +216,15 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryParams p) {
             for (int e = 0; e < V; e += 2) {
               const float co = cs[c][w * (V / 2) + e / 2], si = sn[c][w * (V / 2) + e / 2];
               const float a = x[c][w][e], d = x[c][w][e + 1];
-              o[w][e] = (T)(a * co - d * si);
-              o[w][e + 1] = (T)(d * co + a * si);
+              o[w][e] = (T)__builtin_fmaf(a, co, -(d * si));
+              o[w][e + 1] = (T)__builtin_fmaf(d, co, a * si);
             }
         } else {
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             const float a = x[c][0][e], d = x[c][1][e];
-            o[0][e] = (T)(a * cs[c][e] - d * sn[c][e]);
-            o[1][e] = (T)(d * cs[c][e] + a * sn[c][e]);
+            o[0][e] = (T)__builtin_fmaf(a, cs[c][e], -(d * sn[c][e]));
+            o[1][e] = (T)__builtin_fmaf(d, cs[c][e], a * sn[c][e]);
           }
         }
         if (plain[c]) {  // an infinity there is its own alone
@@ -220,26 +236,36 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryParams p) {
               o[w][e] = plain[c] >> k & 1 ? (T)x[c][w][e] : o[w][e];
             }
         }
-        if (in[c] && live) {
+        if (in[c] && live && h + u < h1) {
           *reinterpret_cast<TV*>(dst + (h + u) * p.yh[kv] + at[c][0]) = o[0];
           *reinterpret_cast<TV*>(dst + (h + u) * p.yh[kv] + at[c][1]) = o[1];
         }
       }
     }
+    h += U;
+    if (h >= h1) break;
+    request(h);
   }
 }
 
 template <typename T, int V, int W, int C, bool IL>
 static int rotary_go(RotaryParams& p, hipStream_t s) {
-  // Heads of one group: as many as leave the card 4096 waves (16 a CU)
-  const long long waves = (p.tokens + 64 / W - 1) / (64 / W);
-  const int total = p.heads[0] + p.heads[1];
-  const int parts = (int)std::min<long long>(total, std::max<long long>(1, (4096 + waves - 1) / waves));
-  p.hpg = (total + parts - 1) / parts;
-  p.blocks[0] = (p.heads[0] + p.hpg - 1) / p.hpg;
-  p.blocks[1] = (p.heads[1] + p.hpg - 1) / p.hpg;
-  const dim3 grid((unsigned)((p.tokens + 256 / W - 1) / (256 / W)), p.blocks[0] + p.blocks[1]);
-  DLM_LAUNCH("rotary_kernel", (rotary_kernel<T, V, W, C, IL>), grid, dim3(256), 0, s, p);
+  // Heads of one group: as many as leave the card 4096 waves (16 a CU), alike in all groups
+  const int tiles = (p.tokens + 256 / W - 1) / (256 / W);
+  const int want = std::max(1, (1024 + tiles - 1) / tiles), total = p.heads[0] + p.heads[1];
+  for (int i = 0; i < 2; ++i) {
+    const int parts = (int)std::min<long long>(p.heads[i], ((long long)want * p.heads[i] + total - 1) / total);
+    p.hpg[i] = parts ? (p.heads[i] + parts - 1) / parts : 1;
+    p.blocks[i] = (p.heads[i] + p.hpg[i] - 1) / p.hpg[i];
+  }
+  const dim3 grid(tiles, p.blocks[0] + p.blocks[1]);
+  const bool many = V > 1 && std::max(p.hpg[0], p.hpg[1]) > 2;
+  auto go = [&](auto kernel) { DLM_LAUNCH("rotary_kernel", kernel, grid, dim3(256), 0, s, p); };
+  constexpr int U = V > 1 ? 4 : 1;
+  if (p.norm)
+    many ? go(rotary_kernel<T, V, W, C, IL, true, U>) : go(rotary_kernel<T, V, W, C, IL, true, 1>);
+  else
+    many ? go(rotary_kernel<T, V, W, C, IL, false, U>) : go(rotary_kernel<T, V, W, C, IL, false, 1>);
   DLM_LAUNCH_CHECK();
   return DLM_OK;
 }
@@ -248,16 +274,11 @@ template <typename T, bool IL>
 static int rotary_by_width(RotaryParams& p, int V, hipStream_t s) {
   const int lanes = p.Dh / (2 * V);  // of one head
   if (V == 8) {
-    if (lanes <= 2) return rotary_go<T, 8, 2, 1, IL>(p, s);
     if (lanes <= 4) return rotary_go<T, 8, 4, 1, IL>(p, s);
     if (lanes <= 8) return rotary_go<T, 8, 8, 1, IL>(p, s);
     return rotary_go<T, 8, 16, 1, IL>(p, s);
   }
-  if (V == 4) {
-    if (lanes <= 8) return rotary_go<T, 4, 8, 1, IL>(p, s);
-    if (lanes <= 16) return rotary_go<T, 4, 16, 1, IL>(p, s);
-    return rotary_go<T, 4, 32, 1, IL>(p, s);
-  }
+  if (V == 4) return lanes <= 16 ? rotary_go<T, 4, 16, 1, IL>(p, s) : rotary_go<T, 4, 32, 1, IL>(p, s);
   return lanes <= 64 ? rotary_go<T, 1, 64, 1, IL>(p, s) : rotary_go<T, 1, 64, 2, IL>(p, s);
 }
 
@@ -415,7 +436,7 @@ static int rotary_run(const char* fn, const dlm_rotary_args* a, hipStream_t s) {
   }
   p.freqs = a->freqs;
   p.P = P, p.Dh = a->Dh, p.norm = a->norm != 0;
-  p.tokens = (long long)a->B * a->S, p.S = a->S, p.eps = a->eps;
+  p.tokens = a->B * a->S, p.S = a->S, p.eps = a->eps;
   p.inv_dh = 1.0f / (float)a->Dh;
   const int V = rotary_vector(a, P);
   if (a->dtype == DLM_DTYPE_F16)
