@@ -9,11 +9,13 @@ int am_run_f16(const AmParams& p, const AmPlan& pl, bool cap, hipStream_t s) { r
 static AmPlan am_plan(const dlm_attention_masked_args* a) {
   const long long heads = (long long)a->B * a->Hkv, rows = (long long)a->Sq * (a->H / a->Hkv);
   AmPlan pl;
-  pl.few = rows <= 64;
+  pl.few = rows <= 32;
   pl.nrb = (int)((rows + (pl.few ? 31 : 127)) / (pl.few ? 32 : 128));
-  const long long blocks = heads * pl.nrb;
-  const long long want = pl.few ? 256 : 512, unit = pl.few ? 512 : 256;
-  pl.splits = (int)std::max<long long>(1, std::min({(want + blocks - 1) / blocks, (long long)(a->Sk + unit - 1) / unit, 64LL}));
+  // A workgroup for every CU, of 256 keys at least.  (us with 1 / 4 / 8 / 16 / 32 parts: one token over
+  // 4096 keys, 32/8 heads of 128: 38 / 19 / 14 / 12 / 12, over 65536: 485 / 132 / 72 / 51 / 50;
+  // 64 tokens over 30001: 420 / 117 / 67 / 45 / 53; 256 over 4096: 68 / 39 / 38 / 50 / 78.)
+  const long long blocks = heads * pl.nrb, most = a->Sk / 256;
+  pl.splits = most < 3 ? 1 : (int)std::min({(256 + blocks - 1) / blocks, most, 64LL});
   return pl;
 }
 

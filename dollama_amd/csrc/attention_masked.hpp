@@ -1006,33 +1006,51 @@ attn_masked_rows_kernel(AmParams p) {
   }
 }
 
-// Joins the parts of every row; a thread takes four dims.
-template <typename T>
+// Joins the parts of a row, a wave each.  A lane knows the weight of one part; groups of
+// DL lanes (four dims a lane) take every 64 / DL-th part, eight requested at a time (one after the other
+// they took half a microsecond each).
+template <typename T, int DL>
 __global__ void __launch_bounds__(256) attn_masked_join_kernel(AmParams p) {
-  const int per = p.Dh / 4;
-  const long long at = blockIdx.x * 256LL + threadIdx.x;
-  const long long total = (long long)p.heads * p.rows;
-  const long long hr = at / per;
-  if (hr >= total) return;
-  const int d = (int)(at - hr * per) * 4;
-  const int head = (int)(hr / p.rows), r = (int)(hr - (long long)head * p.rows);
-  float top = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) top = fmaxf(top, am_part_ml(p, s, head, r)[0]);
-  float sum = 0.0f;
+  constexpr int NG = 64 / DL;
+  const int lane = threadIdx.x & 63, group = lane / DL, d = (lane % DL) * 4;
+  const long long hr = blockIdx.x * 4LL + (threadIdx.x >> 6);
+  if (hr >= (long long)p.heads * p.rows) return;
+  const long long step = (long long)p.heads * p.rows;  // rows between one part and the next
+  const float* po = p.part + hr * p.Dh + d;
+  float2 ml = make_float2(-INFINITY, 0.0f);
+  if (lane < p.splits) ml = *reinterpret_cast<const float2*>(p.part + (p.splits * step) * p.Dh + (lane * step + hr) * 2);
+  const float top = wave_max(ml.x);
+  const bool saw = !(ml.x == -INFINITY && ml.y == 0.0f);
+  const float w = saw ? __builtin_amdgcn_exp2f(ml.x - top) : 0.0f;
+  const float sum = wave_sum(saw ? ml.y * w : 0.0f);
   f32x4 a{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = 0; s < p.splits; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(am_part_ml(p, s, head, r));
-    const f32x4 x = *reinterpret_cast<const f32x4*>(am_part_o(p, s, head, r) + d);
-    if (ml.x == -INFINITY && ml.y == 0.0f) continue;  // saw no key
-    const float w = __builtin_amdgcn_exp2f(ml.x - top);
-    sum = __builtin_fmaf(ml.y, w, sum);
-    a += x * w;
+  for (int s0 = 0; s0 < p.splits; s0 += 8 * NG) {
+    f32x4 x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int s = s0 + i * NG + group;
+      x[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (s < p.splits && d < p.Dh) x[i] = *reinterpret_cast<const f32x4*>(po + s * step * p.Dh);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int s = s0 + i * NG + group;
+      const float ws = __shfl(w, min(s, 63), 64);
+      const bool on = __shfl((int)saw, min(s, 63), 64) != 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a[e] = on ? __builtin_fmaf(x[i][e], ws, a[e]) : a[e];
+    }
   }
+#pragma unroll
+  for (int o = DL; o < 64; o *= 2)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[e] += __shfl_xor(a[e], o, 64);
   const float inv = 1.0f / sum;
 #pragma unroll
   for (int e = 0; e < 4; ++e) a[e] = sum == 0.0f ? 0.0f : a[e] * inv;
+  const int head = (int)(hr / p.rows), r = (int)(hr - (long long)head * p.rows);
   const int b = head / p.Hkv, hk = head - b * p.Hkv, i = r / p.G;
-  am_store4<T>(p, b, i, hk * p.G + r - i * p.G, d, a[0], a[1], a[2], a[3]);
+  if (group == 0 && d < p.Dh) am_store4<T>(p, b, i, hk * p.G + r - i * p.G, d, a[0], a[1], a[2], a[3]);
 }
 
 // ---------------------------------------------------------------------------
@@ -1054,9 +1072,10 @@ static int am_launch(const AmParams& p, const AmPlan& pl, hipStream_t s) {
                dim3(256), 0, s, p);
   DLM_LAUNCH_CHECK();
   if (pl.splits > 1) {
-    const long long n = (long long)p.heads * p.rows * (p.Dh / 4);
-    DLM_LAUNCH("attn_masked_join_kernel", attn_masked_join_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s,
-               p);
+    const dim3 grid((unsigned)(((long long)p.heads * p.rows + 3) / 4));
+    auto join = [&](auto kernel) { DLM_LAUNCH("attn_masked_join_kernel", kernel, grid, dim3(256), 0, s, p); };
+    p.Dh <= 64 ? join(attn_masked_join_kernel<T, 16>)
+               : p.Dh <= 128 ? join(attn_masked_join_kernel<T, 32>) : join(attn_masked_join_kernel<T, 64>);
     DLM_LAUNCH_CHECK();
   }
   return DLM_OK;

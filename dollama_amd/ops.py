@@ -958,16 +958,18 @@ def _heads_dev(t: torch.Tensor, name: str) -> int:
 
 def _heads(t: torch.Tensor, shape, dtype, name: str, dev: int):
     """(batch, token, head) strides of t, which has to be `shape` of `dtype` on device `dev`."""
-    if t.dtype == dtype and t.shape == shape and t.get_device() == dev:
-        st = t.stride()
-        if st[-1] == 1 or shape[-1] == 1:
-            return st[:3] if len(st) == 4 else (0, st[0], st[1])
-        raise ValueError(f"{name} must have consecutive values in a head")
+    st = t.stride()
+    if t.dtype is dtype and t.shape == shape and st[-1] == 1 and t.get_device() == dev:
+        return st[:3] if len(st) == 4 else (0, st[0], st[1])
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
     if t.shape != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    raise ValueError(f"{name} must be on the current device, cuda:{dev}, got {t.device}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} must be on the current device, cuda:{dev}, got {t.device}")
+    if shape[-1] == 1:
+        return st[:3] if len(st) == 4 else (0, st[0], st[1])
+    raise ValueError(f"{name} must have consecutive values in a head")
 
 
 def rotary_freqs(sections: Sequence[int], theta: float = 10000.0, shared: bool = False, device="cuda") -> torch.Tensor:
@@ -984,25 +986,29 @@ def rotary_freqs(sections: Sequence[int], theta: float = 10000.0, shared: bool =
     return torch.tensor(f, dtype=torch.float64).to(device)
 
 
+_NO_STRIDES = (0, 0, 0)
+_SECTIONS_PAD = ((0, 0, 0, 0), (0, 0, 0), (0, 0), (0,), ())
+
+
 def _rotary(name, q, k, q_gamma, k_gamma, positions, freqs, sections, interleaved, norm, eps, q_out, k_out):
     dev = _heads_dev(q, "q")
     shape, dt = q.shape, q.dtype
-    B, (S, H, Dh) = (shape[0] if len(shape) == 4 else 1), shape[-3:]
+    S, H, Dh = shape[-3:]
     sq = _heads(q, shape, dt, "q", dev)
     if q_out is None:
         q_out = torch.empty(shape, dtype=dt, device=q.device)
-    so = _heads(q_out, shape, dt, "q_out", dev)
-    sk = sko = (0, 0, 0)
+    so = sq if q_out is q else _heads(q_out, shape, dt, "q_out", dev)
+    sk = sko = _NO_STRIDES
     pk = pko = Hkv = 0
     if k is not None:
-        if k.dim() != len(shape) or k.shape[-2] < 1:
-            raise ValueError(f"k must have q's dimensions and a head at least, got {list(k.shape)}")
-        Hkv = k.shape[-2]
-        kshape = (*shape[:-2], Hkv, Dh)
+        kshape = k.shape
+        Hkv = kshape[-2] if len(kshape) == len(shape) else 0
+        if Hkv < 1 or kshape[:-2] != shape[:-2] or kshape[-1] != Dh:
+            raise ValueError(f"k must be q's shape but for its heads, {list(shape)}, got {list(kshape)}")
         sk = _heads(k, kshape, dt, "k", dev)
         if k_out is None:
             k_out = torch.empty(kshape, dtype=dt, device=q.device)
-        sko = _heads(k_out, kshape, dt, "k_out", dev)
+        sko = sk if k_out is k else _heads(k_out, kshape, dt, "k_out", dev)
         pk, pko = k.data_ptr(), k_out.data_ptr()
     elif k_out is not None or k_gamma is not None:
         raise ValueError("k_out and k_gamma need k")
@@ -1011,33 +1017,38 @@ def _rotary(name, q, k, q_gamma, k_gamma, positions, freqs, sections, interleave
     axes = len(sections)
     if axes > 4:
         raise ValueError("at most four axes")
-    if any(n < 0 for n in sections):
+    if axes and min(sections) < 0:
         raise ValueError("a section has a negative number of pairs")
     P = sum(sections)
-    pp = pf = pt = 0
-    sp = (0, 0)
+    pp = pf = pt = sp0 = sp1 = 0
     if P > 0:
         if positions is None or freqs is None:
             raise ValueError("sections need positions and freqs")
-        if positions.dtype not in _POS or positions.get_device() != dev:
+        pt = _POS.get(positions.dtype)
+        if pt is None or positions.get_device() != dev:
             raise ValueError(f"positions must be int32, int64 or float32 on the current device, got "
                              f"{positions.dtype} on {positions.device}")
-        pshape = positions.shape
-        if pshape != (S, axes) and pshape != (*shape[:-2], axes):
+        pshape, st = positions.shape, positions.stride()
+        if pshape == (S, axes):
+            sp1 = st[0]
+        elif pshape == (*shape[:-2], axes):
+            sp0, sp1 = st[0], st[1]
+        else:
             raise ValueError(f"positions must be {[*shape[:-2], axes]} or {[S, axes]}, got {list(pshape)}")
-        st = positions.stride()
         if axes > 1 and st[-1] != 1:
             raise ValueError("positions must have consecutive axes")
-        sp = st[:2] if len(st) == 3 else (0, st[0])
-        pp, pt = positions.data_ptr(), _POS[positions.dtype]
+        pp = positions.data_ptr()
         pf = _vector(freqs, P, "freqs", torch.float64, dev)
     elif positions is not None or freqs is not None:
         raise ValueError("positions and freqs need sections")
-    if not q.numel():
+    B = shape[0] if len(shape) == 4 else 1
+    if not (B and S and H and Dh):
         return q_out, k_out
-    args = _pack_rotary(q.data_ptr(), pk, q_out.data_ptr(), pko, *sq, *sk, *so, *sko, gq, gk, pp, *sp, pf, pt, axes,
-                        *sections, *(0,) * (4 - axes), interleaved, norm, eps, _HALF[dt], B, S, H, Hkv, Dh)
-    _lib.check(_entry(name)(args, _stream_of(dev)))
+    args = _pack_rotary(q.data_ptr(), pk, q_out.data_ptr(), pko, *sq, *sk, *so, *sko, gq, gk, pp, sp0, sp1, pf, pt, axes,
+                        *sections, *_SECTIONS_PAD[axes], interleaved, norm, eps, _HALF[dt], B, S, H, Hkv, Dh)
+    st = _entry(name)(args, torch._C._cuda_getCurrentRawStream(dev))
+    if st:
+        _lib.check(st)
     return q_out, k_out
 
 
@@ -1101,7 +1112,7 @@ def _batch_ints(t, B, inner, name, dev):
     if t.shape != inner and t.shape != (B, *inner):
         raise ValueError(f"{name} must be {[B, *inner]} or {list(inner)}, got {list(t.shape)}")
     if t.is_contiguous():
-        return t.data_ptr(), (t.stride(0) if len(t.shape) > len(inner) else 0)
+        return t.data_ptr(), (t.stride(0) if t.dim() > len(inner) else 0)
     if len(t.shape) > len(inner) and t.shape[0] > 0 and t[0].is_contiguous():
         return t.data_ptr(), t.stride(0)
     raise ValueError(f"{name} must be contiguous within a batch")
@@ -1151,11 +1162,13 @@ def attention_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_r
         pb = _vector(rel_bias, H * (2 * R + 1), "rel_bias", torch.float32, dev)
     if scale is None:
         scale = Dh ** -0.5 if Dh else 1.0
-    if not q.numel():
+    if not (B and Sq and H and Dh):
         return out
     args = _pack_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *sq, *sk, *sv, *so, kr, krb, qp, qpb,
                            ps, pb, R, scale, cap, bool(causal), _HALF[dt], B, Sq, Sk, H, Hkv, Dh)
     n = _entry("dlm_attention_masked_workspace_bytes")(args)
-    ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-    _lib.check(_entry("dlm_attention_masked")(args, _p(ws), n, _stream_of(dev)))
+    ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None  # (held until the call is enqueued)
+    st = _entry("dlm_attention_masked")(args, _p(ws), n, torch._C._cuda_getCurrentRawStream(dev))
+    if st:
+        _lib.check(st)
     return out
