@@ -124,6 +124,9 @@ int dlm_attention_masked(const dlm_attention_masked_args* a, void* workspace, si
   p.rows = a->Sq * p.G;
   p.causal = a->causal != 0, p.nrb = pl.nrb, p.heads = a->B * a->Hkv, p.splits = pl.splits;
   p.parts = a->key_range ? 2 : 1;
+  // (more blocks than these even out by themselves, and a head's next to one another share its K and V)
+  const long long blocks = (long long)pl.nrb * p.heads;
+  p.lpt = (a->causal || a->key_range) && pl.splits == 1 && pl.nrb > 1 && blocks <= 8 * 256;
   p.part = (float*)workspace;
   p.c = a->scale * AM_LOG2E;
   if (a->cap > 0.0f) {

@@ -76,6 +76,7 @@ struct AmParams {
   int Sq, Sk, Hkv, G, Dh, rows;  // rows = Sq * G
   int causal, nrb, heads, splits;  // row blocks, B * Hkv, parts of the keys
   int parts;                       // workgroups that may share a block's rows
+  int lpt;                         // row blocks of all heads by their length
   float c;                         // scale, to powers of two
   float ic, cl;                    // scale / cap; the cap, to powers of two
   float small, ct[5];              // q.k up to which, and coefficients with which, the cap is a polynomial
@@ -677,6 +678,36 @@ __device__ __forceinline__ void am_tiles(int lo, int hi, int bk, int splits, int
   t1 = min(b, t0 + per);
 }
 
+// The order in which an XCD's n blocks, from `first` on in the order of heads and, in each, of row blocks
+// from the last to the first, are started where masks make the last row blocks the longest: by row
+// block, those of all heads next to one another, and in rounds of one for each of its 32 CUs, the second
+// round from the shortest up, so that a CU's first two take about as long as any other's.
+__device__ __forceinline__ int am_by_weight(int slot, int first, int n, int nrb) {
+  if (slot >= 32 && slot < 64) slot = 32 + min(32, n - 32) - 1 - (slot - 32);
+  // positions c in a head's order: the first head lacks those below a, the last one those from z on
+  const int a = first % nrb, z = (first + n - 1) % nrb + 1, heads = (a + n + nrb - 1) / nrb;
+  const int lo = min(a, z), hi = max(a, z);
+  const int m1 = heads - (a > 0), m2 = a < z ? heads : heads - 2, m3 = heads - 1;
+  // of n blocks: lo positions of m1 heads each, hi - lo of m2, the rest of m3 (a head that lacks
+  // nothing counts as complete: a = 0, or z = nrb)
+  int c, k;
+  if (slot < lo * m1) {
+    c = slot / m1;
+    k = slot - c * m1;
+  } else if (slot < lo * m1 + (hi - lo) * m2) {
+    const int s = slot - lo * m1;
+    c = s / m2;
+    k = s - c * m2;
+    c += lo;
+  } else {
+    const int s = slot - lo * m1 - (hi - lo) * m2;
+    c = s / m3;
+    k = s - c * m3;
+    c += hi;
+  }
+  return (k + (c < a)) * nrb + c - a;
+}
+
 // ---------------------------------------------------------------------------
 // Many rows: 4 waves of 32 rows share tiles of 64 keys.  The scores of tile t + 1 are
 // issued ahead of tile t's softmax, so a wave's matrix and vector instructions overlap;
@@ -707,7 +738,8 @@ attn_masked_kernel(AmParams p) {
     }
     const int q8 = total >> 3, r8 = total & 7;
     const int x = at & 7, slot = at >> 3;
-    const int logical = x * q8 + (x < r8 ? x : r8) + slot;
+    const int first = x * q8 + (x < r8 ? x : r8), n = q8 + (x < r8);
+    const int logical = first + (p.lpt ? am_by_weight(slot, first, n, p.nrb) : slot);
     const int u = logical / p.splits;
     split = logical - u * p.splits;
     head = u / p.nrb;

@@ -264,6 +264,54 @@ def test_attention_documents_prefix_lengths(gpu, dt):
     attend(q, k, v, "a cache in use up to a length", q_pos=(n - 1)[:, None].to(torch.int32), causal=True, cap=50.0)
 
 
+@pytest.mark.parametrize("dt", HALF, ids=NAMES.get)
+def test_documents_that_share_row_blocks(gpu, dt):
+    """Workgroups of 128 rows that hold the end of one document and the start of others, long
+    and short, apart and not, with the keys in one part and in several."""
+    cases = [(1, 1, 64, [700, 650]), (2, 2, 64, [100, 1300, 90]), (2, 1, 96, [64, 64, 900, 10, 500]),
+             (4, 4, 64, [300, 280, 310, 290, 305]), (1, 1, 128, [1000, 1, 1, 1000]), (6, 3, 80, [257, 700, 3, 385]),
+             (2, 2, 256, [300, 400]), (8, 1, 64, [150, 200, 170])]
+    for H, Hkv, Dh, lengths in cases:
+        S = sum(lengths)
+        q, k, v = qkv(1, S, S, H, Hkv, Dh, dt, S)
+        r = ops.document_ranges(lengths, device="cpu")
+        attend(q, k, v, f"documents {lengths} x{H}/{Hkv}x{Dh} {dt}", key_range=r)
+        attend(q, k, v, f"documents {lengths}, causal, cap", key_range=r, causal=True, cap=20.0)
+
+
+@pytest.mark.parametrize("dt", HALF, ids=NAMES.get)
+@pytest.mark.parametrize("B,S,H,Hkv,Dh", [(1, 129, 3, 3, 64), (2, 700, 5, 5, 40), (3, 400, 7, 7, 64), (1, 1300, 9, 3, 64),
+                                          (5, 260, 4, 2, 128)])
+def test_row_blocks_of_every_head_in_any_order(gpu, B, S, H, Hkv, Dh, dt):
+    """Causal rows of several heads and batches: each row block is taken once."""
+    q, k, v = qkv(B, S, S, H, Hkv, Dh, dt, S)
+    attend(q, k, v, f"causal {B}x{S}x{H}/{Hkv}x{Dh} {dt}", causal=True)
+
+
+@pytest.mark.parametrize("Sq,Sk,H,Hkv,Dh", [(1, 20000, 1, 1, 64), (1, 5000, 2, 1, 128), (1, 4100, 3, 3, 256), (3, 16500, 2, 1, 80),
+                                            (50, 9000, 1, 1, 64), (70, 6000, 2, 2, 128), (40, 3000, 1, 1, 256)])
+def test_keys_in_many_parts(gpu, Sq, Sk, H, Hkv, Dh):
+    q, k, v = qkv(1, Sq, Sk, H, Hkv, Dh, torch.bfloat16, Sk)
+    name = f"{Sq}x{Sk}x{H}/{Hkv}x{Dh}"
+    attend(q, k, v, f"{name} in parts", causal=True)
+    few = torch.tensor([[Sk // 2, Sk // 2 + 40]], dtype=torch.int32).expand(Sq, 2).contiguous()
+    attend(q, k, v, f"{name}, keys in few of the parts", key_range=few)
+    few[::2] = torch.tensor([Sk - 1, 3], dtype=torch.int32)
+    attend(q, k, v, f"{name}, every other row without keys", key_range=few, cap=10.0)
+
+
+@pytest.mark.parametrize("dt", HALF, ids=NAMES.get)
+def test_caps_and_tables_of_any_size(gpu, dt):
+    for Sq, Sk in ((1, 90), (140, 200)):
+        q, k, v = qkv(1, Sq, Sk, 2, 1, 64, dt, Sk)
+        for cap, scale in ((1e6, None), (1e-3, None), (5.0, 1e-3), (3e4, 1.0), (0.5, 1.0), (1e5, 8.0)):
+            attend(q, k, v, f"cap {cap}, scale {scale}, {Sq}x{Sk}", cap=cap, scale=scale)
+        for R in (0, 63, 255, 256, 600):  # in LDS up to 1024 entries of a key head's heads
+            t = rnd((2, 2 * R + 1), R)
+            attend(q, k, v, f"table of R = {R}, {Sq}x{Sk}", rel_bias=t)
+            attend(q, k, v, f"table of R = {R} under a cap, {Sq}x{Sk}", rel_bias=t, cap=6.0, causal=True)
+
+
 def test_attention_of_nothing(gpu):
     announce("no keys, no queries, no batch, a mask of nothing")
     q, k, v = (t.cuda() for t in qkv(2, 3, 0, 4, 2, 64, torch.float16))
