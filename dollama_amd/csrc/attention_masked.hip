@@ -139,7 +139,7 @@ int dlm_attention_masked(const dlm_attention_masked_args* a, void* workspace, si
     double f = (double)a->cap * 1.4426950408889634 * ic;
     for (int i = 0; i < 5; ++i, f *= ic * ic) p.ct[i] = p.small > 0.0f ? (float)(AM_TANH[i] * f) : 0.0f;
   }
-  p.table_lds = a->rel_bias && (2LL * a->R + 1) * p.G <= AM_TABLE_MAX;
+  p.table_lds = a->rel_bias && (2LL * (a->R + AM_TABLE_MARGIN) + 1) * p.G <= AM_TABLE_MAX;
   return a->dtype == DLM_DTYPE_F16 ? am_run_f16(p, pl, a->cap > 0.0f, (hipStream_t)stream)
                                    : am_run_bf16(p, pl, a->cap > 0.0f, (hipStream_t)stream);
 }

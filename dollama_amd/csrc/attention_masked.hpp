@@ -103,7 +103,8 @@ __device__ __forceinline__ int am_wave_max(int v) {
 }
 
 enum { AM_PLAIN, AM_CAP, AM_SLOPE, AM_TABLE, AM_BOTH };  // scores: as they are, capped, with a bias, capped with a bias
-constexpr int AM_TABLE_MAX = 1024;                       // entries of the tables of one key head kept in LDS
+constexpr int AM_TABLE_MAX = 1024;   // entries of the tables of one key head kept in LDS,
+constexpr int AM_TABLE_MARGIN = 96;  // each with its ends repeated behind both: 64 keys and 32 places beyond
 constexpr float AM_LOG2E = 1.4426950408889634f;
 
 // tanh(t) / t in u = t^2 on [0, 1/4]: Chebyshev fit of degree 4, relative error 1.4e-8
@@ -219,10 +220,11 @@ template <int MODE>
 __device__ __forceinline__ bool am_tables(const AmParams& p, int hk, int tid, int threads, float* lds) {
   bool none = !p.table || p.table_lds;
   if (p.table && p.table_lds) {
-    const int n = (2 * p.R + 1) * p.G;
-    const float* tab = p.table + (long long)hk * n;
-    for (int i = tid; i < n; i += threads) {
-      const float x = am_log2(tab[i]);
+    const int n = 2 * p.R + 1, pitch = n + 2 * AM_TABLE_MARGIN;
+    const float* tab = p.table + (long long)hk * p.G * n;
+    for (int i = tid; i < pitch * p.G; i += threads) {
+      const int h = i / pitch, j = i - h * pitch - AM_TABLE_MARGIN;
+      const float x = am_log2(tab[h * n + max(0, min(n - 1, j))]);
       none &= x != -INFINITY;
       if (MODE == AM_TABLE) lds[i] = x;
     }
@@ -389,12 +391,11 @@ struct Core {
       if (k0 + BK - 1 - span.pmin <= -p.R || k0 - span.pmax >= p.R) {
         const float t = row.num(k0 - span.pmax >= p.R ? Row::RIGHT : Row::LEFT);
         f([&](float x, int, int) { return __builtin_fmaf(x, c, t); });
-      } else if (p.table_lds) {
-        const int d0 = k0 + 4 * g - row.get(Row::P), R = p.R;
-        const float DLM_LDS* tab = row.table + row.get(Row::SUB) * (2 * R + 1) + R;
-        f([&](float x, int kb, int e) {
-          return __builtin_fmaf(x, c, tab[max(-R, min(R, d0 + key_of(kb, e)))]);
-        });
+      } else if (p.table_lds && span.pmax - span.pmin < 32) {
+        // (places this near: no distance of the tile passes the margin behind the ends)
+        const int d0 = k0 + 4 * g - row.get(Row::P), pitch = 2 * (p.R + AM_TABLE_MARGIN) + 1;
+        const float DLM_LDS* tab = row.table + row.get(Row::SUB) * pitch + p.R + AM_TABLE_MARGIN + d0;
+        f([&](float x, int kb, int e) { return __builtin_fmaf(x, c, tab[key_of(kb, e)]); });
       } else {
         f([&](float x, int kb, int e) {
           return __builtin_fmaf(x, c, am_table(p, row, k0 + 4 * g + key_of(kb, e)));
@@ -439,6 +440,20 @@ struct Core {
 #pragma unroll
       for (int e = 0; e < 8; e += 2) sum[j & 1] = Hf::dot2(typename Hf::x2{pf[j][e], pf[j][e + 1]}, sum[j & 1]);
     return sum[0] + sum[1];
+  }
+
+  // The base from a first tile that is seen whole, ahead of its exponentials
+  __device__ __forceinline__ void begin(const AmParams& p, const f32x16 (&s)[KB]) {
+    float mt = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[kb][e]);
+    m = am_max_halves(mt * p.c);
+    if (m != -INFINITY) {
+      mref = m - Hf::shift;
+      lim = Hf::limit;
+    }
   }
 
   // A tile's weights against the row's base, given their sum.  No maximum is taken: the sum, which is
@@ -834,6 +849,7 @@ attn_masked_kernel(AmParams p) {
     if (t0 + 1 < t1) c.issue_k(smem + ((t0 ^ even ^ 1) & 1) * C::TILE);
     arrive();
     c.scores(smem + ((t0 ^ even) & 1) * C::TILE, sa, (int)C::here(lane));
+    if (MODE == AM_PLAIN && t0 == f0 && f0 < f1) c.begin(p, sa);
     // a tile that every row sees whole, its scores in sc; the next tile's go to sn (behind the
     // last tile they are made of whatever the buffer holds and not used)
     auto whole = [&](int t, int par, f32x16 (&sc)[2], f32x16 (&sn)[2]) {
