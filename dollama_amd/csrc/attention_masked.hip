@@ -11,11 +11,20 @@ static AmPlan am_plan(const dlm_attention_masked_args* a) {
   AmPlan pl;
   pl.few = rows <= 32;
   pl.nrb = (int)((rows + (pl.few ? 31 : 127)) / (pl.few ? 32 : 128));
-  // A workgroup for every CU, of 256 keys at least.  (us with 1 / 4 / 8 / 16 / 32 parts: one token over
-  // 4096 keys, 32/8 heads of 128: 38 / 19 / 14 / 12 / 12, over 65536: 485 / 132 / 72 / 51 / 50;
-  // 64 tokens over 30001: 420 / 117 / 67 / 45 / 53; 256 over 4096: 68 / 39 / 38 / 50 / 78.)
-  const long long blocks = heads * pl.nrb, most = a->Sk / 256;
-  pl.splits = most < 3 ? 1 : (int)std::min({(256 + blocks - 1) / blocks, most, 64LL});
+  // Parts of 256 keys at least, as many as cost least by a model in us: the keys' time in one part (a
+  // tile of 64 in 1.2, or 55 kB of few rows' K and V a us), the rounds of workgroups over 256 CUs, and the
+  // parts' way through memory.  (us with 1 / 4 / 8 / 16 / 32 parts, 32/8 heads of 128: one token over 4096 keys
+  // 38 / 19 / 14 / 12 / 12, over 65536 485 / 132 / 72 / 51 / 50; 64 tokens over 30001
+  // 420 / 117 / 67 / 45 / 53; 256 over 4096 68 / 39 / 38 / 50 / 78.)
+  const long long blocks = heads * pl.nrb;
+  const double whole = pl.few ? a->Sk * (double)a->Dh * 4 / 55e3 : a->Sk / 64 * 1.2;
+  const double part = (double)heads * rows * (a->Dh + 2) * 8 / 4e6;
+  double best = 0.0;
+  pl.splits = 1;
+  for (int s = 1; s <= std::min(64, std::max(1, a->Sk / 256)); ++s) {
+    const double t = whole * ((blocks * s + 255) / 256) / s + (s > 1 ? 3.0 + part * s : 0.0);
+    if (s == 1 || t < best) best = t, pl.splits = s;
+  }
   return pl;
 }
 
