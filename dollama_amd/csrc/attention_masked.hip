@@ -42,6 +42,7 @@ static int am_check(const char* fn, const dlm_attention_masked_args* a) {
   if (a->Hkv <= 0 || a->H % a->Hkv != 0) return bad("H must be a multiple of Hkv");
   if (!(a->scale > 0.0f && a->scale < INFINITY)) return bad("scale must be positive and finite");
   if (!(a->cap >= 0.0f && a->cap < INFINITY)) return bad("cap must be finite and not negative");
+  if (a->cap > 0.0f && a->scale / a->cap > 1e30f) return bad("cap is too small for the scale");
   if (a->slopes && a->rel_bias) return bad("one bias of distance, slopes or a table");
   if (a->rel_bias && (a->R < 0 || a->R > (1 << 24))) return bad("R must be 0 to 2^24");
   if (a->Sq > (1 << 28) || a->Sk > (1 << 28)) return bad("more than 2^28 queries or keys");
@@ -141,7 +142,7 @@ int dlm_attention_masked(const dlm_attention_masked_args* a, void* workspace, si
   if (a->cap > 0.0f) {
     p.ic = a->scale / a->cap;
     p.cl = a->cap * AM_LOG2E;
-    // tanh_ratio's coefficients for q.k itself; where their powers would leave fp32's range the
+    // AM_TANH's coefficients for q.k itself; where their powers would leave fp32's range the
     // polynomial is not used
     const double ic = (double)a->scale / a->cap;
     p.small = ic > 1e-4 && ic < 1e4 ? (float)(0.5 / ic) : -1.0f;

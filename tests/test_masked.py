@@ -79,7 +79,7 @@ def test_rotary_entries_refuse(lib):
         ("aligned", dict(pos=5 * A + 4, pos_type=1)), ("stride", dict(pos_ss=-1)), ("eps", dict(eps=-1.0)),
         ("eps", dict(eps=float("nan"))), ("eps", dict(eps=float("inf"))), ("aligned", dict(q=A + 1)),
         ("aligned", dict(k_out=4 * A + 1)), ("aligned", dict(q_gamma=7 * A + 1)), ("negative stride", dict(q_ss=-64)),
-        ("2^46", dict(q_sb=1 << 60)), ("2^31", dict(B=1 << 16, S=1 << 16)), ("65535", dict(H=65536)),
+        ("2^46", dict(q_sb=1 << 60)), ("2^30", dict(B=1 << 15, S=1 << 15)), ("65535", dict(H=65536)),
         ("q_out overlaps itself", dict(qo_sh=32)), ("k_out overlaps itself", dict(ko_ss=0)),
         # outputs on inputs, and on one another
         ("q_out overlaps q", dict(q_out=A + 2)), ("q_out overlaps k", dict(q_out=2 * A)), ("k_out overlaps q", dict(k_out=A)),
@@ -151,7 +151,7 @@ def test_attention_entry_refuses(lib):
         ("NULL", dict(q=None)), ("NULL", dict(k=None)), ("NULL", dict(v=None)), ("NULL", dict(o=None)), ("dtype", dict(dtype=2)),
         ("number of keys", dict(Sk=-1)), ("Dh", dict(Dh=60)), ("Dh", dict(Dh=264)), ("multiple of Hkv", dict(Hkv=3)),
         ("multiple of Hkv", dict(Hkv=0)), ("scale", dict(scale=0.0)), ("scale", dict(scale=float("inf"))),
-        ("scale", dict(scale=float("nan"))), ("cap", dict(cap=-1.0)), ("cap", dict(cap=float("nan"))),
+        ("scale", dict(scale=float("nan"))), ("cap", dict(cap=-1.0)), ("cap", dict(cap=float("nan"))), ("cap is too small", dict(cap=1e-38, scale=1.0)),
         ("one bias", dict(slopes=5 * A, rel_bias=6 * A)), ("R must", dict(rel_bias=6 * A, R=-1)),
         ("R must", dict(rel_bias=6 * A, R=(1 << 24) + 1)), ("2^28", dict(Sk=(1 << 28) + 1)), ("rows", dict(Sq=1 << 28)),
         ("rows", dict(B=70000)), ("rows", dict(B=30000, Sq=100000)), ("q: address", dict(q=A + 8)),
