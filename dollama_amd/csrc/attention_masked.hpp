@@ -16,9 +16,10 @@
 // its d.  K and V tiles come by DMA, 16-byte chunks of a row swizzled so that both kinds
 // of read touch every bank once.
 //
-// The softmax keeps a base m per row, moved only when a tile's maximum passes it by
-// 2^8: p = 2^((s - m) c + SH) stays far from fp16's ends (SH = 7: the row's largest p is
-// at least 2^7 times the smallest normal number's 2^14), and the accumulators are rescaled rarely.
+// The softmax keeps a base m per row and takes no maximum of a tile: p = 2^((s - m) c + SH), and the
+// base moves to a tile's maximum only where the tile's sum of p, needed anyway, passes a limit: that
+// of fp16's largest value (SH = 7 then leaves weights down to 2^-21 of the base's normal numbers),
+// 2^10 in bf16, so that the accumulators are rescaled rarely.
 #pragma once
 
 #include <cfloat>
@@ -49,7 +50,7 @@ template <> struct Half<f16> {
 template <> struct Half<__bf16> {
   typedef bf16x8 x8;
   static constexpr float shift = 0.0f;  // fp32's range: no p is too small
-  static constexpr float limit = 0x1p40f;
+  static constexpr float limit = 0x1p10f;  // (times the largest V it has to stay in fp32's range)
   static constexpr unsigned inf = 0x7f80;
   static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -358,8 +359,10 @@ struct Core {
                                               const f32x16 (&s)[KB], int k0, int g, F f) const {
     if constexpr (MODE == AM_PLAIN) f([](float x, int, int) { return x; });
     if constexpr (MODE == AM_CAP) {
-      // c tanh(t), t = x ic: where no t of the wave passes a half, x times a polynomial in x^2 (6
-      // operations against two of a quarter of their rate and 3)
+      // c tanh(t), t = x ic: x times a polynomial in x^2 where t is at most a half (6 operations against
+      // two of a quarter of their rate and 3), else by its exponential.  The form goes by x alone, so
+      // that no score depends on another row's or on masked keys; a wave with none past a half leaves
+      // the second form out.
       float top = 0.0f;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
@@ -368,7 +371,7 @@ struct Core {
       if (__builtin_amdgcn_ballot_w64(!(top <= p.small)) == 0)
         f([&](float x, int, int) { return capped_small(p, x); });
       else
-        f([&](float x, int, int) { return capped(p, x); });
+        f([&](float x, int, int) { return fabsf(x) <= p.small ? capped_small(p, x) : capped(p, x); });
     }
     if constexpr (MODE == AM_SLOPE) {
       // slopes are in powers of two.  Where every key of the tile lies on one side of every row, the

@@ -365,6 +365,40 @@ def test_what_masked_keys_hold_has_no_effect(gpu, Sq, Sk, H, Hkv, Dh, dt):
                 assert not torch.isfinite(got[0][sees[0]]).any()
 
 
+@pytest.mark.parametrize("mode", ["plain", "cap", "slopes", "table", "cap and table"])
+def test_masked_keys_change_no_bit(gpu, mode):
+    """The same bits whatever masked keys hold: zeros, large values, infinities, NaN; short rows
+    and long ones, an interval that ends inside a tile at both ends."""
+    H = 2
+    kw = {"plain": {}, "cap": dict(cap=30.0), "slopes": dict(slopes=torch.tensor([0.1, 0.01]).cuda()),
+          "table": dict(rel_bias=rnd((H, 41), 1).cuda()), "cap and table": dict(cap=30.0, rel_bias=rnd((H, 41), 1).cuda())}[mode]
+    for Sq, Sk in ((3, 200), (150, 300)):
+        q, k, v = (t.cuda() for t in qkv(1, Sq, Sk, H, H, 64, torch.float16, 27))
+        r = torch.tensor([[37, Sk - 45]], dtype=torch.int32, device="cuda").expand(Sq, 2).contiguous()
+        want = None
+        for x in (0.0, 60000.0, float("inf"), -float("inf"), float("nan")):
+            announce(f"masked keys of {x}, {mode}, {Sq}x{Sk}")
+            k2, v2 = k.clone(), v.clone()
+            for t in (k2, v2):
+                t[:, :37] = x
+                t[:, Sk - 45:] = x
+            got = ops.attention_masked(q, k2, v2, key_range=r, **kw)
+            want = got if want is None else want
+            assert torch.isfinite(got).all() and torch.equal(got, want), f"{mode}: {x}"
+
+
+@pytest.mark.parametrize("Sq", [1, 100])
+def test_values_at_the_end_of_bf16s_range(gpu, Sq):
+    """Sums of weights times values stay in fp32 while a row's scores grow from tile to tile."""
+    announce(f"values of 1e36 under growing scores, {Sq} rows")
+    Sk = 500
+    q, k, v = qkv(1, Sq, Sk, 1, 1, 64, torch.bfloat16, 28)
+    k = (k.float() * torch.linspace(0.2, 3, Sk)[None, :, None, None]).bfloat16()
+    small = M.attention(q, k, v)
+    got = ops.attention_masked(q.cuda(), k.cuda(), (v.float() * 2.0 ** 116).bfloat16().cuda()).double() * 2.0 ** -116
+    within(got, small["o"], att_tol(small, Sk, torch.bfloat16, v), "values of 2^116")
+
+
 @pytest.mark.parametrize("dt", HALF, ids=NAMES.get)
 @pytest.mark.parametrize("Sq,Sk", [(1, 400), (150, 150)])
 def test_tables_of_infinities_and_lowest_values(gpu, Sq, Sk, dt):
