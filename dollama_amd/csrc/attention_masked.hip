@@ -15,13 +15,14 @@ static AmPlan am_plan(const dlm_attention_masked_args* a) {
   // tile of 64 in 1.2, or 55 kB of few rows' K and V a us), the rounds of workgroups over 256 CUs, and the
   // parts' way through memory.  (us with 1 / 4 / 8 / 16 / 32 parts, 32/8 heads of 128: one token over 4096 keys
   // 38 / 19 / 14 / 12 / 12, over 65536 485 / 132 / 72 / 51 / 50; 64 tokens over 30001
-  // 420 / 117 / 67 / 45 / 53; 256 over 4096 68 / 39 / 38 / 50 / 78.)
+  // 420 / 117 / 67 / 45 / 53; 256 over 4096 68 / 39 / 38 / 50 / 78.)  Past eight rounds the last one's
+  // share is small, and the parts are large.
   const long long blocks = heads * pl.nrb;
   const double whole = pl.few ? a->Sk * (double)a->Dh * 4 / 55e3 : a->Sk / 64 * 1.2;
   const double part = (double)heads * rows * (a->Dh + 2) * 8 / 4e6;
   double best = 0.0;
   pl.splits = 1;
-  for (int s = 1; s <= std::min(64, std::max(1, a->Sk / 256)); ++s) {
+  for (int s = 1; s <= (blocks <= 8 * 256 ? std::min(64, std::max(1, a->Sk / 256)) : 1); ++s) {
     const double t = whole * ((blocks * s + 255) / 256) / s + (s > 1 ? 3.0 + part * s : 0.0);
     if (s == 1 || t < best) best = t, pl.splits = s;
   }
@@ -141,13 +142,10 @@ int dlm_attention_masked(const dlm_attention_masked_args* a, void* workspace, si
   p.c = a->scale * AM_LOG2E;
   if (a->cap > 0.0f) {
     p.ic = a->scale / a->cap;
-    p.cl = a->cap * AM_LOG2E;
-    // AM_TANH's coefficients for q.k itself; where their powers would leave fp32's range the
-    // polynomial is not used
+    p.cl = std::min(a->cap, FLT_MAX / 2) * AM_LOG2E;
     const double ic = (double)a->scale / a->cap;
-    p.small = ic > 1e-4 && ic < 1e4 ? (float)(0.5 / ic) : -1.0f;
-    double f = (double)a->cap * 1.4426950408889634 * ic;
-    for (int i = 0; i < 5; ++i, f *= ic * ic) p.ct[i] = p.small > 0.0f ? (float)(AM_TANH[i] * f) : 0.0f;
+    p.small = (float)std::min(0.5 / ic, (double)FLT_MAX);
+    for (int i = 0; i < 5; ++i) p.ct[i] = (float)(AM_TANH[i] * a->scale * 1.4426950408889634);
   }
   p.table_lds = a->rel_bias && (2LL * (a->R + AM_TABLE_MARGIN) + 1) * p.G <= AM_TABLE_MAX;
   return a->dtype == DLM_DTYPE_F16 ? am_run_f16(p, pl, a->cap > 0.0f, (hipStream_t)stream)

@@ -80,7 +80,7 @@ struct AmParams {
   int lpt;                         // row blocks of all heads by their length
   float c;                         // scale, to powers of two
   float ic, cl;                    // scale / cap; the cap, to powers of two
-  float small, ct[5];              // q.k up to which, and coefficients with which, the cap is a polynomial
+  float small, ct[5];              // q.k up to which the cap is a polynomial; its coefficients times c
   int table_lds;                   // the table's rows of a key head fit LDS
   float* part;                     // [splits][heads][rows][Dh], then [splits][heads][rows][2]
 };
@@ -112,17 +112,19 @@ constexpr float AM_LOG2E = 1.4426950408889634f;
 constexpr double AM_TANH[5] = {0.9999999870693153, -0.3333307189419686, 0.13324828997687793, -0.052989241174895264,
                                0.017141319047070502};
 __device__ __forceinline__ float capped_small(const AmParams& p, float x) {
-  const float u = x * x;
+  const float t = x * p.ic, u = t * t;
   float r = __builtin_fmaf(p.ct[4], u, p.ct[3]);
   r = __builtin_fmaf(r, u, p.ct[2]);
   r = __builtin_fmaf(r, u, p.ct[1]);
   r = __builtin_fmaf(r, u, p.ct[0]);
   return x * r;
 }
-// tanh(t) = 1 - 2 / (1 + e^2t)
+// ... else tanh(t) = 1 - 2 / (1 + e^2t), whose error, of 1's last bits, would outgrow a small score.
+// The form goes by x alone, so that no score depends on another row's or on masked keys.
 __device__ __forceinline__ float capped(const AmParams& p, float x) {
   const float e = __builtin_amdgcn_exp2f(x * (p.ic * (2.0f * AM_LOG2E)));
-  return __builtin_fmaf(-2.0f * p.cl, __builtin_amdgcn_rcpf(1.0f + e), p.cl);
+  const float far = __builtin_fmaf(-2.0f * p.cl, __builtin_amdgcn_rcpf(1.0f + e), p.cl);
+  return fabsf(x) <= p.small ? capped_small(p, x) : far;
 }
 
 // A bias to powers of two; the lowest values stay finite, -infinity stays what it is.
@@ -359,10 +361,7 @@ struct Core {
                                               const f32x16 (&s)[KB], int k0, int g, F f) const {
     if constexpr (MODE == AM_PLAIN) f([](float x, int, int) { return x; });
     if constexpr (MODE == AM_CAP) {
-      // c tanh(t), t = x ic: x times a polynomial in x^2 where t is at most a half (6 operations against
-      // two of a quarter of their rate and 3), else by its exponential.  The form goes by x alone, so
-      // that no score depends on another row's or on masked keys; a wave with none past a half leaves
-      // the second form out.
+      // a wave with no score past half the cap leaves the second form out
       float top = 0.0f;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
@@ -371,7 +370,7 @@ struct Core {
       if (__builtin_amdgcn_ballot_w64(!(top <= p.small)) == 0)
         f([&](float x, int, int) { return capped_small(p, x); });
       else
-        f([&](float x, int, int) { return fabsf(x) <= p.small ? capped_small(p, x) : capped(p, x); });
+        f([&](float x, int, int) { return capped(p, x); });
     }
     if constexpr (MODE == AM_SLOPE) {
       // slopes are in powers of two.  Where every key of the tile lies on one side of every row, the
@@ -394,7 +393,7 @@ struct Core {
       if (k0 + BK - 1 - span.pmin <= -p.R || k0 - span.pmax >= p.R) {
         const float t = row.num(k0 - span.pmax >= p.R ? Row::RIGHT : Row::LEFT);
         f([&](float x, int, int) { return __builtin_fmaf(x, c, t); });
-      } else if (p.table_lds && span.pmax - span.pmin < 32) {
+      } else if (p.table_lds && (unsigned)span.pmax - (unsigned)span.pmin < 32) {
         // (places this near: no distance of the tile passes the margin behind the ends)
         const int d0 = k0 + 4 * g - row.get(Row::P), pitch = 2 * (p.R + AM_TABLE_MARGIN) + 1;
         const float DLM_LDS* tab = row.table + row.get(Row::SUB) * pitch + p.R + AM_TABLE_MARGIN + d0;

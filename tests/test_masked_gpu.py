@@ -399,6 +399,33 @@ def test_values_at_the_end_of_bf16s_range(gpu, Sq):
     within(got, small["o"], att_tol(small, Sk, torch.bfloat16, v), "values of 2^116")
 
 
+@pytest.mark.parametrize("cap", [0.5, 1e3, 1e4, 1e6, 3e38])
+@pytest.mark.parametrize("bias", [False, True], ids=["cap", "cap and slopes"])
+def test_small_scores_under_large_caps(gpu, cap, bias):
+    """A capped score's error goes by the score, not by the cap (below a half of it, where the cap is a
+    polynomial: 8 units of the score, less than the product's own error, so twice that); above,
+    units of the cap."""
+    for Sq, Sk in ((2, 300), (150, 200)):
+        announce(f"cap {cap}, {Sq}x{Sk}, slopes {bias}")
+        q, k, v = qkv(1, Sq, Sk, 2, 2, 64, torch.float16, 29)
+        kw = dict(slopes=torch.tensor([0.05, 0.01])) if bias else {}
+        ref = M.attention(q, k, v, cap=cap, **kw)
+        ref["err"] = 2 * M.attention(q, k, v, **kw)["err"] + (16 * cap if cap < 100 else 0.0)
+        dev = {n: t.cuda() for n, t in kw.items()}
+        got = ops.attention_masked(q.cuda(), k.cuda(), v.cuda(), cap=cap, **dev)
+        within(got, ref["o"], att_tol(ref, Sk, torch.float16, v), f"cap {cap}")
+
+
+@pytest.mark.parametrize("mode", ["slopes", "table"])
+def test_places_at_both_ends(gpu, mode):
+    """Places of +-2^30 among the rows of one wave."""
+    kw = dict(slopes=torch.tensor([1e-9])) if mode == "slopes" else dict(rel_bias=rnd((1, 11), 3))
+    for Sq in (4, 140):
+        q, k, v = qkv(1, Sq, 90, 1, 1, 64, torch.float16, 30)
+        places = torch.tensor([-(1 << 30), 1 << 30, 0, 89], dtype=torch.int32).repeat(35)[:Sq].contiguous()
+        attend(q, k, v, f"places at both ends, {Sq} rows, {mode}", q_pos=places, **kw)
+
+
 @pytest.mark.parametrize("dt", HALF, ids=NAMES.get)
 @pytest.mark.parametrize("Sq,Sk", [(1, 400), (150, 150)])
 def test_tables_of_infinities_and_lowest_values(gpu, Sq, Sk, dt):
