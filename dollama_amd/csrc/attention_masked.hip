@@ -15,15 +15,18 @@ static AmPlan am_plan(const dlm_attention_masked_args* a) {
   // tile of 64 in 1.2, or 55 kB of few rows' K and V a us), the rounds of workgroups over 256 CUs, and the
   // parts' way through memory.  (us with 1 / 4 / 8 / 16 / 32 parts, 32/8 heads of 128: one token over 4096 keys
   // 38 / 19 / 14 / 12 / 12, over 65536 485 / 132 / 72 / 51 / 50; 64 tokens over 30001
-  // 420 / 117 / 67 / 45 / 53; 256 over 4096 68 / 39 / 38 / 50 / 78.)  Past eight rounds the last one's
-  // share is small, and the parts are large.
+  // 420 / 117 / 67 / 45 / 53; 256 over 4096 68 / 39 / 38 / 50 / 78.)  Few rows, whose
+  // workgroups have a CU to themselves, stay whole past eight rounds, where the last one's share is small;
+  // many rows where there is a workgroup for every CU: a CU runs two or three of them at once, masks leave
+  // less than the model's time, and the parts are large (documents of 426 to 1439 in 8192 tokens x10x64, 640
+  // workgroups: 50 us whole, 102 in two parts, 56 of them to join).
   const long long blocks = heads * pl.nrb;
   const double whole = pl.few ? a->Sk * (double)a->Dh * 4 / 55e3 : a->Sk / 64 * 1.2;
   const double part = (double)heads * rows * (a->Dh + 2) * 8 / 4e6;
   double best = 0.0;
   pl.splits = 1;
-  for (int s = 1; s <= (blocks <= 8 * 256 ? std::min(64, std::max(1, a->Sk / 256)) : 1); ++s) {
-    const double t = whole * ((blocks * s + 255) / 256) / s + (s > 1 ? 3.0 + part * s : 0.0);
+  for (int s = 1; s <= (blocks <= (pl.few ? 8 * 256 : 255) ? std::min(64, std::max(1, a->Sk / 256)) : 1); ++s) {
+    const double t = whole * (double)((blocks * s + 255) / 256) / s + (s > 1 ? 3.0 + part * s : 0.0);
     if (s == 1 || t < best) best = t, pl.splits = s;
   }
   return pl;

@@ -174,6 +174,17 @@ def test_attention_entry_refuses(lib):
     assert lib.dlm_attention_masked_workspace_bytes(ctypes.byref(attention_args())) == 0
 
 
+@pytest.mark.parametrize("B,Sq,Sk,H,Hkv,Dh,parts", [
+    (1, 8192, 8192, 10, 10, 64, False),  # 640 workgroups without parts
+    (2, 4096, 4096, 10, 10, 64, False), (1, 4096, 4096, 32, 8, 128, False), (4, 512, 512, 64, 64, 64, False),
+    (2, 2051, 2051, 12, 12, 80, False), (1 << 10, 1, 4096, 32, 8, 128, False), (1, 1, 511, 32, 8, 128, False),
+    (1, 1, 4096, 32, 8, 128, True), (1, 64, 30001, 32, 32, 128, True), (40, 1, 32768, 32, 8, 128, True),
+])
+def test_keys_are_split_where_workgroups_are_few(lib, B, Sq, Sk, H, Hkv, Dh, parts):
+    a = attention_args(B=B, Sq=Sq, Sk=Sk, H=H, Hkv=Hkv, Dh=Dh)
+    assert (lib.dlm_attention_masked_workspace_bytes(ctypes.byref(a)) > 0) == parts
+
+
 def test_wrappers_refuse_tensors_that_are_not_on_the_gpu():
     q = torch.zeros(1, 2, 2, 64, dtype=torch.float16)
     for call in (lambda: ops.attention_masked(q, q, q), lambda: ops.qk_norm_rotary(q),
