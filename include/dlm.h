@@ -580,8 +580,8 @@ int dlm_linear_q8_f32out(const void* X, int ldx, const float* sx, const void* W,
  * dlm_rotary_axes (norm = 0, gammas NULL) is the rotation alone.
  *
  * dtype is fp16 or bf16 (DLM_DTYPE_*) for every operand but positions and
- * frequencies.  Dh is even and at most 256.  Any alignment of an element is
- * taken; 16-byte aligned heads are fastest.  An output may be its own input
+ * frequencies.  Dh is even and at most 256, tokens (B x S) fewer than 2^26.  Any
+ * alignment of an element is taken; 16-byte aligned heads are fastest.  An output may be its own input
  * (same pointer and strides) and overlap nothing else; slices of one tensor do
  * not overlap.  Uses no workspace.  No counterpart in the reference
  * (src/infer/unet.cu:677-802: no positions, no norm of queries and keys). */
@@ -626,8 +626,9 @@ int dlm_qk_norm_rotary(const dlm_rotary_args* args, void* stream);
  * row's stride is at least Dh and below 2^23.  key_range is int32 [.., Sq, 2] with
  * batch stride kr_sb (elements, 0: one for every batch), 8-byte aligned; q_pos
  * int32 [.., Sq] with batch stride qp_sb; slopes fp32 [H]; rel_bias fp32 [H][2R + 1].
- * scale > 0 and cap >= 0 are finite.  dtype is that of q, k, v and o; scores, softmax and sums are
- * fp32, the probabilities are rounded to dtype for the product with v.
+ * scale > 0 and cap >= 0 are finite, scale / cap at most 1e30.  dtype is that of q, k, v and o; scores,
+ * softmax and sums are fp32, the probabilities are rounded to dtype for the product with v.  Sk
+ * and Sq are at most 2^28, B x Hkv at most 65535.
  * Few queries against many keys are split over the keys; the parts meet in the
  * workspace, of dlm_attention_masked_workspace_bytes(args) bytes (may be 0; it
  * goes by sizes alone), 16-byte aligned, which no other call may use until this one's work is

@@ -79,7 +79,7 @@ def test_rotary_entries_refuse(lib):
         ("aligned", dict(pos=5 * A + 4, pos_type=1)), ("stride", dict(pos_ss=-1)), ("eps", dict(eps=-1.0)),
         ("eps", dict(eps=float("nan"))), ("eps", dict(eps=float("inf"))), ("aligned", dict(q=A + 1)),
         ("aligned", dict(k_out=4 * A + 1)), ("aligned", dict(q_gamma=7 * A + 1)), ("negative stride", dict(q_ss=-64)),
-        ("2^46", dict(q_sb=1 << 60)), ("2^30", dict(B=1 << 15, S=1 << 15)), ("65535", dict(H=65536)),
+        ("2^46", dict(q_sb=1 << 60)), ("2^26", dict(B=1 << 13, S=1 << 13)), ("65535", dict(H=65536)),
         ("q_out overlaps itself", dict(qo_sh=32)), ("k_out overlaps itself", dict(ko_ss=0)),
         # outputs on inputs, and on one another
         ("q_out overlaps q", dict(q_out=A + 2)), ("q_out overlaps k", dict(q_out=2 * A)), ("k_out overlaps q", dict(k_out=A)),
