@@ -631,6 +631,24 @@ def test_calls_on_another_stream_and_repeated(gpu):
         assert torch.equal(g, want)
 
 
+def test_two_calls_at_once(gpu):
+    """Calls with parts of the keys on two streams, each with a workspace of its own."""
+    announce("two streams, parts of 20000 keys")
+    q, k, v = (t.cuda() for t in qkv(1, 4, 20000, 32, 8, 128, torch.bfloat16, 31))
+    other = q * 0.5
+    want = [ops.attention_masked(x, k, v) for x in (q, other)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, x in enumerate((q, other)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.attention_masked(x, k, v))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
 def test_wrappers_refuse_on_the_gpu(gpu):
     announce("refused calls")
     q, k, v = (t.cuda() for t in qkv(2, 4, 9, 4, 2, 64, torch.float16))
