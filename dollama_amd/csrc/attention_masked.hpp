@@ -430,7 +430,8 @@ struct Core {
   __device__ __forceinline__ T weight(const AmParams& p, float s) const {
     return (T)__builtin_amdgcn_exp2f(MODE == AM_PLAIN ? __builtin_fmaf(s, p.c, -mref) : s - mref);
   }
-  // ... of a tile, and this lane's sum of them
+  // ... of a tile, and this lane's sum of them, pairs added in the order of `look_ahead`: which of the
+  // two makes a row's sum goes by the other rows of its wave, and must not show in a bit of it
   __device__ __forceinline__ float weights(const AmParams& p, const f32x16 (&s)[KB], x8 (&pf)[2 * KB]) const {
     float sum[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -438,9 +439,10 @@ struct Core {
 #pragma unroll
       for (int e = 0; e < 16; ++e) pf[2 * kb + (e >> 3)][e & 7] = weight(p, s[kb][e]);
 #pragma unroll
-    for (int j = 0; j < 2 * KB; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) sum[j & 1] = Hf::dot2(typename Hf::x2{pf[j][e], pf[j][e + 1]}, sum[j & 1]);
+    for (int i = 0; i < 8 * KB; ++i) {
+      const int j = i >> 2, e = 2 * (i & 3);
+      sum[i & 1] = Hf::dot2(typename Hf::x2{pf[j][e], pf[j][e + 1]}, sum[i & 1]);
+    }
     return sum[0] + sum[1];
   }
 
