@@ -8,7 +8,7 @@ from test_masked_gpu import HALF, NAMES, announce, qkv, rnd
 
 pytestmark = pytest.mark.gpu
 
-MODES = ["plain", "table"]
+MODES = ["plain", "cap", "table", "cap and table"]
 
 
 def scores_kw(mode, H):
@@ -28,7 +28,7 @@ ROWS = [(24, 640, 40, 64), (150, 640, 40, 64), (150, 640, 40, 128), (700, 640, 4
 @pytest.mark.parametrize("mode", MODES)
 def test_other_rows_change_no_bit(gpu, mode, dt):
     """Every other row of a wave has small scores, or large ones that grow from tile to tile, so that its
-    base moves: the rows between keep their bits."""
+    base moves and a capped score takes its second form: the rows between keep their bits."""
     for Sq, Sk, H, Dh in ROWS:
         announce(f"scores of neighbours, {mode}, {Sq}x{Sk}x{H}x{Dh} {dt}")
         q, k, v = qkv(1, Sq, Sk, H, H, Dh, dt, 3)
