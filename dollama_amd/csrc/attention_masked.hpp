@@ -373,9 +373,11 @@ struct Core {
         f([&](float x, int, int) { return capped(p, x); });
     }
     if constexpr (MODE == AM_SLOPE) {
-      // slopes are in powers of two.  Where every key of the tile lies on one side of every row, the
-      // distance is linear in the key
-      const float c = p.c, f0 = (float)(k0 + 4 * g - row.get(Row::P)), slope = row.num(Row::SLOPE);
+      // slopes are in powers of two.  A row that has every key of the tile on one side takes the bias as
+      // linear in the key, with an operation less; so does a row among others that have not, since the two
+      // are rounded apart
+      const int first = k0 - row.get(Row::P);
+      const float c = p.c, f0 = (float)(first + 4 * g), slope = row.num(Row::SLOPE);
       const bool before = k0 + BK - 1 <= span.pmin;
       if (before || k0 >= span.pmax) {
         const float d = before ? slope : -slope;
@@ -383,8 +385,11 @@ struct Core {
           return __builtin_fmaf(x, c, __builtin_fmaf(d, (float)key_of(kb, e), d * f0));
         });
       } else {
+        const bool side = first + BK - 1 <= 0 || first >= 0;
+        const float d = first < 0 ? slope : -slope;
         f([&](float x, int kb, int e) {
-          return __builtin_fmaf(-slope, fabsf(f0 + (float)key_of(kb, e)), x * c);
+          const float linear = __builtin_fmaf(x, c, __builtin_fmaf(d, (float)key_of(kb, e), d * f0));
+          return side ? linear : __builtin_fmaf(-slope, fabsf(f0 + (float)key_of(kb, e)), x * c);
         });
       }
     }

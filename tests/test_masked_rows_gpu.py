@@ -8,7 +8,7 @@ from test_masked_gpu import HALF, NAMES, announce, qkv, rnd
 
 pytestmark = pytest.mark.gpu
 
-MODES = ["plain", "cap", "table", "cap and table"]
+MODES = ["plain", "cap", "slopes", "table", "cap and slopes", "cap and table"]
 
 
 def scores_kw(mode, H):
