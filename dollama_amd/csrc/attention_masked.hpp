@@ -634,13 +634,21 @@ struct Core {
       }
     }
     if constexpr (MODE >= AM_TABLE) {
-      if (p.table && !guard) {  // an entry of -infinity masks its distance
+      if (p.table) {  // an entry of -infinity masks its distance
         float low = s[0][0];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) low = fminf(low, s[kb][e]);
-        guard = __builtin_amdgcn_ballot_w64(low == -INFINITY) != 0;
+          for (int e = 0; e < 16; ++e) low = __builtin_elementwise_minimum(low, s[kb][e]);
+        guard |= __builtin_amdgcn_ballot_w64(!(low > -INFINITY)) != 0;
+        // ... whatever its key holds: added to infinity or NaN it gave NaN
+        if (__builtin_amdgcn_ballot_w64(low != low) != 0) {
+#pragma unroll
+          for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (s[kb][e] != s[kb][e] && am_table(p, row, k0 + 4 * g + key_of(kb, e)) == -INFINITY) s[kb][e] = -INFINITY;
+        }
       }
     }
     x8 pf[2 * KB];

@@ -1,10 +1,13 @@
 """Masked attention's rows beside one another: no row's result shows what another row's query, keys or
-place hold (GPU)."""
+place hold, nor what keys hold that a table hides from it (GPU)."""
+import math
+
 import pytest
 import torch
 
 from dollama_amd import ops
-from test_masked_gpu import HALF, NAMES, announce, qkv, rnd
+from oracle import masked_ref as M
+from test_masked_gpu import HALF, NAMES, announce, att_tol, qkv, rnd, within
 
 pytestmark = pytest.mark.gpu
 
@@ -76,3 +79,36 @@ def test_places_of_other_rows_change_no_bit(gpu, mode, dt):
             got = ops.attention_masked(q, k, v, q_pos=at, **scores_kw(mode, H))[:, ::2]
             want = got if want is None else want
             assert torch.equal(got, want), f"{mode}, neighbours {far} away: {int((got != want).sum())} values differ"
+
+
+@pytest.mark.parametrize("dt", HALF, ids=NAMES.get)
+@pytest.mark.parametrize("R", [20, 40, 400])  # R = 400: more than LDS holds of both heads
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_keys_that_a_table_hides_may_hold_anything(gpu, cap, R, dt):
+    """Entries of -infinity among others, NaN and infinities in keys and values at their distance: rows that
+    have them hidden keep their bits, and rows that see them show them where the definition does."""
+    t = rnd((2, 2 * R + 1), 6)
+    t[0, 1::4] = -math.inf
+    t[1, R + 3:] = -math.inf  # no key three or more behind the query
+    t[1, :R // 2] = -math.inf
+    for Sq, Sk in ((1, 90), (5, 700), (150, 300), (200, 130)):
+        q, k, v = qkv(1, Sq, Sk, 2, 2, 64, dt, 7)
+        clean = ops.attention_masked(q.cuda(), k.cuda(), v.cuda(), cap=cap, rel_bias=t.cuda()).cpu()
+        ref = M.attention(q, k, v, cap=cap, rel_bias=t)
+        within(clean, ref["o"], att_tol(ref, Sk, dt, v), f"{Sq}x{Sk}, R = {R}, cap {cap}")
+        at = [Sk - 1, Sk - 2, Sk // 2, 3]
+        d = torch.tensor(at)[None] - torch.arange(Sk - Sq, Sk)[:, None]
+        sees = (t[:, d.clamp(-R, R) + R] != -math.inf).any(-1).T  # [query, head]
+        for x in (math.nan, math.inf, -math.inf):
+            announce(f"hidden keys and values of {x}, {Sq}x{Sk}, R = {R}, cap {cap}, {dt}")
+            k2, v2, v3 = k.clone(), v.clone(), v.clone()
+            k2[:, at] = v2[:, at] = x
+            v3[:, at, :, 1] = x
+            both = ops.attention_masked(q.cuda(), k2.cuda(), v2.cuda(), cap=cap, rel_bias=t.cuda()).cpu()
+            assert torch.equal(both[0][~sees], clean[0][~sees]), f"{int((both != clean)[0][~sees].sum())} values differ"
+            one = ops.attention_masked(q.cuda(), k.cuda(), v3.cuda(), cap=cap, rel_bias=t.cuda()).cpu()
+            assert torch.equal(one[0][~sees], clean[0][~sees])
+            shown = one[0][sees][..., 1]
+            assert (shown.isnan() if x != x else shown == x).all()
+            rest = [e for e in range(64) if e != 1]
+            assert torch.equal(one[..., rest], clean[..., rest])
