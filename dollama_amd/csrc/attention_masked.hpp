@@ -19,7 +19,7 @@
 // The softmax keeps a base m per row and takes no maximum of a tile: p = 2^((s - m) c + SH), and the
 // base moves to a tile's maximum only where the tile's sum of p, needed anyway, passes a limit: that
 // of fp16's largest value (SH = 7 then leaves weights down to 2^-21 of the base's normal numbers),
-// 2^10 in bf16, so that the accumulators are rescaled rarely.
+// 2^10 times the base's weight in bf16 (SH = -34), so that the accumulators are rescaled rarely.
 #pragma once
 
 #include <cfloat>
@@ -49,8 +49,10 @@ template <> struct Half<f16> {
 };
 template <> struct Half<__bf16> {
   typedef bf16x8 x8;
-  static constexpr float shift = 0.0f;  // fp32's range: no p is too small
-  static constexpr float limit = 0x1p10f;  // (times the largest V it has to stay in fp32's range)
+  // The sums of p V stay in fp32's range for every finite V: a lane's keys of a tile, 16 or 32, sum to
+  // 2^-24 at most and 2^28 keys to 1; weights down to 2^-92 of the base are normal numbers
+  static constexpr float shift = -34.0f;
+  static constexpr float limit = 0x1p-24f;
   static constexpr unsigned inf = 0x7f80;
   static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);

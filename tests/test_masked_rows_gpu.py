@@ -112,3 +112,22 @@ def test_keys_that_a_table_hides_may_hold_anything(gpu, cap, R, dt):
             assert (shown.isnan() if x != x else shown == x).all()
             rest = [e for e in range(64) if e != 1]
             assert torch.equal(one[..., rest], clean[..., rest])
+
+
+@pytest.mark.parametrize("power", [126, 100, 0, -64])
+@pytest.mark.parametrize("scores", ["equal", "growing", "falling"])
+def test_bf16_values_of_any_size(gpu, scores, power):
+    """Finite values have finite results up to the type's largest, whatever the weights' sum: 500 keys in
+    one part, thousands in several, few rows and many."""
+    for Sq, Sk, H in ((1, 500, 1), (2, 6000, 1), (100, 700, 1), (100, 5000, 1), (100, 500, 260)):
+        announce(f"values of 2^{power}, {scores} scores, {Sq}x{Sk}x{H}")
+        q, k, v = qkv(1, Sq, Sk, H, H, 64, torch.bfloat16, 8)
+        k = k.float() * {"equal": torch.zeros(Sk), "growing": torch.linspace(0.2, 3, Sk),
+                         "falling": torch.linspace(3, 0.2, Sk)}[scores][None, :, None, None]
+        k = k.bfloat16()
+        v = v.abs().clamp(0.5, 1.9) if scores == "equal" else v.clamp(-1.9, 1.9)
+        ref = M.attention(q, k, v)
+        big = (v.double() * 2.0 ** power).bfloat16()
+        assert torch.isfinite(big).all() and torch.equal(big.double() * 2.0 ** -power, v.double())
+        got = ops.attention_masked(q.cuda(), k.cuda(), big.cuda()).double() * 2.0 ** -power
+        within(got, ref["o"], att_tol(ref, Sk, torch.bfloat16, v), f"values of 2^{power}")
