@@ -134,6 +134,12 @@ __device__ __forceinline__ float am_log2(float b) {
   return __builtin_isinf(b) ? b : fmaxf(-FLT_MAX, fminf(FLT_MAX, b * AM_LOG2E));
 }
 
+// A slope to powers of two, held where its product with any distance (below 2^31) is finite
+__device__ __forceinline__ float am_slope(float x) {
+  const float y = x * AM_LOG2E;
+  return y != y ? y : fmaxf(-0x1p96f, fminf(0x1p96f, y));
+}
+
 // What a wave's rows see: keys from the first to behind the last that one of them sees, the
 // keys that all of them see, and their places.
 struct KeySpan {
@@ -210,7 +216,7 @@ __device__ __forceinline__ void am_keep(const AmParams& p, const RowInit& w, Key
     row.set(Row::P, w.p);
     row.set(Row::HEAD, w.h);
     row.set(Row::SUB, w.h % p.G);
-    if (p.slopes) row.set(Row::SLOPE, __float_as_int(p.slopes[w.h] * AM_LOG2E));
+    if (p.slopes) row.set(Row::SLOPE, __float_as_int(am_slope(p.slopes[w.h])));
     if (p.table) {
       const float* tab = p.table + (long long)w.h * (2 * p.R + 1);
       row.set(Row::LEFT, __float_as_int(am_log2(tab[0])));

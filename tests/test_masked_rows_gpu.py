@@ -131,3 +131,25 @@ def test_bf16_values_of_any_size(gpu, scores, power):
         assert torch.isfinite(big).all() and torch.equal(big.double() * 2.0 ** -power, v.double())
         got = ops.attention_masked(q.cuda(), k.cuda(), big.cuda()).double() * 2.0 ** -power
         within(got, ref["o"], att_tol(ref, Sk, torch.bfloat16, v), f"values of 2^{power}")
+
+
+@pytest.mark.parametrize("slope", [3e38, math.inf, -math.inf, 1e-45])
+@pytest.mark.parametrize("mode", ["slopes", "cap and slopes"])
+def test_slopes_of_any_size(gpu, slope, mode):
+    """A slope past every score leaves a query the nearest of its keys alone (the farthest where it is
+    negative); the smallest ones leave the plain result."""
+    for Sq, Sk in ((1, 130), (150, 200)):
+        announce(f"{mode} of {slope}, {Sq}x{Sk}")
+        q, k, v = qkv(1, Sq, Sk, 1, 1, 64, torch.bfloat16, 9)
+        p = torch.arange(Sq, dtype=torch.int32) + Sk - Sq
+        kw = {"cap": 30.0} if "cap" in mode else {}
+        dev = dict(slopes=torch.tensor([slope], device="cuda"), q_pos=p.cuda(), causal=True, **kw)
+        got = ops.attention_masked(q.cuda(), k.cuda(), v.cuda(), **dev).cpu()
+        if abs(slope) < 1:
+            ref = M.attention(q, k, v, causal=True, **kw)
+            within(got, ref["o"], att_tol(ref, Sk, torch.bfloat16, v), "a tiny slope")
+            continue
+        if slope > 0:
+            assert torch.equal(got[0, :, 0], v[0, p.long(), 0])
+        else:
+            assert torch.equal(got[0, :, 0], v[0, :1, 0].expand(Sq, 64))
