@@ -374,8 +374,9 @@ static int rotary_check(const char* fn, const dlm_rotary_args* a, int& P) {
   if (!a->norm && (a->q_gamma || a->k_gamma)) return bad("gamma without the norm");
   for (const void* p : {a->q, (const void*)a->q_out, a->k, (const void*)a->k_out, a->q_gamma, a->k_gamma})
     if ((uintptr_t)p % 2 != 0) return bad("operands must be aligned to their elements");
-  // (a grid's 2^32 threads, 64 a token where heads are wide or unaligned)
-  if ((long long)a->B * a->S >= (1LL << 26)) return bad("2^26 tokens or more");
+  // (a grid has fewer than 2^32 threads: 64 a token where heads are wide or unaligned, in whole blocks of
+  // four tokens)
+  if ((long long)a->B * a->S > (1LL << 26) - 4) return bad("more than 2^26 - 4 tokens");
   if ((long long)a->H + (a->k ? a->Hkv : 0) > 65535) return bad("more than 65535 heads");
   const View v[4] = {{"q", a->q, a->q_sb, a->q_ss, a->q_sh, a->H},
                      {"k", a->k, a->k_sb, a->k_ss, a->k_sh, a->Hkv},

@@ -580,7 +580,7 @@ int dlm_linear_q8_f32out(const void* X, int ldx, const float* sx, const void* W,
  * dlm_rotary_axes (norm = 0, gammas NULL) is the rotation alone.
  *
  * dtype is fp16 or bf16 (DLM_DTYPE_*) for every operand but positions and
- * frequencies.  Dh is even and at most 256, tokens (B x S) fewer than 2^26.  Any
+ * frequencies.  Dh is even and at most 256, tokens (B x S) at most 2^26 - 4.  Any
  * alignment of an element is taken; 16-byte aligned heads are fastest.  An output may be its own input
  * (same pointer and strides) and overlap nothing else; slices of one tensor do
  * not overlap.  Uses no workspace.  No counterpart in the reference
