@@ -11,6 +11,7 @@
 // which only the fraction matters (in fp32 a position of 10^6 would leave errors of
 // 0.06 rad).  v_sin_f32 and v_cos_f32 take turns.
 #include "common.hpp"
+#include "views.hpp"
 
 namespace dlm {
 
@@ -298,57 +299,6 @@ static int rotary_vector(const dlm_rotary_args* a, int P) {
   return 1;
 }
 
-// ---------------------------------------------------------------------------
-// What a call writes against what it reads: [B, S, H, Dh] views with strides
-// ---------------------------------------------------------------------------
-struct View {
-  const char* name;
-  const void* p;
-  long long sb, ss, sh;
-  int H;
-};
-
-// Whether two views of B x S x H x Dh elements share one.  Of views with the same
-// strides, each longer than what lies inside it (slices of one tensor), the places
-// are compared; any others count by their whole extents.
-static bool views_overlap(const View& a, const View& b, int B, int S, int Dh, int elem) {
-  if (!a.p || !b.p) return false;
-  auto extent = [&](const View& v) {
-    return ((B - 1) * v.sb + (S - 1) * v.ss + (v.H - 1) * v.sh + Dh) * (long long)elem;
-  };
-  const long long delta = (long long)((intptr_t)b.p - (intptr_t)a.p);
-  if (delta >= extent(a) || -delta >= extent(b)) return false;
-  if (a.sb != b.sb || a.ss != b.ss || a.sh != b.sh || delta % elem != 0) return true;
-  struct Dim {
-    long long stride;
-    int na, nb;
-  } d[3];
-  int n = 0;
-  auto add = [&](long long st, int na, int nb) {
-    if (na > 1 || nb > 1) d[n++] = {st, na, nb};
-  };
-  add(a.sb, B, B);
-  add(a.ss, S, S);
-  add(a.sh, a.H, b.H);
-  std::sort(d, d + n, [](const Dim& x, const Dim& y) { return x.stride > y.stride; });
-  long long inner = Dh;  // extents of what lies inside a dimension
-  for (int i = n - 1; i >= 0; --i) {
-    if (d[i].stride < inner) return true;
-    inner += (std::max(d[i].na, d[i].nb) - 1) * d[i].stride;
-  }
-  // does some index pair bring b's element box onto a's?
-  auto meet = [&](auto& self, int i, long long off) -> bool {
-    if (i == n) return off < Dh && -off < Dh;
-    const long long st = d[i].stride;
-    const long long k = off >= 0 ? off / st : -((-off + st - 1) / st);
-    // a's index minus b's: only these two leave less than a stride
-    for (const long long t : {k, k + 1})
-      if (t <= d[i].na - 1 && -t <= d[i].nb - 1 && self(self, i + 1, off - t * st)) return true;
-    return false;
-  };
-  return meet(meet, 0, delta / elem);
-}
-
 static int rotary_check(const char* fn, const dlm_rotary_args* a, int& P) {
   auto bad = [&](const std::string& m) { return fail(DLM_ERR_INVALID_ARG, std::string(fn) + ": " + m); };
   if (!a->q || !a->q_out) return bad("NULL operand");
@@ -370,6 +320,8 @@ static int rotary_check(const char* fn, const dlm_rotary_args* a, int& P) {
   if (P > 0 && ((uintptr_t)a->pos % (a->pos_type == DLM_POS_I64 ? 8 : 4) != 0 || (uintptr_t)a->freqs % 8 != 0))
     return bad("positions and frequencies must be aligned to their elements");
   if (P > 0 && (a->pos_sb < 0 || a->pos_ss < 0)) return bad("negative stride of the positions");
+  if (P > 0 && (double)(a->B - 1) * (double)a->pos_sb + (double)(a->S - 1) * (double)a->pos_ss > 0x1p46)
+    return bad("the positions span more than 2^46 elements");
   if (a->norm && !(a->eps >= 0.0f && a->eps < INFINITY)) return bad("eps must be finite and not negative");
   if (!a->norm && (a->q_gamma || a->k_gamma)) return bad("gamma without the norm");
   for (const void* p : {a->q, (const void*)a->q_out, a->k, (const void*)a->k_out, a->q_gamma, a->k_gamma})
@@ -413,6 +365,20 @@ static int rotary_check(const char* fn, const dlm_rotary_args* a, int& P) {
       if (!same && views_overlap(v[i], v[j], a->B, a->S, a->Dh, 2))
         return bad(std::string(v[i].name) + " overlaps " + v[j].name);
     }
+    // nor may it lie on what every head reads
+    const long long vec = 2LL * a->Dh, places = a->pos_type == DLM_POS_I64 ? 8 : 4;
+    const struct {
+      const char* name;
+      const void* p;
+      long long bytes;
+    } shared[4] = {{"q_gamma", a->q_gamma, vec},
+                   {"k_gamma", a->k_gamma, vec},
+                   {"pos", P > 0 ? a->pos : nullptr,
+                    ((a->B - 1) * a->pos_sb + (a->S - 1) * a->pos_ss + a->axes) * places},
+                   {"freqs", P > 0 ? a->freqs : nullptr, 8LL * P}};
+    for (const auto& x : shared)
+      if (view_meets(v[i], a->B, a->S, a->Dh, 2, x.p, x.bytes))
+        return bad(std::string(v[i].name) + " overlaps " + x.name);
   }
   return DLM_OK;
 }

@@ -14,3 +14,48 @@ def test_tokens_that_a_grid_takes(lib):
     for tokens in ((1 << 26) - 3, (1 << 26) - 1, 1 << 26):
         assert qk(lib, B=1, S=tokens) == INVALID and "2^26 - 4 tokens" in err(), (tokens, err())
     assert qk(lib, B=1, S=(1 << 26) - 4, H=65536) == INVALID and "65535" in err()
+
+
+def test_rotary_outputs_on_what_every_head_reads(lib):
+    """Gammas, positions and frequencies on an output are refused; in the gaps between its heads they are not
+    (those calls are refused for their last operand: k_out is q_out)."""
+    qo = 3 * A  # [2, 8, 4, 64], contiguous: 8192 bytes; k_out at 4 A: 4096
+    last = 8192
+    for text, kw in [
+        ("q_out overlaps q_gamma", dict(q_gamma=qo)), ("q_out overlaps q_gamma", dict(q_gamma=qo - 126)),
+        ("q_out overlaps q_gamma", dict(q_gamma=qo + last - 2)), ("q_out overlaps k_gamma", dict(k_gamma=qo + 1000)),
+        ("k_out overlaps k_gamma", dict(k_gamma=4 * A + 4094)), ("k_out overlaps q_gamma", dict(q_gamma=4 * A - 2)),
+        ("q_out overlaps pos", dict(pos=qo + last - 4)), ("q_out overlaps pos", dict(pos=qo - 124)),  # 16 x 2 int32
+        ("q_out overlaps pos", dict(pos=qo - 248, pos_type=1, pos_sb=16)), ("k_out overlaps pos", dict(pos=4 * A)),
+        ("q_out overlaps freqs", dict(freqs=qo + 8)), ("k_out overlaps freqs", dict(freqs=4 * A - 248)),
+        ("k_out overlaps q_out", dict(q_gamma=qo - 128, k_gamma=qo + last, pos=qo - 256, freqs=qo + last, k_out=qo)),
+        ("span more", dict(pos_sb=1 << 60)),
+    ]:
+        assert qk(lib, **kw) == INVALID and text in err(), (kw, err())
+
+
+def test_bytes_on_a_view_against_its_addresses(lib):
+    """q_gamma among the elements of q_out by chance, against the sets of addresses; every call is refused in
+    the end, k_out being q_out."""
+    import itertools
+    import random
+    rng = random.Random(5)
+    told = {True: 0, False: 0}
+    for _ in range(800):
+        B, S, H, Dh = rng.choice([1, 2, 3]), rng.choice([1, 2, 4]), rng.choice([1, 2, 3]), rng.choice([2, 4, 8])
+        size, st = Dh + rng.choice([0, 4, 20]), {}
+        for d in reversed(rng.choice(["bsh", "bhs", "sbh"])):
+            st[d] = size
+            size = size * {"b": B, "s": S, "h": H}[d] + rng.choice([0, 10, 30])
+        at = rng.randrange(-Dh - 2, size + 4)
+        cells = {b * st["b"] + s * st["s"] + h * st["h"] + d
+                 for b, s, h, d in itertools.product(range(B), range(S), range(H), range(Dh))}
+        kw = dict(q=A - 1024 * 1024, k=A + 1024 * 1024, q_out=A, k_out=A, q_gamma=A + 2 * at, B=B, S=S, H=H, Hkv=H, Dh=Dh,
+                  sections=[0, 0])
+        for x in ("q", "qo", "k", "ko"):
+            kw[x + "_sb"], kw[x + "_ss"], kw[x + "_sh"] = st["b"], st["s"], st["h"]
+        clash = bool(cells & set(range(at, at + Dh)))
+        told[clash] += 1
+        assert qk(lib, **kw) == INVALID
+        assert ("q_out overlaps q_gamma" if clash else "k_out overlaps q_out") in err(), (kw, err())
+    assert min(told.values()) > 100, told
