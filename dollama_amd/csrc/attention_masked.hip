@@ -1,6 +1,7 @@
 // Masked attention: the entry points, the choice of a kernel, and the kernels for fp16 (those for bf16
 // are the same in a file of their own, so that the two compile side by side).
 #include "attention_masked.hpp"
+#include "views.hpp"
 
 namespace dlm {
 
@@ -37,7 +38,9 @@ static size_t am_workspace(const dlm_attention_masked_args* a, const AmPlan& pl)
   return (size_t)pl.splits * a->B * a->H * a->Sq * (a->Dh + 2) * 4;
 }
 
-static int am_check(const char* fn, const dlm_attention_masked_args* a) {
+// Every check of a call; its plan where they pass
+static int am_check(const char* fn, const dlm_attention_masked_args* a, const void* workspace, size_t workspace_bytes,
+                    AmPlan& pl) {
   auto bad = [&](const std::string& m) { return fail(DLM_ERR_INVALID_ARG, std::string(fn) + ": " + m); };
   if (!a->q || !a->o || (a->Sk > 0 && (!a->k || !a->v))) return bad("NULL operand");
   if (a->dtype != DLM_DTYPE_F16 && a->dtype != DLM_DTYPE_BF16) return bad("unknown dtype");
@@ -101,6 +104,33 @@ static int am_check(const char* fn, const dlm_attention_masked_args* a) {
       (uintptr_t)a->rel_bias % 4 != 0)
     return bad("key_range must be 8-byte, q_pos, slopes and rel_bias 4-byte aligned");
   if (a->kr_sb < 0 || a->kr_sb % 2 != 0 || a->qp_sb < 0) return bad("batch strides of the masks must be whole and not negative");
+  if ((double)(a->B - 1) * (double)std::max(a->kr_sb, a->qp_sb) > 0x1p46) return bad("the masks span more than 2^46 elements");
+  pl = am_plan(a);
+  const size_t need = am_workspace(a, pl);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return bad("the workspace is too small");
+  if (need > 0 && !dlm_aligned16(workspace)) return bad("the workspace must be 16-byte aligned");
+  // the output may not lie on what every row reads, nor the parts of the keys on anything
+  const struct {
+    const char* name;
+    const void* p;
+    long long bytes;
+  } flat[4] = {{"key_range", a->key_range, ((a->B - 1) * a->kr_sb + 2LL * a->Sq) * 4},
+               {"q_pos", a->q_pos, ((a->B - 1) * a->qp_sb + a->Sq) * 4},
+               {"slopes", a->slopes, 4LL * a->H},
+               {"rel_bias", a->rel_bias, (2LL * a->R + 1) * a->H * 4}};
+  auto meets = [&](const Op& x, const void* q, long long bytes) {
+    return x.S > 0 && view_meets(View{x.name, x.p, x.sb, x.ss, x.sh, x.H}, a->B, x.S, a->Dh, 2, q, bytes);
+  };
+  for (const auto& x : flat)
+    if (meets(ops[3], x.p, x.bytes)) return bad(std::string("o overlaps ") + x.name);
+  if (need > 0) {
+    const uintptr_t at = (uintptr_t)workspace;
+    for (const Op& x : ops)
+      if (meets(x, workspace, (long long)need)) return bad(std::string("the workspace overlaps ") + x.name);
+    for (const auto& x : flat)
+      if (x.p && at < (uintptr_t)x.p + x.bytes && (uintptr_t)x.p < at + need)
+        return bad(std::string("the workspace overlaps ") + x.name);
+  }
   return DLM_OK;
 }
 
@@ -118,13 +148,8 @@ size_t dlm_attention_masked_workspace_bytes(const dlm_attention_masked_args* a) 
 int dlm_attention_masked(const dlm_attention_masked_args* a, void* workspace, size_t workspace_bytes, void* stream) {
   DLM_REQUIRE(a != nullptr, "args is NULL");
   if (a->B <= 0 || a->Sq <= 0 || a->H <= 0 || a->Dh <= 0) return DLM_OK;
-  if (const int st = am_check(__func__, a)) return st;
-  const AmPlan pl = am_plan(a);
-  const size_t need = am_workspace(a, pl);
-  if (need > 0) {
-    DLM_REQUIRE(workspace != nullptr && workspace_bytes >= need, "the workspace is too small");
-    DLM_REQUIRE(dlm_aligned16(workspace), "the workspace must be 16-byte aligned");
-  }
+  AmPlan pl;
+  if (const int st = am_check(__func__, a, workspace, workspace_bytes, pl)) return st;
   AmParams p{};
   p.q = (const char*)a->q, p.k = (const char*)a->k, p.v = (const char*)a->v, p.o = (char*)a->o;
   p.q_sb = a->q_sb, p.q_ss = a->q_ss, p.q_sh = a->q_sh;

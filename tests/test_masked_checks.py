@@ -59,3 +59,39 @@ def test_bytes_on_a_view_against_its_addresses(lib):
         assert qk(lib, **kw) == INVALID
         assert ("q_out overlaps q_gamma" if clash else "k_out overlaps q_out") in err(), (kw, err())
     assert min(told.values()) > 100, told
+
+
+def attend(lib, ws=None, n=0, **kw):
+    return lib.dlm_attention_masked(ctypes.byref(attention_args(**kw)), ws, n, None)
+
+
+def test_attention_outputs_on_masks_and_biases(lib):
+    o, size = 4 * A, 2 * 8 * 4 * 64 * 2  # [2, 8, 4, 64], contiguous
+    table = dict(R=3)  # [4, 7]
+    for text, kw in [
+        ("o overlaps key_range", dict(key_range=o)), ("o overlaps key_range", dict(key_range=o - 56)),
+        ("o overlaps key_range", dict(key_range=o - 112, kr_sb=16)), ("o overlaps key_range", dict(key_range=o + size - 8)),
+        ("o overlaps q_pos", dict(q_pos=o - 28)), ("o overlaps q_pos", dict(q_pos=o - 60, qp_sb=8)),
+        ("o overlaps slopes", dict(slopes=o - 12)), ("o overlaps slopes", dict(slopes=o + size - 4)),
+        ("o overlaps rel_bias", dict(rel_bias=o - 108, **table)), ("o overlaps rel_bias", dict(rel_bias=o + size - 4, **table)),
+        # in the gaps between heads of 64 in 128 they are free (those calls are refused for their table)
+        ("o overlaps rel_bias", dict(o_sh=128, o_ss=512, o_sb=4096, key_range=o + 128, rel_bias=o, **table)),
+        ("o overlaps rel_bias", dict(o_sh=128, o_ss=512, o_sb=4096, q_pos=o + 128, rel_bias=o, **table)),
+        ("span more", dict(q_pos=7 * A, qp_sb=1 << 50)),
+    ]:
+        assert attend(lib, **kw) == INVALID and text in err(), (kw, err())
+
+
+def test_workspaces_on_operands(lib):
+    many = dict(Sq=1, Sk=4096, k_sb=4096 * 128, v_sb=4096 * 128, v=8 * A, q_sb=256, o_sb=256)
+    n = lib.dlm_attention_masked_workspace_bytes(ctypes.byref(attention_args(**many)))
+    assert n > 0
+    keys = 2 * 4096 * 128 * 2
+    for text, ws, kw in [
+        ("workspace overlaps q", A, {}), ("workspace overlaps q", A - n + 16, {}), ("workspace overlaps q", A + 1008, {}),
+        ("workspace overlaps k", 2 * A + keys - 16, {}), ("workspace overlaps v", 8 * A - 16, {}), ("workspace overlaps o", 4 * A, {}),
+        ("workspace overlaps key_range", 9 * A, dict(key_range=9 * A + n - 16)),
+        ("workspace overlaps q_pos", 9 * A, dict(q_pos=9 * A)), ("workspace overlaps slopes", 9 * A, dict(slopes=9 * A - 12)),
+        ("workspace overlaps rel_bias", 9 * A + 16 * 4, dict(rel_bias=9 * A, R=3)),
+    ]:
+        assert attend(lib, ws, n, **{**many, **kw}) == INVALID and text in err(), (ws, kw, err())
