@@ -56,24 +56,18 @@ static int am_check(const char* fn, const dlm_attention_masked_args* a, const vo
   const long long G = a->H / a->Hkv;
   if (a->Sq * G >= (1LL << 29) || (long long)a->B * a->Hkv > 65535) return bad("more rows or heads than a grid takes");
   if ((long long)a->B * a->Hkv * ((a->Sq * G + 31) / 32) >= (1LL << 23)) return bad("more rows than a grid takes");
-  struct Op {
-    const char* name;
-    const void* p;
-    long long sb, ss, sh;
-    int S, H, unit, align;
-  };
-  Op ops[4] = {{"q", a->q, a->q_sb, a->q_ss, a->q_sh, a->Sq, a->H, 8, 16},
-               {"k", a->k, a->k_sb, a->k_ss, a->k_sh, a->Sk, a->Hkv, 8, 16},
-               {"v", a->v, a->v_sb, a->v_ss, a->v_sh, a->Sk, a->Hkv, 8, 16},
-               {"o", a->o, a->o_sb, a->o_ss, a->o_sh, a->Sq, a->H, 4, 8}};
-  uintptr_t lo[4], hi[4];
+  View ops[4] = {{"q", a->q, a->q_sb, a->q_ss, a->q_sh, a->Sq, a->H},
+                 {"k", a->k, a->k_sb, a->k_ss, a->k_sh, a->Sk, a->Hkv},
+                 {"v", a->v, a->v_sb, a->v_ss, a->v_sh, a->Sk, a->Hkv},
+                 {"o", a->o, a->o_sb, a->o_ss, a->o_sh, a->Sq, a->H}};
   for (int i = 0; i < 4; ++i) {
-    Op& x = ops[i];
+    View& x = ops[i];
+    const int unit = i < 3 ? 8 : 4, align = 2 * unit;
     if (a->B == 1) x.sb = 0;  // a dimension of one has no stride
     if (x.S <= 1) x.ss = 0;
     if (x.H == 1) x.sh = 0;
     if (x.sb < 0 || x.ss < 0 || x.sh < 0) return bad(std::string(x.name) + ": negative stride");
-    if ((uintptr_t)x.p % x.align != 0 || x.sb % x.unit != 0 || x.ss % x.unit != 0 || x.sh % x.unit != 0)
+    if ((uintptr_t)x.p % align != 0 || x.sb % unit != 0 || x.ss % unit != 0 || x.sh % unit != 0)
       return bad(std::string(x.name) + (i < 3 ? ": address and strides must keep 16-byte alignment"
                                               : ": address and strides must keep 8-byte alignment"));
     const double last = (double)(a->B - 1) * (double)x.sb + (double)(std::max(x.S, 1) - 1) * (double)x.ss +
@@ -81,8 +75,6 @@ static int am_check(const char* fn, const dlm_attention_masked_args* a, const vo
     if (last > 0x1p46) return bad(std::string(x.name) + " spans more than 2^46 elements");
     if ((i == 1 || i == 2) && x.S > 1 && (x.ss < a->Dh || x.ss >= (1 << 23)))
       return bad(std::string(x.name) + ": a key row's stride must be Dh to 2^23");
-    lo[i] = (uintptr_t)x.p;
-    hi[i] = lo[i] + (uintptr_t)last * 2;
   }
   // an output's own elements have to lie apart
   {
@@ -99,7 +91,7 @@ static int am_check(const char* fn, const dlm_attention_masked_args* a, const vo
     }
   }
   for (int i = 0; i < 3; ++i)
-    if (ops[i].S > 0 && lo[3] < hi[i] && lo[i] < hi[3]) return bad(std::string("o overlaps ") + ops[i].name);
+    if (views_overlap(ops[3], ops[i], a->B, a->Dh, 2)) return bad(std::string("o overlaps ") + ops[i].name);
   if ((uintptr_t)a->key_range % 8 != 0 || (uintptr_t)a->q_pos % 4 != 0 || (uintptr_t)a->slopes % 4 != 0 ||
       (uintptr_t)a->rel_bias % 4 != 0)
     return bad("key_range must be 8-byte, q_pos, slopes and rel_bias 4-byte aligned");
@@ -118,14 +110,12 @@ static int am_check(const char* fn, const dlm_attention_masked_args* a, const vo
                {"q_pos", a->q_pos, ((a->B - 1) * a->qp_sb + a->Sq) * 4},
                {"slopes", a->slopes, 4LL * a->H},
                {"rel_bias", a->rel_bias, (2LL * a->R + 1) * a->H * 4}};
-  auto meets = [&](const Op& x, const void* q, long long bytes) {
-    return x.S > 0 && view_meets(View{x.name, x.p, x.sb, x.ss, x.sh, x.H}, a->B, x.S, a->Dh, 2, q, bytes);
-  };
+  auto meets = [&](const View& x, const void* p, long long bytes) { return view_meets(x, a->B, a->Dh, 2, p, bytes); };
   for (const auto& x : flat)
     if (meets(ops[3], x.p, x.bytes)) return bad(std::string("o overlaps ") + x.name);
   if (need > 0) {
     const uintptr_t at = (uintptr_t)workspace;
-    for (const Op& x : ops)
+    for (const View& x : ops)
       if (meets(x, workspace, (long long)need)) return bad(std::string("the workspace overlaps ") + x.name);
     for (const auto& x : flat)
       if (x.p && at < (uintptr_t)x.p + x.bytes && (uintptr_t)x.p < at + need)

@@ -330,10 +330,10 @@ static int rotary_check(const char* fn, const dlm_rotary_args* a, int& P) {
   // four tokens)
   if ((long long)a->B * a->S > (1LL << 26) - 4) return bad("more than 2^26 - 4 tokens");
   if ((long long)a->H + (a->k ? a->Hkv : 0) > 65535) return bad("more than 65535 heads");
-  const View v[4] = {{"q", a->q, a->q_sb, a->q_ss, a->q_sh, a->H},
-                     {"k", a->k, a->k_sb, a->k_ss, a->k_sh, a->Hkv},
-                     {"q_out", a->q_out, a->qo_sb, a->qo_ss, a->qo_sh, a->H},
-                     {"k_out", a->k_out, a->ko_sb, a->ko_ss, a->ko_sh, a->Hkv}};
+  const View v[4] = {{"q", a->q, a->q_sb, a->q_ss, a->q_sh, a->S, a->H},
+                     {"k", a->k, a->k_sb, a->k_ss, a->k_sh, a->S, a->Hkv},
+                     {"q_out", a->q_out, a->qo_sb, a->qo_ss, a->qo_sh, a->S, a->H},
+                     {"k_out", a->k_out, a->ko_sb, a->ko_ss, a->ko_sh, a->S, a->Hkv}};
   for (const View& x : v) {
     if (!x.p) continue;
     if (x.sb < 0 || x.ss < 0 || x.sh < 0) return bad(std::string(x.name) + ": negative stride");
@@ -362,7 +362,7 @@ static int rotary_check(const char* fn, const dlm_rotary_args* a, int& P) {
       // in place: the very view (a stride of a dimension of one says nothing)
       const bool same = j == i - 2 && v[i].p == v[j].p && (a->B == 1 || v[i].sb == v[j].sb) &&
                         (a->S == 1 || v[i].ss == v[j].ss) && (v[i].H == 1 || v[i].sh == v[j].sh);
-      if (!same && views_overlap(v[i], v[j], a->B, a->S, a->Dh, 2))
+      if (!same && views_overlap(v[i], v[j], a->B, a->Dh, 2))
         return bad(std::string(v[i].name) + " overlaps " + v[j].name);
     }
     // nor may it lie on what every head reads
@@ -377,7 +377,7 @@ static int rotary_check(const char* fn, const dlm_rotary_args* a, int& P) {
                     ((a->B - 1) * a->pos_sb + (a->S - 1) * a->pos_ss + a->axes) * places},
                    {"freqs", P > 0 ? a->freqs : nullptr, 8LL * P}};
     for (const auto& x : shared)
-      if (view_meets(v[i], a->B, a->S, a->Dh, 2, x.p, x.bytes))
+      if (view_meets(v[i], a->B, a->Dh, 2, x.p, x.bytes))
         return bad(std::string(v[i].name) + " overlaps " + x.name);
   }
   return DLM_OK;

@@ -10,31 +10,33 @@ struct View {
   const char* name;
   const void* p;
   long long sb, ss, sh;
-  int H;
+  int S, H;
 };
 
 // Whether two views of B x S x H x Dh elements share one.  Of views with the same
 // strides, each longer than what lies inside it (slices of one tensor), the places
 // are compared; any others count by their whole extents.
-inline bool views_overlap(const View& a, const View& b, int B, int S, int Dh, int elem) {
-  if (!a.p || !b.p) return false;
+inline bool views_overlap(const View& a, const View& b, int B, int Dh, int elem) {
+  if (!a.p || !b.p || a.S <= 0 || b.S <= 0) return false;
   auto extent = [&](const View& v) {
-    return ((B - 1) * v.sb + (S - 1) * v.ss + (v.H - 1) * v.sh + Dh) * (long long)elem;
+    return ((B - 1) * v.sb + (v.S - 1) * v.ss + (v.H - 1) * v.sh + Dh) * (long long)elem;
   };
   const long long delta = (long long)((intptr_t)b.p - (intptr_t)a.p);
   if (delta >= extent(a) || -delta >= extent(b)) return false;
-  if (a.sb != b.sb || a.ss != b.ss || a.sh != b.sh || delta % elem != 0) return true;
   struct Dim {
     long long stride;
     int na, nb;
   } d[3];
   int n = 0;
-  auto add = [&](long long st, int na, int nb) {
-    if (na > 1 || nb > 1) d[n++] = {st, na, nb};
+  bool alike = delta % elem == 0;
+  auto add = [&](long long sa, int na, long long sb, int nb) {
+    if (na > 1 || nb > 1) d[n++] = {na > 1 ? sa : sb, na, nb};
+    alike = alike && (na <= 1 || nb <= 1 || sa == sb);
   };
-  add(a.sb, B, B);
-  add(a.ss, S, S);
-  add(a.sh, a.H, b.H);
+  add(a.sb, B, b.sb, B);
+  add(a.ss, a.S, b.ss, b.S);
+  add(a.sh, a.H, b.sh, b.H);
+  if (!alike) return true;
   std::sort(d, d + n, [](const Dim& x, const Dim& y) { return x.stride > y.stride; });
   long long inner = Dh;  // extents of what lies inside a dimension
   for (int i = n - 1; i >= 0; --i) {
@@ -55,8 +57,8 @@ inline bool views_overlap(const View& a, const View& b, int B, int S, int Dh, in
 }
 
 // Whether one of a view's elements lies in the `bytes` bytes from q on.
-inline bool view_meets(const View& v, int B, int S, int Dh, int elem, const void* q, long long bytes) {
-  if (!v.p || !q || bytes <= 0) return false;
+inline bool view_meets(const View& v, int B, int Dh, int elem, const void* q, long long bytes) {
+  if (!v.p || !q || v.S <= 0 || bytes <= 0) return false;
   struct Dim {
     long long stride;
     int n;
@@ -66,7 +68,7 @@ inline bool view_meets(const View& v, int B, int S, int Dh, int elem, const void
     if (count > 1) d[n++] = {st * elem, count};
   };
   add(v.sb, B);
-  add(v.ss, S);
+  add(v.ss, v.S);
   add(v.sh, v.H);
   std::sort(d, d + n, [](const Dim& x, const Dim& y) { return x.stride > y.stride; });
   long long extent[4];  // of what lies inside a dimension, and of all

@@ -95,3 +95,35 @@ def test_workspaces_on_operands(lib):
         ("workspace overlaps rel_bias", 9 * A + 16 * 4, dict(rel_bias=9 * A, R=3)),
     ]:
         assert attend(lib, ws, n, **{**many, **kw}) == INVALID and text in err(), (ws, kw, err())
+
+
+def test_attention_outputs_among_operands(lib):
+    """The output may be a slice of the tensor that the operands are slices of; against the sets of addresses.
+    Calls without an overlap are refused for their places' alignment."""
+    import itertools
+    import random
+    rng = random.Random(9)
+    told = {True: 0, False: 0}
+    for _ in range(800):
+        B, Sq, Sk, Dh = rng.choice([1, 2, 3]), rng.choice([1, 2, 4]), rng.choice([1, 2, 4]), 8
+        Hkv = rng.choice([1, 2])
+        H = Hkv * rng.choice([1, 2])
+        size, st = Dh + rng.choice([0, 8]), {}
+        for d in reversed(rng.choice(["bsh", "bhs", "sbh"])):
+            st[d] = size
+            size *= {"b": B, "s": 6, "h": 8}[d]
+        k, o = (rng.randrange(0, 6) * st["h"] + rng.randrange(0, 3) * st["s"] for _ in range(2))
+
+        def cells(at, tokens, heads):
+            return {at + b * st["b"] + s * st["s"] + h * st["h"] + d
+                    for b, s, h, d in itertools.product(range(B), range(tokens), range(heads), range(Dh))}
+
+        kw = dict(q=A - 1024 * 1024, v=A + 1024 * 1024, k=A + 2 * k, o=A + 2 * o, B=B, Sq=Sq, Sk=Sk, H=H, Hkv=Hkv, Dh=Dh,
+                  q_pos=7 * A + 2)
+        for x in "qkvo":
+            kw[x + "_sb"], kw[x + "_ss"], kw[x + "_sh"] = st["b"], st["s"], st["h"]
+        clash = bool(cells(k, Sk, Hkv) & cells(o, Sq, H))
+        told[clash] += 1
+        assert attend(lib, **kw) == INVALID
+        assert ("o overlaps k" if clash else "aligned") in err(), (kw, err())
+    assert min(told.values()) > 100, told

@@ -153,3 +153,20 @@ def test_slopes_of_any_size(gpu, slope, mode):
             assert torch.equal(got[0, :, 0], v[0, p.long(), 0])
         else:
             assert torch.equal(got[0, :, 0], v[0, :1, 0].expand(Sq, 64))
+
+
+@pytest.mark.parametrize("dt", HALF, ids=NAMES.get)
+def test_an_output_among_its_operands(gpu, dt):
+    """Queries, keys, values and the output as slices of one tensor: whole heads, or heads' parts."""
+    B, S, H, Hkv, Dh = 2, 100, 4, 2, 64
+    for shape, cut in (((B, S, 2 * H + 2 * Hkv, Dh), lambda t: t.split([H, Hkv, Hkv, H], 2)),
+                       ((B, 2 * H + 2 * Hkv, S, Dh), lambda t: [x.transpose(1, 2) for x in t.split([H, Hkv, Hkv, H], 1)]),
+                       ((B, S, H, 4 * Dh), lambda t: t.split(Dh, 3))):
+        announce(f"slices of {shape} {dt}")
+        x = rnd(shape, 10, dt).cuda()
+        q, k, v, out = cut(x)
+        want = ops.attention_masked(q, k, v, causal=True)
+        before = [t.clone() for t in (q, k, v)]
+        got = ops.attention_masked(q, k, v, causal=True, out=out)
+        assert got is out and torch.equal(out, want)
+        assert all(torch.equal(a, b) for a, b in zip((q, k, v), before))
