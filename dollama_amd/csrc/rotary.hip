@@ -10,6 +10,8 @@
 // store, but for the angle: its turns pos * freq / 2 pi are an fp64 product, of
 // which only the fraction matters (in fp32 a position of 10^6 would leave errors of
 // 0.06 rad).  v_sin_f32 and v_cos_f32 take turns.
+#include <cfloat>
+
 #include "common.hpp"
 #include "views.hpp"
 
@@ -404,7 +406,10 @@ static int rotary_run(const char* fn, const dlm_rotary_args* a, hipStream_t s) {
   }
   p.freqs = a->freqs;
   p.P = P, p.Dh = a->Dh, p.norm = a->norm != 0;
-  p.tokens = a->B * a->S, p.S = a->S, p.eps = a->eps;
+  p.tokens = a->B * a->S, p.S = a->S;
+  // (v_rsq_f32 takes a subnormal number as 0.  A mean of fp16 squares is 2^-56 at least or 0; bf16 heads are
+  // brought into range)
+  p.eps = a->dtype == DLM_DTYPE_F16 && a->eps > 0.0f ? std::max(a->eps, FLT_MIN) : a->eps;
   p.inv_dh = 1.0f / (float)a->Dh;
   const int V = rotary_vector(a, P);
   if (a->dtype == DLM_DTYPE_F16)

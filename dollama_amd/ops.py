@@ -1044,6 +1044,8 @@ def _rotary(name, q, k, q_gamma, k_gamma, positions, freqs, sections, interleave
     B = shape[0] if len(shape) == 4 else 1
     if not (B and S and H and Dh):
         return q_out, k_out
+    if 0.0 < eps < 2.0 ** -149:
+        eps = 2.0 ** -149  # fp32's smallest number, not 0: heads of zeros stay zeros
     args = _pack_rotary(q.data_ptr(), pk, q_out.data_ptr(), pko, *sq, *sk, *so, *sko, gq, gk, pp, sp0, sp1, pf, pt, axes,
                         *sections, *_SECTIONS_PAD[axes], interleaved, norm, eps, _HALF[dt], B, S, H, Hkv, Dh)
     st = _entry(name)(args, torch._C._cuda_getCurrentRawStream(dev))

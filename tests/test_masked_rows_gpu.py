@@ -7,7 +7,7 @@ import torch
 
 from dollama_amd import ops
 from oracle import masked_ref as M
-from test_masked_gpu import HALF, NAMES, announce, att_tol, qkv, rnd, within
+from test_masked_gpu import HALF, NAMES, announce, att_tol, qkv, rnd, turn_tol, within
 
 pytestmark = pytest.mark.gpu
 
@@ -170,3 +170,16 @@ def test_an_output_among_its_operands(gpu, dt):
         got = ops.attention_masked(q, k, v, causal=True, out=out)
         assert got is out and torch.equal(out, want)
         assert all(torch.equal(a, b) for a, b in zip((q, k, v), before))
+
+
+@pytest.mark.parametrize("dt", HALF, ids=NAMES.get)
+@pytest.mark.parametrize("eps", [1e-50, 1e-45, 1e-40, 1e-37])
+def test_heads_of_zeros_under_the_smallest_eps(gpu, eps, dt):
+    """0 / sqrt(0 + eps) is 0 for every eps but 0."""
+    announce(f"norm of zeros, eps = {eps}, {dt}")
+    x = rnd((1, 4, 2, 80), 11, dt)
+    x[0, 1] = 0
+    x[0, 3, 0] = 0
+    got, _ = ops.qk_norm_rotary(x.cuda(), eps=eps)
+    y = M.norm(x, None, eps)
+    within(got, y, turn_tol(y, y.abs(), dt) + 2.0 ** -126, "norm")
