@@ -1164,6 +1164,8 @@ def attention_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_r
         pb = _vector(rel_bias, H * (2 * R + 1), "rel_bias", torch.float32, dev)
     if scale is None:
         scale = Dh ** -0.5 if Dh else 1.0
+    if 0.0 < cap <= 2.0 ** -150:  # 0 in fp32, which is no cap
+        raise ValueError(f"cap is too small, got {cap}")
     if not (B and Sq and H and Dh):
         return out
     args = _pack_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *sq, *sk, *sv, *so, kr, krb, qp, qpb,

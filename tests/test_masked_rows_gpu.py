@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from dollama_amd import ops
+from dollama_amd import _lib, ops
 from oracle import masked_ref as M
 from test_masked_gpu import HALF, NAMES, announce, att_tol, qkv, rnd, turn_tol, within
 
@@ -183,3 +183,13 @@ def test_heads_of_zeros_under_the_smallest_eps(gpu, eps, dt):
     got, _ = ops.qk_norm_rotary(x.cuda(), eps=eps)
     y = M.norm(x, None, eps)
     within(got, y, turn_tol(y, y.abs(), dt) + 2.0 ** -126, "norm")
+
+
+def test_caps_below_every_number_are_refused(gpu):
+    announce("a cap that is no fp32 number")
+    q, k, v = (t.cuda() for t in qkv(1, 3, 9, 2, 2, 64, torch.float16))
+    with pytest.raises(ValueError, match="cap"):
+        ops.attention_masked(q, k, v, cap=1e-46)
+    with pytest.raises(_lib.DlmError, match="cap"):
+        ops.attention_masked(q, k, v, cap=1e-45)
+    ops.attention_masked(q, k, v, cap=1e-45, scale=1e-30)
