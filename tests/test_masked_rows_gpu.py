@@ -1,5 +1,6 @@
 """Masked attention's rows beside one another: no row's result shows what another row's query, keys or
 place hold, nor what keys hold that a table hides from it (GPU)."""
+import ctypes
 import math
 
 import pytest
@@ -7,7 +8,7 @@ import torch
 
 from dollama_amd import _lib, ops
 from oracle import masked_ref as M
-from test_masked_gpu import HALF, NAMES, announce, att_tol, qkv, rnd, turn_tol, within
+from test_masked_gpu import HALF, NAMES, announce, att_tol, attend, qkv, rnd, turn_tol, within
 
 pytestmark = pytest.mark.gpu
 
@@ -193,3 +194,59 @@ def test_caps_below_every_number_are_refused(gpu):
     with pytest.raises(_lib.DlmError, match="cap"):
         ops.attention_masked(q, k, v, cap=1e-45)
     ops.attention_masked(q, k, v, cap=1e-45, scale=1e-30)
+
+
+def in_parts(B, Sq, Sk, H, Hkv, Dh):
+    """Whether a call of these sizes splits its keys."""
+    a = _lib.AttentionMaskedArgs()
+    a.B, a.Sq, a.Sk, a.H, a.Hkv, a.Dh = B, Sq, Sk, H, Hkv, Dh
+    return _lib.hip_lib().dlm_attention_masked_workspace_bytes(ctypes.byref(a)) > 0
+
+
+@pytest.mark.parametrize("dt", HALF, ids=NAMES.get)
+@pytest.mark.parametrize("B,H,Hkv,Dh,lengths", [
+    (1, 43, 43, 64, [310, 300, 90]), (2, 24, 24, 80, [257, 330, 3, 111]), (1, 48, 12, 64, [40, 360, 300]),
+    (1, 37, 37, 40, [500, 260, 10]), (2, 37, 37, 64, [333, 1, 366]), (1, 30, 30, 128, [600, 520, 20]), (1, 29, 29, 256, [400, 390, 360]),
+])
+def test_documents_that_share_row_blocks_of_whole_keys(gpu, B, H, Hkv, Dh, lengths, dt):
+    """More row blocks than CUs, so that keys stay whole: two workgroups store the rows of a block that holds
+    the end of one long document and the start of another, started in the order of their lengths."""
+    S = sum(lengths)
+    blocks = B * Hkv * ((S * (H // Hkv) + 127) // 128)
+    assert blocks > 255 and not in_parts(B, S, S, H, Hkv, Dh)
+    q, k, v = qkv(B, S, S, H, Hkv, Dh, dt, S)
+    r = ops.document_ranges(lengths, device="cpu")
+    name = f"documents {lengths} x{B}x{H}/{Hkv}x{Dh} {dt}, {blocks} row blocks"
+    out = torch.full((B, S, H, Dh), float("nan"), dtype=dt, device="cuda")
+    attend(q, k, v, name, key_range=r, out=out)
+    if Dh != 128:
+        out.fill_(float("nan"))
+        attend(q, k, v, f"{name}, causal", key_range=r, causal=True, out=out)
+
+
+@pytest.mark.parametrize("B,S,H,Hkv,Dh", [(3, 260, 40, 40, 64), (1, 700, 47, 47, 64), (4, 130, 70, 70, 64), (1, 400, 84, 28, 80),
+                                          (2, 513, 30, 30, 128), (5, 129, 29, 29, 40), (1, 1100, 31, 31, 64)])
+def test_row_blocks_by_length_where_keys_are_whole(gpu, B, S, H, Hkv, Dh):
+    """Causal row blocks beyond a first round on 256 CUs, in numbers that 8 divides and does not: each is
+    taken once."""
+    blocks = B * Hkv * ((S * (H // Hkv) + 127) // 128)
+    assert 256 < blocks <= 8 * 256 and not in_parts(B, S, S, H, Hkv, Dh)
+    q, k, v = qkv(B, S, S, H, Hkv, Dh, torch.float16, S)
+    out = torch.full((B, S, H, Dh), float("nan"), dtype=torch.float16, device="cuda")
+    attend(q, k, v, f"causal {B}x{S}x{H}/{Hkv}x{Dh}, {blocks} row blocks", causal=True, out=out)
+
+
+@pytest.mark.parametrize("dt", HALF, ids=NAMES.get)
+@pytest.mark.parametrize("mode", MODES)
+def test_intervals_of_other_rows_change_no_bit(gpu, mode, dt):
+    """Tiles that are whole for a row, and not for its neighbours."""
+    for Sq, Sk, H, Dh in ROWS:
+        announce(f"intervals of neighbours, {mode}, {Sq}x{Sk}x{H}x{Dh} {dt}")
+        q, k, v = (t.cuda() for t in qkv(1, Sq, Sk, H, H, Dh, dt, 12))
+        r = torch.tensor([0, Sk], dtype=torch.int32, device="cuda").repeat(Sq, 1)
+        want = None
+        for lo, hi in ((0, Sk), (0, Sk - 70), (100, Sk), (7, 7), (300, 330)):
+            r[1::2, 0], r[1::2, 1] = lo, hi
+            got = ops.attention_masked(q, k, v, key_range=r, **scores_kw(mode, H))[:, ::2]
+            want = got if want is None else want
+            assert torch.equal(got, want), f"{mode}, neighbours see [{lo}, {hi}): {int((got != want).sum())} values differ"
