@@ -47,7 +47,7 @@ static int am_check(const char* fn, const dlm_attention_masked_args* a, const vo
   if (a->Sk < 0) return bad("negative number of keys");
   if (a->Dh % 8 != 0 || a->Dh > 256) return bad("Dh must be a multiple of 8 and at most 256");
   if (a->Hkv <= 0 || a->H % a->Hkv != 0) return bad("H must be a multiple of Hkv");
-  if (!(a->scale > 0.0f && a->scale < INFINITY)) return bad("scale must be positive and finite");
+  if (!(a->scale > 0.0f && a->scale <= 0x1p127f)) return bad("scale must be positive and at most 2^127");
   if (!(a->cap >= 0.0f && a->cap < INFINITY)) return bad("cap must be finite and not negative");
   if (a->cap > 0.0f && a->scale / a->cap > 1e30f) return bad("cap is too small for the scale");
   if (a->slopes && a->rel_bias) return bad("one bias of distance, slopes or a table");

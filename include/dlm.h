@@ -626,7 +626,7 @@ int dlm_qk_norm_rotary(const dlm_rotary_args* args, void* stream);
  * row's stride is at least Dh and below 2^23.  key_range is int32 [.., Sq, 2] with
  * batch stride kr_sb (elements, 0: one for every batch), 8-byte aligned; q_pos
  * int32 [.., Sq] with batch stride qp_sb; slopes fp32 [H]; rel_bias fp32 [H][2R + 1].
- * scale > 0 and cap >= 0 are finite, scale / cap at most 1e30.  dtype is that of q, k, v and o; scores,
+ * scale > 0 is at most 2^127, cap >= 0 finite, scale / cap at most 1e30.  dtype is that of q, k, v and o; scores,
  * softmax and sums are fp32, the probabilities are rounded to dtype for the product with v.  Sk
  * and Sq are at most 2^28, B x Hkv at most 65535.
  * Few queries against many keys are split over the keys; the parts meet in the

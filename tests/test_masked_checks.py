@@ -127,3 +127,10 @@ def test_attention_outputs_among_operands(lib):
         assert attend(lib, **kw) == INVALID
         assert ("o overlaps k" if clash else "aligned") in err(), (kw, err())
     assert min(told.values()) > 100, told
+
+
+def test_scales_whose_powers_of_two_leave_fp32(lib):
+    """scale log2 e has to be finite: infinity times a product of 0 is NaN."""
+    for cap in (0.0, 1e38):
+        assert attend(lib, scale=3e38, cap=cap) == INVALID and "scale" in err()
+        assert attend(lib, scale=2.0 ** 127, cap=cap, q_pos=7 * A + 2) == INVALID and "aligned" in err()
