@@ -129,9 +129,9 @@ __device__ __forceinline__ float capped(const AmParams& p, float x) {
   return fabsf(x) <= p.small ? capped_small(p, x) : far;
 }
 
-// A bias to powers of two; the lowest values stay finite, -infinity stays what it is.
+// A bias to powers of two; the lowest values stay finite, infinities and NaN what they are.
 __device__ __forceinline__ float am_log2(float b) {
-  return __builtin_isinf(b) ? b : fmaxf(-FLT_MAX, fminf(FLT_MAX, b * AM_LOG2E));
+  return __builtin_isfinite(b) ? fmaxf(-FLT_MAX, fminf(FLT_MAX, b * AM_LOG2E)) : b;
 }
 
 // A slope to powers of two, held where its product with any distance (below 2^31) is finite

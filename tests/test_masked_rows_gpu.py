@@ -40,7 +40,7 @@ def test_other_rows_change_no_bit(gpu, mode, dt):
         k = (k.float() * torch.linspace(0.3, 2, Sk)[None, :, None, None]).to(dt).cuda()
         q[:, ::2] *= 0.5
         want = None
-        for f in (0.0, 0.5, 8.0):
+        for f in (0.0, 0.5, 8.0, math.inf, math.nan):
             x = q.clone()
             x[:, 1::2] *= f
             got = ops.attention_masked(x, k, v, **scores_kw(mode, H))[:, ::2]
@@ -250,3 +250,20 @@ def test_intervals_of_other_rows_change_no_bit(gpu, mode, dt):
             got = ops.attention_masked(q, k, v, key_range=r, **scores_kw(mode, H))[:, ::2]
             want = got if want is None else want
             assert torch.equal(got, want), f"{mode}, neighbours see [{lo}, {hi}): {int((got != want).sum())} values differ"
+
+
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_a_table_shows_its_nan(gpu, cap):
+    """An entry of NaN makes NaN of the rows that see a key at its distance, and of no other."""
+    R = 20
+    t = rnd((1, 2 * R + 1), 13)
+    t[0, R - 7] = math.nan
+    for Sq, Sk in ((2, 90), (150, 200)):
+        announce(f"NaN in a table, {Sq}x{Sk}, cap {cap}")
+        q, k, v = qkv(1, Sq, Sk, 1, 1, 64, torch.float16, 14)
+        p = (torch.arange(Sq) * 9 % Sk).to(torch.int32)
+        clean = p < 7  # no key seven behind them
+        got = ops.attention_masked(q.cuda(), k.cuda(), v.cuda(), rel_bias=t.cuda(), cap=cap, q_pos=p.cuda()).cpu()
+        assert got[0, ~clean].isnan().all()
+        ref = M.attention(q[:, clean], k, v, rel_bias=t.nan_to_num(), cap=cap, q_pos=p[clean])
+        within(got[:, clean], ref["o"], att_tol(ref, Sk, torch.float16, v), "the others")
