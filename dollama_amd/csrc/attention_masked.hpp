@@ -443,14 +443,25 @@ struct Core {
   __device__ __forceinline__ T weight(const AmParams& p, float s) const {
     return (T)__builtin_amdgcn_exp2f(MODE == AM_PLAIN ? __builtin_fmaf(s, p.c, -mref) : s - mref);
   }
+  // The sum that moves a base of m: from 2^26 on every sum does, so that `settle` makes the weights again
+  static __device__ __forceinline__ float limit_at(float m) {
+    return MODE == AM_PLAIN && !(fabsf(m) < 0x1p26f) ? -1.0f : Hf::limit;
+  }
   // ... of a tile, and this lane's sum of them, pairs added in the order of `look_ahead`: which of the
   // two makes a row's sum goes by the other rows of its wave, and must not show in a bit of it
+  // ... LARGE: also of plain scores so large that the base's own rounding, which the fused product has
+  // not, is whole powers of two.  Those are rounded as the base was (one of `first` and `then` is 1)
+  template <bool LARGE = false>
   __device__ __forceinline__ float weights(const AmParams& p, const f32x16 (&s)[KB], x8 (&pf)[2 * KB]) const {
     float sum[2] = {0.0f, 0.0f};
+    const float first = lim < 0.0f ? p.c : 1.0f, then = lim < 0.0f ? 1.0f : p.c;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) pf[2 * kb + (e >> 3)][e & 7] = weight(p, s[kb][e]);
+      for (int e = 0; e < 16; ++e)
+        pf[2 * kb + (e >> 3)][e & 7] = LARGE && MODE == AM_PLAIN
+                                           ? (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][e] * first, then, -mref))
+                                           : weight(p, s[kb][e]);
 #pragma unroll
     for (int i = 0; i < 8 * KB; ++i) {
       const int j = i >> 2, e = 2 * (i & 3);
@@ -469,7 +480,7 @@ struct Core {
     m = am_max_halves(mt * p.c);
     if (m != -INFINITY) {
       mref = m - Hf::shift;
-      lim = Hf::limit;
+      lim = limit_at(m);
     }
   }
 
@@ -490,14 +501,14 @@ struct Core {
       const bool move = am_max_halves(past ? 1.0f : 0.0f) > 0.0f && mt > m;
       const float alpha = move ? __builtin_amdgcn_exp2f(m - mt) : 1.0f;
       m = move ? mt : m;
-      lim = move ? Hf::limit : lim;
+      lim = move ? limit_at(m) : lim;
       mref = m == -INFINITY ? 0.0f : m - Hf::shift;
       l *= alpha;
 #pragma unroll
       for (int dt = 0; dt < DV; ++dt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
-      sum = weights(p, s, pf);
+      sum = weights<true>(p, s, pf);
     }
     l += sum;
   }

@@ -267,3 +267,29 @@ def test_a_table_shows_its_nan(gpu, cap):
         assert got[0, ~clean].isnan().all()
         ref = M.attention(q[:, clean], k, v, rel_bias=t.nan_to_num(), cap=cap, q_pos=p[clean])
         within(got[:, clean], ref["o"], att_tol(ref, Sk, torch.float16, v), "the others")
+
+
+@pytest.mark.parametrize("power,dt", [(n, dt) for dt in HALF for n in (20, 27, 33, 36, 70, 110)
+                                      if n <= 36 or dt == torch.bfloat16], ids=str)
+@pytest.mark.parametrize("mode", ["plain", "slopes", "table"])
+def test_scores_far_beyond_their_differences(gpu, mode, power, dt):
+    """Scores of 1.875 2^20 to 2^110, which no sum rounds, times log2 e, which every product rounds: equal
+    ones share their weight, and the largest have it alone."""
+    a = (power - 6) // 2
+    b = power - 6 - a
+    kw = {"slopes": torch.zeros(2)} if mode == "slopes" else {"rel_bias": torch.zeros(2, 41)} if mode == "table" else {}
+    kw = {n: t.cuda() for n, t in kw.items()}
+    for Sq, Sk in ((3, 100), (2, 3000), (150, 300), (150, 2000)):
+        announce(f"scores of 2^{power}, {mode}, {Sq}x{Sk} {dt}")
+        q, k, v = qkv(1, Sq, Sk, 2, 2, 64, dt, 16)
+        q.fill_(1.25 * 2.0 ** a)
+        k.fill_(1.5 * 2.0 ** b)
+        keep = torch.zeros(Sk, dtype=torch.bool)
+        keep[[Sk // 3, Sk // 2, Sk - 2]] = True
+        half = torch.where(keep, 1.0, 0.5)[None, :, None, None]
+        for what, f, seen in (("equal", 1.0, keep | True), ("equal, below 0", -1.0, keep | True), ("three", half, keep),
+                              ("three, below 0", half - 1.5, keep)):
+            got = ops.attention_masked(q.cuda(), (k.float() * f).to(dt).cuda(), v.cuda(), scale=1.0, **kw)
+            want = v[:, seen].double().mean(1, keepdim=True).expand(1, Sq, 2, 64)
+            ref = {"o": want, "A": v[:, seen].double().abs().mean(1, keepdim=True), "err": torch.zeros(1)}
+            within(got, want, att_tol(ref, Sk, dt, v), f"{what} {Sq}x{Sk}")
