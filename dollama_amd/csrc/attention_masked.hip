@@ -158,16 +158,20 @@ int dlm_attention_masked(const dlm_attention_masked_args* a, void* workspace, si
   p.lpt = (a->causal || a->key_range) && pl.splits == 1 && pl.nrb > 1 && blocks <= 8 * 256;
   p.part = (float*)workspace;
   p.c = a->scale * AM_LOG2E;
-  if (a->cap > 0.0f) {
+  // A cap from 2^126 on changes no softmax: scores up to 2^113 it leaves as they are in fp32, and larger
+  // ones are so far apart that one weight alone is not 0, before it and behind.  Its own terms would pass
+  // fp32's range.
+  const bool cap = a->cap > 0.0f && a->cap < 0x1p126f;
+  if (cap) {
     p.ic = a->scale / a->cap;
-    p.cl = std::min(a->cap, FLT_MAX / 2) * AM_LOG2E;
+    p.cl = a->cap * AM_LOG2E;
     const double ic = (double)a->scale / a->cap;
     p.small = (float)std::min(0.5 / ic, (double)FLT_MAX);
     for (int i = 0; i < 5; ++i) p.ct[i] = (float)(AM_TANH[i] * a->scale * 1.4426950408889634);
   }
   p.table_lds = a->rel_bias && (2LL * (a->R + AM_TABLE_MARGIN) + 1) * p.G <= AM_TABLE_MAX;
-  return a->dtype == DLM_DTYPE_F16 ? am_run_f16(p, pl, a->cap > 0.0f, (hipStream_t)stream)
-                                   : am_run_bf16(p, pl, a->cap > 0.0f, (hipStream_t)stream);
+  return a->dtype == DLM_DTYPE_F16 ? am_run_f16(p, pl, cap, (hipStream_t)stream)
+                                   : am_run_bf16(p, pl, cap, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -293,3 +293,16 @@ def test_scores_far_beyond_their_differences(gpu, mode, power, dt):
             want = v[:, seen].double().mean(1, keepdim=True).expand(1, Sq, 2, 64)
             ref = {"o": want, "A": v[:, seen].double().abs().mean(1, keepdim=True), "err": torch.zeros(1)}
             within(got, want, att_tol(ref, Sk, dt, v), f"{what} {Sq}x{Sk}")
+
+
+@pytest.mark.parametrize("cap", [3e38, 1e38, 2.0 ** 125])
+def test_scores_beyond_half_of_the_largest_caps(gpu, cap):
+    for Sq, Sk in ((1, 100), (140, 100)):
+        announce(f"scores of 1.9e38 under a cap of {cap}, {Sq}x{Sk}")
+        q, k, v = qkv(1, Sq, Sk, 1, 1, 64, torch.bfloat16, 15)
+        q.zero_(), k.zero_()
+        q[..., 0] = 1.5 * 2.0 ** 63
+        k[..., 0] = -1.5 * 2.0 ** 62
+        k[0, 10, 0, 0], k[0, 70, 0, 0] = 1.5 * 2.0 ** 62, 1.5 * 2.0 ** 63
+        got = ops.attention_masked(q.cuda(), k.cuda(), v.cuda(), scale=1.0, cap=cap).cpu()
+        assert torch.equal(got, v[:, 70:71].expand(1, Sq, 1, 64)), "the largest score's value alone"
