@@ -362,9 +362,14 @@ struct Core {
   // key of element e of block kb, against the tile's first key and without the lane's 4 g
   static constexpr __device__ int key_of(int kb, int e) { return kb * 32 + 8 * (e >> 2) + (e & 3); }
 
+  static __device__ __forceinline__ bool near(const KeySpan& span) {
+    return (unsigned)span.pmax - (unsigned)span.pmin < 32;
+  }
+
   // Calls f(z): z(x, kb, e) is the score of element e of block kb in powers of two, made of
-  // its q.k x.  (Plain scores stay q.k: their scale goes into the exponent's one operation.)
-  template <typename F>
+  // its q.k x.  (Plain scores stay q.k: their scale goes into the exponent's one operation.)  WHOLE: of a
+  // tile that every row sees whole.
+  template <bool WHOLE = false, typename F>
   __device__ __forceinline__ void with_scores(const AmParams& p, const KeySpan& span, const Row& row,
                                               const f32x16 (&s)[KB], int k0, int g, F f) const {
     if constexpr (MODE == AM_PLAIN) f([](float x, int, int) { return x; });
@@ -387,7 +392,7 @@ struct Core {
       const int first = k0 - row.get(Row::P);
       const float c = p.c, f0 = (float)(first + 4 * g), slope = row.num(Row::SLOPE);
       const bool before = k0 + BK - 1 <= span.pmin;
-      if (before || k0 >= span.pmax) {
+      if (PB < 512 && (before || k0 >= span.pmax)) {  // (wide heads: one copy of the loop's body, for registers)
         const float d = before ? slope : -slope;
         f([&](float x, int kb, int e) {
           return __builtin_fmaf(x, c, __builtin_fmaf(d, (float)key_of(kb, e), d * f0));
@@ -406,7 +411,7 @@ struct Core {
       if (k0 + BK - 1 - span.pmin <= -p.R || k0 - span.pmax >= p.R) {
         const float t = row.num(k0 - span.pmax >= p.R ? Row::RIGHT : Row::LEFT);
         f([&](float x, int, int) { return __builtin_fmaf(x, c, t); });
-      } else if (p.table_lds && (unsigned)span.pmax - (unsigned)span.pmin < 32) {
+      } else if ((WHOLE && PB == 512) || (p.table_lds && near(span))) {
         // (places this near: no distance of the tile passes the margin behind the ends)
         const int d0 = k0 + 4 * g - row.get(Row::P), pitch = 2 * (p.R + AM_TABLE_MARGIN) + 1;
         const float DLM_LDS* tab = row.table + row.get(Row::SUB) * pitch + p.R + AM_TABLE_MARGIN + d0;
@@ -614,8 +619,8 @@ struct Core {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int count = (int)n[e];
-          if (count & 127) o[dt][e] += INFINITY;
-          if (count >> 7) o[dt][e] -= INFINITY;
+          const float all = o[dt][e] + (count & 127 ? INFINITY : 0.0f) - (count >> 7 ? INFINITY : 0.0f);
+          o[dt][e] = count ? all : o[dt][e];  // (without branches, of which 128 and more kept their masks)
         }
       }
     }
@@ -671,6 +676,7 @@ struct Core {
       }
     }
     x8 pf[2 * KB];
+    bool finite = true;
     if (guard) {
       // V times zeros: NaN where V is not finite (the matrix pipe has room here, the vector pipe
       // has not)
@@ -687,15 +693,15 @@ struct Core {
       float sum = 0.0f;
 #pragma unroll
       for (int e = 0; e < 16; ++e) sum += n[e];
-      if (__builtin_amdgcn_ballot_w64(sum != 0.0f) != 0) {
-        special = true;
-        settle(p, s, pf, weights(p, s, pf));
-        pv_finite(st, pf, lane);
-        return;
-      }
+      finite = __builtin_amdgcn_ballot_w64(sum != 0.0f) == 0;
     }
     settle(p, s, pf, weights(p, s, pf));
-    pv(st, pf, lane);
+    if (finite) {
+      pv(st, pf, lane);
+    } else {
+      special = true;
+      pv_finite(st, pf, lane);
+    }
   }
 };
 
@@ -856,7 +862,9 @@ attn_masked_kernel(AmParams p) {
     f0 = max(t0, (flo + C::BK - 1) / C::BK);
     f1 = min(t1, fhi / C::BK);
     f1 -= (f1 - f0) & 1;
-    if (hidden) f1 = f0;
+    // (wide heads have no registers for a third form of the bias in that loop; f1 may differ among the waves,
+    // which meet once a tile either way)
+    if (hidden || (PB == 512 && MODE == AM_TABLE && !C::near(span))) f1 = f0;
   }
   if (t0 < t1) {
     unsigned char DLM_LDS* const vmem = smem + 2 * C::TILE;
@@ -893,7 +901,7 @@ attn_masked_kernel(AmParams p) {
       copy(t, par);
       typename C::x8 pf[4];
       float sum = 0.0f;
-      c.with_scores(p, span, row, sc, t * C::BK, c.g, [&](auto z) {
+      c.template with_scores<true>(p, span, row, sc, t * C::BK, c.g, [&](auto z) {
         sum = c.look_ahead(p, smem + (par ^ 1) * C::TILE, sn, sc, pf, z, lane);
       });
       c.settle(p, sc, pf, sum);
@@ -1170,6 +1178,8 @@ static int am_by_head(const AmParams& p, const AmPlan& pl, hipStream_t s) {
   if (p.Dh <= 64) return am_launch<T, 128, 4, 2, MODE>(p, pl, s);
   if (p.Dh <= 96) return am_launch<T, 256, 6, 3, MODE>(p, pl, s);
   if (p.Dh <= 128) return am_launch<T, 256, 8, 4, MODE>(p, pl, s);
+  // (These fill all 512 registers.  Accumulators that are spilled to AGPRs in part and to scratch memory in part
+  // come back incomplete, by the assembly; so none of these kernels may use scratch memory.)
   return am_launch<T, 512, 16, 8, MODE>(p, pl, s);
 }
 

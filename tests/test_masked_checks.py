@@ -1,7 +1,11 @@
 """More argument checks of the rotary, norm and masked-attention entry points at the C boundary, without a
 device: every refused call returns before anything is launched (CPU only)."""
 import ctypes
+import struct
 
+import msgpack
+
+from dollama_amd import _lib
 from test_masked import A, INVALID, attention_args, err, lib, rotary_args  # noqa: F401 (lib: a fixture)
 
 
@@ -134,3 +138,45 @@ def test_scales_whose_powers_of_two_leave_fp32(lib):
     for cap in (0.0, 1e38):
         assert attend(lib, scale=3e38, cap=cap) == INVALID and "scale" in err()
         assert attend(lib, scale=2.0 ** 127, cap=cap, q_pos=7 * A + 2) == INVALID and "aligned" in err()
+
+
+def code_objects(path):
+    """The gfx950 code objects that the library holds."""
+    with open(path, "rb") as f:
+        d = f.read()
+    at = d.find(b"__CLANG_OFFLOAD_BUNDLE__")
+    while at >= 0:
+        n, p = struct.unpack_from("<Q", d, at + 24)[0], at + 32
+        for _ in range(n):
+            offset, size, length = struct.unpack_from("<QQQ", d, p)
+            if b"gfx950" in d[p + 24:p + 24 + length]:
+                yield d[at + offset:at + offset + size]
+            p += 24 + length
+        at = d.find(b"__CLANG_OFFLOAD_BUNDLE__", at + 24)
+
+
+def kernels(elf):
+    """Their kernels' metadata: the note of type 32 of a note section."""
+    sections, = struct.unpack_from("<Q", elf, 40)
+    entry, count = struct.unpack_from("<HH", elf, 58)
+    for i in range(count):
+        if struct.unpack_from("<I", elf, sections + i * entry + 4)[0] != 7:
+            continue
+        p, size = struct.unpack_from("<QQ", elf, sections + i * entry + 24)
+        end = p + size
+        while p < end:
+            name, desc, kind = struct.unpack_from("<III", elf, p)
+            p += 12 + (name + 3) // 4 * 4
+            if kind == 32:
+                yield from msgpack.unpackb(elf[p:p + desc])["amdhsa.kernels"]
+            p += (desc + 3) // 4 * 4
+
+
+def test_no_kernel_spills_to_both_kinds_of_place(lib):
+    """A tuple of registers that is spilled to AGPRs in part and to scratch memory in part has come back without
+    one of the former: kernels with AGPRs use no scratch memory."""
+    found = [k for e in code_objects(_lib.HIP_LIB_PATH) for k in kernels(e)]
+    wide = [k for k in found if "attn_masked" in k[".name"] and "Li512E" in k[".name"]]
+    assert len(wide) == 20  # two kernels, five kinds of score, two types
+    both = [k[".name"] for k in found if k[".agpr_count"] and k[".private_segment_fixed_size"]]
+    assert not both, both
