@@ -450,7 +450,8 @@ struct Core {
   }
   // The sum that moves a base of m: from 2^26 on every sum does, so that `settle` makes the weights again
   static __device__ __forceinline__ float limit_at(float m) {
-    return MODE == AM_PLAIN && !(fabsf(m) < 0x1p26f) ? -1.0f : Hf::limit;
+    if (MODE == AM_PLAIN && !(fabsf(m) < 0x1p26f)) return -1.0f;
+    return Hf::shift < 0.0f && !(fabsf(m) < 0x1p30f) ? 0x1p10f : Hf::limit;  // (no shift is left from 2^30 on)
   }
   // ... of a tile, and this lane's sum of them, pairs added in the order of `look_ahead`: which of the
   // two makes a row's sum goes by the other rows of its wave, and must not show in a bit of it
@@ -489,6 +490,9 @@ struct Core {
     }
   }
 
+  // What this wave's sums are in powers of two of: -infinity before the first key
+  __device__ __forceinline__ float unit() const { return m == -INFINITY ? m : mref; }
+
   // A tile's weights against the row's base, given their sum.  No maximum is taken: the sum, which is
   // needed anyway, tells when some weight came near the end of its type; only then (and at a row's first
   // keys) the base moves to the tile's maximum and the weights are made again.  That a row moves goes
@@ -504,10 +508,13 @@ struct Core {
         for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[kb][e]);
       mt = am_max_halves(MODE == AM_PLAIN ? mt * p.c : mt);
       const bool move = am_max_halves(past ? 1.0f : 0.0f) > 0.0f && mt > m;
-      const float alpha = move ? __builtin_amdgcn_exp2f(m - mt) : 1.0f;
+      // (from one base less shift to the next, not from base to base: near 2^24 and beyond the shift is
+      // rounded off them, to more or less)
+      const float next = mt - Hf::shift;
+      const float alpha = !move ? 1.0f : m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mref - next);
       m = move ? mt : m;
       lim = move ? limit_at(m) : lim;
-      mref = m == -INFINITY ? 0.0f : m - Hf::shift;
+      mref = move ? next : mref;
       l *= alpha;
 #pragma unroll
       for (int dt = 0; dt < DV; ++dt)
@@ -963,7 +970,7 @@ attn_masked_kernel(AmParams p) {
       }
     if (c.g == 0) {
       float* ml = q->part + (long long)q->splits * q->heads * q->rows * Dh + at * 2;
-      ml[0] = empty ? -INFINITY : c.m;
+      ml[0] = empty ? -INFINITY : c.unit();
       ml[1] = empty ? 0.0f : l;
     }
     return;
@@ -1050,18 +1057,18 @@ attn_masked_rows_kernel(AmParams p) {
   if (c.special) c.add_special(p, span, row, b, hk, t0 + wave, t1, NW);
   const float l = am_sum_halves(c.l);
   if (lane < 32) {
-    ml[wave][lane][0] = c.m;
+    ml[wave][lane][0] = c.unit();
     ml[wave][lane][1] = l;
   }
   __syncthreads();
-  // this wave's sums in the units of the largest base, then all waves' together
+  // this wave's sums in the largest unit, then all waves' together
   float top = -INFINITY, sum = 0.0f;
 #pragma unroll
   for (int w = 0; w < NW; ++w) top = fmaxf(top, ml[w][lane & 31][0]);
   auto weight = [&](float m) { return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top); };
 #pragma unroll
   for (int w = 0; w < NW; ++w) sum += ml[w][lane & 31][1] * weight(ml[w][lane & 31][0]);
-  const float mine = weight(c.m);
+  const float mine = weight(c.unit());
   float DLM_LDS* part = (float DLM_LDS*)smem_g;  // [wave][d][row]
 #pragma unroll
   for (int dt = 0; dt < DV; ++dt)

@@ -306,3 +306,32 @@ def test_scores_beyond_half_of_the_largest_caps(gpu, cap):
         k[0, 10, 0, 0], k[0, 70, 0, 0] = 1.5 * 2.0 ** 62, 1.5 * 2.0 ** 63
         got = ops.attention_masked(q.cuda(), k.cuda(), v.cuda(), scale=1.0, cap=cap).cpu()
         assert torch.equal(got, v[:, 70:71].expand(1, Sq, 1, 64)), "the largest score's value alone"
+
+
+@pytest.mark.parametrize("mode", ["plain", "table"])
+@pytest.mark.parametrize("dt,high,first,rise", [(torch.float16, 12, 32, 18), (torch.bfloat16, 13, 64, 20)], ids=["fp16", "bf16"])
+def test_bases_that_round(gpu, dt, high, first, rise, mode):
+    """One key above 60000 others by a few powers of two, all scores near 2^24 or 2^25, where every number is a
+    multiple of 2 or 4: what was summed against the first base counts against the second as its score says."""
+    scale = float(torch.tensor(math.log(2)))  # to powers of two: 1
+    Sk, at = 60000, 50000
+    for Sq in (1, 70):
+        for B in (1, 260):  # with the keys in parts, and whole
+            if B > 1 and (Sq == 1) != (mode == "plain"):
+                continue
+            announce(f"scores of {first} to {first + rise} above 2^{12 + high}, {mode}, {B}x{Sq} {dt}")
+            q = torch.zeros(1, Sq, 1, 16, dtype=dt)
+            k = torch.zeros(1, Sk, 1, 16, dtype=dt)
+            q[..., 0], q[..., 1] = 2.0 ** high, 1.0
+            k[..., 0], k[..., 1] = 2.0 ** 12, first
+            k[0, at, 0, 1] = first + rise
+            v = torch.ones(1, Sk, 1, 16, dtype=dt)
+            v[0, at] = 0
+            kw = {"rel_bias": torch.zeros(B, 1).cuda()} if mode == "table" else {}
+            # the batches as heads, so that one tensor does for all
+            got = ops.attention_masked(q.expand(1, Sq, B, 16).contiguous().cuda(), k.cuda().expand(1, Sk, B, 16),
+                                       v.cuda().expand(1, Sk, B, 16), scale=scale, **kw).double().cpu()
+            w = (Sk - 1) * 2.0 ** -rise
+            want = torch.full((1, Sq, B, 16), w / (1 + w), dtype=torch.float64)
+            ref = {"o": want, "A": want, "err": torch.zeros(1)}
+            within(got, want, att_tol(ref, Sk, dt, v), f"{B}x{Sq}")
