@@ -13,7 +13,7 @@ static AmPlan am_plan(const dlm_attention_masked_args* a) {
   pl.few = rows <= 32;
   pl.nrb = (int)((rows + (pl.few ? 31 : 127)) / (pl.few ? 32 : 128));
   // Parts of 256 keys at least, as many as cost least by a model in us: the keys' time in one part (a
-  // tile of 64 in 1.2, or 55 kB of few rows' K and V a us), the rounds of workgroups over 256 CUs, and the
+  // tile of 64 in 1.2, as of heads of 128; or 55 kB of few rows' K and V a us), the rounds of workgroups over 256 CUs, and the
   // parts' way through memory.  (us with 1 / 4 / 8 / 16 / 32 parts, 32/8 heads of 128: one token over 4096 keys
   // 38 / 19 / 14 / 12 / 12, over 65536 485 / 132 / 72 / 51 / 50; 64 tokens over 30001
   // 420 / 117 / 67 / 45 / 53; 256 over 4096 68 / 39 / 38 / 50 / 78.)  Few rows, whose

@@ -934,9 +934,10 @@ def linear_q8(xq: torch.Tensor, sx: torch.Tensor, wq: torch.Tensor, sw: torch.Te
 
 # ---------------------------------------------------------------------------
 # Attention with positions, masks and biases.  Operands are [batch, token, head, Dh] or
-# [token, head, Dh] views, fp16 or bf16, with any strides as long as a head's values are
-# consecutive: slices of a fused projection, a cache's used part, head-major layouts
-# seen through transpose.
+# [token, head, Dh] views, fp16 or bf16, a head's values consecutive: slices of a fused
+# projection, a cache's used part, head-major layouts seen through transpose.  The rotation
+# and the norms take any strides and alignment; attention takes strides that are multiples of
+# 8 (out: 4) at 16-byte (out: 8-byte) aligned addresses.
 # ---------------------------------------------------------------------------
 _HALF = {torch.float16: 0, torch.bfloat16: 1}
 _POS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
@@ -1135,7 +1136,12 @@ def attention_masked(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, key_r
     A query sees the keys lo <= j < hi of its key_range (int32 [(batch,) Sq, 2]:
     ``document_ranges``, ``prefix_ranges``, lengths, windows; None: all) and, where
     causal, only j <= p.  So a cache in use up to n keys is q_pos = n - 1 with causal.
-    A query that sees nothing gives 0; what masked keys hold has no effect."""
+    Nor does it see a key whose rel_bias is -infinity.  A query that sees nothing gives 0; what
+    masked and hidden keys hold, infinities and NaN too, has no effect, nor have other queries.
+
+    Strides of q, k and v are multiples of 8, of out of 4, addresses 16-byte and 8-byte aligned.
+    out may be a slice of the tensor that the operands are slices of, and overlaps nothing.
+    Some calls split the keys, through a workspace that the call allocates."""
     dev = _heads_dev(q, "q")
     shape, dt = q.shape, q.dtype
     if k.dim() != len(shape) or k.shape[-2] < 1:

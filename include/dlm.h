@@ -572,7 +572,8 @@ int dlm_linear_q8_f32out(const void* X, int ldx, const float* sx, const void* W,
  * Element (b, s, h, d) of an operand is at b sb + s ss + h sh + d; positions are
  * at b pos_sb + s pos_ss + axis (pos_sb = 0: one line of positions for every
  * batch), int32, int64 or fp32 (DLM_POS_*).  freqs are fp64, and so is the
- * angle, reduced to a turn before its sine; all else is fp32, rounded once.
+ * angle, reduced to a turn; its sine and cosine, the hardware's, are within
+ * 2^-21.  All else is fp32, rounded once.
  *
  * dlm_qk_norm_rotary (norm = 1) first makes every head of q and of k
  * x / sqrt(mean(x^2) + eps) * gamma, with q_gamma and k_gamma [Dh] of the
@@ -582,8 +583,8 @@ int dlm_linear_q8_f32out(const void* X, int ldx, const float* sx, const void* W,
  * dtype is fp16 or bf16 (DLM_DTYPE_*) for every operand but positions and
  * frequencies.  Dh is even and at most 256, tokens (B x S) at most 2^26 - 4.  Any
  * alignment of an element is taken; 16-byte aligned heads are fastest.  An output may be its own input
- * (same pointer and strides) and overlap nothing else; slices of one tensor do
- * not overlap.  Uses no workspace.  No counterpart in the reference
+ * (same pointer and strides) and overlap nothing else, gammas, positions and
+ * frequencies included; slices of one tensor do not overlap.  Uses no workspace.  No counterpart in the reference
  * (src/infer/unet.cu:677-802: no positions, no norm of queries and keys). */
 typedef struct dlm_rotary_args {
   const void* q;
@@ -616,9 +617,10 @@ int dlm_qk_norm_rotary(const dlm_rotary_args* args, void* stream);
  * Query i of batch b sees key j when lo <= j < hi of its interval
  * key_range[b, i] = (lo, hi) (NULL: every key; hi past Sk counts as Sk), and,
  * where causal, j <= p_i.  p_i = q_pos[b, i] is the query's place among the keys
- * (NULL: i + Sk - Sq), within +-2^30.  A query that sees no key, or whose scores
- * are all -infinity, is 0.  What masked keys hold, infinities and NaN too, has
- * no effect.
+ * (NULL: i + Sk - Sq), within +-2^30.  A rel_bias of -infinity hides its key as
+ * well; slopes count as 2^96 / log2(e) at most, in either direction.  A query that
+ * sees no key, or whose scores are all -infinity, is 0.  What masked and hidden
+ * keys hold, infinities and NaN too, has no effect, nor have other queries' values.
  * Query head h reads key / value head h / (H / Hkv).  Element (b, s, h, d) of an
  * operand is at b sb + s ss + h sh + d.  Dh is a multiple of 8 up to 256.  q, k
  * and v start at 16-byte aligned addresses and have strides that are multiples
@@ -631,8 +633,9 @@ int dlm_qk_norm_rotary(const dlm_rotary_args* args, void* stream);
  * and Sq are at most 2^28, B x Hkv at most 65535.
  * Few queries against many keys are split over the keys; the parts meet in the
  * workspace, of dlm_attention_masked_workspace_bytes(args) bytes (may be 0; it
- * goes by sizes alone), 16-byte aligned, which no other call may use until this one's work is
- * done.  o may not overlap q, k or v.  A query's result is reproducible bit for bit.
+ * goes by sizes alone), 16-byte aligned, which overlaps no operand and which no other call may
+ * use until this one's work is done.  o may not overlap q, k, v, masks or biases; slices of one
+ * tensor do not overlap.  A query's result is reproducible bit for bit.
  * No counterpart in the reference (src/kernels/attention.cuh:53-73 has neither
  * masks nor biases). */
 typedef struct dlm_attention_masked_args {

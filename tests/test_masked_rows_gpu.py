@@ -1,5 +1,6 @@
 """Masked attention's rows beside one another: no row's result shows what another row's query, keys or
-place hold, nor what keys hold that a table hides from it (GPU)."""
+place hold, nor what keys hold that a table hides from it; scores, values, slopes and caps at the ends of their
+ranges; row blocks that workgroups share (GPU)."""
 import ctypes
 import math
 
