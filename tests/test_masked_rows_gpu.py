@@ -25,8 +25,9 @@ def scores_kw(mode, H):
     return kw
 
 
-# queries, keys, heads, Dh: few rows, many rows with their keys in parts, many rows whole
-ROWS = [(24, 640, 40, 64), (150, 640, 40, 64), (150, 640, 40, 128), (700, 640, 48, 64)]
+# queries, keys, heads, Dh: few rows, many rows with their keys in parts, many rows whole; every width
+ROWS = [(24, 640, 40, 64), (150, 640, 40, 64), (150, 640, 40, 128), (700, 640, 48, 64), (20, 640, 20, 256), (150, 640, 20, 256),
+        (150, 640, 20, 80)]
 
 
 @pytest.mark.parametrize("dt", HALF, ids=NAMES.get)
@@ -336,3 +337,22 @@ def test_bases_that_round(gpu, dt, high, first, rise, mode):
             want = torch.full((1, Sq, B, 16), w / (1 + w), dtype=torch.float64)
             ref = {"o": want, "A": want, "err": torch.zeros(1)}
             within(got, want, att_tol(ref, Sk, dt, v), f"{B}x{Sq}")
+
+
+@pytest.mark.parametrize("dt", HALF, ids=NAMES.get)
+@pytest.mark.parametrize("Dh", [64, 256])
+def test_places_near_and_far_in_one_workgroup(gpu, Dh, dt):
+    """Waves whose rows' places lie within a table's margin beside waves whose places do not: each takes its
+    own way through the tiles, and all meet at every tile."""
+    table = rnd((3, 2 * 40 + 1), 17)
+    for Sq, Sk, H in ((128, 700, 3), (300, 512, 3), (130, 900, 90)):
+        q, k, v = qkv(1, Sq, Sk, H, H, Dh, dt, 18)
+        g = torch.Generator().manual_seed(Sq)
+        p = torch.arange(Sq, dtype=torch.int32) + 100
+        for at in (0, 64, 160):
+            n = len(p[at:at + 32])
+            p[at:at + 32] = torch.randint(0, Sk, (n,), generator=g).to(torch.int32)
+        t = table.repeat(H // 3, 1)
+        attend(q, k, v, f"places near and far, {Sq}x{Sk}x{H}x{Dh} {dt}", q_pos=p, rel_bias=t)
+        r = torch.tensor([17, Sk - 5], dtype=torch.int32).repeat(Sq, 1)
+        attend(q, k, v, f"places near and far, interval, {Sq}x{Sk}x{H}x{Dh} {dt}", q_pos=p, rel_bias=t, key_range=r)
